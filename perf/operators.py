@@ -325,7 +325,7 @@ def _own_beam(s):
     kda = _package()
     kda.paged_free(s["table"], s["lens"], s["refs"], s["dst"])
     forked = kda.paged_fork(s["pool"], s["table"], s["lens"], s["refs"], s["src"], s["dst"])
-    grown = kda.paged_reserve(s["table"], s["lens"], s["refs"], s["more"])
+    grown = kda.paged_reserve(s["table"], s["lens"], s["refs"], s["more"], s["case"]["page"])
     return {"table": s["table"], "lens": s["lens"], "refs": s["refs"], "forked": forked, "grown": grown,
             "pool": _bits(s["pool"])}
 
