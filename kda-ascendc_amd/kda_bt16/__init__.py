@@ -11,7 +11,9 @@ Beyond the reference: the backward (``kda_bt16_bwd``, and autograd through
 fp32, the decode step and an on-GPU gold) and ``kda_decode_step``; FLA's
 ``chunk_kda`` / ``fused_recurrent_kda`` calling convention (``kda_bt16.fla``)
 and a per-function backend dispatch that registers these kernels
-(``kda_bt16.dispatch``).
+(``kda_bt16.dispatch``); and, for models that alternate KDA layers with
+softmax attention, attention over a paged cache of keys and values and the
+work on its pages (``kda_bt16.paged``).
 """
 
 from . import dispatch
@@ -28,6 +30,15 @@ from .kernels import (
     kda_recurrent_fwd,
     set_backward_recompute,
 )
+from .paged import (
+    paged_append,
+    paged_attention,
+    paged_compact,
+    paged_copy,
+    paged_fork,
+    paged_free,
+    paged_reserve,
+)
 
 __all__ = [
     "kda_bt16_fwd",
@@ -43,5 +54,12 @@ __all__ = [
     "chunk_kda",
     "fused_recurrent_kda",
     "dispatch",
+    "paged_attention",
+    "paged_append",
+    "paged_reserve",
+    "paged_free",
+    "paged_fork",
+    "paged_copy",
+    "paged_compact",
 ]
 __version__ = "0.1.0"

@@ -1,4 +1,5 @@
-"""ctypes binding of ``libkda_bt16_hip.so`` (C ABI in ``include/kda_bt16_hip.h``).
+"""ctypes binding of ``libkda_bt16_hip.so`` (C ABI in ``include/kda_bt16_hip.h``
+and ``include/kda_paged_hip.h``).
 
 The library is loaded lazily on first use.  There is no fallback: if the
 library is missing or fails to load, every call raises.
@@ -52,6 +53,27 @@ EXPORTED_SYMBOLS = (
     "kda_bt16_fused_aborts",
     "kda_bt16_strerror",
     "kda_bt16_abi_version",
+)
+
+
+# include/kda_paged_hip.h
+PAGED_ABI_VERSION = 1
+PAGED_BF16 = 0
+PAGED_FP16 = 1
+PAGED_CAUSAL = 1 << 0
+PAGED_MAX_POOLS = 8
+
+PAGED_SYMBOLS = (
+    "kda_paged_attn_workspace_bytes",
+    "kda_paged_attn_hip",
+    "kda_paged_append_hip",
+    "kda_pages_workspace_bytes",
+    "kda_pages_reserve_hip",
+    "kda_pages_free_hip",
+    "kda_pages_fork_hip",
+    "kda_pages_copy_hip",
+    "kda_pages_compact_hip",
+    "kda_paged_abi_version",
 )
 
 
@@ -117,6 +139,94 @@ class KdaBt16BwdArgs(ctypes.Structure):
     ]
 
 
+class KdaPagedArgs(ctypes.Structure):
+    """Mirror of ``struct KdaPagedArgs``."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("N", ctypes.c_int32),
+        ("T", ctypes.c_int32),
+        ("HQ", ctypes.c_int32),
+        ("HKV", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("P", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("M", ctypes.c_int32),
+        ("flags", ctypes.c_uint32),
+        ("window", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("cu_seqlens_dtype", ctypes.c_int32),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_page", ctypes.c_int64),
+        ("k_token", ctypes.c_int64),
+        ("k_head", ctypes.c_int64),
+        ("v_page", ctypes.c_int64),
+        ("v_token", ctypes.c_int64),
+        ("v_head", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("q_row", ctypes.c_int64),
+        ("q_token", ctypes.c_int64),
+        ("q_head", ctypes.c_int64),
+        ("o", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("new_k", ctypes.c_void_p),
+        ("new_v", ctypes.c_void_p),
+        ("nk_row", ctypes.c_int64),
+        ("nk_token", ctypes.c_int64),
+        ("nk_head", ctypes.c_int64),
+        ("nv_row", ctypes.c_int64),
+        ("nv_token", ctypes.c_int64),
+        ("nv_head", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class KdaPagePool(ctypes.Structure):
+    """Mirror of ``struct KdaPagePool``."""
+
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("lead", ctypes.c_int64),
+        ("page_bytes", ctypes.c_int64),
+    ]
+
+
+class KdaPagesArgs(ctypes.Structure):
+    """Mirror of ``struct KdaPagesArgs``."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("N", ctypes.c_int32),
+        ("M", ctypes.c_int32),
+        ("P", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("F", ctypes.c_int32),
+        ("num_pools", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("pools", KdaPagePool * PAGED_MAX_POOLS),
+        ("page_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("page_refs", ctypes.c_void_p),
+        ("src", ctypes.c_void_p),
+        ("dst", ctypes.c_void_p),
+        ("new_tokens", ctypes.c_void_p),
+        ("ok", ctypes.c_void_p),
+        ("out_table", ctypes.c_void_p),
+        ("out_refs", ctypes.c_void_p),
+        ("out_live", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class KdaHipError(RuntimeError):
     """A non-zero return code from the HIP library."""
 
@@ -175,6 +285,24 @@ def lib() -> ctypes.CDLL:
         h.kda_bt16_strerror.argtypes = [ctypes.c_int]
         h.kda_bt16_abi_version.restype = ctypes.c_int
         h.kda_bt16_abi_version.argtypes = []
+        for name in ("kda_paged_attn_hip", "kda_paged_append_hip"):
+            fn = getattr(h, name)
+            fn.restype = ctypes.c_int
+            fn.argtypes = [ctypes.POINTER(KdaPagedArgs), ctypes.c_void_p]
+        for name in ("kda_pages_reserve_hip", "kda_pages_free_hip", "kda_pages_fork_hip",
+                     "kda_pages_copy_hip", "kda_pages_compact_hip"):
+            fn = getattr(h, name)
+            fn.restype = ctypes.c_int
+            fn.argtypes = [ctypes.POINTER(KdaPagesArgs), ctypes.c_void_p]
+        h.kda_paged_attn_workspace_bytes.restype = ctypes.c_size_t
+        h.kda_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(KdaPagedArgs)]
+        h.kda_pages_workspace_bytes.restype = ctypes.c_size_t
+        h.kda_pages_workspace_bytes.argtypes = [ctypes.POINTER(KdaPagesArgs)]
+        h.kda_paged_abi_version.restype = ctypes.c_int
+        h.kda_paged_abi_version.argtypes = []
+        if h.kda_paged_abi_version() != PAGED_ABI_VERSION:
+            raise ImportError(f"{LIB_PATH.name} has paged-cache ABI version {h.kda_paged_abi_version()}, "
+                              f"expected {PAGED_ABI_VERSION}")
         got = h.kda_bt16_abi_version()
         if got != ABI_VERSION:
             raise ImportError(f"{LIB_PATH.name} has ABI version {got}, expected {ABI_VERSION}")

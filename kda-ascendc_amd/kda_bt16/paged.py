@@ -1,0 +1,466 @@
+"""A paged cache of keys and values on MI355X: attention of new tokens over
+it, their append, and the work on its pages.
+
+For models that alternate KDA layers with softmax-attention layers: the KDA
+layers keep a state of fixed size (:func:`kda_bt16.kda_decode_step`), the
+attention layers a cache that grows with every token.  No counterpart in the
+reference, which has no attention cache.
+
+The cache of a layer is a pool of pages for its keys and one for its values,
+``[P, page_size, HKV, D]`` each: views of any layout whose last dimension is
+contiguous (tokens of a head together, ``[P, HKV, page_size, D]`` transposed,
+read in longer pieces).  One table serves all layers:
+
+* ``page_table`` ``[N, M]`` int32: the pages of each sequence, -1 for none;
+* ``seq_lens`` ``[N]`` int32: its cached tokens, those of the call included;
+* ``page_refs`` ``[P]`` int32: the sequences that hold each page, 0 if it is
+  free.
+
+All of it stays on the device: no call here waits for the GPU or reads a
+length on the host.  A step of a serving loop::
+
+    ok = paged_reserve(page_table, seq_lens, page_refs, new_tokens, page_size)
+    for layer in layers:
+        paged_append(k, v, layer.k_cache, layer.v_cache, page_table, seq_lens)
+        o = paged_attention(q, layer.k_cache, layer.v_cache, page_table, seq_lens)
+
+The new tokens of a sequence are its last ones: token i of T sits at position
+``seq_lens - T + i``.  Entries outside ``[0, P)``, lengths beyond the table's
+rows and row numbers outside ``[0, N)`` give unspecified results but never an
+access outside the tensors.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _hip, workspace
+from .kernels import _raw_stream, _require_gpu
+
+_CACHE_DTYPES = {torch.bfloat16: _hip.PAGED_BF16, torch.float16: _hip.PAGED_FP16}
+
+
+def _int32(name: str, t: torch.Tensor, ndim: int, device: torch.device) -> None:
+    if t.ndim != ndim:
+        raise ValueError(f"{name} must be {ndim}D, got {t.ndim}D with shape {tuple(t.shape)}")
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32, got {t.dtype}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name} must be contiguous")
+    if t.device != device:
+        raise ValueError(f"{name} device {t.device} must match ({device})")
+
+
+def _check_table(page_table, seq_lens, device) -> None:
+    _int32("page_table", page_table, 2, device)
+    _int32("seq_lens", seq_lens, 1, device)
+    if page_table.shape[0] < 1 or page_table.shape[1] < 1:
+        raise ValueError(f"page_table dimensions must be positive, got shape {tuple(page_table.shape)}")
+    if seq_lens.shape[0] != page_table.shape[0]:
+        raise ValueError(
+            f"seq_lens must have one entry a row of page_table, {page_table.shape[0]}, got {seq_lens.shape[0]}")
+    if page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]:
+        raise ValueError("rows of page_table must not overlap")
+
+
+def _check_page_size(size: int) -> None:
+    if size < 16 or size > 1024 or size & (size - 1):
+        raise ValueError(f"the page size must be a power of two from 16 to 1024, got {size}")
+
+
+def _check_strided(name: str, t: torch.Tensor) -> None:
+    """16-byte accesses at any (page, token, head)."""
+    if t.stride(-1) != 1:
+        raise ValueError(f"{name}'s last dimension must be contiguous")
+    if t.data_ptr() % 16 or any(t.stride(i) % 8 for i in range(t.ndim - 1) if t.shape[i] > 1):
+        raise ValueError(f"{name} must be 16-byte aligned, its strides multiples of 8 elements; "
+                         f"got strides {t.stride()}")
+
+
+def _check_cache(k_cache, v_cache, page_table, seq_lens) -> None:
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if t.ndim != 4:
+            raise ValueError(f"{name} must be 4D [P, page_size, HKV, D], got {t.ndim}D with shape {tuple(t.shape)}")
+        if t.dtype not in _CACHE_DTYPES:
+            raise TypeError(f"{name} must be bfloat16 or float16, got {t.dtype}")
+    if v_cache.shape != k_cache.shape:
+        raise ValueError(f"v_cache.shape {tuple(v_cache.shape)} must match k_cache {tuple(k_cache.shape)}")
+    if v_cache.dtype != k_cache.dtype:
+        raise TypeError(f"v_cache must be {k_cache.dtype} like k_cache, got {v_cache.dtype}")
+    P, size, HKV, D = k_cache.shape
+    if P < 1 or HKV < 1:
+        raise ValueError(f"cache dimensions must be positive, got P={P}, HKV={HKV}")
+    _check_page_size(size)
+    if D not in (64, 128):
+        raise ValueError(f"the head size must be 64 or 128, got {D}")
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        _check_strided(name, t)
+        if t.stride(1) < D or (P > 1 and t.stride(0) < 1) or (HKV > 1 and t.stride(2) < D):
+            raise ValueError(f"{name}'s tokens must not overlap, got strides {t.stride()}")
+    if v_cache.device != k_cache.device:
+        raise ValueError(f"v_cache device {v_cache.device} must match k_cache ({k_cache.device})")
+    _check_table(page_table, seq_lens, k_cache.device)
+
+
+def _check_new(name: str, t: torch.Tensor, heads: int | None, k_cache, page_table, cu_seqlens) -> None:
+    """Tensors of the new tokens: [N, T, heads, D], or [1, T, heads, D] packed."""
+    if t.ndim != 4:
+        raise ValueError(f"{name} must be 4D [B, T, H, D], got {t.ndim}D with shape {tuple(t.shape)}")
+    if t.dtype != k_cache.dtype:
+        raise TypeError(f"{name} must be {k_cache.dtype} like the cache, got {t.dtype}")
+    if t.device != k_cache.device:
+        raise ValueError(f"{name} device {t.device} must match k_cache ({k_cache.device})")
+    B, T, H, D = t.shape
+    if D != k_cache.shape[-1]:
+        raise ValueError(f"{name} must have the cache's head size {k_cache.shape[-1]}, got {D}")
+    if heads is not None and H != heads:
+        raise ValueError(f"{name} must have the cache's {heads} heads, got {H}")
+    if T < 1 or H < 1:
+        raise ValueError(f"{name} dimensions must be positive, got T={T}, H={H}")
+    N = page_table.shape[0]
+    if cu_seqlens is None:
+        if B != N:
+            raise ValueError(f"{name} must have one row a row of page_table, {N}, got {B}")
+    else:
+        if B != 1:
+            raise ValueError(
+                f"The batch size is expected to be 1 rather than {B} when using `cu_seqlens`. "
+                "Please flatten variable-length inputs before processing.")
+        if cu_seqlens.ndim != 1 or cu_seqlens.shape[0] != N + 1:
+            raise ValueError(f"cu_seqlens must have {N + 1} entries, one more than the rows of page_table, "
+                             f"got shape {tuple(cu_seqlens.shape)}")
+        if cu_seqlens.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"cu_seqlens must be int32 or int64, got {cu_seqlens.dtype}")
+        if not cu_seqlens.is_contiguous():
+            raise ValueError("cu_seqlens must be contiguous")
+        if cu_seqlens.device != t.device:
+            raise ValueError(f"cu_seqlens device {cu_seqlens.device} must match {name} ({t.device})")
+    _check_strided(name, t)
+
+
+def _cache_args(k_cache, v_cache, page_table, seq_lens, N, T, HQ, cu_seqlens) -> _hip.KdaPagedArgs:
+    P, size, HKV, D = k_cache.shape
+    a = _hip.KdaPagedArgs(
+        _hip.PAGED_ABI_VERSION, N, T, HQ, HKV, D, _CACHE_DTYPES[k_cache.dtype], P, size, page_table.shape[1], 0, 0,
+        1.0, 0, None, page_table.data_ptr(), max(page_table.stride(0), page_table.shape[1]), seq_lens.data_ptr(),
+        k_cache.data_ptr(), v_cache.data_ptr(), *_strides(k_cache), *_strides(v_cache))
+    if cu_seqlens is not None:
+        a.cu_seqlens = cu_seqlens.data_ptr()
+        a.cu_seqlens_dtype = _hip.DTYPE_I64 if cu_seqlens.dtype == torch.int64 else _hip.DTYPE_I32
+    return a
+
+
+def _strides(t: torch.Tensor) -> tuple[int, int, int]:
+    """The first three strides; of a dimension of one element, 0."""
+    s, n = t.stride(), t.shape
+    return (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
+
+
+def paged_attention(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    page_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    *,
+    scale: float | None = None,
+    causal: bool = True,
+    window: int | None = None,
+    cu_seqlens: torch.Tensor | None = None,
+    return_lse: bool = False,
+):
+    """Softmax attention of new tokens over their sequences' cached keys and
+    values (the new tokens' own among them, :func:`paged_append`).
+
+    ``q`` is ``[N, T, HQ, D]``, T new tokens of each sequence (one: a decode
+    step), or with ``cu_seqlens`` ``[1, total, HQ, D]``, chunks of any lengths
+    packed.  HQ is a multiple of HKV; query head h reads the cache's head
+    ``h // (HQ // HKV)``; D is 64 or 128; bfloat16 or float16, like the cache.
+    ``q`` may be a view (a slice of a fused projection).
+
+    A query at position p sees the keys up to p (``causal``; else all), with
+    ``window`` those above ``p - window`` only.  ``scale`` (above 0) is
+    ``D ** -0.5`` by default.  Sums and the softmax are held in fp32; the
+    exponentials are rounded to q's type for the product with the values.
+
+    Returns ``o`` in q's shape and type, with ``return_lse`` also the log of
+    the sum of the exponentials, fp32 ``[N, T, HQ]``.  A query that sees no
+    key (an empty sequence) has o = 0 and -inf.  What the pages hold beyond
+    ``seq_lens`` does not matter; keys and values before it have to be finite.
+    Forward only: raises if q requires a gradient.
+    """
+    _check_cache(k_cache, v_cache, page_table, seq_lens)
+    _check_new("q", q, None, k_cache, page_table, cu_seqlens)
+    B, T, HQ, D = q.shape
+    HKV = k_cache.shape[2]
+    if HQ % HKV != 0:
+        raise ValueError(f"HQ must be a multiple of HKV, got HQ={HQ}, HKV={HKV}")
+    if scale is None:
+        scale = D ** -0.5
+    if not scale > 0:
+        raise ValueError(f"scale must be positive, got {scale}")
+    if window is not None:
+        if window < 1:
+            raise ValueError(f"window must be at least 1, got {window}")
+        if not causal:
+            raise ValueError("window needs causal=True")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k_cache, v_cache)):
+        raise NotImplementedError("paged_attention is forward only: inputs require grad")
+    _require_gpu(q)
+    o = torch.empty((B, T, HQ, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, T, HQ), dtype=torch.float32, device=q.device) if return_lse else None
+    a = _cache_args(k_cache, v_cache, page_table, seq_lens, page_table.shape[0], T, HQ, cu_seqlens)
+    a.flags = _hip.PAGED_CAUSAL if causal else 0
+    a.window = window or 0
+    a.scale = scale
+    a.q, a.o = q.data_ptr(), o.data_ptr()
+    a.q_row, a.q_token, a.q_head = _strides(q)
+    if lse is not None:
+        a.lse = lse.data_ptr()
+    with torch.cuda.device(q.device):
+        nbytes = int(_hip.lib().kda_paged_attn_workspace_bytes(ctypes.byref(a)))
+        if nbytes:
+            ws = workspace.scratch(q.device, nbytes)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        _hip.call("kda_paged_attn_hip", a, _raw_stream(q.device))
+    return (o, lse) if return_lse else o
+
+
+def paged_append(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    page_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    *,
+    cu_seqlens: torch.Tensor | None = None,
+) -> None:
+    """Writes the new tokens' keys and values into their places in the pages.
+
+    ``k`` and ``v`` are ``[N, T, HKV, D]`` or, with ``cu_seqlens``, packed
+    ``[1, total, HKV, D]``, of the cache's type; they may be views.
+    ``seq_lens`` counts the new tokens already (:func:`paged_reserve`).
+    Tokens at negative positions, or whose page the table does not have, are
+    left out.
+    """
+    _check_cache(k_cache, v_cache, page_table, seq_lens)
+    for name, t in (("k", k), ("v", v)):
+        _check_new(name, t, k_cache.shape[2], k_cache, page_table, cu_seqlens)
+    if v.shape != k.shape:
+        raise ValueError(f"v.shape {tuple(v.shape)} must match k {tuple(k.shape)}")
+    _require_gpu(k)
+    a = _cache_args(k_cache, v_cache, page_table, seq_lens, page_table.shape[0], k.shape[1], 0, cu_seqlens)
+    a.new_k, a.new_v = k.data_ptr(), v.data_ptr()
+    a.nk_row, a.nk_token, a.nk_head = _strides(k)
+    a.nv_row, a.nv_token, a.nv_head = _strides(v)
+    with torch.cuda.device(k.device):
+        _hip.call("kda_paged_append_hip", a, _raw_stream(k.device))
+
+
+def _pools(pools) -> list[torch.Tensor]:
+    """The pools of a call, checked: ``[..., P, a, b, c]`` each."""
+    ts = [pools] if isinstance(pools, torch.Tensor) else list(pools)
+    if not 1 <= len(ts) <= _hip.PAGED_MAX_POOLS:
+        raise ValueError(f"between 1 and {_hip.PAGED_MAX_POOLS} pools, got {len(ts)}")
+    P = ts[0].shape[-4] if ts[0].ndim >= 4 else 0
+    for i, t in enumerate(ts):
+        if t.ndim < 4:
+            raise ValueError(f"pool {i} must be at least 4D [..., P, a, b, c], got shape {tuple(t.shape)}")
+        if not t.is_contiguous():
+            raise ValueError(f"pool {i} must be contiguous")
+        if t.numel() == 0:
+            raise ValueError(f"pool {i} dimensions must be positive, got shape {tuple(t.shape)}")
+        if t.shape[-4] != P:
+            raise ValueError(f"pool {i} must have {P} pages like the first, got {t.shape[-4]}")
+        if t.device != ts[0].device:
+            raise ValueError(f"pool {i} device {t.device} must match the first's ({ts[0].device})")
+        if t.data_ptr() % 16 or t.stride(-4) * t.element_size() % 16:
+            raise ValueError(f"pool {i} must be 16-byte aligned, its pages multiples of 16 bytes")
+    return ts
+
+
+def _pages_args(P: int, pools=(), page_table=None, seq_lens=None, page_refs=None, page_size: int = 16):
+    a = _hip.KdaPagesArgs()
+    a.abi_version, a.P, a.page_size = _hip.PAGED_ABI_VERSION, P, page_size
+    a.num_pools = len(pools)
+    for i, t in enumerate(pools):
+        page = t.stride(-4) * t.element_size()
+        a.pools[i] = _hip.KdaPagePool(t.data_ptr(), t.numel() * t.element_size() // (P * page), page)
+    if page_table is not None:
+        a.N, a.M = page_table.shape
+        a.page_table, a.table_stride = page_table.data_ptr(), max(page_table.stride(0), a.M)
+    if seq_lens is not None:
+        a.seq_lens = seq_lens.data_ptr()
+    if page_refs is not None:
+        a.page_refs = page_refs.data_ptr()
+    return a
+
+
+def _check_refs(page_refs, device) -> None:
+    _int32("page_refs", page_refs, 1, device)
+    if page_refs.shape[0] < 1:
+        raise ValueError("page_refs must not be empty")
+    if page_refs.data_ptr() % 16:
+        raise ValueError("page_refs must be 16-byte aligned")
+
+
+def _with_workspace(a, device) -> torch.Tensor:
+    ws = workspace.scratch(device, int(_hip.lib().kda_pages_workspace_bytes(ctypes.byref(a))))
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    return ws
+
+
+def _check_rows(pairs, device) -> None:
+    for name, t in pairs:
+        _int32(name, t, 1, device)
+        if t.shape[0] != pairs[0][1].shape[0]:
+            raise ValueError(f"{name} must have {pairs[0][1].shape[0]} entries like {pairs[0][0]}, got {t.shape[0]}")
+
+
+def paged_reserve(
+    page_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    page_refs: torch.Tensor,
+    new_tokens: torch.Tensor,
+    page_size: int,
+) -> torch.Tensor:
+    """Room for ``new_tokens[n]`` (int32 ``[N]``) more tokens of every
+    sequence: the lowest free pages, in the sequences' order, until they run
+    out; ``seq_lens`` grows by as many.
+
+    Returns a bool ``[N]``: False for a sequence whose pages cannot all be
+    had, or do not fit its row; it keeps what it has.
+    """
+    device = page_table.device
+    _check_table(page_table, seq_lens, device)
+    _check_refs(page_refs, device)
+    _check_rows([("seq_lens", seq_lens), ("new_tokens", new_tokens)], device)
+    _check_page_size(page_size)
+    _require_gpu(page_table)
+    ok = torch.empty(seq_lens.shape[0], dtype=torch.bool, device=device)
+    a = _pages_args(page_refs.shape[0], (), page_table, seq_lens, page_refs, page_size)
+    a.new_tokens, a.ok = new_tokens.data_ptr(), ok.data_ptr()
+    with torch.cuda.device(device):
+        ws = _with_workspace(a, device)  # noqa: F841  (held until the launch)
+        _hip.call("kda_pages_reserve_hip", a, _raw_stream(device))
+    return ok
+
+
+def paged_free(
+    page_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    page_refs: torch.Tensor,
+    rows: torch.Tensor,
+) -> None:
+    """The sequences ``rows`` (int32) end: their pages lose a holder each,
+    their entries become -1, their lengths 0."""
+    device = page_table.device
+    _check_table(page_table, seq_lens, device)
+    _check_refs(page_refs, device)
+    _check_rows([("rows", rows)], device)
+    _require_gpu(page_table)
+    a = _pages_args(page_refs.shape[0], (), page_table, seq_lens, page_refs)
+    a.F, a.dst = rows.shape[0], rows.data_ptr()
+    with torch.cuda.device(device):
+        _hip.call("kda_pages_free_hip", a, _raw_stream(device))
+
+
+def paged_fork(
+    pools,
+    page_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    page_refs: torch.Tensor,
+    src: torch.Tensor,
+    dst: torch.Tensor,
+    *,
+    page_size: int | None = None,
+) -> torch.Tensor:
+    """Row ``dst[i]`` (empty) becomes a copy of row ``src[i]`` (int32): whole
+    pages are shared, the tokens of a last partial page copied, in every pool,
+    to the lowest free page not taken by an earlier fork.
+
+    ``pools`` is a tensor ``[..., P, page_size, HKV, D]`` or a sequence of
+    them (up to 8): keys and values of all layers in one, or apart.  With
+    another order of a page's dimensions (``[..., P, HKV, page_size, D]``)
+    give ``page_size``.  Rows of ``dst`` are distinct and none is in ``src``;
+    a row of ``src`` may be forked several times.
+
+    Returns a bool per fork: False where no page was left; the row stays empty.
+    """
+    ts = _pools(pools)
+    device = ts[0].device
+    _check_table(page_table, seq_lens, device)
+    _check_refs(page_refs, device)
+    _check_rows([("src", src), ("dst", dst)], device)
+    page_size = ts[0].shape[-3] if page_size is None else page_size
+    _check_page_size(page_size)
+    P = ts[0].shape[-4]
+    if page_refs.shape[0] != P:
+        raise ValueError(f"page_refs must have one entry a page, {P}, got {page_refs.shape[0]}")
+    _require_gpu(ts[0])
+    ok = torch.empty(src.shape[0], dtype=torch.bool, device=device)
+    a = _pages_args(P, ts, page_table, seq_lens, page_refs, page_size)
+    a.F, a.src, a.dst, a.ok = src.shape[0], src.data_ptr(), dst.data_ptr(), ok.data_ptr()
+    with torch.cuda.device(device):
+        ws = _with_workspace(a, device)  # noqa: F841
+        _hip.call("kda_pages_fork_hip", a, _raw_stream(device))
+    return ok
+
+
+def paged_copy(pools, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """``pool[..., dst[i], :, :, :] = pool[..., src[i], :, :, :]`` for every
+    pool, ``[..., P, a, b, c]``, in one launch.
+
+    Pages of a cache, or whatever else goes along with a sequence: recurrent
+    states ``[layers, rows, HV, 128, 128]`` are a pool of ``rows`` pages.
+    Pairs outside ``[0, P)`` are left out; no page is in ``src`` and in
+    ``dst``, or in ``dst`` twice.
+    """
+    ts = _pools(pools)
+    device = ts[0].device
+    _check_rows([("src", src), ("dst", dst)], device)
+    _require_gpu(ts[0])
+    a = _pages_args(ts[0].shape[-4], ts)
+    a.F, a.src, a.dst = src.shape[0], src.data_ptr(), dst.data_ptr()
+    with torch.cuda.device(device):
+        _hip.call("kda_pages_copy_hip", a, _raw_stream(device))
+
+
+def paged_compact(
+    pools,
+    page_table: torch.Tensor,
+    page_refs: torch.Tensor,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Moves the held pages into the first ``live`` places of every pool,
+    live being their number: the i-th held page at or above ``live`` goes to
+    the i-th free place below it.
+
+    Returns ``(page_table, page_refs, live)``, new tensors (live: int32
+    ``[1]``).  The old table and counts stay as they are, and the pages moved
+    away from keep their contents: a launch on another stream that still reads
+    by the old table stays right until those pages are handed out again.
+    """
+    ts = _pools(pools)
+    device = ts[0].device
+    P = ts[0].shape[-4]
+    _int32("page_table", page_table, 2, device)
+    if page_table.shape[0] < 1 or page_table.shape[1] < 1:
+        raise ValueError(f"page_table dimensions must be positive, got shape {tuple(page_table.shape)}")
+    if page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]:
+        raise ValueError("rows of page_table must not overlap")
+    _check_refs(page_refs, device)
+    if page_refs.shape[0] != P:
+        raise ValueError(f"page_refs must have one entry a page, {P}, got {page_refs.shape[0]}")
+    _require_gpu(ts[0])
+    table = torch.empty(page_table.shape, dtype=torch.int32, device=device)
+    refs = torch.empty_like(page_refs)
+    live = torch.empty(1, dtype=torch.int32, device=device)
+    a = _pages_args(P, ts, page_table, None, page_refs)
+    a.out_table, a.out_refs, a.out_live = table.data_ptr(), refs.data_ptr(), live.data_ptr()
+    with torch.cuda.device(device):
+        ws = _with_workspace(a, device)  # noqa: F841
+        _hip.call("kda_pages_compact_hip", a, _raw_stream(device))
+    return table, refs, live
