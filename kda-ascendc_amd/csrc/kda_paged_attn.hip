@@ -52,9 +52,21 @@ struct FP16 {
 };
 
 constexpr int WAVES = 4;
-constexpr int ROWS = 32;            // rows a wave
-constexpr int MT = WAVES * ROWS;    // rows a work-group
-constexpr int TK = 64;              // keys a tile
+constexpr int ROWS = 32;  // rows of a wave's products
+
+// Two ways over the keys.  Few rows (a decode step, a draft): every wave of a
+// work-group has the same 32 rows and keys of its own.  Many rows (a chunk):
+// every wave has rows of its own, and the work-group's keys are shared.
+constexpr int FEW = 0, MANY = 1, MIXED = 2;
+template <int KIND>
+struct Shape {
+    static constexpr int MT = KIND == FEW ? ROWS : WAVES * ROWS;  // rows a work-group
+    static constexpr int TK = KIND == FEW ? 32 : 64;              // keys a tile
+    // Tiles a work-group takes at least, where keys are split among several.
+    static constexpr int LEAST = KIND == FEW ? 8 : 4;
+};
+// Work-groups the keys are split for: two on each of 256 CUs.
+constexpr int SLOTS = 512;
 
 // A tile of keys (or values) in LDS: rows of D elements, in each the 16-byte
 // piece c at place c ^ swizzle(row).  The swizzle keeps two reads free of bank
@@ -102,94 +114,377 @@ __device__ __forceinline__ u32x2 read_v(const uint8_t* lds, int key, int db, int
 
 __device__ __forceinline__ float other_half(float x) { return shfl(x, (threadIdx.x & 63) ^ 32); }
 
-// Work-group -> (sequence, kv head, row tile): sequence by sequence, its row
-// tiles last first (those of a causal chunk see the most keys), heads
-// innermost.  Every lane counts one sequence's work-groups.
+// Maximum and sum of the softmax over one tile's scores (16 * NB a lane, of
+// keys key0 + 32 * b + 8 * (i / 4) + i % 4), and its weights as operands of the
+// second product: m in the scores' unit, c = scale * log2 e.  Returns the
+// factor by which sums so far shrink.
+template <class E, int NB>
+__device__ __forceinline__ float softmax_tile(f32x16 (&st)[NB], int key0, int lo, int hi, bool edge, float c, float& m,
+                                              float& l, u32x4 (&pt)[2 * NB]) {
+    float mx = -INFINITY;
+    if (edge) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = key0 + 32 * b + 8 * (i >> 2) + (i & 3);
+                if (key < lo || key >= hi) st[b][i] = -INFINITY;
+            }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[b][i]);
+    mx = fmaxf(mx, other_half(mx));
+    // (a row that has seen no key yet keeps m = -inf and subtracts 0)
+    const float m2 = fmaxf(m, mx);
+    const float sub = m2 == -INFINITY ? 0.f : m2 * c;
+    const float alpha = fast_exp2(fmaf(m, c, -sub));
+    m = m2;
+    float sum = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const float e0 = fast_exp2(fmaf(st[b][i], c, -sub)), e1 = fast_exp2(fmaf(st[b][i + 1], c, -sub));
+            sum += e0 + e1;
+            pt[2 * b + (i >> 3)][(i & 7) >> 1] = E::pack(e0, e1);
+        }
+    l = fmaf(l, alpha, sum);
+    return alpha;
+}
+
+// ---- the split ----
+
+// What a sequence is to a launch of one kind: row tiles (0: not of this kind)
+// and the tiles of keys that a row tile sees at most.
+struct SeqWork {
+    int mt, tiles;
+};
+template <int KIND>
+__device__ __forceinline__ SeqWork seq_work(const PagedParams& p, const NewTokens& s) {
+    constexpr int MT = Shape<KIND>::MT, TK = Shape<KIND>::TK;
+    const int rows = s.count * p.G;
+    SeqWork w = {(rows + MT - 1) / MT, (s.len + TK - 1) / TK};
+    if (p.cu_seqlens && (rows <= ROWS) != (KIND == FEW)) w.mt = 0;
+    if (p.window) {
+        // the tokens of a row tile and the window before the first
+        const int64_t span = (int64_t)min(s.count, MT / p.G + 2) + p.window;
+        w.tiles = (int)min((int64_t)w.tiles, (span + 2 * TK - 2) / TK);
+    }
+    return w;
+}
+
+__device__ __forceinline__ int wave_prefix(int x, int lane) {  // inclusive
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+
+// A part of the work: row tile m of (sequence n, kv head h) over part `part` of
+// `parts` of its keys; with several parts, its place in the workspace (that of
+// part 0 is `slot - part * stride`).
 struct Unit {
-    int n, h, m;
+    int n, h, m, part, parts, slot;
     NewTokens s;
 };
+
+// Work-group (COMBINE: row tile) `id` -> its part.  The keys are split so that the parts are
+// about SLOTS: a part has at most S = ceil(all tiles / SLOTS) tiles, at least
+// LEAST.  Sequence by sequence, a sequence's row tiles last first (those of a
+// causal chunk see the most keys), then its parts, heads innermost.  Every
+// lane counts one sequence; all work-groups come to the same split, from the
+// lengths on the device.  Parts of split row tiles number at most 2 * SLOTS:
+// a row tile of t > S tiles has ceil(t / S) < 2 t / S.
+template <int KIND, bool COMBINE>
 __device__ __forceinline__ bool find_unit(const PagedParams& p, int id, int lane, Unit& u) {
+    int64_t all = 0;
     for (int n0 = 0; n0 < p.N; n0 += 64) {
-        int tiles = 0;
+        int64_t x = 0;
         if (n0 + lane < p.N) {
-            const NewTokens s = new_tokens(p, n0 + lane);
-            tiles = (s.count * p.G + MT - 1) / MT;
+            const SeqWork w = seq_work<KIND>(p, new_tokens(p, n0 + lane));
+            x = (int64_t)w.mt * w.tiles;
         }
-        int end = tiles * p.HKV;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int x = __shfl_up(end, d);
-            if (lane >= d) end += x;
-        }
+        for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+        all += x;
+    }
+    const int64_t share = (all * p.HKV + SLOTS - 1) / SLOTS;
+    const int S = __builtin_amdgcn_readfirstlane((int)(share > 0x7fffffff ? 0x7fffffff : max((int64_t)Shape<KIND>::LEAST, share)));
+    int slots = 0;
+    for (int n0 = 0; n0 < p.N; n0 += 64) {
+        SeqWork w = {0, 0};
+        if (n0 + lane < p.N) w = seq_work<KIND>(p, new_tokens(p, n0 + lane));
+        const int parts = max(1, (w.tiles + S - 1) / S);
+        const int end = wave_prefix(w.mt * p.HKV * (COMBINE ? 1 : parts), lane);
+        const int slot_end = wave_prefix(parts > 1 ? w.mt * p.HKV * parts : 0, lane);
         const int total = __builtin_amdgcn_readlane(end, 63);
         if (id < total) {
             const int at = __builtin_ctzll(__ballot(end > id));
             const int before = at > 0 ? __builtin_amdgcn_readlane(end, at - 1) : 0;
-            const int mt = __builtin_amdgcn_readlane(tiles, at);
+            const int slot0 = slots + (at > 0 ? __builtin_amdgcn_readlane(slot_end, at - 1) : 0);
+            const int mt = __builtin_amdgcn_readlane(w.mt, at);
+            u.parts = __builtin_amdgcn_readlane(parts, at);
             u.n = __builtin_amdgcn_readfirstlane(n0 + at);
-            const int x = id - before;
+            int x = id - before;
             u.h = x % p.HKV;
-            u.m = mt - 1 - x / p.HKV;
+            x /= p.HKV;
+            u.part = 0;
+            if (!COMBINE) {
+                u.part = x % u.parts;
+                x /= u.parts;
+            }
+            u.m = mt - 1 - x;
+            u.slot = slot0 + (x * p.HKV + u.h) * u.parts + u.part;
             u.s = new_tokens(p, u.n);
             return true;
         }
         id -= total;
+        slots += __builtin_amdgcn_readlane(slot_end, 63);
     }
     return false;
 }
 
+// A part's rows in the workspace: m (times c), l, then the row tile's O.
+template <int KIND, int D>
+struct Partial {
+    static constexpr int MT = Shape<KIND>::MT;
+    static constexpr int64_t FLOATS = MT * (D + 2);
+    static __device__ __forceinline__ float* at(float* ws, int slot) { return ws + slot * FLOATS; }
+};
+// Floats of the workspace before the parts of kind MANY.
+template <int D>
+constexpr int64_t few_floats() { return 2 * SLOTS * Partial<FEW, D>::FLOATS; }
+
+// What a row sees: keys [lo, hi) of its sequence.
+struct Row {
+    int tok, head, lo, hi;
+    bool live;
+};
+__device__ __forceinline__ Row row_of(const PagedParams& p, const Unit& u, int r) {
+    Row x;
+    const int rows = u.s.count * p.G;
+    x.live = r < rows;
+    const int rc = min(r, rows - 1);  // (rows past the last: its values again, unstored)
+    x.tok = rc / p.G;
+    x.head = u.h * p.G + (rc - x.tok * p.G);
+    const int pos = u.s.pos + x.tok;
+    x.hi = p.causal ? max(0, min(pos + 1, u.s.len)) : u.s.len;
+    x.lo = p.window ? max(0, pos + 1 - p.window) : 0;
+    return x;
+}
+
+// The tiles of keys of a part: those that rows r0 .. r1 see, its share.
+struct Tiles {
+    int begin, end;
+};
+template <int KIND>
+__device__ __forceinline__ Tiles tiles_of(const PagedParams& p, const Unit& u) {
+    constexpr int MT = Shape<KIND>::MT, TK = Shape<KIND>::TK;
+    const int rows = u.s.count * p.G;
+    const int first = u.m * MT / p.G, last = (min(rows, u.m * MT + MT) - 1) / p.G;
+    const int hi = p.causal ? max(0, min(u.s.pos + last + 1, u.s.len)) : u.s.len;
+    const int lo = p.window ? min(hi, max(0, u.s.pos + first + 1 - p.window)) : 0;
+    const int t0 = lo / TK, t1 = (hi + TK - 1) / TK;
+    const int64_t count = max(0, t1 - t0);
+    return {t0 + (int)(count * u.part / u.parts), t0 + (int)(count * (u.part + 1) / u.parts)};
+}
+
+__device__ __forceinline__ int64_t out_row(const PagedParams& p, const Unit& u, const Row& x) {
+    return (p.cu_seqlens ? (int64_t)u.s.first + x.tok : (int64_t)u.n * p.T + x.tok) * p.HQ + x.head;
+}
+
+template <int D>
+__device__ __forceinline__ void load_q(const PagedParams& p, const Unit& u, const Row& x, int half, u32x4 (&q)[D / 16]) {
+    const uint16_t* at = p.q + (p.cu_seqlens ? u.s.first * p.q_token : u.n * p.q_row) + x.tok * p.q_token + x.head * p.q_head;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) q[s] = *reinterpret_cast<const u32x4*>(at + 16 * s + 8 * half);
+}
+
+// 16 keys from `key` on (a multiple of 16) into LDS: they share a page.
+template <int D>
+__device__ __forceinline__ void load_keys(const PagedParams& p, const uint16_t* cache, int64_t page_stride, int64_t token,
+                                          int64_t head, int page, int key, int len, int lane, uint8_t* lds) {
+    const int rows = page < 0 ? 0 : min(len - key, 16);
+    const int64_t pg = page < 0 ? 0 : page;
+    const int in = key & ((1 << p.page_shift) - 1);
+    load_rows<D>(cache + pg * page_stride + in * token + head, token, rows, lane, lds);
+}
+
+__device__ __forceinline__ int page_at(const PagedParams& p, const Unit& u, int key) {
+    return key < u.s.len ? page_of(p, u.n, key >> p.page_shift) : -1;
+}
+
+// This wave's LDS reads have returned: what they read may be loaded over.
+__device__ __forceinline__ void reads_done() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt 0
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Output or partial of one row's four elements from d on.
 template <class E, int D>
-__global__ __launch_bounds__(256) void paged_attn_kernel(PagedParams p) {
-    constexpr int STEPS = D / 16, DB = D / 32;
-    __shared__ alignas(1024) uint8_t kt[TK * D * 2];
-    __shared__ alignas(1024) uint8_t vt[TK * D * 2];
+__device__ __forceinline__ void store_o(const PagedParams& p, int64_t out, int d, float a, float b, float c, float e) {
+    *reinterpret_cast<u32x2*>(p.o + out * D + d) = u32x2{E::pack(a, b), E::pack(c, e)};
+}
+__device__ __forceinline__ float log_sum(float mc, float l) {
+    return l > 0.f ? (mc + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+}
+
+// ---- few rows ----
+
+// Each wave goes over every fourth tile of 32 keys, through LDS of its own:
+// while it multiplies keys the values arrive, and the other way round.  The
+// four waves' sums are joined at the end.
+template <class E, int D>
+__device__ void few_rows(const PagedParams& p, const Unit& u, uint8_t* kt, uint8_t* vt, float* joint) {
+    constexpr int STEPS = D / 16, DB = D / 32, TK = 32;
+    constexpr int TILE = TK * D * 2;
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    Unit u;
-    if (!find_unit(p, blockIdx.x, lane, u)) return;
-
-    // This lane's query; rows past the last compute its values again, unstored.
-    const int rows = u.s.count * p.G;
-    const int r = u.m * MT + wave * ROWS + (lane & 31);
-    const bool live = r < rows;
-    const int rc = min(r, rows - 1);
-    const int tok = rc / p.G, head = u.h * p.G + (rc - tok * p.G);
-    const int64_t row0 = p.cu_seqlens ? u.s.first : 0;
-    u32x4 q[STEPS];
-    {
-        const uint16_t* qp = p.q + (p.cu_seqlens ? 0 : u.n * p.q_row) + (row0 + tok) * p.q_token + head * p.q_head;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) q[s] = *reinterpret_cast<const u32x4*>(qp + 16 * s + 8 * half);
-    }
-    // The keys it sees, [lo, hi), and the tile's.
-    const int pos = u.s.pos + tok;
-    const int hi = p.causal ? max(0, min(pos + 1, u.s.len)) : u.s.len;
-    const int lo = p.window ? max(0, pos + 1 - p.window) : 0;
-    const int first_tok = u.m * MT / p.G, last_tok = min(rows - 1, u.m * MT + MT - 1) / p.G;
-    const int tile_hi = p.causal ? max(0, min(u.s.pos + last_tok + 1, u.s.len)) : u.s.len;
-    const int tile_lo = p.window ? max(0, u.s.pos + first_tok + 1 - p.window) : 0;
-
+    const Row x = row_of(p, u, u.m * ROWS + (lane & 31));
+    const Tiles tl = tiles_of<FEW>(p, u);
+    uint8_t* kw = kt + wave * TILE;
+    uint8_t* vw = vt + wave * TILE;
     const float c = p.scale * LOG2E;
     float m = -INFINITY, l = 0.f;
     f32x16 acc[DB];
 #pragma unroll
     for (int i = 0; i < DB; ++i) acc[i] = f32x16{};
 
-    for (int t0 = tile_lo & -TK; t0 < tile_hi; t0 += TK) {
+    int t = tl.begin + wave;
+    int pages[2], next[2];
+    auto look_up = [&](int tile, int (&pg)[2]) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) pg[g] = tile < tl.end ? page_at(p, u, tile * TK + 16 * g) : -1;
+    };
+    auto load_k = [&](int tile, const int (&pg)[2]) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+            load_keys<D>(p, p.k, p.k_page, p.k_token, u.h * p.k_head, pg[g], tile * TK + 16 * g, u.s.len, lane, kw + g * (TILE / 2));
+    };
+    auto load_v = [&](int tile, const int (&pg)[2]) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+            load_keys<D>(p, p.v, p.v_page, p.v_token, u.h * p.v_head, pg[g], tile * TK + 16 * g, u.s.len, lane, vw + g * (TILE / 2));
+    };
+    look_up(t, pages);
+    if (t < tl.end) {
+        load_k(t, pages);
+        load_v(t, pages);
+    }
+    look_up(t + WAVES, next);
+    u32x4 q[STEPS];
+    load_q<D>(p, u, x, half, q);
+    for (; t < tl.end; t += WAVES) {
+        f32x16 st[1] = {f32x16{}};
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) st[0] = E::mfma(read_k<D>(kw, lane & 31, 2 * s + half), q[s], st[0]);
+        reads_done();
+        if (t + WAVES < tl.end) load_k(t + WAVES, next);
+        u32x4 pt[2];
+        const float alpha = softmax_tile<E, 1>(st, t * TK + 4 * half, x.lo, x.hi, true, c, m, l, pt);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            acc[d] *= alpha;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const u32x2 v0 = read_v<D>(vw, 16 * k + 4 * half, d, lane);
+                const u32x2 v1 = read_v<D>(vw, 16 * k + 8 + 4 * half, d, lane);
+                acc[d] = E::mfma(u32x4{v0.x, v0.y, v1.x, v1.y}, pt[k], acc[d]);
+            }
+        }
+        reads_done();
+        if (t + WAVES < tl.end) load_v(t + WAVES, next);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) pages[g] = next[g];
+        look_up(t + 2 * WAVES, next);
+    }
+    l += other_half(l);
+
+    // Join: every wave's m and l, then its O over the tiles' LDS, row by row
+    // in pieces of four (the rows' pieces turned by the row, so that the lanes
+    // of a half, one row each, write different banks).
+    const int row = lane & 31;
+    if (half == 0) {
+        joint[wave * 2 * ROWS + row] = m * c;
+        joint[wave * 2 * ROWS + ROWS + row] = l;
+    }
+    __syncthreads();
+    float* own = reinterpret_cast<float*>(wave < 2 ? kt : vt) + (wave & 1) * (ROWS * D);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int piece = (32 * d + 2 * i + 4 * half) / 4;
+            *reinterpret_cast<f32x4*>(own + row * D + ((piece + row) & (D / 4 - 1)) * 4) =
+                f32x4{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
+        }
+    __syncthreads();
+    float* part = u.parts > 1 ? Partial<FEW, D>::at(p.ws, u.slot) : nullptr;
+    for (int e = threadIdx.x; e < ROWS * (D / 4); e += 256) {
+        const int r = e / (D / 4), piece = e % (D / 4);
+        const Row y = row_of(p, u, u.m * ROWS + r);
+        if (!y.live) break;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) mx = fmaxf(mx, joint[w * 2 * ROWS + r]);
+        const float sub = mx == -INFINITY ? 0.f : mx;
+        float sum = 0.f;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float f = fast_exp2(joint[w * 2 * ROWS + r] - sub);
+            sum = fmaf(f, joint[w * 2 * ROWS + ROWS + r], sum);
+            const float* src = reinterpret_cast<const float*>(w < 2 ? kt : vt) + (w & 1) * (ROWS * D);
+            const f32x4 v = *reinterpret_cast<const f32x4*>(src + r * D + ((piece + r) & (D / 4 - 1)) * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = fmaf(f, v[i], o[i]);
+        }
+        if (part) {
+            *reinterpret_cast<f32x4*>(part + 2 * ROWS + r * D + piece * 4) = o;
+            if (piece == 0) {
+                part[r] = mx;
+                part[ROWS + r] = sum;
+            }
+        } else {
+            const float inv = sum > 0.f ? 1.f / sum : 0.f;
+            const int64_t out = out_row(p, u, y);
+            store_o<E, D>(p, out, piece * 4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+            if (p.lse && piece == 0) p.lse[out] = log_sum(mx, sum);
+        }
+    }
+}
+
+// ---- many rows ----
+
+template <class E, int D>
+__device__ void many_rows(const PagedParams& p, const Unit& u, uint8_t* kt, uint8_t* vt) {
+    constexpr int STEPS = D / 16, DB = D / 32, TK = Shape<MANY>::TK, MT = Shape<MANY>::MT;
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = wave * ROWS + (lane & 31);
+    const Row x = row_of(p, u, u.m * MT + row);
+    const Tiles tl = tiles_of<MANY>(p, u);
+    u32x4 q[STEPS];
+    load_q<D>(p, u, x, half, q);
+    const float c = p.scale * LOG2E;
+    float m = -INFINITY, l = 0.f;
+    f32x16 acc[DB];
+#pragma unroll
+    for (int i = 0; i < DB; ++i) acc[i] = f32x16{};
+
+    for (int t = tl.begin; t < tl.end; ++t) {
+        const int t0 = t * TK;
         __syncthreads();
         {
-            // 16 rows a wave, all of one page
-            const int key = t0 + 16 * wave;
-            const int left = u.s.len - key;
-            const int page = left > 0 ? page_of(p, u.n, key >> p.page_shift) : -1;
-            const int in = key & ((1 << p.page_shift) - 1);
-            const int n = page < 0 ? 0 : min(left, 16);
-            const int64_t pg = page < 0 ? 0 : page;
-            load_rows<D>(p.k + pg * p.k_page + in * p.k_token + u.h * p.k_head, p.k_token, n, lane,
-                         kt + wave * (16 * D * 2));
-            load_rows<D>(p.v + pg * p.v_page + in * p.v_token + u.h * p.v_head, p.v_token, n, lane,
-                         vt + wave * (16 * D * 2));
+            // 16 keys a wave
+            const int key = t0 + 16 * wave, page = page_at(p, u, key);
+            load_keys<D>(p, p.k, p.k_page, p.k_token, u.h * p.k_head, page, key, u.s.len, lane, kt + wave * (16 * D * 2));
+            load_keys<D>(p, p.v, p.v_page, p.v_token, u.h * p.v_head, page, key, u.s.len, lane, vt + wave * (16 * D * 2));
         }
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
@@ -202,32 +497,8 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedParams p) {
             for (int s = 0; s < STEPS; ++s)
                 st[b] = E::mfma(read_k<D>(kt, 32 * b + (lane & 31), 2 * s + half), q[s], st[b]);
         }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = t0 + 32 * b + 8 * (i >> 2) + 4 * half + (i & 3);
-                if (key < lo || key >= hi) st[b][i] = -INFINITY;
-                mx = fmaxf(mx, st[b][i]);
-            }
-        mx = fmaxf(mx, other_half(mx));
-        // (a row that has seen no key yet keeps m = -inf and subtracts 0)
-        const float m2 = fmaxf(m, mx);
-        const float sub = m2 == -INFINITY ? 0.f : m2 * c;
-        const float alpha = fast_exp2(fmaf(m, c, -sub));
-        m = m2;
-        float sum = 0.f;
         u32x4 pt[4];
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float e0 = fast_exp2(fmaf(st[b][i], c, -sub)), e1 = fast_exp2(fmaf(st[b][i + 1], c, -sub));
-                sum += e0 + e1;
-                pt[2 * b + (i >> 3)][(i & 7) >> 1] = E::pack(e0, e1);
-            }
-        l = fmaf(l, alpha, sum);
+        const float alpha = softmax_tile<E, 2>(st, t0 + 4 * half, x.lo, x.hi, true, c, m, l, pt);
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
             acc[d] *= alpha;
@@ -241,36 +512,149 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedParams p) {
     }
 
     l += other_half(l);
-    if (!live) return;
-    const int64_t out = (p.cu_seqlens ? row0 + tok : (int64_t)u.n * p.T + tok) * p.HQ + head;
+    if (!x.live) return;
+    if (u.parts > 1) {
+        float* part = Partial<MANY, D>::at(p.ws + few_floats<D>(), u.slot);
+        if (half == 0) {
+            part[row] = m * c;
+            part[MT + row] = l;
+        }
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<f32x4*>(part + 2 * MT + row * D + 32 * d + 2 * i + 4 * half) =
+                    f32x4{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
+        return;
+    }
+    const int64_t out = out_row(p, u, x);
     const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const u32x2 w = {E::pack(acc[d][i] * inv, acc[d][i + 1] * inv),
-                             E::pack(acc[d][i + 2] * inv, acc[d][i + 3] * inv)};
-            *reinterpret_cast<u32x2*>(p.o + out * D + 32 * d + 2 * i + 4 * half) = w;
+        for (int i = 0; i < 16; i += 4)
+            store_o<E, D>(p, out, 32 * d + 2 * i + 4 * half, acc[d][i] * inv, acc[d][i + 1] * inv, acc[d][i + 2] * inv,
+                          acc[d][i + 3] * inv);
+    if (p.lse && half == 0) p.lse[out] = log_sum(m * c, l);
+}
+
+// ---- kernels ----
+
+// KIND MIXED: the first `few` work-groups take the sequences of few rows, the
+// others the rest.
+template <class E, int D, int KIND>
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedParams p, int few) {
+    constexpr int BYTES = (KIND == MANY ? 64 : 128) * D * 2;
+    __shared__ alignas(1024) uint8_t kt[BYTES];
+    __shared__ alignas(1024) uint8_t vt[BYTES];
+    __shared__ float joint[KIND == MANY ? 1 : WAVES * 2 * ROWS];
+    const int lane = threadIdx.x & 63;
+    Unit u;
+    if (KIND == FEW || (KIND == MIXED && (int)blockIdx.x < few)) {
+        if (find_unit<FEW, false>(p, blockIdx.x, lane, u)) few_rows<E, D>(p, u, kt, vt, joint);
+    } else {
+        if (find_unit<MANY, false>(p, blockIdx.x - few, lane, u)) many_rows<E, D>(p, u, kt, vt);
+    }
+}
+
+// The parts of one row tile joined.
+template <class E, int D, int KIND>
+__device__ void combine(const PagedParams& p, const Unit& u, const float* ws) {
+    constexpr int MT = Shape<KIND>::MT;
+    const float* first = ws + u.slot * Partial<KIND, D>::FLOATS;
+    for (int e = threadIdx.x; e < MT * (D / 4); e += 256) {
+        const int r = e / (D / 4), piece = e % (D / 4);
+        const Row y = row_of(p, u, u.m * MT + r);
+        if (!y.live) break;
+        float mx = -INFINITY;
+        for (int j = 0; j < u.parts; ++j) mx = fmaxf(mx, first[j * Partial<KIND, D>::FLOATS + r]);
+        const float sub = mx == -INFINITY ? 0.f : mx;
+        float sum = 0.f;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < u.parts; ++j) {
+            const float* part = first + j * Partial<KIND, D>::FLOATS;
+            const float f = fast_exp2(part[r] - sub);
+            sum = fmaf(f, part[MT + r], sum);
+            const f32x4 v = *reinterpret_cast<const f32x4*>(part + 2 * MT + r * D + piece * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = fmaf(f, v[i], o[i]);
         }
-    if (p.lse && half == 0)
-        p.lse[out] = l > 0.f ? (m * c + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        const int64_t out = out_row(p, u, y);
+        store_o<E, D>(p, out, piece * 4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+        if (p.lse && piece == 0) p.lse[out] = log_sum(mx, sum);
+    }
+}
+template <class E, int D, int KIND>
+__global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p, int few) {
+    const int lane = threadIdx.x & 63;
+    Unit u;
+    if (KIND == FEW || (KIND == MIXED && (int)blockIdx.x < few)) {
+        if (find_unit<FEW, true>(p, blockIdx.x, lane, u) && u.parts > 1) combine<E, D, FEW>(p, u, p.ws);
+    } else {
+        if (find_unit<MANY, true>(p, blockIdx.x - few, lane, u) && u.parts > 1)
+            combine<E, D, MANY>(p, u, p.ws + few_floats<D>());
+    }
+}
+
+// ---- launches ----
+
+// What a call's kinds are from what the host knows: packed sequences may be of
+// both, unless their tokens cannot be of many rows.
+int kind_of(const PagedParams& p) {
+    if ((int64_t)p.T * p.G <= ROWS) return FEW;
+    return p.cu_seqlens ? MIXED : MANY;
+}
+
+// Row tiles of a kind at most, and whether their keys may be split.
+template <int KIND>
+int64_t most_units(const PagedParams& p) {
+    constexpr int MT = Shape<KIND>::MT;
+    const int64_t rows = (int64_t)p.T * p.G;
+    if (!p.cu_seqlens) return (int64_t)p.N * ((rows + MT - 1) / MT) * p.HKV;
+    return (KIND == FEW ? (int64_t)p.N : rows / MT + p.N) * p.HKV;
+}
+template <int KIND>
+bool may_split(const PagedParams& p) {
+    return ((int64_t)p.M << p.page_shift) > Shape<KIND>::LEAST * Shape<KIND>::TK;
+}
+
+template <class E, int D, int KIND>
+hipError_t launch(const PagedParams& p, hipStream_t stream) {
+    const int64_t fu = KIND == MANY ? 0 : most_units<FEW>(p), mu = KIND == FEW ? 0 : most_units<MANY>(p);
+    const bool fs = KIND != MANY && may_split<FEW>(p), ms = KIND != FEW && may_split<MANY>(p);
+    // (splitting adds at most SLOTS work-groups: the parts are at most one a
+    // row tile and one for every S tiles)
+    const int64_t fw = fu + (fs ? SLOTS : 0), mw = mu + (ms ? SLOTS : 0);
+    paged_attn_kernel<E, D, KIND><<<dim3((unsigned)(fw + mw)), 256, 0, stream>>>(p, (int)fw);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !(fs || ms)) return e;
+    paged_combine_kernel<E, D, KIND><<<dim3((unsigned)(fu + mu)), 256, 0, stream>>>(p, (int)fu);
+    return hipGetLastError();
 }
 
 template <class E, int D>
-hipError_t launch(const PagedParams& p, hipStream_t stream) {
-    // at most this many (packed sequences each leave one tile unfilled)
-    const int64_t tiles = p.cu_seqlens ? ((int64_t)p.T * p.G) / MT + p.N : (int64_t)p.N * (((int64_t)p.T * p.G + MT - 1) / MT);
-    paged_attn_kernel<E, D><<<dim3((unsigned)(tiles * p.HKV)), dim3(256), 0, stream>>>(p);
-    return hipGetLastError();
+hipError_t launch_kind(const PagedParams& p, hipStream_t stream) {
+    switch (kind_of(p)) {
+        case FEW: return launch<E, D, FEW>(p, stream);
+        case MANY: return launch<E, D, MANY>(p, stream);
+        default: return launch<E, D, MIXED>(p, stream);
+    }
 }
 
 }  // namespace
 
-size_t paged_attn_workspace(const PagedParams&, int) { return 0; }
+size_t paged_attn_workspace(const PagedParams& p, int D) {
+    const int kind = kind_of(p);
+    const bool fs = kind != MANY && may_split<FEW>(p), ms = kind != FEW && may_split<MANY>(p);
+    if (!fs && !ms) return 0;
+    const int64_t few = 2 * SLOTS * (int64_t)Shape<FEW>::MT * (D + 2), many = 2 * SLOTS * (int64_t)Shape<MANY>::MT * (D + 2);
+    return (size_t)(few + (ms ? many : 0)) * 4;
+}
 
 hipError_t launch_paged_attn(const PagedParams& p, int D, hipStream_t stream) {
-    if (D == 128) return p.fp16 ? launch<FP16, 128>(p, stream) : launch<BF16, 128>(p, stream);
-    return p.fp16 ? launch<FP16, 64>(p, stream) : launch<BF16, 64>(p, stream);
+    if (D == 128) return p.fp16 ? launch_kind<FP16, 128>(p, stream) : launch_kind<BF16, 128>(p, stream);
+    return p.fp16 ? launch_kind<FP16, 64>(p, stream) : launch_kind<BF16, 64>(p, stream);
 }
 
 }  // namespace kda
