@@ -140,22 +140,78 @@ def _check_new(name: str, t: torch.Tensor, heads: int | None, k_cache, page_tabl
     _check_strided(name, t)
 
 
-def _cache_args(k_cache, v_cache, page_table, seq_lens, N, T, HQ, cu_seqlens) -> _hip.KdaPagedArgs:
-    P, size, HKV, D = k_cache.shape
-    a = _hip.KdaPagedArgs(
-        _hip.PAGED_ABI_VERSION, N, T, HQ, HKV, D, _CACHE_DTYPES[k_cache.dtype], P, size, page_table.shape[1], 0, 0,
-        1.0, 0, None, page_table.data_ptr(), max(page_table.stride(0), page_table.shape[1]), seq_lens.data_ptr(),
-        k_cache.data_ptr(), v_cache.data_ptr(), *_strides(k_cache), *_strides(v_cache))
-    if cu_seqlens is not None:
-        a.cu_seqlens = cu_seqlens.data_ptr()
-        a.cu_seqlens_dtype = _hip.DTYPE_I64 if cu_seqlens.dtype == torch.int64 else _hip.DTYPE_I32
-    return a
+_PAGE_SIZES = (16, 32, 64, 128, 256, 512, 1024)
+
+
+def _plain_cache(k, v, table, lens) -> bool:
+    """Whether these are an ordinary cache and table on a GPU that
+    :func:`_check_cache` accepts, each tensor looked at once: a small call's
+    time is the host's, and the checks in the order of their messages are half
+    of it.  False says nothing: the full checks then accept or raise."""
+    shape, s, dt, dev = k.shape, k.stride(), k.dtype, k.get_device()
+    if dev < 0 or len(shape) != 4 or v.shape != shape or v.dtype is not dt or v.get_device() != dev:
+        return False
+    t, D = v.stride(), shape[3]
+    if not (
+        (dt is torch.bfloat16 or dt is torch.float16) and (D == 128 or D == 64) and shape[1] in _PAGE_SIZES
+        and s[3] == 1 and t[3] == 1 and s[0] > 0 and t[0] > 0 and s[1] >= D and s[2] >= D and t[1] >= D and t[2] >= D
+        and (s[0] | s[1] | s[2] | t[0] | t[1] | t[2]) % 8 == 0 and (k.data_ptr() | v.data_ptr()) % 16 == 0
+        and shape[0] > 0 and shape[2] > 0
+    ):
+        return False
+    return _plain_table(table, lens, dev)
+
+
+def _plain_table(table, lens, dev) -> bool:
+    """As :func:`_plain_cache`, for :func:`_check_table`."""
+    n = table.shape
+    return (
+        len(n) == 2 and n[1] > 0 and lens.shape == n[:1] and table.dtype is torch.int32 and lens.dtype is torch.int32
+        and table.is_contiguous() and lens.is_contiguous() and table.get_device() == dev and lens.get_device() == dev
+        and n[0] > 0
+    )
+
+
+def _plain_new(x, rows, heads, D, dt, dev) -> bool:
+    """As :func:`_plain_cache`, for :func:`_check_new` without cu_seqlens
+    (``heads`` 0: any)."""
+    n, s = x.shape, x.stride()
+    return (
+        len(n) == 4 and n[0] == rows and n[3] == D and n[1] > 0 and (n[2] == heads if heads else n[2] > 0)
+        and x.dtype is dt and x.get_device() == dev and s[3] == 1 and (s[0] | s[1] | s[2]) % 8 == 0
+        and x.data_ptr() % 16 == 0
+    )
 
 
 def _strides(t: torch.Tensor) -> tuple[int, int, int]:
     """The first three strides; of a dimension of one element, 0."""
     s, n = t.stride(), t.shape
     return (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
+
+
+def _cache_args(k_cache, v_cache, page_table, seq_lens, new, HQ, cu_seqlens, flags=0, window=0, scale=1.0,
+                rest=()) -> _hip.KdaPagedArgs:
+    """The arguments of a call, in the order of the fields (setting each by
+    name takes twice the time); ``rest`` from ``q`` on."""
+    P, size, HKV, D = k_cache.shape
+    N, M = page_table.shape
+    cu, cu_dtype = None, 0
+    if cu_seqlens is not None:
+        cu = cu_seqlens.data_ptr()
+        cu_dtype = _hip.DTYPE_I64 if cu_seqlens.dtype == torch.int64 else _hip.DTYPE_I32
+    return _hip.KdaPagedArgs(
+        _hip.PAGED_ABI_VERSION, N, new.shape[1], HQ, HKV, D, _CACHE_DTYPES[k_cache.dtype], P, size, M, flags, window,
+        scale, cu_dtype, cu, page_table.data_ptr(), page_table.stride(0) if N > 1 else M, seq_lens.data_ptr(),
+        k_cache.data_ptr(), v_cache.data_ptr(), *_strides(k_cache), *_strides(v_cache), *rest)
+
+
+def _launch(name: str, a, device: torch.device) -> None:
+    """The entry point on the tensors' device and its current stream."""
+    if torch._C._cuda_getDevice() == device.index:
+        _hip.call(name, a, _raw_stream(device))
+        return
+    with torch.cuda.device(device):
+        _hip.call(name, a, _raw_stream(device))
 
 
 def paged_attention(
@@ -191,8 +247,10 @@ def paged_attention(
     ``seq_lens`` does not matter; keys and values before it have to be finite.
     Forward only: raises if q requires a gradient.
     """
-    _check_cache(k_cache, v_cache, page_table, seq_lens)
-    _check_new("q", q, None, k_cache, page_table, cu_seqlens)
+    if not (cu_seqlens is None and _plain_cache(k_cache, v_cache, page_table, seq_lens)
+            and _plain_new(q, page_table.shape[0], 0, k_cache.shape[3], k_cache.dtype, k_cache.get_device())):
+        _check_cache(k_cache, v_cache, page_table, seq_lens)
+        _check_new("q", q, None, k_cache, page_table, cu_seqlens)
     B, T, HQ, D = q.shape
     HKV = k_cache.shape[2]
     if HQ % HKV != 0:
@@ -206,25 +264,20 @@ def paged_attention(
             raise ValueError(f"window must be at least 1, got {window}")
         if not causal:
             raise ValueError("window needs causal=True")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k_cache, v_cache)):
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise NotImplementedError("paged_attention is forward only: inputs require grad")
     _require_gpu(q)
-    o = torch.empty((B, T, HQ, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, T, HQ), dtype=torch.float32, device=q.device) if return_lse else None
-    a = _cache_args(k_cache, v_cache, page_table, seq_lens, page_table.shape[0], T, HQ, cu_seqlens)
-    a.flags = _hip.PAGED_CAUSAL if causal else 0
-    a.window = window or 0
-    a.scale = scale
-    a.q, a.o = q.data_ptr(), o.data_ptr()
-    a.q_row, a.q_token, a.q_head = _strides(q)
-    if lse is not None:
-        a.lse = lse.data_ptr()
-    with torch.cuda.device(q.device):
-        nbytes = int(_hip.lib().kda_paged_attn_workspace_bytes(ctypes.byref(a)))
-        if nbytes:
-            ws = workspace.scratch(q.device, nbytes)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-        _hip.call("kda_paged_attn_hip", a, _raw_stream(q.device))
+    device = q.device
+    o = torch.empty((B, T, HQ, D), dtype=q.dtype, device=device)
+    lse = torch.empty((B, T, HQ), dtype=torch.float32, device=device) if return_lse else None
+    a = _cache_args(
+        k_cache, v_cache, page_table, seq_lens, q, HQ, cu_seqlens, _hip.PAGED_CAUSAL if causal else 0, window or 0, scale,
+        (q.data_ptr(), *_strides(q), o.data_ptr(), None if lse is None else lse.data_ptr()))
+    nbytes = _hip.lib().kda_paged_attn_workspace_bytes(ctypes.byref(a))
+    if nbytes:
+        ws = workspace.scratch(device, nbytes)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    _launch("kda_paged_attn_hip", a, device)
     return (o, lse) if return_lse else o
 
 
@@ -246,18 +299,19 @@ def paged_append(
     Tokens at negative positions, or whose page the table does not have, are
     left out.
     """
-    _check_cache(k_cache, v_cache, page_table, seq_lens)
-    for name, t in (("k", k), ("v", v)):
-        _check_new(name, t, k_cache.shape[2], k_cache, page_table, cu_seqlens)
-    if v.shape != k.shape:
-        raise ValueError(f"v.shape {tuple(v.shape)} must match k {tuple(k.shape)}")
+    dt, dev = k_cache.dtype, k_cache.get_device()
+    if not (cu_seqlens is None and _plain_cache(k_cache, v_cache, page_table, seq_lens) and v.shape == k.shape
+            and _plain_new(k, page_table.shape[0], k_cache.shape[2], k_cache.shape[3], dt, dev)
+            and _plain_new(v, page_table.shape[0], k_cache.shape[2], k_cache.shape[3], dt, dev)):
+        _check_cache(k_cache, v_cache, page_table, seq_lens)
+        for name, t in (("k", k), ("v", v)):
+            _check_new(name, t, k_cache.shape[2], k_cache, page_table, cu_seqlens)
+        if v.shape != k.shape:
+            raise ValueError(f"v.shape {tuple(v.shape)} must match k {tuple(k.shape)}")
     _require_gpu(k)
-    a = _cache_args(k_cache, v_cache, page_table, seq_lens, page_table.shape[0], k.shape[1], 0, cu_seqlens)
-    a.new_k, a.new_v = k.data_ptr(), v.data_ptr()
-    a.nk_row, a.nk_token, a.nk_head = _strides(k)
-    a.nv_row, a.nv_token, a.nv_head = _strides(v)
-    with torch.cuda.device(k.device):
-        _hip.call("kda_paged_append_hip", a, _raw_stream(k.device))
+    _launch("kda_paged_append_hip", _cache_args(
+        k_cache, v_cache, page_table, seq_lens, k, 0, cu_seqlens, rest=(
+            None, 0, 0, 0, None, None, k.data_ptr(), v.data_ptr(), *_strides(k), *_strides(v))), k.device)
 
 
 def _pools(pools) -> list[torch.Tensor]:
@@ -282,21 +336,30 @@ def _pools(pools) -> list[torch.Tensor]:
     return ts
 
 
-def _pages_args(P: int, pools=(), page_table=None, seq_lens=None, page_refs=None, page_size: int = 16):
-    a = _hip.KdaPagesArgs()
-    a.abi_version, a.P, a.page_size = _hip.PAGED_ABI_VERSION, P, page_size
-    a.num_pools = len(pools)
-    for i, t in enumerate(pools):
-        page = t.stride(-4) * t.element_size()
-        a.pools[i] = _hip.KdaPagePool(t.data_ptr(), t.numel() * t.element_size() // (P * page), page)
+def _pages_args(P, pools=(), page_table=None, seq_lens=None, page_refs=None, page_size=16, rest=()):
+    """The arguments of a call on the pages, in the order of the fields;
+    ``rest`` from ``F`` on: F, then src, dst, new_tokens, ok, out_table,
+    out_refs, out_live as tensors or None."""
+    N = M = stride = 0
+    table = None
     if page_table is not None:
-        a.N, a.M = page_table.shape
-        a.page_table, a.table_stride = page_table.data_ptr(), max(page_table.stride(0), a.M)
-    if seq_lens is not None:
-        a.seq_lens = seq_lens.data_ptr()
-    if page_refs is not None:
-        a.page_refs = page_refs.data_ptr()
-    return a
+        N, M = page_table.shape
+        table, stride = page_table.data_ptr(), page_table.stride(0) if N > 1 else M
+    arr = _NO_POOLS
+    if pools:
+        arr = (_hip.KdaPagePool * _hip.PAGED_MAX_POOLS)()
+        for i, t in enumerate(pools):
+            size = t.element_size()
+            page = t.stride(-4) * size
+            arr[i] = (t.data_ptr(), t.numel() * size // (P * page), page)
+    F, *tensors = rest
+    return _hip.KdaPagesArgs(
+        _hip.PAGED_ABI_VERSION, N, M, P, page_size, F, len(pools), 0, arr, table, stride,
+        None if seq_lens is None else seq_lens.data_ptr(), None if page_refs is None else page_refs.data_ptr(),
+        *[None if t is None else t.data_ptr() for t in tensors])
+
+
+_NO_POOLS = (_hip.KdaPagePool * _hip.PAGED_MAX_POOLS)()
 
 
 def _check_refs(page_refs, device) -> None:
@@ -307,17 +370,33 @@ def _check_refs(page_refs, device) -> None:
         raise ValueError("page_refs must be 16-byte aligned")
 
 
-def _with_workspace(a, device) -> torch.Tensor:
-    ws = workspace.scratch(device, int(_hip.lib().kda_pages_workspace_bytes(ctypes.byref(a))))
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    return ws
+def _launch_with_workspace(name: str, a, device) -> None:
+    nbytes = _hip.lib().kda_pages_workspace_bytes(ctypes.byref(a))
+    ws = workspace.scratch(device, nbytes)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    _launch(name, a, device)
 
 
 def _check_rows(pairs, device) -> None:
+    dev = device.index
+    if dev is not None:
+        n = pairs[0][1].shape
+        if len(n) == 1 and all(t.shape == n and t.dtype is torch.int32 and t.is_contiguous() and t.get_device() == dev
+                               for _, t in pairs):
+            return
     for name, t in pairs:
         _int32(name, t, 1, device)
         if t.shape[0] != pairs[0][1].shape[0]:
             raise ValueError(f"{name} must have {pairs[0][1].shape[0]} entries like {pairs[0][0]}, got {t.shape[0]}")
+
+
+def _check_counts(page_table, seq_lens, page_refs) -> torch.device:
+    """Table, lengths and counts of one cache; their device."""
+    device = page_table.device
+    if not (page_table.is_cuda and _plain_table(page_table, seq_lens, page_table.get_device())):
+        _check_table(page_table, seq_lens, device)
+    _check_refs(page_refs, device)
+    return device
 
 
 def paged_reserve(
@@ -334,18 +413,14 @@ def paged_reserve(
     Returns a bool ``[N]``: False for a sequence whose pages cannot all be
     had, or do not fit its row; it keeps what it has.
     """
-    device = page_table.device
-    _check_table(page_table, seq_lens, device)
-    _check_refs(page_refs, device)
+    device = _check_counts(page_table, seq_lens, page_refs)
     _check_rows([("seq_lens", seq_lens), ("new_tokens", new_tokens)], device)
     _check_page_size(page_size)
     _require_gpu(page_table)
     ok = torch.empty(seq_lens.shape[0], dtype=torch.bool, device=device)
-    a = _pages_args(page_refs.shape[0], (), page_table, seq_lens, page_refs, page_size)
-    a.new_tokens, a.ok = new_tokens.data_ptr(), ok.data_ptr()
-    with torch.cuda.device(device):
-        ws = _with_workspace(a, device)  # noqa: F841  (held until the launch)
-        _hip.call("kda_pages_reserve_hip", a, _raw_stream(device))
+    a = _pages_args(page_refs.shape[0], (), page_table, seq_lens, page_refs, page_size,
+                    (0, None, None, new_tokens, ok))
+    _launch_with_workspace("kda_pages_reserve_hip", a, device)
     return ok
 
 
@@ -357,15 +432,11 @@ def paged_free(
 ) -> None:
     """The sequences ``rows`` (int32) end: their pages lose a holder each,
     their entries become -1, their lengths 0."""
-    device = page_table.device
-    _check_table(page_table, seq_lens, device)
-    _check_refs(page_refs, device)
+    device = _check_counts(page_table, seq_lens, page_refs)
     _check_rows([("rows", rows)], device)
     _require_gpu(page_table)
-    a = _pages_args(page_refs.shape[0], (), page_table, seq_lens, page_refs)
-    a.F, a.dst = rows.shape[0], rows.data_ptr()
-    with torch.cuda.device(device):
-        _hip.call("kda_pages_free_hip", a, _raw_stream(device))
+    _launch("kda_pages_free_hip", _pages_args(page_refs.shape[0], (), page_table, seq_lens, page_refs, 16,
+                                              (rows.shape[0], None, rows)), device)
 
 
 def paged_fork(
@@ -392,8 +463,8 @@ def paged_fork(
     """
     ts = _pools(pools)
     device = ts[0].device
-    _check_table(page_table, seq_lens, device)
-    _check_refs(page_refs, device)
+    if _check_counts(page_table, seq_lens, page_refs) != device:
+        raise ValueError(f"page_table device {page_table.device} must match ({device})")
     _check_rows([("src", src), ("dst", dst)], device)
     page_size = ts[0].shape[-3] if page_size is None else page_size
     _check_page_size(page_size)
@@ -402,11 +473,8 @@ def paged_fork(
         raise ValueError(f"page_refs must have one entry a page, {P}, got {page_refs.shape[0]}")
     _require_gpu(ts[0])
     ok = torch.empty(src.shape[0], dtype=torch.bool, device=device)
-    a = _pages_args(P, ts, page_table, seq_lens, page_refs, page_size)
-    a.F, a.src, a.dst, a.ok = src.shape[0], src.data_ptr(), dst.data_ptr(), ok.data_ptr()
-    with torch.cuda.device(device):
-        ws = _with_workspace(a, device)  # noqa: F841
-        _hip.call("kda_pages_fork_hip", a, _raw_stream(device))
+    a = _pages_args(P, ts, page_table, seq_lens, page_refs, page_size, (src.shape[0], src, dst, None, ok))
+    _launch_with_workspace("kda_pages_fork_hip", a, device)
     return ok
 
 
@@ -423,10 +491,7 @@ def paged_copy(pools, src: torch.Tensor, dst: torch.Tensor) -> None:
     device = ts[0].device
     _check_rows([("src", src), ("dst", dst)], device)
     _require_gpu(ts[0])
-    a = _pages_args(ts[0].shape[-4], ts)
-    a.F, a.src, a.dst = src.shape[0], src.data_ptr(), dst.data_ptr()
-    with torch.cuda.device(device):
-        _hip.call("kda_pages_copy_hip", a, _raw_stream(device))
+    _launch("kda_pages_copy_hip", _pages_args(ts[0].shape[-4], ts, rest=(src.shape[0], src, dst)), device)
 
 
 def paged_compact(
@@ -458,9 +523,6 @@ def paged_compact(
     table = torch.empty(page_table.shape, dtype=torch.int32, device=device)
     refs = torch.empty_like(page_refs)
     live = torch.empty(1, dtype=torch.int32, device=device)
-    a = _pages_args(P, ts, page_table, None, page_refs)
-    a.out_table, a.out_refs, a.out_live = table.data_ptr(), refs.data_ptr(), live.data_ptr()
-    with torch.cuda.device(device):
-        ws = _with_workspace(a, device)  # noqa: F841
-        _hip.call("kda_pages_compact_hip", a, _raw_stream(device))
+    a = _pages_args(P, ts, page_table, None, page_refs, 16, (0, None, None, None, None, table, refs, live))
+    _launch_with_workspace("kda_pages_compact_hip", a, device)
     return table, refs, live
