@@ -112,16 +112,47 @@ __device__ __forceinline__ u32x2 read_v(const uint8_t* lds, int key, int db, int
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at));
 }
 
-__device__ __forceinline__ float other_half(float x) { return shfl(x, (threadIdx.x & 63) ^ 32); }
+// Maximum and sum of x and the value of lane ^ 32: the swap exchanges the upper
+// half of its first operand with the lower half of its second.  (The elements
+// go through scalars: a bit cast of a vector's element takes the first one.)
+struct Halves {
+    float lower, upper;
+};
+__device__ __forceinline__ Halves halves(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t a = r[0], b = r[1];
+    return {__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
+}
+__device__ __forceinline__ float max_halves(float x) {
+    const Halves h = halves(x);
+    return fmaxf(h.lower, h.upper);
+}
+__device__ __forceinline__ float sum_halves(float x) {
+    const Halves h = halves(x);
+    return h.lower + h.upper;
+}
 
-// Maximum and sum of the softmax over one tile's scores (16 * NB a lane, of
-// keys key0 + 32 * b + 8 * (i / 4) + i % 4), and its weights as operands of the
-// second product: m in the scores' unit, c = scale * log2 e.  Returns the
-// factor by which sums so far shrink.
+// The softmax over one tile's scores (16 * NB a lane, of keys key0 + 32 * b +
+// 8 * (i / 4) + i % 4): its weights as operands of the second product, and the
+// running m (in the scores' unit; c = scale * log2 e) and l.  Returns whether
+// the sums so far have to shrink, by `alpha`.
+// m follows the maximum only when a row's grows by more than a factor of 2^8
+// (any m does as long as nothing overflows: weights stay at most 2^8, and fp32
+// sums and 16-bit weights keep their relative precision), so that the rescaling
+// of O, 64 multiplications a lane against the softmax's ~130 operations, is
+// rare after the first tiles.
+constexpr float GROWTH = 8.f;
+struct Running {
+    float m = -INFINITY;  // -inf: no key seen yet
+    float mc = 0.f;       // m * c, or 0 with m = -inf: what the exponents subtract
+    float l = 0.f;
+    // (the two halves' sums joined) m * c for the join of several parts
+    __device__ __forceinline__ float log2_max() const { return m == -INFINITY ? m : mc; }
+};
 template <class E, int NB>
-__device__ __forceinline__ float softmax_tile(f32x16 (&st)[NB], int key0, int lo, int hi, bool edge, float c, float& m,
-                                              float& l, u32x4 (&pt)[2 * NB]) {
-    float mx = -INFINITY;
+__device__ __forceinline__ bool softmax_tile(f32x16 (&st)[NB], int key0, int lo, int hi, bool edge, float c,
+                                             Running& run, u32x4 (&pt)[2 * NB], float& alpha) {
     if (edge) {
 #pragma unroll
         for (int b = 0; b < NB; ++b)
@@ -131,16 +162,21 @@ __device__ __forceinline__ float softmax_tile(f32x16 (&st)[NB], int key0, int lo
                 if (key < lo || key >= hi) st[b][i] = -INFINITY;
             }
     }
+    float mx = st[0][0];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[b][i]);
-    mx = fmaxf(mx, other_half(mx));
-    // (a row that has seen no key yet keeps m = -inf and subtracts 0)
-    const float m2 = fmaxf(m, mx);
-    const float sub = m2 == -INFINITY ? 0.f : m2 * c;
-    const float alpha = fast_exp2(fmaf(m, c, -sub));
-    m = m2;
+    mx = max_halves(mx);
+    const bool grow = __any((mx - run.m) * c > GROWTH);  // (-inf - -inf is no growth)
+    if (grow) {
+        const float m2 = fmaxf(run.m, mx), mc2 = m2 == -INFINITY ? 0.f : m2 * c;
+        alpha = run.m == -INFINITY ? 0.f : fast_exp2(run.mc - mc2);
+        run.m = m2;
+        run.mc = mc2;
+        run.l *= alpha;
+    }
+    const float sub = run.mc;
     float sum = 0.f;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -150,8 +186,8 @@ __device__ __forceinline__ float softmax_tile(f32x16 (&st)[NB], int key0, int lo
             sum += e0 + e1;
             pt[2 * b + (i >> 3)][(i & 7) >> 1] = E::pack(e0, e1);
         }
-    l = fmaf(l, alpha, sum);
-    return alpha;
+    run.l += sum;
+    return grow;
 }
 
 // ---- the split ----
@@ -334,26 +370,30 @@ __device__ __forceinline__ float log_sum(float mc, float l) {
     return l > 0.f ? (mc + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
 }
 
+// A work-group's LDS: two tiles of 64 keys and their values (few rows: a tile
+// of 32 of each for every wave; at the end every wave's sums), four variables
+// so that the compiler sees which loads a read has to wait for.
+struct Lds {
+    uint8_t *k0, *v0, *k1, *v1;
+    __device__ __forceinline__ float* of_wave(int w) const {
+        return reinterpret_cast<float*>(w == 0 ? k0 : w == 1 ? v0 : w == 2 ? k1 : v1);
+    }
+};
+
 // ---- few rows ----
 
 // Each wave goes over every fourth tile of 32 keys, through LDS of its own:
 // while it multiplies keys the values arrive, and the other way round.  The
 // four waves' sums are joined at the end.
 template <class E, int D>
-__device__ void few_rows(const PagedParams& p, const Unit& u, uint8_t* kt, uint8_t* vt, float* joint) {
+__device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, uint8_t* kw, uint8_t* vw, int wave,
+                                         Running& run, f32x16 (&acc)[D / 32]) {
     constexpr int STEPS = D / 16, DB = D / 32, TK = 32;
     constexpr int TILE = TK * D * 2;
     const int lane = threadIdx.x & 63, half = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Row x = row_of(p, u, u.m * ROWS + (lane & 31));
     const Tiles tl = tiles_of<FEW>(p, u);
-    uint8_t* kw = kt + wave * TILE;
-    uint8_t* vw = vt + wave * TILE;
     const float c = p.scale * LOG2E;
-    float m = -INFINITY, l = 0.f;
-    f32x16 acc[DB];
-#pragma unroll
-    for (int i = 0; i < DB; ++i) acc[i] = f32x16{};
 
     int t = tl.begin + wave;
     int pages[2], next[2];
@@ -386,10 +426,13 @@ __device__ void few_rows(const PagedParams& p, const Unit& u, uint8_t* kt, uint8
         reads_done();
         if (t + WAVES < tl.end) load_k(t + WAVES, next);
         u32x4 pt[2];
-        const float alpha = softmax_tile<E, 1>(st, t * TK + 4 * half, x.lo, x.hi, true, c, m, l, pt);
+        float alpha;
+        if (softmax_tile<E, 1>(st, t * TK + 4 * half, x.lo, x.hi, true, c, run, pt, alpha)) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d) acc[d] *= alpha;
+        }
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-            acc[d] *= alpha;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const u32x2 v0 = read_v<D>(vw, 16 * k + 4 * half, d, lane);
@@ -403,18 +446,31 @@ __device__ void few_rows(const PagedParams& p, const Unit& u, uint8_t* kt, uint8
         for (int g = 0; g < 2; ++g) pages[g] = next[g];
         look_up(t + 2 * WAVES, next);
     }
-    l += other_half(l);
+    run.l = sum_halves(run.l);
+}
+
+template <class E, int D>
+__device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, const Lds& lds, float* joint) {
+    constexpr int DB = D / 32, TILE = 32 * D * 2;
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Running run;
+    f32x16 acc[DB];
+#pragma unroll
+    for (int i = 0; i < DB; ++i) acc[i] = f32x16{};
+    if (wave < 2) few_loop<E, D>(p, u, lds.k0 + wave * TILE, lds.v0 + wave * TILE, wave, run, acc);
+    else few_loop<E, D>(p, u, lds.k1 + (wave - 2) * TILE, lds.v1 + (wave - 2) * TILE, wave, run, acc);
 
     // Join: every wave's m and l, then its O over the tiles' LDS, row by row
     // in pieces of four (the rows' pieces turned by the row, so that the lanes
     // of a half, one row each, write different banks).
     const int row = lane & 31;
     if (half == 0) {
-        joint[wave * 2 * ROWS + row] = m * c;
-        joint[wave * 2 * ROWS + ROWS + row] = l;
+        joint[wave * 2 * ROWS + row] = run.log2_max();
+        joint[wave * 2 * ROWS + ROWS + row] = run.l;
     }
     __syncthreads();
-    float* own = reinterpret_cast<float*>(wave < 2 ? kt : vt) + (wave & 1) * (ROWS * D);
+    float* own = lds.of_wave(wave);
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -439,7 +495,7 @@ __device__ void few_rows(const PagedParams& p, const Unit& u, uint8_t* kt, uint8
         for (int w = 0; w < WAVES; ++w) {
             const float f = fast_exp2(joint[w * 2 * ROWS + r] - sub);
             sum = fmaf(f, joint[w * 2 * ROWS + ROWS + r], sum);
-            const float* src = reinterpret_cast<const float*>(w < 2 ? kt : vt) + (w & 1) * (ROWS * D);
+            const float* src = lds.of_wave(w);
             const f32x4 v = *reinterpret_cast<const f32x4*>(src + r * D + ((piece + r) & (D / 4 - 1)) * 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = fmaf(f, v[i], o[i]);
@@ -461,34 +517,44 @@ __device__ void few_rows(const PagedParams& p, const Unit& u, uint8_t* kt, uint8
 
 // ---- many rows ----
 
+// Two tiles of 64 keys in turn: while one is worked on the other arrives.  A
+// wave loads 16 keys of each.
 template <class E, int D>
-__device__ void many_rows(const PagedParams& p, const Unit& u, uint8_t* kt, uint8_t* vt) {
+__device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, const Lds& lds) {
     constexpr int STEPS = D / 16, DB = D / 32, TK = Shape<MANY>::TK, MT = Shape<MANY>::MT;
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = wave * ROWS + (lane & 31);
     const Row x = row_of(p, u, u.m * MT + row);
     const Tiles tl = tiles_of<MANY>(p, u);
-    u32x4 q[STEPS];
-    load_q<D>(p, u, x, half, q);
+    // the keys that every row of this wave sees, and those that any does
+    const int all_lo = __builtin_amdgcn_readlane(x.lo, 31), all_hi = __builtin_amdgcn_readlane(x.hi, 0);
+    const int any_lo = __builtin_amdgcn_readlane(x.lo, 0), any_hi = __builtin_amdgcn_readlane(x.hi, 31);
     const float c = p.scale * LOG2E;
-    float m = -INFINITY, l = 0.f;
+    Running run;
     f32x16 acc[DB];
 #pragma unroll
     for (int i = 0; i < DB; ++i) acc[i] = f32x16{};
 
-    for (int t = tl.begin; t < tl.end; ++t) {
-        const int t0 = t * TK;
-        __syncthreads();
-        {
-            // 16 keys a wave
-            const int key = t0 + 16 * wave, page = page_at(p, u, key);
-            load_keys<D>(p, p.k, p.k_page, p.k_token, u.h * p.k_head, page, key, u.s.len, lane, kt + wave * (16 * D * 2));
-            load_keys<D>(p, p.v, p.v_page, p.v_token, u.h * p.v_head, page, key, u.s.len, lane, vt + wave * (16 * D * 2));
-        }
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
+    auto load = [&](int t, int page, uint8_t* kt, uint8_t* vt) {
+        const int key = t * TK + 16 * wave;
+        load_keys<D>(p, p.k, p.k_page, p.k_token, u.h * p.k_head, page, key, u.s.len, lane, kt + wave * (16 * D * 2));
+        load_keys<D>(p, p.v, p.v_page, p.v_token, u.h * p.v_head, page, key, u.s.len, lane, vt + wave * (16 * D * 2));
+    };
+    auto look_up = [&](int t) { return t < tl.end ? page_at(p, u, t * TK + 16 * wave) : -1; };
+    u32x4 q[STEPS];
+    int page = look_up(tl.begin);
+    if (tl.begin < tl.end) load(tl.begin, page, lds.k0, lds.v0);
+    page = look_up(tl.begin + 1);
+    load_q<D>(p, u, x, half, q);
 
+    // Tile t, in (kt, vt); the next goes to (kn, vn).
+    auto step = [&](int t, const uint8_t* kt, const uint8_t* vt, uint8_t* kn, uint8_t* vn) {
+        __syncthreads();  // (with the wave's loads complete)
+        if (t + 1 < tl.end) load(t + 1, page, kn, vn);
+        page = look_up(t + 2);
+        const int t0 = t * TK;
+        if (t0 >= any_hi || t0 + TK <= any_lo) return;
         f32x16 st[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -498,10 +564,13 @@ __device__ void many_rows(const PagedParams& p, const Unit& u, uint8_t* kt, uint
                 st[b] = E::mfma(read_k<D>(kt, 32 * b + (lane & 31), 2 * s + half), q[s], st[b]);
         }
         u32x4 pt[4];
-        const float alpha = softmax_tile<E, 2>(st, t0 + 4 * half, x.lo, x.hi, true, c, m, l, pt);
+        float alpha;
+        if (softmax_tile<E, 2>(st, t0 + 4 * half, x.lo, x.hi, t0 < all_lo || t0 + TK > all_hi, c, run, pt, alpha)) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d) acc[d] *= alpha;
+        }
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-            acc[d] *= alpha;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const u32x2 v0 = read_v<D>(vt, 16 * k + 4 * half, d, lane);
@@ -509,14 +578,18 @@ __device__ void many_rows(const PagedParams& p, const Unit& u, uint8_t* kt, uint
                 acc[d] = E::mfma(u32x4{v0.x, v0.y, v1.x, v1.y}, pt[k], acc[d]);
             }
         }
+    };
+    for (int t = tl.begin; t < tl.end; t += 2) {
+        step(t, lds.k0, lds.v0, lds.k1, lds.v1);
+        if (t + 1 < tl.end) step(t + 1, lds.k1, lds.v1, lds.k0, lds.v0);
     }
 
-    l += other_half(l);
+    const float l = sum_halves(run.l);
     if (!x.live) return;
     if (u.parts > 1) {
         float* part = Partial<MANY, D>::at(p.ws + few_floats<D>(), u.slot);
         if (half == 0) {
-            part[row] = m * c;
+            part[row] = run.log2_max();
             part[MT + row] = l;
         }
 #pragma unroll
@@ -535,7 +608,7 @@ __device__ void many_rows(const PagedParams& p, const Unit& u, uint8_t* kt, uint
         for (int i = 0; i < 16; i += 4)
             store_o<E, D>(p, out, 32 * d + 2 * i + 4 * half, acc[d][i] * inv, acc[d][i + 1] * inv, acc[d][i + 2] * inv,
                           acc[d][i + 3] * inv);
-    if (p.lse && half == 0) p.lse[out] = log_sum(m * c, l);
+    if (p.lse && half == 0) p.lse[out] = log_sum(run.mc, l);
 }
 
 // ---- kernels ----
@@ -544,16 +617,18 @@ __device__ void many_rows(const PagedParams& p, const Unit& u, uint8_t* kt, uint
 // others the rest.
 template <class E, int D, int KIND>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedParams p, int few) {
-    constexpr int BYTES = (KIND == MANY ? 64 : 128) * D * 2;
-    __shared__ alignas(1024) uint8_t kt[BYTES];
-    __shared__ alignas(1024) uint8_t vt[BYTES];
+    __shared__ alignas(1024) uint8_t k0[64 * D * 2];
+    __shared__ alignas(1024) uint8_t v0[64 * D * 2];
+    __shared__ alignas(1024) uint8_t k1[64 * D * 2];
+    __shared__ alignas(1024) uint8_t v1[64 * D * 2];
+    const Lds lds = {k0, v0, k1, v1};
     __shared__ float joint[KIND == MANY ? 1 : WAVES * 2 * ROWS];
     const int lane = threadIdx.x & 63;
     Unit u;
     if (KIND == FEW || (KIND == MIXED && (int)blockIdx.x < few)) {
-        if (find_unit<FEW, false>(p, blockIdx.x, lane, u)) few_rows<E, D>(p, u, kt, vt, joint);
+        if (find_unit<FEW, false>(p, blockIdx.x, lane, u)) few_rows<E, D>(p, u, lds, joint);
     } else {
-        if (find_unit<MANY, false>(p, blockIdx.x - few, lane, u)) many_rows<E, D>(p, u, kt, vt);
+        if (find_unit<MANY, false>(p, blockIdx.x - few, lane, u)) many_rows<E, D>(p, u, lds);
     }
 }
 
