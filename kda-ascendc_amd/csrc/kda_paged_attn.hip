@@ -19,6 +19,8 @@
 #include "kda_common.h"
 #include "kda_paged.h"
 
+#include <algorithm>
+
 namespace kda {
 namespace {
 
@@ -64,6 +66,8 @@ struct Shape {
     static constexpr int TK = KIND == FEW ? 32 : 64;              // keys a tile
     // Tiles a work-group takes at least, where keys are split among several.
     static constexpr int LEAST = KIND == FEW ? 8 : 4;
+    // Places for partial results in the workspace.
+    static constexpr int PLACES = KIND == FEW ? 2 * 512 : 512;
 };
 // Work-groups the keys are split for: two on each of 256 CUs.
 constexpr int SLOTS = 512;
@@ -190,19 +194,116 @@ __device__ __forceinline__ bool softmax_tile(f32x16 (&st)[NB], int key0, int lo,
     return grow;
 }
 
-// ---- the split ----
+// ---- the work and its split ----
 
-// What a sequence is to a launch of one kind: row tiles (0: not of this kind)
-// and the tiles of keys that a row tile sees at most.
-struct SeqWork {
-    int mt, tiles;
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t x, int lane) {  // inclusive
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+
+// Row tile m of (sequence n, kv head h), and which of its tiles of keys
+// [begin, end); `slot`: its place in the workspace, or -1 where these are all.
+struct Unit {
+    int n, h, m, begin, end, slot;
+    NewTokens s;
+};
+
+// The tiles of keys that rows [m * MT, m * MT + MT) of a sequence see.
+struct Tiles {
+    int begin, end;
 };
 template <int KIND>
-__device__ __forceinline__ SeqWork seq_work(const PagedParams& p, const NewTokens& s) {
+__device__ __forceinline__ Tiles tiles_of(const PagedParams& p, const NewTokens& s, int m) {
     constexpr int MT = Shape<KIND>::MT, TK = Shape<KIND>::TK;
     const int rows = s.count * p.G;
-    SeqWork w = {(rows + MT - 1) / MT, (s.len + TK - 1) / TK};
-    if (p.cu_seqlens && (rows <= ROWS) != (KIND == FEW)) w.mt = 0;
+    const int first = m * MT / p.G, last = (min(rows, m * MT + MT) - 1) / p.G;
+    const int hi = p.causal ? max(0, min(s.pos + last + 1, s.len)) : s.len;
+    const int lo = p.window ? min(hi, max(0, s.pos + first + 1 - p.window)) : 0;
+    return {lo / TK, max(lo / TK, (hi + TK - 1) / TK)};
+}
+
+// Whether a sequence is of the kind: packed ones are told apart by their rows.
+template <int KIND>
+__device__ __forceinline__ bool of_kind(const PagedParams& p, const NewTokens& s) {
+    return s.count > 0 && (!p.cu_seqlens || (s.count * p.G <= ROWS) == (KIND == FEW));
+}
+
+// Few rows.  The tiles of all sequences and heads, one after the other (at
+// least one a row tile, so that rows that see nothing are written too), are
+// cut into pieces of `size`, one a work-group: the end of one row tile, whole
+// ones, the start of another.  The two that a piece may not have whole go to
+// places 2 b (its first) and 2 b + 1 of the workspace.  With many row tiles the
+// pieces are the SLOTS that run at once, equal whatever the lengths (pieces of
+// one row tile each left half of a second round empty).  With few each row
+// tile is filled up to whole pieces, so that none has two, one after the other:
+// SLOTS pieces hold what the tiles and the fillings come to.
+// All work-groups come to the same cut, from the lengths on the device; every
+// lane counts one sequence.
+constexpr uint32_t FEW_UNITS = SLOTS / 4;
+struct Cut {
+    uint32_t tiles, size;
+    bool filled;
+    int first;  // few_tiles of sequence `lane`
+    // Tiles of a row tile of c with its filling.
+    __device__ __forceinline__ uint32_t span(uint32_t c) const { return filled ? (c + size - 1) / size * size : c; }
+};
+__device__ __forceinline__ int few_tiles(const PagedParams& p, int n) {
+    if (n >= p.N) return 0;
+    const NewTokens s = new_tokens(p, n);
+    if (!of_kind<FEW>(p, s)) return 0;
+    const Tiles t = tiles_of<FEW>(p, s, 0);
+    return max(1, t.end - t.begin);
+}
+__device__ __forceinline__ Cut few_cut(const PagedParams& p, int lane) {
+    Cut c;
+    uint32_t all = 0, units = 0;
+    for (int n0 = 0; n0 < p.N; n0 += 64) {
+        const int x = few_tiles(p, n0 + lane);
+        if (n0 == 0) c.first = x;
+        all += (uint32_t)__builtin_amdgcn_readlane(wave_prefix(x, lane), 63);
+        units += __popcll(__ballot(x > 0));
+    }
+    c.tiles = all * p.HKV;
+    units *= p.HKV;
+    c.filled = units <= FEW_UNITS;
+    const uint32_t pieces = c.filled ? SLOTS - units : SLOTS;
+    c.size = __builtin_amdgcn_readfirstlane(max((uint32_t)Shape<FEW>::LEAST, (c.tiles + pieces - 1) / pieces));
+    return c;
+}
+// Sequence by sequence, the first tile (of all, with fillings) of each lane's
+// sequence n0 + lane, and the tiles of one of its heads.
+struct FewSpans {
+    int tiles;
+    uint32_t span, upto;  // with its filling; the heads' sum up to its end
+};
+__device__ __forceinline__ FewSpans few_spans(const PagedParams& p, const Cut& cut, int n0, int lane) {
+    FewSpans x;
+    x.tiles = n0 == 0 ? cut.first : few_tiles(p, n0 + lane);
+    x.span = cut.span(x.tiles);
+    x.upto = wave_prefix(x.span * p.HKV, lane);
+    return x;
+}
+
+// Many rows.  Row tiles are taken whole where they are enough to fill the
+// card, else their keys are cut into parts: S = ceil(all tiles / SLOTS), at
+// least LEAST, and t / S parts (rounded down: all parts then run at once).
+// Sequence by sequence, a sequence's row tiles last first (those of a causal
+// chunk see the most keys), then its parts, heads innermost: work-groups go
+// round the XCDs, so that with 8 heads each XCD's L2 has the keys of one.
+// Parts of cut row tiles number at most SLOTS.
+struct ManyWork {
+    int mt, tiles;  // row tiles, and tiles of keys that one sees at most
+};
+__device__ __forceinline__ ManyWork many_work(const PagedParams& p, int n) {
+    constexpr int MT = Shape<MANY>::MT, TK = Shape<MANY>::TK;
+    if (n >= p.N) return {0, 0};
+    const NewTokens s = new_tokens(p, n);
+    if (!of_kind<MANY>(p, s)) return {0, 0};
+    ManyWork w = {(s.count * p.G + MT - 1) / MT, (s.len + TK - 1) / TK};
     if (p.window) {
         // the tokens of a row tile and the window before the first
         const int64_t span = (int64_t)min(s.count, MT / p.G + 2) + p.window;
@@ -210,72 +311,51 @@ __device__ __forceinline__ SeqWork seq_work(const PagedParams& p, const NewToken
     }
     return w;
 }
-
-__device__ __forceinline__ int wave_prefix(int x, int lane) {  // inclusive
+// Work-group (JOIN: row tile, its parts' first place and number) `id`'s part.
+template <bool JOIN>
+__device__ __forceinline__ bool many_unit(const PagedParams& p, int id, bool cut, int lane, Unit& u, int& parts) {
+    int S = 0x7fffffff;
+    if (cut) {
+        int64_t all = 0;
+        for (int n0 = 0; n0 < p.N; n0 += 64) {
+            const ManyWork w = many_work(p, n0 + lane);
+            int64_t x = (int64_t)w.mt * w.tiles;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
-    return x;
-}
-
-// A part of the work: row tile m of (sequence n, kv head h) over part `part` of
-// `parts` of its keys; with several parts, its place in the workspace (that of
-// part 0 is `slot - part * stride`).
-struct Unit {
-    int n, h, m, part, parts, slot;
-    NewTokens s;
-};
-
-// Work-group (COMBINE: row tile) `id` -> its part.  The keys are split so that the parts are
-// about SLOTS: a part has at most S = ceil(all tiles / SLOTS) tiles, at least
-// LEAST.  Sequence by sequence, a sequence's row tiles last first (those of a
-// causal chunk see the most keys), then its parts, heads innermost.  Every
-// lane counts one sequence; all work-groups come to the same split, from the
-// lengths on the device.  Parts of split row tiles number at most 2 * SLOTS:
-// a row tile of t > S tiles has ceil(t / S) < 2 t / S.
-template <int KIND, bool COMBINE>
-__device__ __forceinline__ bool find_unit(const PagedParams& p, int id, int lane, Unit& u) {
-    int64_t all = 0;
-    for (int n0 = 0; n0 < p.N; n0 += 64) {
-        int64_t x = 0;
-        if (n0 + lane < p.N) {
-            const SeqWork w = seq_work<KIND>(p, new_tokens(p, n0 + lane));
-            x = (int64_t)w.mt * w.tiles;
+            for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+            all += x;
         }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-        all += x;
+        const int64_t share = (all * p.HKV + SLOTS - 1) / SLOTS;
+        S = __builtin_amdgcn_readfirstlane((int)min((int64_t)S, max((int64_t)Shape<MANY>::LEAST, share)));
     }
-    const int64_t share = (all * p.HKV + SLOTS - 1) / SLOTS;
-    const int S = __builtin_amdgcn_readfirstlane((int)(share > 0x7fffffff ? 0x7fffffff : max((int64_t)Shape<KIND>::LEAST, share)));
     int slots = 0;
     for (int n0 = 0; n0 < p.N; n0 += 64) {
-        SeqWork w = {0, 0};
-        if (n0 + lane < p.N) w = seq_work<KIND>(p, new_tokens(p, n0 + lane));
-        const int parts = max(1, (w.tiles + S - 1) / S);
-        const int end = wave_prefix(w.mt * p.HKV * (COMBINE ? 1 : parts), lane);
-        const int slot_end = wave_prefix(parts > 1 ? w.mt * p.HKV * parts : 0, lane);
+        const ManyWork w = many_work(p, n0 + lane);
+        const int np = max(1, w.tiles / S);
+        const uint32_t end = wave_prefix(w.mt * p.HKV * (JOIN ? 1 : np), lane);
+        const uint32_t slot_end = wave_prefix(np > 1 ? w.mt * p.HKV * np : 0, lane);
         const int total = __builtin_amdgcn_readlane(end, 63);
         if (id < total) {
-            const int at = __builtin_ctzll(__ballot(end > id));
+            const int at = __builtin_ctzll(__ballot((int)end > id));
             const int before = at > 0 ? __builtin_amdgcn_readlane(end, at - 1) : 0;
             const int slot0 = slots + (at > 0 ? __builtin_amdgcn_readlane(slot_end, at - 1) : 0);
             const int mt = __builtin_amdgcn_readlane(w.mt, at);
-            u.parts = __builtin_amdgcn_readlane(parts, at);
+            parts = __builtin_amdgcn_readlane(np, at);
             u.n = __builtin_amdgcn_readfirstlane(n0 + at);
             int x = id - before;
             u.h = x % p.HKV;
             x /= p.HKV;
-            u.part = 0;
-            if (!COMBINE) {
-                u.part = x % u.parts;
-                x /= u.parts;
+            int part = 0;
+            if (!JOIN) {
+                part = x % parts;
+                x /= parts;
             }
             u.m = mt - 1 - x;
-            u.slot = slot0 + (x * p.HKV + u.h) * u.parts + u.part;
+            u.slot = parts > 1 ? slot0 + (x * p.HKV + u.h) * parts + part : -1;
             u.s = new_tokens(p, u.n);
+            const Tiles t = tiles_of<MANY>(p, u.s, u.m);
+            const int64_t count = t.end - t.begin;
+            u.begin = t.begin + (int)(count * part / parts);
+            u.end = t.begin + (int)(count * (part + 1) / parts);
             return true;
         }
         id -= total;
@@ -293,7 +373,7 @@ struct Partial {
 };
 // Floats of the workspace before the parts of kind MANY.
 template <int D>
-constexpr int64_t few_floats() { return 2 * SLOTS * Partial<FEW, D>::FLOATS; }
+constexpr int64_t few_floats() { return Shape<FEW>::PLACES * Partial<FEW, D>::FLOATS; }
 
 // What a row sees: keys [lo, hi) of its sequence.
 struct Row {
@@ -311,22 +391,6 @@ __device__ __forceinline__ Row row_of(const PagedParams& p, const Unit& u, int r
     x.hi = p.causal ? max(0, min(pos + 1, u.s.len)) : u.s.len;
     x.lo = p.window ? max(0, pos + 1 - p.window) : 0;
     return x;
-}
-
-// The tiles of keys of a part: those that rows r0 .. r1 see, its share.
-struct Tiles {
-    int begin, end;
-};
-template <int KIND>
-__device__ __forceinline__ Tiles tiles_of(const PagedParams& p, const Unit& u) {
-    constexpr int MT = Shape<KIND>::MT, TK = Shape<KIND>::TK;
-    const int rows = u.s.count * p.G;
-    const int first = u.m * MT / p.G, last = (min(rows, u.m * MT + MT) - 1) / p.G;
-    const int hi = p.causal ? max(0, min(u.s.pos + last + 1, u.s.len)) : u.s.len;
-    const int lo = p.window ? min(hi, max(0, u.s.pos + first + 1 - p.window)) : 0;
-    const int t0 = lo / TK, t1 = (hi + TK - 1) / TK;
-    const int64_t count = max(0, t1 - t0);
-    return {t0 + (int)(count * u.part / u.parts), t0 + (int)(count * (u.part + 1) / u.parts)};
 }
 
 __device__ __forceinline__ int64_t out_row(const PagedParams& p, const Unit& u, const Row& x) {
@@ -392,7 +456,7 @@ __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, ui
     constexpr int TILE = TK * D * 2;
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const Row x = row_of(p, u, u.m * ROWS + (lane & 31));
-    const Tiles tl = tiles_of<FEW>(p, u);
+    const Tiles tl = {u.begin, u.end};
     const float c = p.scale * LOG2E;
 
     int t = tl.begin + wave;
@@ -480,7 +544,7 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, co
                 f32x4{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
         }
     __syncthreads();
-    float* part = u.parts > 1 ? Partial<FEW, D>::at(p.ws, u.slot) : nullptr;
+    float* part = u.slot >= 0 ? Partial<FEW, D>::at(p.ws, u.slot) : nullptr;
     for (int e = threadIdx.x; e < ROWS * (D / 4); e += 256) {
         const int r = e / (D / 4), piece = e % (D / 4);
         const Row y = row_of(p, u, u.m * ROWS + r);
@@ -515,6 +579,38 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, co
     }
 }
 
+// Work-group b's piece of the cut, row tile by row tile.
+template <class E, int D>
+__device__ __forceinline__ void few_piece(const PagedParams& p, int b, const Lds& lds, float* joint) {
+    const int lane = threadIdx.x & 63;
+    const Cut cut = few_cut(p, lane);
+    const uint32_t first = b * cut.size, end = first + cut.size;
+    uint32_t cur = first, base = 0;
+    for (int n0 = 0; n0 < p.N && cur < end; n0 += 64) {
+        const FewSpans x = few_spans(p, cut, n0, lane);
+        const uint32_t total = __builtin_amdgcn_readlane(x.upto, 63);
+        while (cur < end && cur < base + total) {
+            const int at = __builtin_ctzll(__ballot(x.upto > cur - base));
+            const uint32_t c = __builtin_amdgcn_readlane(x.tiles, at), span = __builtin_amdgcn_readlane(x.span, at);
+            const uint32_t in = cur - base - (__builtin_amdgcn_readlane(x.upto, at) - span * p.HKV);
+            Unit u;
+            u.n = __builtin_amdgcn_readfirstlane(n0 + at);
+            u.h = in / span;
+            u.m = 0;
+            u.s = new_tokens(p, u.n);
+            const uint32_t t = in - u.h * span, stop = min(span, t + (end - cur));
+            const int t0 = tiles_of<FEW>(p, u.s, 0).begin;
+            u.begin = t0 + t;
+            u.end = t0 + min(c, stop);
+            u.slot = t == 0 && stop >= c ? -1 : 2 * b + (cur == first ? 0 : 1);
+            if (cur != first) __syncthreads();  // the last row tile's join is over
+            few_rows<E, D>(p, u, lds, joint);
+            cur += stop - t;
+        }
+        base += total;
+    }
+}
+
 // ---- many rows ----
 
 // Two tiles of 64 keys in turn: while one is worked on the other arrives.  A
@@ -526,7 +622,7 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, c
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = wave * ROWS + (lane & 31);
     const Row x = row_of(p, u, u.m * MT + row);
-    const Tiles tl = tiles_of<MANY>(p, u);
+    const Tiles tl = {u.begin, u.end};
     // the keys that every row of this wave sees, and those that any does
     const int all_lo = __builtin_amdgcn_readlane(x.lo, 31), all_hi = __builtin_amdgcn_readlane(x.hi, 0);
     const int any_lo = __builtin_amdgcn_readlane(x.lo, 0), any_hi = __builtin_amdgcn_readlane(x.hi, 31);
@@ -550,7 +646,10 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, c
 
     // Tile t, in (kt, vt); the next goes to (kn, vn).
     auto step = [&](int t, const uint8_t* kt, const uint8_t* vt, uint8_t* kn, uint8_t* vn) {
-        __syncthreads();  // (with the wave's loads complete)
+        // This wave's loads into LDS are complete, then every wave's (the barrier
+        // alone does not wait for them).
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0
+        __syncthreads();
         if (t + 1 < tl.end) load(t + 1, page, kn, vn);
         page = look_up(t + 2);
         const int t0 = t * TK;
@@ -586,7 +685,7 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, c
 
     const float l = sum_halves(run.l);
     if (!x.live) return;
-    if (u.parts > 1) {
+    if (u.slot >= 0) {
         float* part = Partial<MANY, D>::at(p.ws + few_floats<D>(), u.slot);
         if (half == 0) {
             part[row] = run.log2_max();
@@ -616,59 +715,123 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, c
 // KIND MIXED: the first `few` work-groups take the sequences of few rows, the
 // others the rest.
 template <class E, int D, int KIND>
-__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedParams p, int few) {
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedParams p, int few, bool cut) {
     __shared__ alignas(1024) uint8_t k0[64 * D * 2];
     __shared__ alignas(1024) uint8_t v0[64 * D * 2];
     __shared__ alignas(1024) uint8_t k1[64 * D * 2];
     __shared__ alignas(1024) uint8_t v1[64 * D * 2];
     const Lds lds = {k0, v0, k1, v1};
     __shared__ float joint[KIND == MANY ? 1 : WAVES * 2 * ROWS];
-    const int lane = threadIdx.x & 63;
-    Unit u;
     if (KIND == FEW || (KIND == MIXED && (int)blockIdx.x < few)) {
-        if (find_unit<FEW, false>(p, blockIdx.x, lane, u)) few_rows<E, D>(p, u, lds, joint);
+        few_piece<E, D>(p, blockIdx.x, lds, joint);
     } else {
-        if (find_unit<MANY, false>(p, blockIdx.x - few, lane, u)) many_rows<E, D>(p, u, lds);
+        Unit u;
+        int parts;
+        if (many_unit<false>(p, (int)blockIdx.x - few, cut, threadIdx.x & 63, u, parts)) many_rows<E, D>(p, u, lds);
     }
 }
 
-// The parts of one row tile joined.
-template <class E, int D, int KIND>
-__device__ void combine(const PagedParams& p, const Unit& u, const float* ws) {
-    constexpr int MT = Shape<KIND>::MT;
-    const float* first = ws + u.slot * Partial<KIND, D>::FLOATS;
-    for (int e = threadIdx.x; e < MT * (D / 4); e += 256) {
-        const int r = e / (D / 4), piece = e % (D / 4);
-        const Row y = row_of(p, u, u.m * MT + r);
-        if (!y.live) break;
-        float mx = -INFINITY;
-        for (int j = 0; j < u.parts; ++j) mx = fmaxf(mx, first[j * Partial<KIND, D>::FLOATS + r]);
+// Joins the partial results of one row tile: four elements of a row a thread,
+// SLICES threads' parts in turn.  place(j): the j-th part's rows.
+constexpr int SLICES = 4;  // few rows: the waves
+template <class E, int D, int KIND, class Place>
+__device__ __forceinline__ void join(const PagedParams& p, const Unit& u, int group, int parts, Place place, float* lds) {
+    constexpr int MT = Shape<KIND>::MT, NS = KIND == FEW ? SLICES : 1;
+    const int slice = KIND == FEW ? threadIdx.x >> 6 : 0;
+    const int e = group * (256 / NS) + threadIdx.x % (256 / NS);
+    const int r = e / (D / 4), piece = e % (D / 4);
+    const Row y = row_of(p, u, u.m * MT + r);
+    float mx = -INFINITY, sum = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (y.live) {
+#pragma unroll 8
+        for (int j = slice; j < parts; j += NS) mx = fmaxf(mx, place(j)[r]);
         const float sub = mx == -INFINITY ? 0.f : mx;
-        float sum = 0.f;
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        for (int j = 0; j < u.parts; ++j) {
-            const float* part = first + j * Partial<KIND, D>::FLOATS;
+#pragma unroll 4
+        for (int j = slice; j < parts; j += NS) {
+            const float* part = place(j);
             const float f = fast_exp2(part[r] - sub);
             sum = fmaf(f, part[MT + r], sum);
             const f32x4 v = *reinterpret_cast<const f32x4*>(part + 2 * MT + r * D + piece * 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = fmaf(f, v[i], o[i]);
         }
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
-        const int64_t out = out_row(p, u, y);
-        store_o<E, D>(p, out, piece * 4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-        if (p.lse && piece == 0) p.lse[out] = log_sum(mx, sum);
     }
+    if constexpr (NS > 1) {
+        // the slices' sums, six numbers a thread
+        const int t = threadIdx.x;
+        lds[t] = mx;
+        lds[256 + t] = sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lds[(2 + i) * 256 + t] = o[i];
+        __syncthreads();
+        if (slice != 0) return;  // (no barrier follows in here)
+        float top = mx;
+#pragma unroll
+        for (int w = 1; w < NS; ++w) top = fmaxf(top, lds[w * 64 + t]);
+        const float sub = top == -INFINITY ? 0.f : top;
+        float f = fast_exp2(mx - sub);
+        sum *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] *= f;
+#pragma unroll
+        for (int w = 1; w < NS; ++w) {
+            f = fast_exp2(lds[w * 64 + t] - sub);
+            sum = fmaf(f, lds[256 + w * 64 + t], sum);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = fmaf(f, lds[(2 + i) * 256 + w * 64 + t], o[i]);
+        }
+        mx = top;
+    }
+    if (!y.live) return;
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const int64_t out = out_row(p, u, y);
+    store_o<E, D>(p, out, piece * 4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (p.lse && piece == 0) p.lse[out] = log_sum(mx, sum);
 }
+
+// A work-group a row tile (few rows: `few_groups` of them).
 template <class E, int D, int KIND>
-__global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p, int few) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int few, int few_groups, bool cut_many) {
+    __shared__ float lds[KIND == MANY ? 1 : 6 * 256];
     const int lane = threadIdx.x & 63;
     Unit u;
     if (KIND == FEW || (KIND == MIXED && (int)blockIdx.x < few)) {
-        if (find_unit<FEW, true>(p, blockIdx.x, lane, u) && u.parts > 1) combine<E, D, FEW>(p, u, p.ws);
+        const int id = blockIdx.x / few_groups;
+        const Cut cut = few_cut(p, lane);
+        u.n = id / p.HKV;
+        u.h = id - u.n * p.HKV;
+        u.m = 0;
+        uint32_t first = 0, c = 0;  // its tiles [first, first + c) of all
+        for (int n0 = 0; n0 <= u.n; n0 += 64) {
+            const FewSpans x = few_spans(p, cut, n0, lane);
+            if (u.n < n0 + 64) {
+                c = __builtin_amdgcn_readlane(x.tiles, u.n - n0);
+                const uint32_t span = __builtin_amdgcn_readlane(x.span, u.n - n0);
+                first += __builtin_amdgcn_readlane(x.upto, u.n - n0) - (p.HKV - u.h) * span;
+            } else {
+                first += __builtin_amdgcn_readlane(x.upto, 63);
+            }
+        }
+        if (c == 0) return;
+        const uint32_t b0 = first / cut.size, b1 = (first + c - 1) / cut.size;
+        if (b0 == b1) return;
+        u.s = new_tokens(p, u.n);
+        const int items = u.s.count * p.G * (D / 4);
+        for (int group = blockIdx.x % few_groups; group * 64 < items; group += few_groups) {
+            join<E, D, FEW>(p, u, group, b1 - b0 + 1, [&](int j) {
+                const uint32_t b = b0 + j;
+                return Partial<FEW, D>::at(p.ws, 2 * b + (b * cut.size >= first ? 0 : 1));
+            }, lds);
+            __syncthreads();
+        }
     } else {
-        if (find_unit<MANY, true>(p, blockIdx.x - few, lane, u) && u.parts > 1)
-            combine<E, D, MANY>(p, u, p.ws + few_floats<D>());
+        int parts;
+        if (!many_unit<true>(p, (int)blockIdx.x - few, cut_many, lane, u, parts) || parts == 1) return;
+        for (int group = 0; group < Shape<MANY>::MT * (D / 4) / 256; ++group)
+            join<E, D, MANY>(p, u, group, parts, [&](int j) {
+                return Partial<MANY, D>::at(p.ws + few_floats<D>(), u.slot + j);
+            }, lds);
     }
 }
 
@@ -681,30 +844,35 @@ int kind_of(const PagedParams& p) {
     return p.cu_seqlens ? MIXED : MANY;
 }
 
-// Row tiles of a kind at most, and whether their keys may be split.
-template <int KIND>
-int64_t most_units(const PagedParams& p) {
-    constexpr int MT = Shape<KIND>::MT;
+// Row tiles of many rows at most (packed sequences each leave one unfilled).
+int64_t many_units(const PagedParams& p) {
+    constexpr int MT = Shape<MANY>::MT;
     const int64_t rows = (int64_t)p.T * p.G;
-    if (!p.cu_seqlens) return (int64_t)p.N * ((rows + MT - 1) / MT) * p.HKV;
-    return (KIND == FEW ? (int64_t)p.N : rows / MT + p.N) * p.HKV;
+    return (p.cu_seqlens ? rows / MT + p.N : p.N * ((rows + MT - 1) / MT)) * p.HKV;
 }
-template <int KIND>
-bool may_split(const PagedParams& p) {
-    return ((int64_t)p.M << p.page_shift) > Shape<KIND>::LEAST * Shape<KIND>::TK;
+
+// Whether a row tile's keys may go to several work-groups.  (Many rows: row
+// tiles that fill half of SLOTS are taken whole.)
+bool may_cut(const PagedParams& p, int kind) {
+    const int64_t keys = (int64_t)p.M << p.page_shift;
+    if (kind == FEW) return keys > Shape<FEW>::TK;
+    return keys >= 2 * Shape<MANY>::LEAST * Shape<MANY>::TK && many_units(p) <= SLOTS / 2;
 }
 
 template <class E, int D, int KIND>
 hipError_t launch(const PagedParams& p, hipStream_t stream) {
-    const int64_t fu = KIND == MANY ? 0 : most_units<FEW>(p), mu = KIND == FEW ? 0 : most_units<MANY>(p);
-    const bool fs = KIND != MANY && may_split<FEW>(p), ms = KIND != FEW && may_split<MANY>(p);
-    // (splitting adds at most SLOTS work-groups: the parts are at most one a
-    // row tile and one for every S tiles)
-    const int64_t fw = fu + (fs ? SLOTS : 0), mw = mu + (ms ? SLOTS : 0);
-    paged_attn_kernel<E, D, KIND><<<dim3((unsigned)(fw + mw)), 256, 0, stream>>>(p, (int)fw);
+    const bool fc = KIND != MANY && may_cut(p, FEW), mc = KIND != FEW && may_cut(p, MANY);
+    const int64_t units = KIND == FEW ? 0 : many_units(p);
+    const int64_t few = KIND == MANY ? 0 : SLOTS, many = units + (mc ? SLOTS : 0);
+    paged_attn_kernel<E, D, KIND><<<dim3((unsigned)(few + many)), 256, 0, stream>>>(p, (int)few, mc);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !(fs || ms)) return e;
-    paged_combine_kernel<E, D, KIND><<<dim3((unsigned)(fu + mu)), 256, 0, stream>>>(p, (int)fu);
+    if (e != hipSuccess || !(fc || mc)) return e;
+    // work-groups a row tile: one for every 64 fours of what rows there can be, up to 4
+    const int64_t rows = p.cu_seqlens || (int64_t)p.T * p.G > ROWS ? ROWS : p.T * p.G;
+    const int groups = (int)std::min((rows * (D / 4) + 63) / 64, (int64_t)4);
+    const int64_t few_joins = fc ? (int64_t)p.N * p.HKV * groups : 0;
+    const int64_t many_joins = mc ? units : 0;
+    paged_join_kernel<E, D, KIND><<<dim3((unsigned)(few_joins + many_joins)), 256, 0, stream>>>(p, (int)few_joins, groups, mc);
     return hipGetLastError();
 }
 
@@ -721,10 +889,11 @@ hipError_t launch_kind(const PagedParams& p, hipStream_t stream) {
 
 size_t paged_attn_workspace(const PagedParams& p, int D) {
     const int kind = kind_of(p);
-    const bool fs = kind != MANY && may_split<FEW>(p), ms = kind != FEW && may_split<MANY>(p);
-    if (!fs && !ms) return 0;
-    const int64_t few = 2 * SLOTS * (int64_t)Shape<FEW>::MT * (D + 2), many = 2 * SLOTS * (int64_t)Shape<MANY>::MT * (D + 2);
-    return (size_t)(few + (ms ? many : 0)) * 4;
+    const bool fc = kind != MANY && may_cut(p, FEW), mc = kind != FEW && may_cut(p, MANY);
+    if (!fc && !mc) return 0;
+    const int64_t few = (int64_t)Shape<FEW>::PLACES * Shape<FEW>::MT * (D + 2);
+    const int64_t many = (int64_t)Shape<MANY>::PLACES * Shape<MANY>::MT * (D + 2);
+    return (size_t)(few + (mc ? many : 0)) * 4;
 }
 
 hipError_t launch_paged_attn(const PagedParams& p, int D, hipStream_t stream) {

@@ -89,7 +89,11 @@ int attn_params(const KdaPagedArgs* a, PagedParams& p) {
     if (a->HQ <= 0 || a->HQ % a->HKV != 0) return KDA_BT16_EINVAL;
     if (a->window < 0 || !(a->scale > 0.0f)) return KDA_BT16_EINVAL;
     if (a->window > 0 && !p.causal) return KDA_BT16_EUNSUPPORTED;
-    // Rows (token, head of a group) and work-groups are counted in 32 bits.
+    // Tiles of 32 keys of all sequences and heads (with up to as many again to
+    // fill pieces), rows (token, head of a group) and work-groups are counted in
+    // 32 bits.
+    const int64_t tiles = ((((int64_t)a->M * a->page_size) >> 5) + 2) * a->HKV;
+    if (tiles > I32_MAX / a->N) return KDA_BT16_EUNSUPPORTED;
     const int64_t tokens = a->cu_seqlens ? a->T : (int64_t)a->N * a->T;
     if ((tokens + (int64_t)a->N * 128) * a->HQ > I32_MAX / 4) return KDA_BT16_EUNSUPPORTED;
     if (!a->q || !a->o) return KDA_BT16_EINVAL;
