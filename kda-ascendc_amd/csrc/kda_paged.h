@@ -24,8 +24,9 @@ struct PagedParams {
     const int32_t* seq_lens;
     uint16_t* k;
     uint16_t* v;
-    int64_t k_page, k_token, k_head;
-    int64_t v_page, v_token, v_head;
+    uint32_t k_page, v_page;    // below 2^31
+    int32_t k_token, v_token;   // a page of one head spans less than 2^30
+    int64_t k_head, v_head;
     const uint16_t* q;
     int64_t q_row, q_token, q_head;
     uint16_t* o;
@@ -66,12 +67,13 @@ __device__ __forceinline__ NewTokens new_tokens(const PagedParams& p, int n) {
     return s;
 }
 
-// The i-th page of sequence n, or -1 where there is none.
-__device__ __forceinline__ int page_of(const PagedParams& p, int n, int i) {
+// Entry i of sequence n's row of the page table: the last one for any i past
+// it.  A page only if is_page().
+__device__ __forceinline__ int table_entry(const PagedParams& p, int n, int i) {
     typedef __attribute__((address_space(4))) const int32_t c_i32;
-    const int x = ((c_i32*)(p.page_table + (int64_t)n * p.table_stride))[i];
-    return (unsigned)x < (unsigned)p.P ? x : -1;
+    return ((c_i32*)(p.page_table + (int64_t)n * p.table_stride))[i < p.M ? i : p.M - 1];
 }
+__device__ __forceinline__ bool is_page(const PagedParams& p, int x) { return (unsigned)x < (unsigned)p.P; }
 
 // Pools and counts of a call on the pages (kda_paged_hip.h).
 struct PagesParams {

@@ -53,7 +53,6 @@ struct FP16 {
     }
 };
 
-constexpr int WAVES = 4;
 constexpr int ROWS = 32;  // rows of a wave's products
 
 // Two ways over the keys.  Few rows (a decode step, a draft): every wave of a
@@ -62,15 +61,17 @@ constexpr int ROWS = 32;  // rows of a wave's products
 constexpr int FEW = 0, MANY = 1, MIXED = 2;
 template <int KIND>
 struct Shape {
+    static constexpr int WAVES = KIND == FEW ? 4 : 8;
     static constexpr int MT = KIND == FEW ? ROWS : WAVES * ROWS;  // rows a work-group
     static constexpr int TK = KIND == FEW ? 32 : 64;              // keys a tile
     // Tiles a work-group takes at least, where keys are split among several.
-    static constexpr int LEAST = KIND == FEW ? 8 : 4;
+    static constexpr int LEAST = KIND == FEW ? 4 : 4;
+    // Work-groups that run at once (LDS and registers: two of few rows on each
+    // of 256 CUs, one of many): the parts that keys are split into.
+    static constexpr int SLOTS = KIND == FEW ? 512 : 256;
     // Places for partial results in the workspace.
-    static constexpr int PLACES = KIND == FEW ? 2 * 512 : 512;
+    static constexpr int PLACES = KIND == FEW ? 2 * SLOTS : SLOTS;
 };
-// Work-groups the keys are split for: two on each of 256 CUs.
-constexpr int SLOTS = 512;
 
 // A tile of keys (or values) in LDS: rows of D elements, in each the 16-byte
 // piece c at place c ^ swizzle(row).  The swizzle keeps two reads free of bank
@@ -82,21 +83,51 @@ __device__ __forceinline__ int swizzle(int row) {
     return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
 }
 
-// 16 rows of a page into LDS (`rows` of them exist, the others become zeros:
-// the descriptor ends with the last one).  Each load takes 1 KiB, lane l's 16
-// bytes going to byte 16 * l of it.
-template <int D>
-__device__ __forceinline__ void load_rows(const uint16_t* head, int64_t token, int rows, int lane, uint8_t* lds) {
-    constexpr int PIECES = D / 8, R = 64 / PIECES;
-    const int bytes = rows > 0 ? (int)((rows - 1) * token + D) * 2 : 0;
-    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)head, 0, bytes, BUF_RAW);
-#pragma unroll
-    for (int j = 0; j < 16 / R; ++j) {
-        const int row = j * R + lane / PIECES;
-        const int off = (int)(row * token) * 2 + (((lane & (PIECES - 1)) ^ swizzle<D>(row)) << 4);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_u8*)(lds + j * 1024), 16, off, 0, 0, 0);
-    }
+// 16 bytes a lane from a buffer straight into LDS, lane l's to `lds` + 16 * l
+// (a byte address, wave-uniform).  Written as an instruction: the compiler
+// cannot tell the tiles of a ring apart and would wait, before any LDS read,
+// for every such load under way.  So nothing but wait_loads() waits for it;
+// it has no result in registers, and other loads' waits only become longer.
+__device__ __forceinline__ void load_lds(u32x4 rsrc, int off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(lds)
+                 : "memory");
 }
+// All but the last `n` of this wave's loads have arrived.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const uint8_t* p) {
+    return (uint32_t)reinterpret_cast<uintptr_t>((lds_u8*)p);
+}
+
+// What a wave loads of a tile: NROWS keys (or values) of one head, all of one
+// page, 1 KiB a load.
+template <int D, int NROWS>
+struct Loader {
+    static constexpr int PIECES = D / 8, R = 64 / PIECES, LOADS = NROWS / R;
+    uint64_t head;            // byte address of the head in page 0
+    uint32_t page_bytes, token_bytes;
+    int off[LOADS];           // this lane's bytes of each load, within the rows
+    // row0: the first row's place in its 16.
+    __device__ __forceinline__ Loader(const uint16_t* cache, uint32_t page_stride, int token, int64_t h, int row0, int lane)
+        : head(reinterpret_cast<uint64_t>(cache + h)), page_bytes(page_stride), token_bytes(token * 2) {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int row = j * R + lane / PIECES;
+            off[j] = row * (int)token_bytes + (((lane & (PIECES - 1)) ^ swizzle<D>(row0 + row)) << 4);
+        }
+    }
+    // Rows `in` on of a page (an entry of the table) to LDS: `rows` of them
+    // exist, the others become zeros (the descriptor ends with the last one).
+    __device__ __forceinline__ void load(const PagedParams& p, int page, int in, int rows, uint32_t lds) const {
+        const int n = is_page(p, page) ? min(rows, NROWS) : 0;
+        const uint64_t at = head + ((uint64_t)(n > 0 ? (uint32_t)page : 0u) * page_bytes << 1) + (uint32_t)in * token_bytes;
+        const u32x4 rsrc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, n > 0 ? (n - 1) * token_bytes + D * 2 : 0u, BUF_RAW};
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) load_lds(rsrc, off[j], lds + j * 1024);
+    }
+};
 
 // Operand of the first product: rows lane & 31, elements 16 * s + 8 * (lane >> 5) .. +7.
 template <int D>
@@ -243,7 +274,7 @@ __device__ __forceinline__ bool of_kind(const PagedParams& p, const NewTokens& s
 // SLOTS pieces hold what the tiles and the fillings come to.
 // All work-groups come to the same cut, from the lengths on the device; every
 // lane counts one sequence.
-constexpr uint32_t FEW_UNITS = SLOTS / 4;
+constexpr uint32_t FEW_UNITS = Shape<FEW>::SLOTS / 4;
 struct Cut {
     uint32_t tiles, size;
     bool filled;
@@ -270,7 +301,7 @@ __device__ __forceinline__ Cut few_cut(const PagedParams& p, int lane) {
     c.tiles = all * p.HKV;
     units *= p.HKV;
     c.filled = units <= FEW_UNITS;
-    const uint32_t pieces = c.filled ? SLOTS - units : SLOTS;
+    const uint32_t pieces = c.filled ? Shape<FEW>::SLOTS - units : Shape<FEW>::SLOTS;
     c.size = __builtin_amdgcn_readfirstlane(max((uint32_t)Shape<FEW>::LEAST, (c.tiles + pieces - 1) / pieces));
     return c;
 }
@@ -324,7 +355,7 @@ __device__ __forceinline__ bool many_unit(const PagedParams& p, int id, bool cut
             for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
             all += x;
         }
-        const int64_t share = (all * p.HKV + SLOTS - 1) / SLOTS;
+        const int64_t share = (all * p.HKV + Shape<MANY>::SLOTS - 1) / Shape<MANY>::SLOTS;
         S = __builtin_amdgcn_readfirstlane((int)min((int64_t)S, max((int64_t)Shape<MANY>::LEAST, share)));
     }
     int slots = 0;
@@ -404,20 +435,6 @@ __device__ __forceinline__ void load_q(const PagedParams& p, const Unit& u, cons
     for (int s = 0; s < D / 16; ++s) q[s] = *reinterpret_cast<const u32x4*>(at + 16 * s + 8 * half);
 }
 
-// 16 keys from `key` on (a multiple of 16) into LDS: they share a page.
-template <int D>
-__device__ __forceinline__ void load_keys(const PagedParams& p, const uint16_t* cache, int64_t page_stride, int64_t token,
-                                          int64_t head, int page, int key, int len, int lane, uint8_t* lds) {
-    const int rows = page < 0 ? 0 : min(len - key, 16);
-    const int64_t pg = page < 0 ? 0 : page;
-    const int in = key & ((1 << p.page_shift) - 1);
-    load_rows<D>(cache + pg * page_stride + in * token + head, token, rows, lane, lds);
-}
-
-__device__ __forceinline__ int page_at(const PagedParams& p, const Unit& u, int key) {
-    return key < u.s.len ? page_of(p, u.n, key >> p.page_shift) : -1;
-}
-
 // This wave's LDS reads have returned: what they read may be loaded over.
 __device__ __forceinline__ void reads_done() {
     __builtin_amdgcn_sched_barrier(0);
@@ -434,25 +451,16 @@ __device__ __forceinline__ float log_sum(float mc, float l) {
     return l > 0.f ? (mc + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
 }
 
-// A work-group's LDS: two tiles of 64 keys and their values (few rows: a tile
-// of 32 of each for every wave; at the end every wave's sums), four variables
-// so that the compiler sees which loads a read has to wait for.
-struct Lds {
-    uint8_t *k0, *v0, *k1, *v1;
-    __device__ __forceinline__ float* of_wave(int w) const {
-        return reinterpret_cast<float*>(w == 0 ? k0 : w == 1 ? v0 : w == 2 ? k1 : v1);
-    }
-};
-
 // ---- few rows ----
 
 // Each wave goes over every fourth tile of 32 keys, through LDS of its own:
 // while it multiplies keys the values arrive, and the other way round.  The
-// four waves' sums are joined at the end.
+// four waves' sums are joined at the end, in the same LDS (2 * TILE bytes a
+// wave: a tile of keys, one of values; 32 rows of D floats).
 template <class E, int D>
 __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, uint8_t* kw, uint8_t* vw, int wave,
                                          Running& run, f32x16 (&acc)[D / 32]) {
-    constexpr int STEPS = D / 16, DB = D / 32, TK = 32;
+    constexpr int STEPS = D / 16, DB = D / 32, TK = Shape<FEW>::TK, WAVES = Shape<FEW>::WAVES;
     constexpr int TILE = TK * D * 2;
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const Row x = row_of(p, u, u.m * ROWS + (lane & 31));
@@ -460,70 +468,73 @@ __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, ui
     const float c = p.scale * LOG2E;
 
     int t = tl.begin + wave;
-    int pages[2], next[2];
+    const Loader<D, 16> k0(p.k, p.k_page, p.k_token, u.h * p.k_head, 0, lane);
+    const Loader<D, 16> v0(p.v, p.v_page, p.v_token, u.h * p.v_head, 0, lane);
+    const int in_page = (1 << p.page_shift) - 1;
+    int pages[2], next[2];  // of the tile's first and second 16 keys
     auto look_up = [&](int tile, int (&pg)[2]) {
 #pragma unroll
-        for (int g = 0; g < 2; ++g) pg[g] = tile < tl.end ? page_at(p, u, tile * TK + 16 * g) : -1;
+        for (int g = 0; g < 2; ++g) pg[g] = table_entry(p, u.n, (tile * TK + 16 * g) >> p.page_shift);
     };
-    auto load_k = [&](int tile, const int (&pg)[2]) {
+    auto load = [&](const Loader<D, 16>& from, int tile, const int (&pg)[2], uint8_t* to) {
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
-            load_keys<D>(p, p.k, p.k_page, p.k_token, u.h * p.k_head, pg[g], tile * TK + 16 * g, u.s.len, lane, kw + g * (TILE / 2));
-    };
-    auto load_v = [&](int tile, const int (&pg)[2]) {
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-            load_keys<D>(p, p.v, p.v_page, p.v_token, u.h * p.v_head, pg[g], tile * TK + 16 * g, u.s.len, lane, vw + g * (TILE / 2));
+        for (int g = 0; g < 2; ++g) {
+            const int key = tile * TK + 16 * g;
+            from.load(p, pg[g], key & in_page, u.s.len - key, lds_address(to) + g * (TILE / 2));
+        }
     };
     look_up(t, pages);
     if (t < tl.end) {
-        load_k(t, pages);
-        load_v(t, pages);
+        load(k0, t, pages, kw);
+        load(v0, t, pages, vw);
     }
     look_up(t + WAVES, next);
     u32x4 q[STEPS];
     load_q<D>(p, u, x, half, q);
+    // (once here, where the compiler sees it: else it waits for q in every turn)
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0
+    constexpr int LOADS = TILE / 1024;  // of a tile of keys, or of values
     for (; t < tl.end; t += WAVES) {
         f32x16 st[1] = {f32x16{}};
+        wait_loads<LOADS>();  // but for the values'
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) st[0] = E::mfma(read_k<D>(kw, lane & 31, 2 * s + half), q[s], st[0]);
         reads_done();
-        if (t + WAVES < tl.end) load_k(t + WAVES, next);
+        if (t + WAVES < tl.end) load(k0, t + WAVES, next, kw);
         u32x4 pt[2];
         float alpha;
         if (softmax_tile<E, 1>(st, t * TK + 4 * half, x.lo, x.hi, true, c, run, pt, alpha)) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) acc[d] *= alpha;
         }
+        if (t + WAVES < tl.end) wait_loads<LOADS>();  // but for the next keys'
+        else wait_loads<0>();
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const u32x2 v0 = read_v<D>(vw, 16 * k + 4 * half, d, lane);
-                const u32x2 v1 = read_v<D>(vw, 16 * k + 8 + 4 * half, d, lane);
-                acc[d] = E::mfma(u32x4{v0.x, v0.y, v1.x, v1.y}, pt[k], acc[d]);
+                const u32x2 a = read_v<D>(vw, 16 * k + 4 * half, d, lane);
+                const u32x2 b = read_v<D>(vw, 16 * k + 8 + 4 * half, d, lane);
+                acc[d] = E::mfma(u32x4{a.x, a.y, b.x, b.y}, pt[k], acc[d]);
             }
         }
         reads_done();
-        if (t + WAVES < tl.end) load_v(t + WAVES, next);
-#pragma unroll
-        for (int g = 0; g < 2; ++g) pages[g] = next[g];
+        if (t + WAVES < tl.end) load(v0, t + WAVES, next, vw);
         look_up(t + 2 * WAVES, next);
     }
     run.l = sum_halves(run.l);
 }
 
 template <class E, int D>
-__device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, const Lds& lds, float* joint) {
-    constexpr int DB = D / 32, TILE = 32 * D * 2;
+__device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, uint8_t* lds, float* joint) {
+    constexpr int DB = D / 32, TILE = Shape<FEW>::TK * D * 2, WAVES = Shape<FEW>::WAVES;
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Running run;
     f32x16 acc[DB];
 #pragma unroll
     for (int i = 0; i < DB; ++i) acc[i] = f32x16{};
-    if (wave < 2) few_loop<E, D>(p, u, lds.k0 + wave * TILE, lds.v0 + wave * TILE, wave, run, acc);
-    else few_loop<E, D>(p, u, lds.k1 + (wave - 2) * TILE, lds.v1 + (wave - 2) * TILE, wave, run, acc);
+    few_loop<E, D>(p, u, lds + wave * (2 * TILE), lds + wave * (2 * TILE) + TILE, wave, run, acc);
 
     // Join: every wave's m and l, then its O over the tiles' LDS, row by row
     // in pieces of four (the rows' pieces turned by the row, so that the lanes
@@ -534,7 +545,7 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, co
         joint[wave * 2 * ROWS + ROWS + row] = run.l;
     }
     __syncthreads();
-    float* own = lds.of_wave(wave);
+    float* own = reinterpret_cast<float*>(lds + wave * (2 * TILE));
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -559,7 +570,7 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, co
         for (int w = 0; w < WAVES; ++w) {
             const float f = fast_exp2(joint[w * 2 * ROWS + r] - sub);
             sum = fmaf(f, joint[w * 2 * ROWS + ROWS + r], sum);
-            const float* src = lds.of_wave(w);
+            const float* src = reinterpret_cast<const float*>(lds + w * (2 * TILE));
             const f32x4 v = *reinterpret_cast<const f32x4*>(src + r * D + ((piece + r) & (D / 4 - 1)) * 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = fmaf(f, v[i], o[i]);
@@ -581,7 +592,7 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, co
 
 // Work-group b's piece of the cut, row tile by row tile.
 template <class E, int D>
-__device__ __forceinline__ void few_piece(const PagedParams& p, int b, const Lds& lds, float* joint) {
+__device__ __forceinline__ void few_piece(const PagedParams& p, int b, uint8_t* lds, float* joint) {
     const int lane = threadIdx.x & 63;
     const Cut cut = few_cut(p, lane);
     const uint32_t first = b * cut.size, end = first + cut.size;
@@ -613,74 +624,160 @@ __device__ __forceinline__ void few_piece(const PagedParams& p, int b, const Lds
 
 // ---- many rows ----
 
-// Two tiles of 64 keys in turn: while one is worked on the other arrives.  A
-// wave loads 16 keys of each.
+// The work-group meets; the wave's LDS reads have returned.  The clobber keeps
+// LDS accesses on their side.
+__device__ __forceinline__ void meet() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // (known to be zero: no waits for reads before)
+}
+
+// Eight waves, two on each SIMD, in two groups: while one group's waves form
+// products (phase M: O += V^T P^T of the last tile, S of this one) the other
+// group's do the softmax of theirs (phase S), and they meet after each phase.
+// Left to themselves the two waves of a SIMD fell into step, each pipe idle
+// half of the time (@PINGPONG@).
+//   slot     2t             2t + 1         2t + 2
+//   group 0  M(t)           S(t)           M(t + 1)
+//   group 1  S(t - 1)       M(t)           S(t)
+// Keys and values go through three tiles of LDS each: slot 2t begins the loads
+// of K(t + 2) and V(t + 1) over tiles last read in slot 2t - 1; slot 2t + 2
+// reads K(t + 1) and V(t), which every wave has waited for by its end of slot
+// 2t + 1.  Each wave loads 8 keys of a tile.
 template <class E, int D>
-__device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, const Lds& lds) {
+__device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, uint8_t* kt, uint8_t* vt) {
     constexpr int STEPS = D / 16, DB = D / 32, TK = Shape<MANY>::TK, MT = Shape<MANY>::MT;
+    constexpr int TILE = TK * D * 2;
+    constexpr int SHARE = TK / Shape<MANY>::WAVES, LOADS = SHARE * D * 2 / 1024;  // keys and loads a wave and tile
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool second = wave >= 4;
     const int row = wave * ROWS + (lane & 31);
     const Row x = row_of(p, u, u.m * MT + row);
-    const Tiles tl = {u.begin, u.end};
+    const int count = u.end - u.begin;
     // the keys that every row of this wave sees, and those that any does
     const int all_lo = __builtin_amdgcn_readlane(x.lo, 31), all_hi = __builtin_amdgcn_readlane(x.hi, 0);
-    const int any_lo = __builtin_amdgcn_readlane(x.lo, 0), any_hi = __builtin_amdgcn_readlane(x.hi, 31);
+    const int any_lo = __builtin_amdgcn_readlane(x.lo, 0);
+    const int any_hi = u.m * MT + wave * ROWS < u.s.count * p.G ? __builtin_amdgcn_readlane(x.hi, 31) : 0;
     const float c = p.scale * LOG2E;
     Running run;
-    f32x16 acc[DB];
+    f32x16 acc[DB], st[2];
+    u32x4 pt[4];
 #pragma unroll
     for (int i = 0; i < DB; ++i) acc[i] = f32x16{};
 
-    auto load = [&](int t, int page, uint8_t* kt, uint8_t* vt) {
-        const int key = t * TK + 16 * wave;
-        load_keys<D>(p, p.k, p.k_page, p.k_token, u.h * p.k_head, page, key, u.s.len, lane, kt + wave * (16 * D * 2));
-        load_keys<D>(p, p.v, p.v_page, p.v_token, u.h * p.v_head, page, key, u.s.len, lane, vt + wave * (16 * D * 2));
+    const Loader<D, SHARE> k0(p.k, p.k_page, p.k_token, u.h * p.k_head, SHARE * wave & 15, lane);
+    const Loader<D, SHARE> v0(p.v, p.v_page, p.v_token, u.h * p.v_head, SHARE * wave & 15, lane);
+    const uint32_t k_lds = lds_address(kt) + wave * (SHARE * D * 2), v_lds = lds_address(vt) + wave * (SHARE * D * 2);
+    const int in_page = (1 << p.page_shift) - 1;
+    auto look_up = [&](int t) { return table_entry(p, u.n, ((u.begin + t) * TK + SHARE * wave) >> p.page_shift); };
+    auto load = [&](const Loader<D, SHARE>& from, int t, int page, uint32_t to) {
+        if (t >= count) return;
+        const int key = (u.begin + t) * TK + SHARE * wave;
+        from.load(p, page, key & in_page, u.s.len - key, to);
     };
-    auto look_up = [&](int t) { return t < tl.end ? page_at(p, u, t * TK + 16 * wave) : -1; };
+    // Table entries of tiles t + 1 and t + 2 as slot 2t begins.
+    int page1 = look_up(0), page2 = look_up(1);
+    load(k0, 0, page1, k_lds);
+    load(k0, 1, page2, k_lds + TILE);
+    load(v0, 0, page1, v_lds);
+    page1 = page2;
+    page2 = look_up(2);
     u32x4 q[STEPS];
-    int page = look_up(tl.begin);
-    if (tl.begin < tl.end) load(tl.begin, page, lds.k0, lds.v0);
-    page = look_up(tl.begin + 1);
     load_q<D>(p, u, x, half, q);
 
-    // Tile t, in (kt, vt); the next goes to (kn, vn).
-    auto step = [&](int t, const uint8_t* kt, const uint8_t* vt, uint8_t* kn, uint8_t* vn) {
-        // This wave's loads into LDS are complete, then every wave's (the barrier
-        // alone does not wait for them).
-        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0
-        __syncthreads();
-        if (t + 1 < tl.end) load(t + 1, page, kn, vn);
-        page = look_up(t + 2);
-        const int t0 = t * TK;
-        if (t0 >= any_hi || t0 + TK <= any_lo) return;
-        f32x16 st[2];
+    auto sees = [&](int t) {
+        const int t0 = (u.begin + t) * TK;
+        return t0 < any_hi && t0 + TK > any_lo;
+    };
+    auto begin_loads = [&](int t, int kbuf, int vbuf) {
+        load(k0, t + 2, page2, k_lds + kbuf * TILE);
+        load(v0, t + 1, page1, v_lds + vbuf * TILE);
+        page1 = page2;
+        page2 = look_up(t + 3);
+    };
+    // K(t + 1) and V(t) have arrived: what was begun after them, in slot 2t, may be under way.
+    auto arrived = [&](int t) {
+        if (t + 2 < count) wait_loads<2 * LOADS>();
+        else wait_loads<0>();
+    };
+    // The products' operands are read one group of matrix ops ahead of their
+    // use, a read between two matrix ops: an LDS read takes several of them.
+    auto scores = [&](const uint8_t* ks) {
+        u32x4 a[2][4];
+        auto read = [&](int g, int i) {
+            return read_k<D>(ks, 32 * (i & 1) + (lane & 31), 2 * (2 * g + (i >> 1)) + half);
+        };
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            st[b] = f32x16{};
+        for (int i = 0; i < 4; ++i) a[0][i] = read(0, i);
+        st[0] = st[1] = f32x16{};
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s)
-                st[b] = E::mfma(read_k<D>(kt, 32 * b + (lane & 31), 2 * s + half), q[s], st[b]);
-        }
-        u32x4 pt[4];
+        for (int g = 0; g < STEPS / 2; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (g + 1 < STEPS / 2) a[(g + 1) & 1][i] = read(g + 1, i);
+                st[i & 1] = E::mfma(a[g & 1][i], q[2 * g + (i >> 1)], st[i & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    };
+    auto outputs = [&](const uint8_t* vs) {
+        u32x4 a[2][DB];
+        auto read = [&](int k, int d) {
+            const u32x2 v0 = read_v<D>(vs, 16 * k + 4 * half, d, lane);
+            const u32x2 v1 = read_v<D>(vs, 16 * k + 8 + 4 * half, d, lane);
+            return u32x4{v0.x, v0.y, v1.x, v1.y};
+        };
+#pragma unroll
+        for (int d = 0; d < DB; ++d) a[0][d] = read(0, d);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                if (k + 1 < 4) a[(k + 1) & 1][d] = read(k + 1, d);
+                acc[d] = E::mfma(a[k & 1][d], pt[k], acc[d]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    };
+    auto products = [&](int t, const uint8_t* ks, const uint8_t* vs) {
+        __builtin_amdgcn_s_setprio(1);
+        if (t > 0 && sees(t - 1)) outputs(vs);
+        if (sees(t)) scores(ks);
+        __builtin_amdgcn_s_setprio(0);
+    };
+    auto softmax = [&](int t) {
+        if (!sees(t)) return;
+        const int t0 = (u.begin + t) * TK;
         float alpha;
         if (softmax_tile<E, 2>(st, t0 + 4 * half, x.lo, x.hi, t0 < all_lo || t0 + TK > all_hi, c, run, pt, alpha)) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) acc[d] *= alpha;
         }
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const u32x2 v0 = read_v<D>(vt, 16 * k + 4 * half, d, lane);
-                const u32x2 v1 = read_v<D>(vt, 16 * k + 8 + 4 * half, d, lane);
-                acc[d] = E::mfma(u32x4{v0.x, v0.y, v1.x, v1.y}, pt[k], acc[d]);
-            }
-        }
     };
-    for (int t = tl.begin; t < tl.end; t += 2) {
-        step(t, lds.k0, lds.v0, lds.k1, lds.v1);
-        if (t + 1 < tl.end) step(t + 1, lds.k1, lds.v1, lds.k0, lds.v0);
+    // Tile t, in place I = t % 3 of the rings.
+    auto step = [&](int t, int I) {
+        if (!second) begin_loads(t, (I + 2) % 3, (I + 1) % 3);
+        products(t, kt + I * TILE, vt + (I + 2) % 3 * TILE);
+        if (second) arrived(t);
+        meet();
+        if (second) begin_loads(t + 1, I, (I + 2) % 3);
+        softmax(t);
+        if (!second) arrived(t);
+        meet();
+    };
+    if (count > 0) {
+        // (where the compiler sees it: else it waits for q in every turn)
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0
+        meet();
+        if (second) {
+            begin_loads(0, 2, 1);
+            meet();
+        }
+        for (int t = 0; t < count; t += 3) {
+            step(t, 0);
+            if (t + 1 < count) step(t + 1, 1);
+            if (t + 2 < count) step(t + 2, 2);
+        }
+        if (sees(count - 1)) outputs(vt + (count - 1) % 3 * TILE);
+        if (!second) meet();
     }
 
     const float l = sum_halves(run.l);
@@ -712,23 +809,20 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, c
 
 // ---- kernels ----
 
-// KIND MIXED: the first `few` work-groups take the sequences of few rows, the
-// others the rest.
-template <class E, int D, int KIND>
-__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedParams p, int few, bool cut) {
-    __shared__ alignas(1024) uint8_t k0[64 * D * 2];
-    __shared__ alignas(1024) uint8_t v0[64 * D * 2];
-    __shared__ alignas(1024) uint8_t k1[64 * D * 2];
-    __shared__ alignas(1024) uint8_t v1[64 * D * 2];
-    const Lds lds = {k0, v0, k1, v1};
-    __shared__ float joint[KIND == MANY ? 1 : WAVES * 2 * ROWS];
-    if (KIND == FEW || (KIND == MIXED && (int)blockIdx.x < few)) {
-        few_piece<E, D>(p, blockIdx.x, lds, joint);
-    } else {
-        Unit u;
-        int parts;
-        if (many_unit<false>(p, (int)blockIdx.x - few, cut, threadIdx.x & 63, u, parts)) many_rows<E, D>(p, u, lds);
-    }
+template <class E, int D>
+__global__ __launch_bounds__(256, 2) void paged_few_kernel(PagedParams p) {
+    __shared__ alignas(1024) uint8_t lds[Shape<FEW>::WAVES * 2 * Shape<FEW>::TK * D * 2];
+    __shared__ float joint[Shape<FEW>::WAVES * 2 * ROWS];
+    few_piece<E, D>(p, blockIdx.x, lds, joint);
+}
+
+template <class E, int D>
+__global__ __launch_bounds__(512, 2) void paged_many_kernel(PagedParams p, bool cut) {
+    __shared__ alignas(1024) uint8_t kt[3 * Shape<MANY>::TK * D * 2];
+    __shared__ alignas(1024) uint8_t vt[3 * Shape<MANY>::TK * D * 2];
+    Unit u;
+    int parts;
+    if (many_unit<false>(p, blockIdx.x, cut, threadIdx.x & 63, u, parts)) many_rows<E, D>(p, u, kt, vt);
 }
 
 // Joins the partial results of one row tile: four elements of a row a thread,
@@ -856,15 +950,16 @@ int64_t many_units(const PagedParams& p) {
 bool may_cut(const PagedParams& p, int kind) {
     const int64_t keys = (int64_t)p.M << p.page_shift;
     if (kind == FEW) return keys > Shape<FEW>::TK;
-    return keys >= 2 * Shape<MANY>::LEAST * Shape<MANY>::TK && many_units(p) <= SLOTS / 2;
+    return keys >= 2 * Shape<MANY>::LEAST * Shape<MANY>::TK && many_units(p) <= Shape<MANY>::SLOTS / 2;
 }
 
 template <class E, int D, int KIND>
 hipError_t launch(const PagedParams& p, hipStream_t stream) {
     const bool fc = KIND != MANY && may_cut(p, FEW), mc = KIND != FEW && may_cut(p, MANY);
     const int64_t units = KIND == FEW ? 0 : many_units(p);
-    const int64_t few = KIND == MANY ? 0 : SLOTS, many = units + (mc ? SLOTS : 0);
-    paged_attn_kernel<E, D, KIND><<<dim3((unsigned)(few + many)), 256, 0, stream>>>(p, (int)few, mc);
+    if (KIND != MANY) paged_few_kernel<E, D><<<Shape<FEW>::SLOTS, 256, 0, stream>>>(p);
+    if (KIND != FEW)
+        paged_many_kernel<E, D><<<dim3((unsigned)(units + (mc ? Shape<MANY>::SLOTS : 0))), 512, 0, stream>>>(p, mc);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !(fc || mc)) return e;
     // work-groups a row tile: one for every 64 fours of what rows there can be, up to 4

@@ -52,6 +52,7 @@ int paged_params(const KdaPagedArgs* a, PagedParams& p) {
     if (!strides_ok(a->k_page, a->k_token, a->k_head) || !strides_ok(a->v_page, a->v_token, a->v_head))
         return KDA_BT16_EINVAL;
     if (!page_span_ok(a, a->k_token) || !page_span_ok(a, a->v_token)) return KDA_BT16_EUNSUPPORTED;
+    if (a->k_page > I32_MAX || a->v_page > I32_MAX) return KDA_BT16_EUNSUPPORTED;
     // Positions are 32-bit.
     if (((int64_t)a->M << shift) > I32_MAX / 2) return KDA_BT16_EUNSUPPORTED;
 
@@ -74,11 +75,11 @@ int paged_params(const KdaPagedArgs* a, PagedParams& p) {
     p.seq_lens = a->seq_lens;
     p.k = static_cast<uint16_t*>(a->k);
     p.v = static_cast<uint16_t*>(a->v);
-    p.k_page = a->k_page;
-    p.k_token = a->k_token;
+    p.k_page = (uint32_t)a->k_page;
+    p.k_token = (int32_t)a->k_token;
     p.k_head = a->k_head;
-    p.v_page = a->v_page;
-    p.v_token = a->v_token;
+    p.v_page = (uint32_t)a->v_page;
+    p.v_token = (int32_t)a->v_token;
     p.v_head = a->v_head;
     return KDA_BT16_OK;
 }

@@ -37,14 +37,14 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedParams p, int to
     const int tok = p.cu_seqlens ? t - s.first : t - n * p.T;
     const int pos = s.pos + tok;
     if (tok < 0 || tok >= s.count || pos < 0) return;
-    const int page = page_of(p, n, pos >> p.page_shift);
-    if (page < 0) return;
+    const int64_t page = table_entry(p, n, pos >> p.page_shift);
+    if (!is_page(p, (int)page)) return;
     const int in = pos & ((1 << p.page_shift) - 1);
     const int64_t row = p.cu_seqlens ? 0 : n, at = p.cu_seqlens ? t : tok;
     const u32x4 k = *reinterpret_cast<const u32x4*>(p.nk + row * p.nk_row + at * p.nk_token + h * p.nk_head + 8 * piece);
     const u32x4 v = *reinterpret_cast<const u32x4*>(p.nv + row * p.nv_row + at * p.nv_token + h * p.nv_head + 8 * piece);
-    *reinterpret_cast<u32x4*>(p.k + page * p.k_page + in * p.k_token + h * p.k_head + 8 * piece) = k;
-    *reinterpret_cast<u32x4*>(p.v + page * p.v_page + in * p.v_token + h * p.v_head + 8 * piece) = v;
+    *reinterpret_cast<u32x4*>(p.k + page * p.k_page + (int64_t)in * p.k_token + h * p.k_head + 8 * piece) = k;
+    *reinterpret_cast<u32x4*>(p.v + page * p.v_page + (int64_t)in * p.v_token + h * p.v_head + 8 * piece) = v;
 }
 
 // ---- scans ----
