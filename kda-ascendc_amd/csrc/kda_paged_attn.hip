@@ -639,10 +639,10 @@ __device__ __forceinline__ void meet() {
 //   slot     2t             2t + 1         2t + 2
 //   group 0  M(t)           S(t)           M(t + 1)
 //   group 1  S(t - 1)       M(t)           S(t)
-// Keys and values go through three tiles of LDS each: slot 2t begins the loads
-// of K(t + 2) and V(t + 1) over tiles last read in slot 2t - 1; slot 2t + 2
-// reads K(t + 1) and V(t), which every wave has waited for by its end of slot
-// 2t + 1.  Each wave loads 8 keys of a tile.
+// Keys and values go through three tiles of LDS each.  The softmax of tile t
+// begins with this wave's loads (8 keys) of K(t + 2) and V(t + 1), over tiles
+// last read in slot 2t - 1; slot 2t + 2 is the first to read K(t + 1) and V(t),
+// which every wave has waited for by its end of slot 2t + 1.
 template <class E, int D>
 __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, uint8_t* kt, uint8_t* vt) {
     constexpr int STEPS = D / 16, DB = D / 32, TK = Shape<MANY>::TK, MT = Shape<MANY>::MT;
@@ -675,7 +675,7 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
         const int key = (u.begin + t) * TK + SHARE * wave;
         from.load(p, page, key & in_page, u.s.len - key, to);
     };
-    // Table entries of tiles t + 1 and t + 2 as slot 2t begins.
+    // Table entries of tiles t + 1 and t + 2 as the softmax of t begins.
     int page1 = look_up(0), page2 = look_up(1);
     load(k0, 0, page1, k_lds);
     load(k0, 1, page2, k_lds + TILE);
@@ -695,7 +695,7 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
         page1 = page2;
         page2 = look_up(t + 3);
     };
-    // K(t + 1) and V(t) have arrived: what was begun after them, in slot 2t, may be under way.
+    // K(t + 1) and V(t) have arrived: what was begun after them may be under way.
     auto arrived = [&](int t) {
         if (t + 2 < count) wait_loads<2 * LOADS>();
         else wait_loads<0>();
@@ -754,11 +754,10 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
     };
     // Tile t, in place I = t % 3 of the rings.
     auto step = [&](int t, int I) {
-        if (!second) begin_loads(t, (I + 2) % 3, (I + 1) % 3);
         products(t, kt + I * TILE, vt + (I + 2) % 3 * TILE);
-        if (second) arrived(t);
+        if (second) wait_loads<0>();
         meet();
-        if (second) begin_loads(t + 1, I, (I + 2) % 3);
+        begin_loads(t, (I + 2) % 3, (I + 1) % 3);
         softmax(t);
         if (!second) arrived(t);
         meet();
@@ -767,10 +766,7 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
         // (where the compiler sees it: else it waits for q in every turn)
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0
         meet();
-        if (second) {
-            begin_loads(0, 2, 1);
-            meet();
-        }
+        if (second) meet();
         for (int t = 0; t < count; t += 3) {
             step(t, 0);
             if (t + 1 < count) step(t + 1, 1);
