@@ -88,9 +88,20 @@ __device__ __forceinline__ int swizzle(int row) {
 // cannot tell the tiles of a ring apart and would wait, before any LDS read,
 // for every such load under way.  So nothing but wait_loads() waits for it;
 // it has no result in registers, and other loads' waits only become longer.
+// STREAM: for what is read once, past the caches' lines of other work (the
+// decode step of 64 sequences of 3024 tokens, 32 / 8 heads: 141 us without,
+// 124 us with, 6.4 TB/s; a long chunk's keys, read again by other work-groups,
+// lose by it).
+template <bool STREAM>
 __device__ __forceinline__ void load_lds(u32x4 rsrc, int off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(lds)
-                 : "memory");
+    if constexpr (STREAM)
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds" ::"v"(off), "s"(rsrc),
+                     "s"(lds)
+                     : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc),
+                     "s"(lds)
+                     : "memory");
 }
 // All but the last `n` of this wave's loads have arrived.
 template <int N>
@@ -103,7 +114,7 @@ __device__ __forceinline__ uint32_t lds_address(const uint8_t* p) {
 
 // What a wave loads of a tile: NROWS keys (or values) of one head, all of one
 // page, 1 KiB a load.
-template <int D, int NROWS>
+template <int D, int NROWS, bool STREAM>
 struct Loader {
     static constexpr int PIECES = D / 8, R = 64 / PIECES, LOADS = NROWS / R;
     uint64_t head;            // byte address of the head in page 0
@@ -125,7 +136,7 @@ struct Loader {
         const uint64_t at = head + ((uint64_t)(n > 0 ? (uint32_t)page : 0u) * page_bytes << 1) + (uint32_t)in * token_bytes;
         const u32x4 rsrc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, n > 0 ? (n - 1) * token_bytes + D * 2 : 0u, BUF_RAW};
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) load_lds(rsrc, off[j], lds + j * 1024);
+        for (int j = 0; j < LOADS; ++j) load_lds<STREAM>(rsrc, off[j], lds + j * 1024);
     }
 };
 
@@ -468,15 +479,15 @@ __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, ui
     const float c = p.scale * LOG2E;
 
     int t = tl.begin + wave;
-    const Loader<D, 16> k0(p.k, p.k_page, p.k_token, u.h * p.k_head, 0, lane);
-    const Loader<D, 16> v0(p.v, p.v_page, p.v_token, u.h * p.v_head, 0, lane);
+    const Loader<D, 16, true> k0(p.k, p.k_page, p.k_token, u.h * p.k_head, 0, lane);
+    const Loader<D, 16, true> v0(p.v, p.v_page, p.v_token, u.h * p.v_head, 0, lane);
     const int in_page = (1 << p.page_shift) - 1;
     int pages[2], next[2];  // of the tile's first and second 16 keys
     auto look_up = [&](int tile, int (&pg)[2]) {
 #pragma unroll
         for (int g = 0; g < 2; ++g) pg[g] = table_entry(p, u.n, (tile * TK + 16 * g) >> p.page_shift);
     };
-    auto load = [&](const Loader<D, 16>& from, int tile, const int (&pg)[2], uint8_t* to) {
+    auto load = [&](const Loader<D, 16, true>& from, int tile, const int (&pg)[2], uint8_t* to) {
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             const int key = tile * TK + 16 * g;
@@ -665,12 +676,12 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
 #pragma unroll
     for (int i = 0; i < DB; ++i) acc[i] = f32x16{};
 
-    const Loader<D, SHARE> k0(p.k, p.k_page, p.k_token, u.h * p.k_head, SHARE * wave & 15, lane);
-    const Loader<D, SHARE> v0(p.v, p.v_page, p.v_token, u.h * p.v_head, SHARE * wave & 15, lane);
+    const Loader<D, SHARE, false> k0(p.k, p.k_page, p.k_token, u.h * p.k_head, SHARE * wave & 15, lane);
+    const Loader<D, SHARE, false> v0(p.v, p.v_page, p.v_token, u.h * p.v_head, SHARE * wave & 15, lane);
     const uint32_t k_lds = lds_address(kt) + wave * (SHARE * D * 2), v_lds = lds_address(vt) + wave * (SHARE * D * 2);
     const int in_page = (1 << p.page_shift) - 1;
     auto look_up = [&](int t) { return table_entry(p, u.n, ((u.begin + t) * TK + SHARE * wave) >> p.page_shift); };
-    auto load = [&](const Loader<D, SHARE>& from, int t, int page, uint32_t to) {
+    auto load = [&](const Loader<D, SHARE, false>& from, int t, int page, uint32_t to) {
         if (t >= count) return;
         const int key = (u.begin + t) * TK + SHARE * wave;
         from.load(p, page, key & in_page, u.s.len - key, to);
