@@ -268,6 +268,12 @@ __device__ __forceinline__ Tiles tiles_of(const PagedParams& p, const NewTokens&
     return {lo / TK, max(lo / TK, (hi + TK - 1) / TK)};
 }
 
+// Lane `at`'s.
+__device__ __forceinline__ NewTokens of_lane(const NewTokens& s, int at) {
+    return {__builtin_amdgcn_readlane(s.first, at), __builtin_amdgcn_readlane(s.count, at),
+            __builtin_amdgcn_readlane(s.len, at), __builtin_amdgcn_readlane(s.pos, at)};
+}
+
 // Whether a sequence is of the kind: packed ones are told apart by their rows.
 template <int KIND>
 __device__ __forceinline__ bool of_kind(const PagedParams& p, const NewTokens& s) {
@@ -285,46 +291,57 @@ __device__ __forceinline__ bool of_kind(const PagedParams& p, const NewTokens& s
 // SLOTS pieces hold what the tiles and the fillings come to.
 // All work-groups come to the same cut, from the lengths on the device; every
 // lane counts one sequence.
+// !cut: row tiles whole, each filled up to a piece of FEW_WHOLE keys, which
+// no row of the table exceeds.
+constexpr int FEW_WHOLE = 24 * Shape<FEW>::TK;
 constexpr uint32_t FEW_UNITS = Shape<FEW>::SLOTS / 4;
 struct Cut {
     uint32_t tiles, size;
     bool filled;
-    int first;  // few_tiles of sequence `lane`
+    NewTokens s0;  // of sequence `lane`, and its few_tiles
+    int first;
     // Tiles of a row tile of c with its filling.
     __device__ __forceinline__ uint32_t span(uint32_t c) const { return filled ? (c + size - 1) / size * size : c; }
 };
-__device__ __forceinline__ int few_tiles(const PagedParams& p, int n) {
+__device__ __forceinline__ int few_tiles(const PagedParams& p, int n, NewTokens& s) {
     if (n >= p.N) return 0;
-    const NewTokens s = new_tokens(p, n);
+    s = new_tokens(p, n);
     if (!of_kind<FEW>(p, s)) return 0;
     const Tiles t = tiles_of<FEW>(p, s, 0);
     return max(1, t.end - t.begin);
 }
-__device__ __forceinline__ Cut few_cut(const PagedParams& p, int lane) {
+__device__ __forceinline__ Cut few_cut(const PagedParams& p, bool cut, int lane) {
     Cut c;
     uint32_t all = 0, units = 0;
     for (int n0 = 0; n0 < p.N; n0 += 64) {
-        const int x = few_tiles(p, n0 + lane);
-        if (n0 == 0) c.first = x;
+        NewTokens s = {};
+        const int x = few_tiles(p, n0 + lane, s);
+        if (n0 == 0) {
+            c.first = x;
+            c.s0 = s;
+        }
         all += (uint32_t)__builtin_amdgcn_readlane(wave_prefix(x, lane), 63);
         units += __popcll(__ballot(x > 0));
     }
     c.tiles = all * p.HKV;
     units *= p.HKV;
-    c.filled = units <= FEW_UNITS;
+    c.filled = !cut || units <= FEW_UNITS;
     const uint32_t pieces = c.filled ? Shape<FEW>::SLOTS - units : Shape<FEW>::SLOTS;
-    c.size = __builtin_amdgcn_readfirstlane(max((uint32_t)Shape<FEW>::LEAST, (c.tiles + pieces - 1) / pieces));
+    c.size = cut ? max((uint32_t)Shape<FEW>::LEAST, (c.tiles + pieces - 1) / pieces) : FEW_WHOLE / Shape<FEW>::TK;
+    c.size = __builtin_amdgcn_readfirstlane(c.size);
     return c;
 }
-// Sequence by sequence, the first tile (of all, with fillings) of each lane's
-// sequence n0 + lane, and the tiles of one of its heads.
+// Each lane's sequence n0 + lane: the tiles of one of its heads.
 struct FewSpans {
+    NewTokens s;
     int tiles;
     uint32_t span, upto;  // with its filling; the heads' sum up to its end
 };
 __device__ __forceinline__ FewSpans few_spans(const PagedParams& p, const Cut& cut, int n0, int lane) {
     FewSpans x;
-    x.tiles = n0 == 0 ? cut.first : few_tiles(p, n0 + lane);
+    x.s = cut.s0;
+    x.tiles = cut.first;
+    if (n0 > 0) x.tiles = few_tiles(p, n0 + lane, x.s);
     x.span = cut.span(x.tiles);
     x.upto = wave_prefix(x.span * p.HKV, lane);
     return x;
@@ -338,14 +355,18 @@ __device__ __forceinline__ FewSpans few_spans(const PagedParams& p, const Cut& c
 // round the XCDs, so that with 8 heads each XCD's L2 has the keys of one.
 // Parts of cut row tiles number at most SLOTS.
 struct ManyWork {
-    int mt, tiles;  // row tiles, and tiles of keys that one sees at most
+    int mt = 0, tiles = 0;  // row tiles, and tiles of keys that one sees at most
+    NewTokens s;
 };
 __device__ __forceinline__ ManyWork many_work(const PagedParams& p, int n) {
     constexpr int MT = Shape<MANY>::MT, TK = Shape<MANY>::TK;
-    if (n >= p.N) return {0, 0};
+    ManyWork w;
+    if (n >= p.N) return w;
     const NewTokens s = new_tokens(p, n);
-    if (!of_kind<MANY>(p, s)) return {0, 0};
-    ManyWork w = {(s.count * p.G + MT - 1) / MT, (s.len + TK - 1) / TK};
+    if (!of_kind<MANY>(p, s)) return w;
+    w.s = s;
+    w.mt = (s.count * p.G + MT - 1) / MT;
+    w.tiles = (s.len + TK - 1) / TK;
     if (p.window) {
         // the tokens of a row tile and the window before the first
         const int64_t span = (int64_t)min(s.count, MT / p.G + 2) + p.window;
@@ -393,7 +414,7 @@ __device__ __forceinline__ bool many_unit(const PagedParams& p, int id, bool cut
             }
             u.m = mt - 1 - x;
             u.slot = parts > 1 ? slot0 + (x * p.HKV + u.h) * parts + part : -1;
-            u.s = new_tokens(p, u.n);
+            u.s = of_lane(w.s, at);
             const Tiles t = tiles_of<MANY>(p, u.s, u.m);
             const int64_t count = t.end - t.begin;
             u.begin = t.begin + (int)(count * part / parts);
@@ -603,9 +624,9 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, ui
 
 // Work-group b's piece of the cut, row tile by row tile.
 template <class E, int D>
-__device__ __forceinline__ void few_piece(const PagedParams& p, int b, uint8_t* lds, float* joint) {
+__device__ __forceinline__ void few_piece(const PagedParams& p, int b, bool may_cut, uint8_t* lds, float* joint) {
     const int lane = threadIdx.x & 63;
-    const Cut cut = few_cut(p, lane);
+    const Cut cut = few_cut(p, may_cut, lane);
     const uint32_t first = b * cut.size, end = first + cut.size;
     uint32_t cur = first, base = 0;
     for (int n0 = 0; n0 < p.N && cur < end; n0 += 64) {
@@ -619,7 +640,7 @@ __device__ __forceinline__ void few_piece(const PagedParams& p, int b, uint8_t* 
             u.n = __builtin_amdgcn_readfirstlane(n0 + at);
             u.h = in / span;
             u.m = 0;
-            u.s = new_tokens(p, u.n);
+            u.s = of_lane(x.s, at);
             const uint32_t t = in - u.h * span, stop = min(span, t + (end - cur));
             const int t0 = tiles_of<FEW>(p, u.s, 0).begin;
             u.begin = t0 + t;
@@ -817,10 +838,10 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
 // ---- kernels ----
 
 template <class E, int D>
-__global__ __launch_bounds__(256, 2) void paged_few_kernel(PagedParams p) {
+__global__ __launch_bounds__(256, 2) void paged_few_kernel(PagedParams p, bool cut) {
     __shared__ alignas(1024) uint8_t lds[Shape<FEW>::WAVES * 2 * Shape<FEW>::TK * D * 2];
     __shared__ float joint[Shape<FEW>::WAVES * 2 * ROWS];
-    few_piece<E, D>(p, blockIdx.x, lds, joint);
+    few_piece<E, D>(p, blockIdx.x, cut, lds, joint);
 }
 
 template <class E, int D>
@@ -845,17 +866,18 @@ __device__ __forceinline__ void join(const PagedParams& p, const Unit& u, int gr
     float mx = -INFINITY, sum = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     if (y.live) {
-#pragma unroll 8
-        for (int j = slice; j < parts; j += NS) mx = fmaxf(mx, place(j)[r]);
-        const float sub = mx == -INFINITY ? 0.f : mx;
+        // one pass, so that no load waits for another
 #pragma unroll 4
         for (int j = slice; j < parts; j += NS) {
             const float* part = place(j);
-            const float f = fast_exp2(part[r] - sub);
-            sum = fmaf(f, part[MT + r], sum);
+            const float mj = part[r], lj = part[MT + r];
             const f32x4 v = *reinterpret_cast<const f32x4*>(part + 2 * MT + r * D + piece * 4);
+            const float top = fmaxf(mx, mj), sub = top == -INFINITY ? 0.f : top;
+            const float f0 = fast_exp2(mx - sub), f = fast_exp2(mj - sub);
+            mx = top;
+            sum = fmaf(f, lj, sum * f0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = fmaf(f, v[i], o[i]);
+            for (int i = 0; i < 4; ++i) o[i] = fmaf(f, v[i], o[i] * f0);
         }
     }
     if constexpr (NS > 1) {
@@ -899,7 +921,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int few,
     Unit u;
     if (KIND == FEW || (KIND == MIXED && (int)blockIdx.x < few)) {
         const int id = blockIdx.x / few_groups;
-        const Cut cut = few_cut(p, lane);
+        const Cut cut = few_cut(p, true, lane);
         u.n = id / p.HKV;
         u.h = id - u.n * p.HKV;
         u.m = 0;
@@ -908,6 +930,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int few,
             const FewSpans x = few_spans(p, cut, n0, lane);
             if (u.n < n0 + 64) {
                 c = __builtin_amdgcn_readlane(x.tiles, u.n - n0);
+                u.s = of_lane(x.s, u.n - n0);
                 const uint32_t span = __builtin_amdgcn_readlane(x.span, u.n - n0);
                 first += __builtin_amdgcn_readlane(x.upto, u.n - n0) - (p.HKV - u.h) * span;
             } else {
@@ -917,7 +940,6 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int few,
         if (c == 0) return;
         const uint32_t b0 = first / cut.size, b1 = (first + c - 1) / cut.size;
         if (b0 == b1) return;
-        u.s = new_tokens(p, u.n);
         const int items = u.s.count * p.G * (D / 4);
         for (int group = blockIdx.x % few_groups; group * 64 < items; group += few_groups) {
             join<E, D, FEW>(p, u, group, b1 - b0 + 1, [&](int j) {
@@ -952,11 +974,12 @@ int64_t many_units(const PagedParams& p) {
     return (p.cu_seqlens ? rows / MT + p.N : p.N * ((rows + MT - 1) / MT)) * p.HKV;
 }
 
-// Whether a row tile's keys may go to several work-groups.  (Many rows: row
-// tiles that fill half of SLOTS are taken whole.)
+// Whether a row tile's keys may go to several work-groups.  Few rows: not where
+// the table's rows hold so few keys that the join costs more (@WHOLE@).  Many
+// rows: row tiles that fill half of SLOTS are taken whole.
 bool may_cut(const PagedParams& p, int kind) {
     const int64_t keys = (int64_t)p.M << p.page_shift;
-    if (kind == FEW) return keys > Shape<FEW>::TK;
+    if (kind == FEW) return keys > FEW_WHOLE;
     return keys >= 2 * Shape<MANY>::LEAST * Shape<MANY>::TK && many_units(p) <= Shape<MANY>::SLOTS / 2;
 }
 
@@ -964,7 +987,9 @@ template <class E, int D, int KIND>
 hipError_t launch(const PagedParams& p, hipStream_t stream) {
     const bool fc = KIND != MANY && may_cut(p, FEW), mc = KIND != FEW && may_cut(p, MANY);
     const int64_t units = KIND == FEW ? 0 : many_units(p);
-    if (KIND != MANY) paged_few_kernel<E, D><<<Shape<FEW>::SLOTS, 256, 0, stream>>>(p);
+    // (uncut: one piece a row tile)
+    if (KIND != MANY)
+        paged_few_kernel<E, D><<<dim3((unsigned)(fc ? Shape<FEW>::SLOTS : (int64_t)p.N * p.HKV)), 256, 0, stream>>>(p, fc);
     if (KIND != FEW)
         paged_many_kernel<E, D><<<dim3((unsigned)(units + (mc ? Shape<MANY>::SLOTS : 0))), 512, 0, stream>>>(p, mc);
     hipError_t e = hipGetLastError();
