@@ -8,6 +8,7 @@ library is missing or fails to load, every call raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -227,6 +228,28 @@ class KdaPagesArgs(ctypes.Structure):
     ]
 
 
+def _packer(fields) -> struct.Struct:
+    """A packer of C fields in their order and native alignment: the bytes of
+    a struct in a third of the time ctypes takes to fill one, for calls whose
+    time is the host's."""
+    codes = {ctypes.c_int32: "i", ctypes.c_uint32: "I", ctypes.c_float: "f", ctypes.c_int64: "q",
+             ctypes.c_void_p: "P", ctypes.c_size_t: "N"}
+    out = ""
+    for _, t in fields:
+        if issubclass(t, ctypes.Array):
+            out += "".join(codes[u] for _, u in t._type_._fields_) * t._length_
+        else:
+            out += codes[t]
+    return struct.Struct("@" + out)
+
+
+# The arguments up to the workspace, and the workspace (pointer, bytes).
+PAGED_PACK = _packer(KdaPagedArgs._fields_[:-2])
+PAGES_PACK = _packer(KdaPagesArgs._fields_[:-2])
+WORKSPACE_PACK = _packer(KdaPagedArgs._fields_[-2:])
+NO_WORKSPACE = WORKSPACE_PACK.pack(0, 0)
+
+
 class KdaHipError(RuntimeError):
     """A non-zero return code from the HIP library."""
 
@@ -285,19 +308,11 @@ def lib() -> ctypes.CDLL:
         h.kda_bt16_strerror.argtypes = [ctypes.c_int]
         h.kda_bt16_abi_version.restype = ctypes.c_int
         h.kda_bt16_abi_version.argtypes = []
-        for name in ("kda_paged_attn_hip", "kda_paged_append_hip"):
+        # (c_void_p: a struct by reference, or its packed bytes)
+        for name in PAGED_SYMBOLS[:-1]:
             fn = getattr(h, name)
-            fn.restype = ctypes.c_int
-            fn.argtypes = [ctypes.POINTER(KdaPagedArgs), ctypes.c_void_p]
-        for name in ("kda_pages_reserve_hip", "kda_pages_free_hip", "kda_pages_fork_hip",
-                     "kda_pages_copy_hip", "kda_pages_compact_hip"):
-            fn = getattr(h, name)
-            fn.restype = ctypes.c_int
-            fn.argtypes = [ctypes.POINTER(KdaPagesArgs), ctypes.c_void_p]
-        h.kda_paged_attn_workspace_bytes.restype = ctypes.c_size_t
-        h.kda_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(KdaPagedArgs)]
-        h.kda_pages_workspace_bytes.restype = ctypes.c_size_t
-        h.kda_pages_workspace_bytes.argtypes = [ctypes.POINTER(KdaPagesArgs)]
+            fn.restype = ctypes.c_size_t if name.endswith("_bytes") else ctypes.c_int
+            fn.argtypes = [ctypes.c_void_p] if name.endswith("_bytes") else [ctypes.c_void_p, ctypes.c_void_p]
         h.kda_paged_abi_version.restype = ctypes.c_int
         h.kda_paged_abi_version.argtypes = []
         if h.kda_paged_abi_version() != PAGED_ABI_VERSION:
@@ -377,5 +392,12 @@ def call_saved(name: str, args, saved: int, nbytes: int, stream: int) -> None:
 
 def call(name: str, args, stream: int) -> None:
     rc = getattr(_lib or lib(), name)(ctypes.byref(args), stream)
+    if rc != 0:
+        raise KdaHipError(name, rc, lib().kda_bt16_strerror(rc).decode())
+
+
+def call_packed(name: str, args: bytes, stream: int) -> None:
+    """:func:`call` with packed arguments."""
+    rc = getattr(_lib or lib(), name)(args, stream)
     if rc != 0:
         raise KdaHipError(name, rc, lib().kda_bt16_strerror(rc).decode())

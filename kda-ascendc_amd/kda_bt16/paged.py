@@ -32,8 +32,6 @@ access outside the tensors.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _hip, workspace
@@ -143,27 +141,9 @@ def _check_new(name: str, t: torch.Tensor, heads: int | None, k_cache, page_tabl
 _PAGE_SIZES = (16, 32, 64, 128, 256, 512, 1024)
 
 
-def _plain_cache(k, v, table, lens) -> bool:
-    """Whether these are an ordinary cache and table on a GPU that
-    :func:`_check_cache` accepts, each tensor looked at once: a small call's
-    time is the host's, and the checks in the order of their messages are half
-    of it.  False says nothing: the full checks then accept or raise."""
-    shape, s, dt, dev = k.shape, k.stride(), k.dtype, k.get_device()
-    if dev < 0 or len(shape) != 4 or v.shape != shape or v.dtype is not dt or v.get_device() != dev:
-        return False
-    t, D = v.stride(), shape[3]
-    if not (
-        (dt is torch.bfloat16 or dt is torch.float16) and (D == 128 or D == 64) and shape[1] in _PAGE_SIZES
-        and s[3] == 1 and t[3] == 1 and s[0] > 0 and t[0] > 0 and s[1] >= D and s[2] >= D and t[1] >= D and t[2] >= D
-        and (s[0] | s[1] | s[2] | t[0] | t[1] | t[2]) % 8 == 0 and (k.data_ptr() | v.data_ptr()) % 16 == 0
-        and shape[0] > 0 and shape[2] > 0
-    ):
-        return False
-    return _plain_table(table, lens, dev)
-
-
 def _plain_table(table, lens, dev) -> bool:
-    """As :func:`_plain_cache`, for :func:`_check_table`."""
+    """Whether these are an ordinary table and lengths on device ``dev`` that
+    :func:`_check_table` accepts."""
     n = table.shape
     return (
         len(n) == 2 and n[1] > 0 and lens.shape == n[:1] and table.dtype is torch.int32 and lens.dtype is torch.int32
@@ -172,15 +152,32 @@ def _plain_table(table, lens, dev) -> bool:
     )
 
 
-def _plain_new(x, rows, heads, D, dt, dev) -> bool:
-    """As :func:`_plain_cache`, for :func:`_check_new` without cu_seqlens
-    (``heads`` 0: any)."""
-    n, s = x.shape, x.stride()
-    return (
-        len(n) == 4 and n[0] == rows and n[3] == D and n[1] > 0 and (n[2] == heads if heads else n[2] > 0)
-        and x.dtype is dt and x.get_device() == dev and s[3] == 1 and (s[0] | s[1] | s[2]) % 8 == 0
-        and x.data_ptr() % 16 == 0
-    )
+def _plain_fields(k, v, table, lens, x, heads) -> tuple | None:
+    """The argument fields of an ordinary call without cu_seqlens on a GPU,
+    whose cache, table and new tokens ``x`` (``heads`` of them, 0: any) the
+    full checks accept, each tensor looked at once: a small call's time is the
+    host's, and the checks in the order of their messages are half of it.  None
+    says nothing: the full checks then accept or raise."""
+    shape, s, t, dt, dev = k.shape, k.stride(), v.stride(), k.dtype, k.get_device()
+    n, u, rows = x.shape, x.stride(), table.shape
+    if dev < 0 or len(shape) != 4 or len(n) != 4 or v.shape != shape:
+        return None
+    P, size, HKV, D = shape
+    s0, s1, s2, s3 = s
+    t0, t1, t2, t3 = t
+    u0, u1, u2, u3 = u
+    kp, vp = k.data_ptr(), v.data_ptr()
+    if not (
+        dt in _CACHE_DTYPES and v.dtype is dt and x.dtype is dt and (D == 128 or D == 64) and size in _PAGE_SIZES
+        and s3 == 1 and t3 == 1 and u3 == 1 and s0 > 0 and t0 > 0 and s1 >= D and s2 >= D and t1 >= D and t2 >= D
+        and (s0 | s1 | s2 | t0 | t1 | t2 | u0 | u1 | u2) % 8 == 0 and (kp | vp | x.data_ptr()) % 16 == 0
+        and P > 0 and HKV > 0 and n[0] == rows[0] and n[3] == D and n[1] > 0
+        and (n[2] == heads if heads else n[2] > 0) and v.get_device() == dev and x.get_device() == dev
+        and _plain_table(table, lens, dev)
+    ):
+        return None
+    return (rows[0], n[1], n[2], HKV, D, _CACHE_DTYPES[dt], P, size, rows[1], 0, 0, table.data_ptr(), rows[1],
+            lens.data_ptr(), kp, vp, s0, s1, s2, t0, t1, t2, u0, u1, u2)
 
 
 def _strides(t: torch.Tensor) -> tuple[int, int, int]:
@@ -189,29 +186,36 @@ def _strides(t: torch.Tensor) -> tuple[int, int, int]:
     return (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
 
 
-def _cache_args(k_cache, v_cache, page_table, seq_lens, new, HQ, cu_seqlens, flags=0, window=0, scale=1.0,
-                rest=()) -> _hip.KdaPagedArgs:
-    """The arguments of a call, in the order of the fields (setting each by
-    name takes twice the time); ``rest`` from ``q`` on."""
-    P, size, HKV, D = k_cache.shape
-    N, M = page_table.shape
-    cu, cu_dtype = None, 0
+def _fields(k, v, table, lens, x, cu_seqlens) -> tuple:
+    """:func:`_plain_fields` of any call that the full checks accept."""
+    P, size, HKV, D = k.shape
+    N, M = table.shape
+    cu_dtype = cu = 0
     if cu_seqlens is not None:
-        cu = cu_seqlens.data_ptr()
         cu_dtype = _hip.DTYPE_I64 if cu_seqlens.dtype == torch.int64 else _hip.DTYPE_I32
-    return _hip.KdaPagedArgs(
-        _hip.PAGED_ABI_VERSION, N, new.shape[1], HQ, HKV, D, _CACHE_DTYPES[k_cache.dtype], P, size, M, flags, window,
-        scale, cu_dtype, cu, page_table.data_ptr(), page_table.stride(0) if N > 1 else M, seq_lens.data_ptr(),
-        k_cache.data_ptr(), v_cache.data_ptr(), *_strides(k_cache), *_strides(v_cache), *rest)
+        cu = cu_seqlens.data_ptr()
+    return (N, x.shape[1], x.shape[2], HKV, D, _CACHE_DTYPES[k.dtype], P, size, M, cu_dtype, cu, table.data_ptr(),
+            table.stride(0) if N > 1 else M, lens.data_ptr(), k.data_ptr(), v.data_ptr(), *_strides(k), *_strides(v),
+            *_strides(x))
 
 
-def _launch(name: str, a, device: torch.device) -> None:
+def _launch(name: str, args: bytes, device: torch.device) -> None:
     """The entry point on the tensors' device and its current stream."""
     if torch._C._cuda_getDevice() == device.index:
-        _hip.call(name, a, _raw_stream(device))
+        _hip.call_packed(name, args, _raw_stream(device))
         return
     with torch.cuda.device(device):
-        _hip.call(name, a, _raw_stream(device))
+        _hip.call_packed(name, args, _raw_stream(device))
+
+
+def _launch_in(name: str, args: bytes, nbytes: int, device: torch.device) -> None:
+    """:func:`_launch` with a workspace of ``nbytes``, the caller's stream's
+    again once the launches are queued."""
+    if nbytes == 0:
+        _launch(name, args + _hip.NO_WORKSPACE, device)
+        return
+    ws = workspace.scratch(device, nbytes)
+    _launch(name, args + _hip.WORKSPACE_PACK.pack(ws.data_ptr(), nbytes), device)
 
 
 def paged_attention(
@@ -247,10 +251,12 @@ def paged_attention(
     ``seq_lens`` does not matter; keys and values before it have to be finite.
     Forward only: raises if q requires a gradient.
     """
-    if not (cu_seqlens is None and _plain_cache(k_cache, v_cache, page_table, seq_lens)
-            and _plain_new(q, page_table.shape[0], 0, k_cache.shape[3], k_cache.dtype, k_cache.get_device())):
+    f = _plain_fields(k_cache, v_cache, page_table, seq_lens, q, 0) if cu_seqlens is None else None
+    if f is None:
         _check_cache(k_cache, v_cache, page_table, seq_lens)
         _check_new("q", q, None, k_cache, page_table, cu_seqlens)
+        _require_gpu(q)
+        f = _fields(k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
     B, T, HQ, D = q.shape
     HKV = k_cache.shape[2]
     if HQ % HKV != 0:
@@ -266,18 +272,17 @@ def paged_attention(
             raise ValueError("window needs causal=True")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise NotImplementedError("paged_attention is forward only: inputs require grad")
-    _require_gpu(q)
     device = q.device
     o = torch.empty((B, T, HQ, D), dtype=q.dtype, device=device)
     lse = torch.empty((B, T, HQ), dtype=torch.float32, device=device) if return_lse else None
-    a = _cache_args(
-        k_cache, v_cache, page_table, seq_lens, q, HQ, cu_seqlens, _hip.PAGED_CAUSAL if causal else 0, window or 0, scale,
-        (q.data_ptr(), *_strides(q), o.data_ptr(), None if lse is None else lse.data_ptr()))
-    nbytes = _hip.lib().kda_paged_attn_workspace_bytes(ctypes.byref(a))
-    if nbytes:
-        ws = workspace.scratch(device, nbytes)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-    _launch("kda_paged_attn_hip", a, device)
+    (N, T, HQ, HKV, D, dt, P, size, M, cu_dtype, cu, table, table_stride, lens, kp, vp, s0, s1, s2, t0, t1, t2, u0, u1,
+     u2) = f
+    args = _hip.PAGED_PACK.pack(
+        _hip.PAGED_ABI_VERSION, N, T, HQ, HKV, D, dt, P, size, M, _hip.PAGED_CAUSAL if causal else 0, window or 0, scale,
+        cu_dtype, cu, table, table_stride, lens, kp, vp, s0, s1, s2, t0, t1, t2, q.data_ptr(), u0, u1, u2, o.data_ptr(),
+        0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0)
+    nbytes = _hip.lib().kda_paged_attn_workspace_bytes(args + _hip.NO_WORKSPACE)
+    _launch_in("kda_paged_attn_hip", args, nbytes, device)
     return (o, lse) if return_lse else o
 
 
@@ -299,19 +304,24 @@ def paged_append(
     Tokens at negative positions, or whose page the table does not have, are
     left out.
     """
-    dt, dev = k_cache.dtype, k_cache.get_device()
-    if not (cu_seqlens is None and _plain_cache(k_cache, v_cache, page_table, seq_lens) and v.shape == k.shape
-            and _plain_new(k, page_table.shape[0], k_cache.shape[2], k_cache.shape[3], dt, dev)
-            and _plain_new(v, page_table.shape[0], k_cache.shape[2], k_cache.shape[3], dt, dev)):
+    f = None
+    if cu_seqlens is None and v.shape == k.shape and v.stride() == k.stride() and v.dtype is k.dtype and (
+            v.data_ptr() % 16 == 0 and v.get_device() == k.get_device()):
+        f = _plain_fields(k_cache, v_cache, page_table, seq_lens, k, k_cache.shape[2])
+    if f is None:
         _check_cache(k_cache, v_cache, page_table, seq_lens)
         for name, t in (("k", k), ("v", v)):
             _check_new(name, t, k_cache.shape[2], k_cache, page_table, cu_seqlens)
         if v.shape != k.shape:
             raise ValueError(f"v.shape {tuple(v.shape)} must match k {tuple(k.shape)}")
-    _require_gpu(k)
-    _launch("kda_paged_append_hip", _cache_args(
-        k_cache, v_cache, page_table, seq_lens, k, 0, cu_seqlens, rest=(
-            None, 0, 0, 0, None, None, k.data_ptr(), v.data_ptr(), *_strides(k), *_strides(v))), k.device)
+        _require_gpu(k)
+        f = _fields(k_cache, v_cache, page_table, seq_lens, k, cu_seqlens) + _strides(v)
+    (N, T, HQ, HKV, D, dt, P, size, M, cu_dtype, cu, table, table_stride, lens, kp, vp, s0, s1, s2, t0, t1, t2, u0, u1,
+     u2), w = f[:25], f[25:] or f[22:]
+    _launch("kda_paged_append_hip", _hip.PAGED_PACK.pack(
+        _hip.PAGED_ABI_VERSION, N, T, HQ, HKV, D, dt, P, size, M, 0, 0, 1.0, cu_dtype, cu, table, table_stride, lens, kp,
+        vp, s0, s1, s2, t0, t1, t2, 0, 0, 0, 0, 0, 0, k.data_ptr(), v.data_ptr(), u0, u1, u2, *w) + _hip.NO_WORKSPACE,
+        k.device)
 
 
 def _pools(pools) -> list[torch.Tensor]:
@@ -336,30 +346,30 @@ def _pools(pools) -> list[torch.Tensor]:
     return ts
 
 
-def _pages_args(P, pools=(), page_table=None, seq_lens=None, page_refs=None, page_size=16, rest=()):
-    """The arguments of a call on the pages, in the order of the fields;
+_NO_POOLS = (0,) * (3 * _hip.PAGED_MAX_POOLS)
+
+
+def _pages_args(P, pools=(), page_table=None, seq_lens=None, page_refs=None, page_size=16, rest=()) -> bytes:
+    """The packed arguments of a call on the pages, up to the workspace;
     ``rest`` from ``F`` on: F, then src, dst, new_tokens, ok, out_table,
-    out_refs, out_live as tensors or None."""
-    N = M = stride = 0
-    table = None
+    out_refs, out_live as tensors or None, as many as there are."""
+    N = M = stride = table = 0
     if page_table is not None:
         N, M = page_table.shape
         table, stride = page_table.data_ptr(), page_table.stride(0) if N > 1 else M
     arr = _NO_POOLS
     if pools:
-        arr = (_hip.KdaPagePool * _hip.PAGED_MAX_POOLS)()
-        for i, t in enumerate(pools):
+        arr = []
+        for t in pools:
             size = t.element_size()
             page = t.stride(-4) * size
-            arr[i] = (t.data_ptr(), t.numel() * size // (P * page), page)
-    F, *tensors = rest
-    return _hip.KdaPagesArgs(
-        _hip.PAGED_ABI_VERSION, N, M, P, page_size, F, len(pools), 0, arr, table, stride,
-        None if seq_lens is None else seq_lens.data_ptr(), None if page_refs is None else page_refs.data_ptr(),
-        *[None if t is None else t.data_ptr() for t in tensors])
-
-
-_NO_POOLS = (_hip.KdaPagePool * _hip.PAGED_MAX_POOLS)()
+            arr += (t.data_ptr(), t.numel() * size // (P * page), page)
+        arr += _NO_POOLS[len(arr):]
+    tail = [0 if t is None else t.data_ptr() for t in rest[1:]]
+    tail += [0] * (7 - len(tail))
+    return _hip.PAGES_PACK.pack(
+        _hip.PAGED_ABI_VERSION, N, M, P, page_size, rest[0], len(pools), 0, *arr, table, stride,
+        0 if seq_lens is None else seq_lens.data_ptr(), 0 if page_refs is None else page_refs.data_ptr(), *tail)
 
 
 def _check_refs(page_refs, device) -> None:
@@ -370,11 +380,9 @@ def _check_refs(page_refs, device) -> None:
         raise ValueError("page_refs must be 16-byte aligned")
 
 
-def _launch_with_workspace(name: str, a, device) -> None:
-    nbytes = _hip.lib().kda_pages_workspace_bytes(ctypes.byref(a))
-    ws = workspace.scratch(device, nbytes)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-    _launch(name, a, device)
+def _launch_pages(name: str, args: bytes, device) -> None:
+    """A call on the pages that takes a workspace."""
+    _launch_in(name, args, _hip.lib().kda_pages_workspace_bytes(args + _hip.NO_WORKSPACE), device)
 
 
 def _check_rows(pairs, device) -> None:
@@ -420,7 +428,7 @@ def paged_reserve(
     ok = torch.empty(seq_lens.shape[0], dtype=torch.bool, device=device)
     a = _pages_args(page_refs.shape[0], (), page_table, seq_lens, page_refs, page_size,
                     (0, None, None, new_tokens, ok))
-    _launch_with_workspace("kda_pages_reserve_hip", a, device)
+    _launch_pages("kda_pages_reserve_hip", a, device)
     return ok
 
 
@@ -436,7 +444,7 @@ def paged_free(
     _check_rows([("rows", rows)], device)
     _require_gpu(page_table)
     _launch("kda_pages_free_hip", _pages_args(page_refs.shape[0], (), page_table, seq_lens, page_refs, 16,
-                                              (rows.shape[0], None, rows)), device)
+                                              (rows.shape[0], None, rows)) + _hip.NO_WORKSPACE, device)
 
 
 def paged_fork(
@@ -474,7 +482,7 @@ def paged_fork(
     _require_gpu(ts[0])
     ok = torch.empty(src.shape[0], dtype=torch.bool, device=device)
     a = _pages_args(P, ts, page_table, seq_lens, page_refs, page_size, (src.shape[0], src, dst, None, ok))
-    _launch_with_workspace("kda_pages_fork_hip", a, device)
+    _launch_pages("kda_pages_fork_hip", a, device)
     return ok
 
 
@@ -491,7 +499,8 @@ def paged_copy(pools, src: torch.Tensor, dst: torch.Tensor) -> None:
     device = ts[0].device
     _check_rows([("src", src), ("dst", dst)], device)
     _require_gpu(ts[0])
-    _launch("kda_pages_copy_hip", _pages_args(ts[0].shape[-4], ts, rest=(src.shape[0], src, dst)), device)
+    _launch("kda_pages_copy_hip", _pages_args(ts[0].shape[-4], ts, rest=(src.shape[0], src, dst))
+            + _hip.NO_WORKSPACE, device)
 
 
 def paged_compact(
@@ -524,5 +533,5 @@ def paged_compact(
     refs = torch.empty_like(page_refs)
     live = torch.empty(1, dtype=torch.int32, device=device)
     a = _pages_args(P, ts, page_table, None, page_refs, 16, (0, None, None, None, None, table, refs, live))
-    _launch_with_workspace("kda_pages_compact_hip", a, device)
+    _launch_pages("kda_pages_compact_hip", a, device)
     return table, refs, live
