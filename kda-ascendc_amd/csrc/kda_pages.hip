@@ -168,12 +168,16 @@ __global__ __launch_bounds__(256) void pages_free_kernel(PagesParams p) {
 
 // ---- copies ----
 
-// Threads move 16 bytes each, COPY_UNROLL at a time: a work-group 16 KiB of
-// a page at most.
-constexpr int COPY_UNROLL = 4;
+// Threads move 16 bytes each, COPY_UNROLL at a time: a work-group 8 KiB of a
+// page at most (more in flight a thread was slower: a compaction that moves
+// 0.5 GB @COPY@).
+constexpr int COPY_UNROLL = 2;
 constexpr int COPY_BYTES = 256 * 16 * COPY_UNROLL;
 
-// Piece `seg` of page `src` of one pool's part `lead` to page `dst`.
+// Piece `seg` of page `src` of one pool's part `lead` to page `dst`.  What is
+// written is not read here again: stored past the caches, and with STREAM read
+// past them too (not for a fork, whose source others fork as well).
+template <bool STREAM>
 __device__ __forceinline__ void copy_piece(const PagesParams& p, const KdaPagePool& x, int64_t lead, int src, int dst,
                                            int64_t seg) {
     char* base = static_cast<char*>(x.data) + lead * p.P * x.page_bytes;
@@ -183,17 +187,21 @@ __device__ __forceinline__ void copy_piece(const PagesParams& p, const KdaPagePo
     u32x4 w[COPY_UNROLL];
 #pragma unroll
     for (int i = 0; i < COPY_UNROLL; ++i)
-        if (off + i * 4096 < x.page_bytes) w[i] = *reinterpret_cast<const u32x4*>(from + off + i * 4096);
+        if (off + i * 4096 < x.page_bytes) {
+            const u32x4* at = reinterpret_cast<const u32x4*>(from + off + i * 4096);
+            w[i] = STREAM ? __builtin_nontemporal_load(at) : *at;
+        }
 #pragma unroll
     for (int i = 0; i < COPY_UNROLL; ++i)
-        if (off + i * 4096 < x.page_bytes) *reinterpret_cast<u32x4*>(to + off + i * 4096) = w[i];
+        if (off + i * 4096 < x.page_bytes)
+            __builtin_nontemporal_store(w[i], reinterpret_cast<u32x4*>(to + off + i * 4096));
 }
 
 // Work items of all pools for `count` pairs: (pool, lead, pair, piece), pieces
 // innermost.
 __host__ __device__ inline int64_t pieces_of(const KdaPagePool& x) { return (x.page_bytes + COPY_BYTES - 1) / COPY_BYTES; }
 
-template <class Pair>
+template <bool STREAM, class Pair>
 __device__ __forceinline__ void copy_items(const PagesParams& p, int64_t count, Pair pair) {
     int64_t first = 0;
     for (int i = 0; i < p.num_pools; ++i) {
@@ -205,13 +213,13 @@ __device__ __forceinline__ void copy_items(const PagesParams& p, int64_t count, 
         for (; id < items; id += gridDim.x) {
             const int64_t pr = id / seg, lead = pr / count;
             int src, dst;
-            if (pair((int)(pr - lead * count), src, dst)) copy_piece(p, x, lead, src, dst, id - pr * seg);
+            if (pair((int)(pr - lead * count), src, dst)) copy_piece<STREAM>(p, x, lead, src, dst, id - pr * seg);
         }
         first += items;
     }
 }
 
-constexpr int COPY_GRID = 256 * 16;
+constexpr int COPY_GRID = 256 * 64;
 
 int copy_grid(const PagesParams& p, int64_t count) {
     int64_t items = 0;
@@ -220,7 +228,7 @@ int copy_grid(const PagesParams& p, int64_t count) {
 }
 
 __global__ __launch_bounds__(256) void pages_copy_kernel(PagesParams p) {
-    copy_items(p, p.F, [&](int i, int& src, int& dst) {
+    copy_items<true>(p, p.F, [&](int i, int& src, int& dst) {
         src = p.src[i];
         dst = p.dst[i];
         return (unsigned)src < (unsigned)p.P && (unsigned)dst < (unsigned)p.P;
@@ -308,7 +316,7 @@ __global__ __launch_bounds__(256) void pages_fork_copy_kernel(PagesParams p) {
     const int* fresh = whence + p.F;
     for (int i = blockIdx.x * 256 + threadIdx.x; i < p.F; i += gridDim.x * 256)
         if (fresh[i] >= 0) p.refs[fresh[i]] = 1;
-    copy_items(p, p.F, [&](int i, int& src, int& dst) {
+    copy_items<false>(p, p.F, [&](int i, int& src, int& dst) {
         src = whence[i];
         dst = fresh[i];
         return (unsigned)src < (unsigned)p.P && dst >= 0;
@@ -317,17 +325,23 @@ __global__ __launch_bounds__(256) void pages_fork_copy_kernel(PagesParams p) {
 
 // ---- compact ----
 
-// The held pages of each 4096: counts for the lists.
+// The held pages of each 4096: counts for the lists of a large pool.
 constexpr int LIST_PAGES = 4096;
+// Up to here every work-group of the lists counts all pages itself, 16 at a
+// time a thread: a launch less (256 pages, a compaction @COUNT@ us).
+constexpr int COUNT_PAGES = 16 * LIST_PAGES;
+__device__ __forceinline__ int held_of(const PagesParams& p, int i) {
+    int r[4], cnt = 0;
+    read_refs(p, i, r);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) cnt += i + j < p.P && r[j] != 0;
+    return cnt;
+}
 __global__ __launch_bounds__(1024) void pages_count_kernel(PagesParams p) {
     __shared__ int lds[16];
-    int r[4], total;
-    read_refs(p, blockIdx.x * LIST_PAGES + 4 * threadIdx.x, r);
-    int cnt = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) cnt += r[j] == 0;
-    block_scan<1024>(cnt, lds, total);
-    if (threadIdx.x == 0) p.ws[3 * (int64_t)p.P + blockIdx.x] = min(LIST_PAGES, p.P - blockIdx.x * LIST_PAGES) - total;
+    int total;
+    block_scan<1024>(held_of(p, blockIdx.x * LIST_PAGES + 4 * threadIdx.x), lds, total);
+    if (threadIdx.x == 0) p.ws[3 * (int64_t)p.P + blockIdx.x] = total;
 }
 
 // Free places below `live` (the number of held pages), held pages at or above
@@ -352,15 +366,25 @@ __global__ __launch_bounds__(1024) void pages_list_kernel(PagesParams p) {
     __shared__ int lds[16];
     const CompactLists x = compact_lists(p);
     const int tid = threadIdx.x;
-    int live = 0, before = 0;
-    for (int b0 = 0; b0 < x.blocks; b0 += 1024) {
-        int total;
-        const int c = b0 + tid < x.blocks ? x.counts[b0 + tid] : 0;
-        block_scan<1024>(b0 + tid < (int)blockIdx.x ? c : 0, lds, total);
-        before += total;
-        block_scan<1024>(c, lds, total);
-        live += total;
+    // held pages of the work-groups before, and of all
+    int mine = 0, all = 0;
+    if (p.P <= COUNT_PAGES) {
+#pragma unroll 4
+        for (int b = 0; b < x.blocks; ++b) {
+            const int c = held_of(p, b * LIST_PAGES + 4 * tid);
+            all += c;
+            mine += b < (int)blockIdx.x ? c : 0;
+        }
+    } else {
+        for (int b = tid; b < x.blocks; b += 1024) {
+            const int c = x.counts[b];
+            all += c;
+            mine += b < (int)blockIdx.x ? c : 0;
+        }
     }
+    int before, live;
+    block_scan<1024>(mine, lds, before);
+    block_scan<1024>(all, lds, live);
     int r[4], total, cnt = 0;
     const int i = blockIdx.x * LIST_PAGES + 4 * tid;
     read_refs(p, i, r);
@@ -403,7 +427,7 @@ __global__ __launch_bounds__(256) void pages_move_kernel(PagesParams p) {
         p.out_refs[x.holes[i]] = p.refs[from];
         p.out_refs[from] = 0;
     }
-    copy_items(p, places, [&](int i, int& src, int& dst) {
+    copy_items<true>(p, places, [&](int i, int& src, int& dst) {
         src = x.movers[places - 1 - i];
         dst = x.holes[i];
         return true;
@@ -447,9 +471,12 @@ hipError_t launch_pages_fork(const PagesParams& p, hipStream_t stream) {
 
 hipError_t launch_pages_compact(const PagesParams& p, hipStream_t stream) {
     const int blocks = compact_lists(p).blocks;
-    pages_count_kernel<<<blocks, 1024, 0, stream>>>(p);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    hipError_t e = hipSuccess;
+    if (p.P > COUNT_PAGES) {
+        pages_count_kernel<<<blocks, 1024, 0, stream>>>(p);
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
     pages_list_kernel<<<blocks, 1024, 0, stream>>>(p);
     e = hipGetLastError();
     if (e != hipSuccess) return e;

@@ -37,6 +37,7 @@ import torch
 from . import _hip, workspace
 from .kernels import _raw_stream, _require_gpu
 
+_CU_DTYPES = {torch.int32: _hip.DTYPE_I32, torch.int64: _hip.DTYPE_I64}
 _CACHE_DTYPES = {torch.bfloat16: _hip.PAGED_BF16, torch.float16: _hip.PAGED_FP16}
 
 
@@ -152,10 +153,10 @@ def _plain_table(table, lens, dev) -> bool:
     )
 
 
-def _plain_fields(k, v, table, lens, x, heads) -> tuple | None:
-    """The argument fields of an ordinary call without cu_seqlens on a GPU,
-    whose cache, table and new tokens ``x`` (``heads`` of them, 0: any) the
-    full checks accept, each tensor looked at once: a small call's time is the
+def _plain_fields(k, v, table, lens, x, heads, cu) -> tuple | None:
+    """The argument fields of an ordinary call on a GPU, whose cache, table,
+    new tokens ``x`` (``heads`` of them, 0: any) and offsets ``cu`` the full
+    checks accept, each tensor looked at once: a small call's time is the
     host's, and the checks in the order of their messages are half of it.  None
     says nothing: the full checks then accept or raise."""
     shape, s, t, dt, dev = k.shape, k.stride(), v.stride(), k.dtype, k.get_device()
@@ -171,12 +172,18 @@ def _plain_fields(k, v, table, lens, x, heads) -> tuple | None:
         dt in _CACHE_DTYPES and v.dtype is dt and x.dtype is dt and (D == 128 or D == 64) and size in _PAGE_SIZES
         and s3 == 1 and t3 == 1 and u3 == 1 and s0 > 0 and t0 > 0 and s1 >= D and s2 >= D and t1 >= D and t2 >= D
         and (s0 | s1 | s2 | t0 | t1 | t2 | u0 | u1 | u2) % 8 == 0 and (kp | vp | x.data_ptr()) % 16 == 0
-        and P > 0 and HKV > 0 and n[0] == rows[0] and n[3] == D and n[1] > 0
+        and P > 0 and HKV > 0 and n[0] == (rows[0] if cu is None else 1) and n[3] == D and n[1] > 0
         and (n[2] == heads if heads else n[2] > 0) and v.get_device() == dev and x.get_device() == dev
         and _plain_table(table, lens, dev)
     ):
         return None
-    return (rows[0], n[1], n[2], HKV, D, _CACHE_DTYPES[dt], P, size, rows[1], 0, 0, table.data_ptr(), rows[1],
+    cu_dtype = cu_ptr = 0
+    if cu is not None:
+        cu_dtype = _CU_DTYPES.get(cu.dtype)
+        if cu_dtype is None or cu.shape != (rows[0] + 1,) or not cu.is_contiguous() or cu.get_device() != dev:
+            return None
+        cu_ptr = cu.data_ptr()
+    return (rows[0], n[1], n[2], HKV, D, _CACHE_DTYPES[dt], P, size, rows[1], cu_dtype, cu_ptr, table.data_ptr(), rows[1],
             lens.data_ptr(), kp, vp, s0, s1, s2, t0, t1, t2, u0, u1, u2)
 
 
@@ -192,7 +199,7 @@ def _fields(k, v, table, lens, x, cu_seqlens) -> tuple:
     N, M = table.shape
     cu_dtype = cu = 0
     if cu_seqlens is not None:
-        cu_dtype = _hip.DTYPE_I64 if cu_seqlens.dtype == torch.int64 else _hip.DTYPE_I32
+        cu_dtype = _CU_DTYPES[cu_seqlens.dtype]
         cu = cu_seqlens.data_ptr()
     return (N, x.shape[1], x.shape[2], HKV, D, _CACHE_DTYPES[k.dtype], P, size, M, cu_dtype, cu, table.data_ptr(),
             table.stride(0) if N > 1 else M, lens.data_ptr(), k.data_ptr(), v.data_ptr(), *_strides(k), *_strides(v),
@@ -251,7 +258,7 @@ def paged_attention(
     ``seq_lens`` does not matter; keys and values before it have to be finite.
     Forward only: raises if q requires a gradient.
     """
-    f = _plain_fields(k_cache, v_cache, page_table, seq_lens, q, 0) if cu_seqlens is None else None
+    f = _plain_fields(k_cache, v_cache, page_table, seq_lens, q, 0, cu_seqlens)
     if f is None:
         _check_cache(k_cache, v_cache, page_table, seq_lens)
         _check_new("q", q, None, k_cache, page_table, cu_seqlens)
@@ -305,9 +312,9 @@ def paged_append(
     left out.
     """
     f = None
-    if cu_seqlens is None and v.shape == k.shape and v.stride() == k.stride() and v.dtype is k.dtype and (
+    if v.shape == k.shape and v.stride() == k.stride() and v.dtype is k.dtype and (
             v.data_ptr() % 16 == 0 and v.get_device() == k.get_device()):
-        f = _plain_fields(k_cache, v_cache, page_table, seq_lens, k, k_cache.shape[2])
+        f = _plain_fields(k_cache, v_cache, page_table, seq_lens, k, k_cache.shape[2], cu_seqlens)
     if f is None:
         _check_cache(k_cache, v_cache, page_table, seq_lens)
         for name, t in (("k", k), ("v", v)):
