@@ -127,12 +127,11 @@ typedef struct KdaPagesArgs {
     int32_t* out_table;        /* compact: [N, M] contiguous */
     int32_t* out_refs;         /* compact: [P] */
     int32_t* out_live;         /* compact: [1] */
-    void* workspace;           /* kda_pages_workspace_bytes() bytes, 256-byte aligned */
+    void* workspace;           /* compact: kda_pages_workspace_bytes() bytes, 256-byte aligned */
     size_t workspace_bytes;
 } KdaPagesArgs;
 
-/* Workspace of kda_pages_reserve_hip, kda_pages_fork_hip and
- * kda_pages_compact_hip (N, P and F read). */
+/* Workspace of kda_pages_compact_hip (P read). */
 size_t kda_pages_workspace_bytes(const KdaPagesArgs* args);
 
 /* Room for new_tokens[n] more tokens of every sequence n: the lowest free

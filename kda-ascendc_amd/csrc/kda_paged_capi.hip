@@ -210,16 +210,14 @@ int kda_paged_append_hip(const KdaPagedArgs* args, void* stream) {
 
 size_t kda_pages_workspace_bytes(const KdaPagesArgs* args) {
     if (args == nullptr || args->abi_version != KDA_PAGED_ABI_VERSION || args->P <= 0) return 0;
-    // Compact: three lists of pages and the counts of each 4096 (kda_pages.hip).  Reserve: a list and the
-    // sequences' first ranks.  Fork: its pairs.
-    const int64_t P = args->P, N = args->N > 0 ? args->N : 0, F = args->F > 0 ? args->F : 0;
-    const int64_t ints = 3 * P + P / 4096 + 2 + N + 2 * F;
+    // three lists of pages and the counts of each 4096 (kda_pages.hip)
+    const int64_t P = args->P, ints = 3 * P + P / 4096 + 2;
     return (size_t)((ints * 4 + 255) / 256 * 256);
 }
 
 int kda_pages_reserve_hip(const KdaPagesArgs* args, void* stream) {
     PagesParams p;
-    int rc = pages_params(args, p, TABLE | REFS | WS);
+    int rc = pages_params(args, p, TABLE | REFS);
     if (rc == KDA_BT16_OK) rc = pages_lens(args, p);
     if (rc != KDA_BT16_OK) return rc;
     if (!args->new_tokens || misaligned(args->new_tokens, 4) || !args->ok) return KDA_BT16_EINVAL;
@@ -239,7 +237,7 @@ int kda_pages_free_hip(const KdaPagesArgs* args, void* stream) {
 
 int kda_pages_fork_hip(const KdaPagesArgs* args, void* stream) {
     PagesParams p;
-    int rc = pages_params(args, p, POOLS | TABLE | REFS | SRC | DST | WS);
+    int rc = pages_params(args, p, POOLS | TABLE | REFS | SRC | DST);
     if (rc == KDA_BT16_OK) rc = pages_lens(args, p);
     if (rc != KDA_BT16_OK) return rc;
     if (p.F == 0) return KDA_BT16_OK;

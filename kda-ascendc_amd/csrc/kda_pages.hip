@@ -8,6 +8,8 @@
 #include "kda_common.h"
 #include "kda_paged.h"
 
+#include <algorithm>
+
 namespace kda {
 namespace {
 
@@ -92,16 +94,47 @@ __device__ __forceinline__ void read_refs(const PagesParams& p, int i, int (&r)[
     }
 }
 
+// Free pages from `from` on in rising order, by a whole work-group: calls
+// take(rank, page) for the first `want` of them (rank from 0) and returns how
+// many there are, at most `want`; `next`: where a later search goes on.
+template <int THREADS, class Take>
+__device__ __forceinline__ int find_free(const PagesParams& p, int from, int want, int* lds, int& next, Take take) {
+    constexpr int EACH = 4, STEP = THREADS * 4 * EACH;  // pages a thread and turn: 16, read together
+    int found = 0;
+    next = from;
+    for (int i0 = from; i0 < p.P && found < want; i0 += STEP) {
+        const int first = i0 + 4 * EACH * (int)threadIdx.x;
+        int r[EACH][4], cnt = 0, total;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) read_refs(p, first + 4 * e, r[e]);
+#pragma unroll
+        for (int j = 0; j < 4 * EACH; ++j) cnt += r[j >> 2][j & 3] == 0;
+        int at = found + block_scan<THREADS>(cnt, lds, total);
+#pragma unroll
+        for (int j = 0; j < 4 * EACH; ++j)
+            if (r[j >> 2][j & 3] == 0) {
+                if (at < want) take(at, first + j);
+                ++at;
+            }
+        found += total;
+        next = i0;
+    }
+    return min(found, want);
+}
+
 // ---- reserve ----
 
-// One work-group: the pages each sequence needs and their first rank among
-// all that are needed, the list of as many free pages, and their entries.
+// One work-group, SEQS sequences at a time: the first rank of each among the
+// pages that are needed; then, RANKS at a time, the free pages in order, each
+// to the entry that its rank falls to, a thread a rank.
+constexpr int SEQS = 4096, RANKS = 4096;
 __global__ __launch_bounds__(1024) void pages_reserve_kernel(PagesParams p) {
     __shared__ int lds[16];
-    int* list = p.ws;
-    int* rank = p.ws + p.P;
+    __shared__ int start[SEQS], had[SEQS];
+    __shared__ int list[RANKS];
     const int tid = threadIdx.x;
     const int64_t most = (int64_t)p.M << p.page_shift;
+    // pages that sequence n needs beyond those it has; -1: more than a row holds
     auto need_of = [&](int n, int& have) {
         const int len = max(0, p.lens[n]);
         have = pages_for(len, p.page_shift);
@@ -109,57 +142,70 @@ __global__ __launch_bounds__(1024) void pages_reserve_kernel(PagesParams p) {
         if (want > most) return -1;
         return max(0, pages_for((int)want, p.page_shift) - have);
     };
-    int needed = 0;
-    for (int n0 = 0; n0 < p.N; n0 += 1024) {
-        int have, total;
-        const int need = n0 + tid < p.N ? max(0, need_of(n0 + tid, have)) : 0;
-        const int before = block_scan<1024>(need, lds, total);
-        if (n0 + tid < p.N) rank[n0 + tid] = needed + before;
-        needed += total;
-    }
-    int found = 0;
-    for (int i0 = 0; i0 < p.P && found < needed; i0 += 4096) {
-        int r[4], total;
-        read_refs(p, i0 + 4 * tid, r);
-        int cnt = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) cnt += r[j] == 0;
-        int at = found + block_scan<1024>(cnt, lds, total);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (r[j] == 0) {
-                if (at < needed) list[at] = i0 + 4 * tid + j;
-                ++at;
+    int from = 0;
+    for (int n0 = 0; n0 < p.N; n0 += SEQS) {
+        const int count = min(SEQS, p.N - n0);
+        int needed = 0;
+        for (int i0 = 0; i0 < count; i0 += 1024) {
+            int have = 0, total;
+            const int need = i0 + tid < count ? max(0, need_of(n0 + i0 + tid, have)) : 0;
+            const int before = block_scan<1024>(need, lds, total);
+            if (i0 + tid < count) {
+                start[i0 + tid] = needed + before;
+                had[i0 + tid] = have;
             }
-        found += total;
-    }
-    __syncthreads();
-    // a wave a sequence: its entries
-    const int lane = tid & 63;
-    for (int n = tid >> 6; n < p.N; n += 16) {
-        int have;
-        const int need = need_of(n, have), start = rank[n];
-        const bool ok = need == 0 || (need > 0 && start + need <= found);
-        for (int i = lane; ok && i < need; i += 64) {
-            const int page = list[start + i];
-            p.table[n * p.table_stride + have + i] = page;
-            p.refs[page] = 1;
+            needed += total;
         }
-        if (lane == 0) {
-            if (ok) p.lens[n] = max(0, p.lens[n]) + max(0, p.more[n]);
+        int found = 0;
+        for (int base = 0; base < needed && found == base; base += RANKS) {
+            int next;
+            const int got = find_free<1024>(p, from, min(RANKS, needed - base), lds, next,
+                                            [&](int rank, int page) { list[rank] = page; });
+            from = next;
+            __syncthreads();
+            for (int k = tid; k < got; k += 1024) {
+                // the last sequence that starts at or before the rank (those
+                // without need start where the next one does)
+                int lo = 0, hi = count - 1;
+                while (lo < hi) {
+                    const int mid = (lo + hi + 1) >> 1;
+                    if (start[mid] <= base + k) lo = mid;
+                    else hi = mid - 1;
+                }
+                p.table[(n0 + lo) * p.table_stride + had[lo] + base + k - start[lo]] = list[k];
+                p.refs[list[k]] = 1;
+            }
+            found += got;
+            __syncthreads();
+        }
+        for (int i = tid; i < count; i += 1024) {
+            int have;
+            const int n = n0 + i, need = need_of(n, have);
+            const bool ok = need == 0 || (need > 0 && start[i] + need <= found);
+            if (ok) {
+                p.lens[n] = max(0, p.lens[n]) + max(0, p.more[n]);
+            } else if (need > 0) {
+                // pages ran out inside it: what it got goes back
+                for (int j = 0; start[i] + j < found; ++j) {
+                    int32_t* entry = p.table + n * p.table_stride + have + j;
+                    p.refs[*entry] = 0;
+                    *entry = -1;
+                }
+            }
             p.ok[n] = ok;
         }
+        __syncthreads();
     }
 }
 
 // ---- free ----
 
-__global__ __launch_bounds__(256) void pages_free_kernel(PagesParams p) {
+__global__ __launch_bounds__(512) void pages_free_kernel(PagesParams p) {
     const int n = p.dst[blockIdx.x];
     if ((unsigned)n >= (unsigned)p.N) return;
     int32_t* row = p.table + n * p.table_stride;
     // (the exchange: a row named twice gives its pages back once)
-    for (int i = threadIdx.x; i < p.M; i += 256) {
+    for (int i = threadIdx.x; i < p.M; i += 512) {
         const int page = atomicExch(row + i, -1);
         if ((unsigned)page < (unsigned)p.P) atomicSub(p.refs + page, 1);
     }
@@ -197,38 +243,38 @@ __device__ __forceinline__ void copy_piece(const PagesParams& p, const KdaPagePo
             __builtin_nontemporal_store(w[i], reinterpret_cast<u32x4*>(to + off + i * 4096));
 }
 
-// Work items of all pools for `count` pairs: (pool, lead, pair, piece), pieces
-// innermost.
 __host__ __device__ inline int64_t pieces_of(const KdaPagePool& x) { return (x.page_bytes + COPY_BYTES - 1) / COPY_BYTES; }
 
-template <bool STREAM, class Pair>
-__device__ __forceinline__ void copy_items(const PagesParams& p, int64_t count, Pair pair) {
-    int64_t first = 0;
+// Copies `count` pairs in all parts of all pools: (pool, part, pair, piece),
+// pieces innermost, so that the work-groups that run together are in one part
+// and finish whole pages (pair by pair, or a piece of every pair in turn, a
+// compaction that moves 0.5 GB took 196 us, so 187).
+template <class Pair>
+__device__ __forceinline__ void copy_pairs(const PagesParams& p, int64_t count, Pair pair) {
+    int64_t id = blockIdx.x;
     for (int i = 0; i < p.num_pools; ++i) {
         const KdaPagePool& x = p.pools[i];
         const int64_t seg = pieces_of(x), items = x.lead * count * seg;
-        // the first of this work-group's items in this pool
-        int64_t id = blockIdx.x - first % gridDim.x;
-        if (id < 0) id += gridDim.x;
         for (; id < items; id += gridDim.x) {
             const int64_t pr = id / seg, lead = pr / count;
             int src, dst;
-            if (pair((int)(pr - lead * count), src, dst)) copy_piece<STREAM>(p, x, lead, src, dst, id - pr * seg);
+            if (pair((int)(pr - lead * count), src, dst)) copy_piece<true>(p, x, lead, src, dst, id - pr * seg);
         }
-        first += items;
+        id -= items;
     }
 }
 
-constexpr int COPY_GRID = 256 * 64;
-
-int copy_grid(const PagesParams& p, int64_t count) {
-    int64_t items = 0;
-    for (int i = 0; i < p.num_pools; ++i) items += p.pools[i].lead * count * pieces_of(p.pools[i]);
-    return (int)(items < 1 ? 1 : (items > COPY_GRID ? COPY_GRID : items));
+int64_t copy_pieces(const PagesParams& p) {  // of a pair
+    int64_t pieces = 0;
+    for (int i = 0; i < p.num_pools; ++i) pieces += p.pools[i].lead * pieces_of(p.pools[i]);
+    return pieces;
+}
+unsigned copy_grid(const PagesParams& p, int64_t pairs) {
+    return (unsigned)std::min(std::max(copy_pieces(p) * pairs, (int64_t)1), (int64_t)256 * 64);
 }
 
 __global__ __launch_bounds__(256) void pages_copy_kernel(PagesParams p) {
-    copy_items<true>(p, p.F, [&](int i, int& src, int& dst) {
+    copy_pairs(p, p.F, [&](int i, int& src, int& dst) {
         src = p.src[i];
         dst = p.dst[i];
         return (unsigned)src < (unsigned)p.P && (unsigned)dst < (unsigned)p.P;
@@ -240,12 +286,11 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(PagesParams p) {
 // A work-group a fork.  Shared pages gain a holder, which makes no free page
 // of theirs, so that every work-group can look for its own free page while the
 // others count; the pages found are marked by the copy that follows.
-__global__ __launch_bounds__(256) void pages_fork_kernel(PagesParams p) {
-    __shared__ int lds[4];
-    __shared__ int found;
+constexpr int FORK_THREADS = 512;
+__global__ __launch_bounds__(FORK_THREADS) void pages_fork_kernel(PagesParams p) {
+    __shared__ int lds[FORK_THREADS / 64];
+    __shared__ int fresh;
     const int i = blockIdx.x, tid = threadIdx.x;
-    int* whence = p.ws;
-    int* fresh = whence + p.F;
     auto len_of = [&](int j) {
         const int s = p.src[j];
         if ((unsigned)s >= (unsigned)p.N) return 0;
@@ -257,42 +302,24 @@ __global__ __launch_bounds__(256) void pages_fork_kernel(PagesParams p) {
     const bool rows_ok = (unsigned)s < (unsigned)p.N && (unsigned)d < (unsigned)p.N;
     const int len = len_of(i), full = len >> p.page_shift;
     const bool part = rows_ok && (len & mask) != 0;
-    // the forks before it that need a page
-    int rank = 0;
-    for (int j0 = 0; j0 < i; j0 += 256) {
-        int total;
-        const int j = j0 + tid;
-        const bool need = j < i && (unsigned)p.dst[j] < (unsigned)p.N && (len_of(j) & mask) != 0;
-        block_scan<256>(need, lds, total);
-        rank += total;
-    }
-    if (tid == 0) found = -1;
-    __syncthreads();
+    if (tid == 0) fresh = -1;
     if (part) {
-        int seen = 0;
-        for (int i0 = 0; i0 < p.P && seen <= rank; i0 += 1024) {
-            int r[4], total;
-            read_refs(p, i0 + 4 * tid, r);
-            int cnt = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) cnt += r[j] == 0;
-            int at = seen + block_scan<256>(cnt, lds, total);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (r[j] == 0) {
-                    if (at == rank) found = i0 + 4 * tid + j;
-                    ++at;
-                }
-            seen += total;
-        }
+        // the forks before it that need a page
+        int before = 0, rank;
+        for (int j = tid; j < i; j += FORK_THREADS) before += (unsigned)p.dst[j] < (unsigned)p.N && (len_of(j) & mask) != 0;
+        block_scan<FORK_THREADS>(before, lds, rank);
+        int next;
+        find_free<FORK_THREADS>(p, 0, rank + 1, lds, next, [&](int at, int page) {
+            if (at == rank) fresh = page;
+        });
         __syncthreads();
     }
-    const int page = found;
+    const int page = part ? fresh : -1;
     const bool ok = rows_ok && (!part || page >= 0);
     if (ok) {
         const int32_t* from = p.table + s * p.table_stride;
         int32_t* to = p.table + d * p.table_stride;
-        for (int j = tid; j < p.M; j += 256) {
+        for (int j = tid; j < p.M; j += FORK_THREADS) {
             int x = -1;
             if (j < full) {
                 x = from[j];
@@ -306,21 +333,34 @@ __global__ __launch_bounds__(256) void pages_fork_kernel(PagesParams p) {
     if (tid == 0) {
         if (ok) p.lens[d] = len;
         p.ok[i] = ok;
-        whence[i] = ok && part ? p.table[s * p.table_stride + full] : -1;
-        fresh[i] = ok && part ? page : -1;
     }
 }
 
-__global__ __launch_bounds__(256) void pages_fork_copy_kernel(PagesParams p) {
-    const int* whence = p.ws;
-    const int* fresh = whence + p.F;
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < p.F; i += gridDim.x * 256)
-        if (fresh[i] >= 0) p.refs[fresh[i]] = 1;
-    copy_items<false>(p, p.F, [&](int i, int& src, int& dst) {
-        src = whence[i];
-        dst = fresh[i];
-        return (unsigned)src < (unsigned)p.P && dst >= 0;
-    });
+// Fork i's last page, if it has one of its own: from the rows that the fork
+// left.
+__device__ __forceinline__ bool forked_page(const PagesParams& p, int i, int& src, int& dst) {
+    if (!p.ok[i]) return false;
+    const int s = p.src[i], d = p.dst[i], len = p.lens[d], full = len >> p.page_shift;
+    if (len - (full << p.page_shift) == 0) return false;
+    src = p.table[s * p.table_stride + full];
+    dst = p.table[d * p.table_stride + full];
+    return (unsigned)dst < (unsigned)p.P;
+}
+// `share` work-groups a fork, which look its page up once and move every
+// share-th piece of it in all parts of all pools.
+__global__ __launch_bounds__(256) void pages_fork_copy_kernel(PagesParams p, int share) {
+    int src, dst;
+    const int f = blockIdx.x % p.F;
+    if (!forked_page(p, f, src, dst)) return;
+    int64_t piece = blockIdx.x / p.F;
+    if (piece == 0 && threadIdx.x == 0) p.refs[dst] = 1;
+    if ((unsigned)src >= (unsigned)p.P) return;
+    for (int i = 0; i < p.num_pools; ++i) {
+        const KdaPagePool& x = p.pools[i];
+        const int64_t seg = pieces_of(x), items = x.lead * seg;
+        for (; piece < items; piece += share) copy_piece<false>(p, x, piece / seg, src, dst, piece % seg);
+        piece -= items;
+    }
 }
 
 // ---- compact ----
@@ -427,7 +467,7 @@ __global__ __launch_bounds__(256) void pages_move_kernel(PagesParams p) {
         p.out_refs[x.holes[i]] = p.refs[from];
         p.out_refs[from] = 0;
     }
-    copy_items<true>(p, places, [&](int i, int& src, int& dst) {
+    copy_pairs(p, places, [&](int i, int& src, int& dst) {
         src = x.movers[places - 1 - i];
         dst = x.holes[i];
         return true;
@@ -452,7 +492,7 @@ hipError_t launch_pages_reserve(const PagesParams& p, hipStream_t stream) {
 }
 
 hipError_t launch_pages_free(const PagesParams& p, hipStream_t stream) {
-    pages_free_kernel<<<p.F, 256, 0, stream>>>(p);
+    pages_free_kernel<<<p.F, 512, 0, stream>>>(p);
     return hipGetLastError();
 }
 
@@ -462,10 +502,13 @@ hipError_t launch_pages_copy(const PagesParams& p, hipStream_t stream) {
 }
 
 hipError_t launch_pages_fork(const PagesParams& p, hipStream_t stream) {
-    pages_fork_kernel<<<p.F, 256, 0, stream>>>(p);
+    pages_fork_kernel<<<p.F, FORK_THREADS, 0, stream>>>(p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    pages_fork_copy_kernel<<<copy_grid(p, p.F), 256, 0, stream>>>(p);
+    // a piece each where there are few, up to 4 where there are many
+    const int64_t pieces = copy_pieces(p), each = std::min(std::max(pieces * p.F / 2048, (int64_t)1), (int64_t)4);
+    const int64_t share = std::min((pieces + each - 1) / each, std::max((int64_t)256 * 64 / p.F, (int64_t)1));
+    pages_fork_copy_kernel<<<dim3((unsigned)(share * p.F)), 256, 0, stream>>>(p, (int)share);
     return hipGetLastError();
 }
 

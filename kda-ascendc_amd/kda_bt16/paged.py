@@ -387,11 +387,6 @@ def _check_refs(page_refs, device) -> None:
         raise ValueError("page_refs must be 16-byte aligned")
 
 
-def _launch_pages(name: str, args: bytes, device) -> None:
-    """A call on the pages that takes a workspace."""
-    _launch_in(name, args, _hip.lib().kda_pages_workspace_bytes(args + _hip.NO_WORKSPACE), device)
-
-
 def _check_rows(pairs, device) -> None:
     dev = device.index
     if dev is not None:
@@ -435,7 +430,7 @@ def paged_reserve(
     ok = torch.empty(seq_lens.shape[0], dtype=torch.bool, device=device)
     a = _pages_args(page_refs.shape[0], (), page_table, seq_lens, page_refs, page_size,
                     (0, None, None, new_tokens, ok))
-    _launch_pages("kda_pages_reserve_hip", a, device)
+    _launch("kda_pages_reserve_hip", a + _hip.NO_WORKSPACE, device)
     return ok
 
 
@@ -489,7 +484,7 @@ def paged_fork(
     _require_gpu(ts[0])
     ok = torch.empty(src.shape[0], dtype=torch.bool, device=device)
     a = _pages_args(P, ts, page_table, seq_lens, page_refs, page_size, (src.shape[0], src, dst, None, ok))
-    _launch_pages("kda_pages_fork_hip", a, device)
+    _launch("kda_pages_fork_hip", a + _hip.NO_WORKSPACE, device)
     return ok
 
 
@@ -540,5 +535,5 @@ def paged_compact(
     refs = torch.empty_like(page_refs)
     live = torch.empty(1, dtype=torch.int32, device=device)
     a = _pages_args(P, ts, page_table, None, page_refs, 16, (0, None, None, None, None, table, refs, live))
-    _launch_pages("kda_pages_compact_hip", a, device)
+    _launch_in("kda_pages_compact_hip", a, _hip.lib().kda_pages_workspace_bytes(a + _hip.NO_WORKSPACE), device)
     return table, refs, live
