@@ -348,12 +348,12 @@ __device__ __forceinline__ FewSpans few_spans(const PagedParams& p, const Cut& c
 }
 
 // Many rows.  Row tiles are taken whole where they are enough to fill the
-// card, else their keys are cut into parts: S = ceil(all tiles / SLOTS), at
-// least LEAST, and t / S parts (rounded down: all parts then run at once).
+// card, else the keys of one with t tiles are cut into t * SLOTS / all parts,
+// all being the tiles of all (rounded down: the parts of all then number at
+// most SLOTS and run at once), of LEAST tiles at least.
 // Sequence by sequence, a sequence's row tiles last first (those of a causal
 // chunk see the most keys), then its parts, heads innermost: work-groups go
 // round the XCDs, so that with 8 heads each XCD's L2 has the keys of one.
-// Parts of cut row tiles number at most SLOTS.
 struct ManyWork {
     int mt = 0, tiles = 0;  // row tiles, and tiles of keys that one sees at most
     NewTokens s;
@@ -377,9 +377,8 @@ __device__ __forceinline__ ManyWork many_work(const PagedParams& p, int n) {
 // Work-group (JOIN: row tile, its parts' first place and number) `id`'s part.
 template <bool JOIN>
 __device__ __forceinline__ bool many_unit(const PagedParams& p, int id, bool cut, int lane, Unit& u, int& parts) {
-    int S = 0x7fffffff;
+    int64_t all = 0;
     if (cut) {
-        int64_t all = 0;
         for (int n0 = 0; n0 < p.N; n0 += 64) {
             const ManyWork w = many_work(p, n0 + lane);
             int64_t x = (int64_t)w.mt * w.tiles;
@@ -387,13 +386,14 @@ __device__ __forceinline__ bool many_unit(const PagedParams& p, int id, bool cut
             for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
             all += x;
         }
-        const int64_t share = (all * p.HKV + Shape<MANY>::SLOTS - 1) / Shape<MANY>::SLOTS;
-        S = __builtin_amdgcn_readfirstlane((int)min((int64_t)S, max((int64_t)Shape<MANY>::LEAST, share)));
+        all *= p.HKV;
     }
     int slots = 0;
     for (int n0 = 0; n0 < p.N; n0 += 64) {
         const ManyWork w = many_work(p, n0 + lane);
-        const int np = max(1, w.tiles / S);
+        const int np = cut && w.tiles >= 2 * Shape<MANY>::LEAST
+                           ? max(1, min(w.tiles / Shape<MANY>::LEAST, (int)((int64_t)w.tiles * Shape<MANY>::SLOTS / all)))
+                           : 1;
         const uint32_t end = wave_prefix(w.mt * p.HKV * (JOIN ? 1 : np), lane);
         const uint32_t slot_end = wave_prefix(np > 1 ? w.mt * p.HKV * np : 0, lane);
         const int total = __builtin_amdgcn_readlane(end, 63);
@@ -913,9 +913,9 @@ __device__ __forceinline__ void join(const PagedParams& p, const Unit& u, int gr
     if (p.lse && piece == 0) p.lse[out] = log_sum(mx, sum);
 }
 
-// A work-group a row tile (few rows: `few_groups` of them).
+// `few_groups` or `many_groups` work-groups a row tile.
 template <class E, int D, int KIND>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int few, int few_groups, bool cut_many) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int few, int few_groups, int many_groups, bool cut_many) {
     __shared__ float lds[KIND == MANY ? 1 : 6 * 256];
     const int lane = threadIdx.x & 63;
     Unit u;
@@ -950,8 +950,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int few,
         }
     } else {
         int parts;
-        if (!many_unit<true>(p, (int)blockIdx.x - few, cut_many, lane, u, parts) || parts == 1) return;
-        for (int group = 0; group < Shape<MANY>::MT * (D / 4) / 256; ++group)
+        const int x = (int)blockIdx.x - few;
+        if (!many_unit<true>(p, x / many_groups, cut_many, lane, u, parts) || parts == 1) return;
+        const int items = min(Shape<MANY>::MT, u.s.count * p.G - u.m * Shape<MANY>::MT) * (D / 4);
+        for (int group = x % many_groups; group * 256 < items; group += many_groups)
             join<E, D, MANY>(p, u, group, parts, [&](int j) {
                 return Partial<MANY, D>::at(p.ws + few_floats<D>(), u.slot + j);
             }, lds);
@@ -998,8 +1000,9 @@ hipError_t launch(const PagedParams& p, hipStream_t stream) {
     const int64_t rows = p.cu_seqlens || (int64_t)p.T * p.G > ROWS ? ROWS : p.T * p.G;
     const int groups = (int)std::min((rows * (D / 4) + 63) / 64, (int64_t)4);
     const int64_t few_joins = fc ? (int64_t)p.N * p.HKV * groups : 0;
-    const int64_t many_joins = mc ? units : 0;
-    paged_join_kernel<E, D, KIND><<<dim3((unsigned)(few_joins + many_joins)), 256, 0, stream>>>(p, (int)few_joins, groups, mc);
+    const int many_groups = (int)std::min(std::max((int64_t)1024 / std::max(units, (int64_t)1), (int64_t)1), (int64_t)Shape<MANY>::MT * (D / 4) / 256);
+    const int64_t many_joins = mc ? units * many_groups : 0;
+    paged_join_kernel<E, D, KIND><<<dim3((unsigned)(few_joins + many_joins)), 256, 0, stream>>>(p, (int)few_joins, groups, many_groups, mc);
     return hipGetLastError();
 }
 
