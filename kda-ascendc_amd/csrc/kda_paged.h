@@ -24,7 +24,7 @@ struct PagedParams {
     const int32_t* seq_lens;
     uint16_t* k;
     uint16_t* v;
-    uint32_t k_page, v_page;    // below 2^31
+    uint32_t k_page, v_page;    // below 2^31 (bytes in 32 bits)
     int32_t k_token, v_token;   // a page of one head spans less than 2^30
     int64_t k_head, v_head;
     const uint16_t* q;

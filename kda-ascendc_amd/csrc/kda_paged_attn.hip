@@ -112,34 +112,6 @@ __device__ __forceinline__ uint32_t lds_address(const uint8_t* p) {
     return (uint32_t)reinterpret_cast<uintptr_t>((lds_u8*)p);
 }
 
-// What a wave loads of a tile: NROWS keys (or values) of one head, all of one
-// page, 1 KiB a load.
-template <int D, int NROWS, bool STREAM>
-struct Loader {
-    static constexpr int PIECES = D / 8, R = 64 / PIECES, LOADS = NROWS / R;
-    uint64_t head;            // byte address of the head in page 0
-    uint32_t page_bytes, token_bytes;
-    int off[LOADS];           // this lane's bytes of each load, within the rows
-    // row0: the first row's place in its 16.
-    __device__ __forceinline__ Loader(const uint16_t* cache, uint32_t page_stride, int token, int64_t h, int row0, int lane)
-        : head(reinterpret_cast<uint64_t>(cache + h)), page_bytes(page_stride), token_bytes(token * 2) {
-#pragma unroll
-        for (int j = 0; j < LOADS; ++j) {
-            const int row = j * R + lane / PIECES;
-            off[j] = row * (int)token_bytes + (((lane & (PIECES - 1)) ^ swizzle<D>(row0 + row)) << 4);
-        }
-    }
-    // Rows `in` on of a page (an entry of the table) to LDS: `rows` of them
-    // exist, the others become zeros (the descriptor ends with the last one).
-    __device__ __forceinline__ void load(const PagedParams& p, int page, int in, int rows, uint32_t lds) const {
-        const int n = is_page(p, page) ? min(rows, NROWS) : 0;
-        const uint64_t at = head + ((uint64_t)(n > 0 ? (uint32_t)page : 0u) * page_bytes << 1) + (uint32_t)in * token_bytes;
-        const u32x4 rsrc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, n > 0 ? (n - 1) * token_bytes + D * 2 : 0u, BUF_RAW};
-#pragma unroll
-        for (int j = 0; j < LOADS; ++j) load_lds<STREAM>(rsrc, off[j], lds + j * 1024);
-    }
-};
-
 // Operand of the first product: rows lane & 31, elements 16 * s + 8 * (lane >> 5) .. +7.
 template <int D>
 __device__ __forceinline__ u32x4 read_k(const uint8_t* lds, int row, int piece) {
@@ -247,16 +219,17 @@ __device__ __forceinline__ uint32_t wave_prefix(uint32_t x, int lane) {  // incl
     return x;
 }
 
-// Row tile m of (sequence n, kv head h), and which of its tiles of keys
-// [begin, end); `slot`: its place in the workspace, or -1 where these are all.
+// Row tile m of (sequence n, kv head h), the keys [lo, hi) that any of its rows
+// sees, and which of their tiles [begin, end); `slot`: its place in the
+// workspace, or -1 where these are all.
 struct Unit {
-    int n, h, m, begin, end, slot;
+    int n, h, m, lo, hi, begin, end, slot;
     NewTokens s;
 };
 
-// The tiles of keys that rows [m * MT, m * MT + MT) of a sequence see.
+// The keys that rows [m * MT, m * MT + MT) of a sequence see, and their tiles.
 struct Tiles {
-    int begin, end;
+    int lo, hi, begin, end;
 };
 template <int KIND>
 __device__ __forceinline__ Tiles tiles_of(const PagedParams& p, const NewTokens& s, int m) {
@@ -265,7 +238,7 @@ __device__ __forceinline__ Tiles tiles_of(const PagedParams& p, const NewTokens&
     const int first = m * MT / p.G, last = (min(rows, m * MT + MT) - 1) / p.G;
     const int hi = p.causal ? max(0, min(s.pos + last + 1, s.len)) : s.len;
     const int lo = p.window ? min(hi, max(0, s.pos + first + 1 - p.window)) : 0;
-    return {lo / TK, max(lo / TK, (hi + TK - 1) / TK)};
+    return {lo, hi, lo / TK, max(lo / TK, (hi + TK - 1) / TK)};
 }
 
 // Lane `at`'s.
@@ -417,6 +390,8 @@ __device__ __forceinline__ bool many_unit(const PagedParams& p, int id, bool cut
             u.s = of_lane(w.s, at);
             const Tiles t = tiles_of<MANY>(p, u.s, u.m);
             const int64_t count = t.end - t.begin;
+            u.lo = t.lo;
+            u.hi = t.hi;
             u.begin = t.begin + (int)(count * part / parts);
             u.end = t.begin + (int)(count * (part + 1) / parts);
             return true;
@@ -467,6 +442,38 @@ __device__ __forceinline__ void load_q(const PagedParams& p, const Unit& u, cons
     for (int s = 0; s < D / 16; ++s) q[s] = *reinterpret_cast<const u32x4*>(at + 16 * s + 8 * half);
 }
 
+// What a wave loads of a tile: NROWS keys (or values) of one head, all of one
+// page, 1 KiB a load.
+template <int D, int NROWS, bool STREAM>
+struct Loader {
+    static constexpr int PIECES = D / 8, R = 64 / PIECES, LOADS = NROWS / R;
+    uint64_t head;            // byte address of the head in page 0
+    uint32_t page_bytes, token_bytes;
+    int off[LOADS];           // this lane's bytes of each load, within the rows
+    // row0: the first row's place in its 16.
+    __device__ __forceinline__ Loader(const uint16_t* cache, uint32_t page_stride, int token, int64_t h, int row0, int lane)
+        : head(reinterpret_cast<uint64_t>(cache + h)), page_bytes(page_stride * 2), token_bytes(token * 2) {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int row = j * R + lane / PIECES;
+            off[j] = row * (int)token_bytes + (((lane & (PIECES - 1)) ^ swizzle<D>(row0 + row)) << 4);
+        }
+    }
+    // Keys `key` on, of a page (an entry of the table), to LDS.  Keys past the
+    // last that the row tile sees become zeros (the descriptor ends with it),
+    // and so do all where it sees none of them or there is no page: whatever
+    // pages hold beyond a sequence, or had before its window, does not reach
+    // the products.
+    __device__ __forceinline__ void load(const PagedParams& p, const Unit& u, int page, int key, uint32_t lds) const {
+        const int n = is_page(p, page) && key + NROWS > u.lo ? min(u.hi - key, NROWS) : 0;
+        const int in = key & ((1 << p.page_shift) - 1);
+        const uint64_t at = head + (uint64_t)(n > 0 ? (uint32_t)page : 0u) * page_bytes + (uint32_t)in * token_bytes;
+        const u32x4 rsrc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, n > 0 ? (n - 1) * token_bytes + D * 2 : 0u, BUF_RAW};
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) load_lds<STREAM>(rsrc, off[j], lds + j * 1024);
+    }
+};
+
 // This wave's LDS reads have returned: what they read may be loaded over.
 __device__ __forceinline__ void reads_done() {
     __builtin_amdgcn_sched_barrier(0);
@@ -496,13 +503,11 @@ __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, ui
     constexpr int TILE = TK * D * 2;
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const Row x = row_of(p, u, u.m * ROWS + (lane & 31));
-    const Tiles tl = {u.begin, u.end};
     const float c = p.scale * LOG2E;
 
-    int t = tl.begin + wave;
+    int t = u.begin + wave;
     const Loader<D, 16, true> k0(p.k, p.k_page, p.k_token, u.h * p.k_head, 0, lane);
     const Loader<D, 16, true> v0(p.v, p.v_page, p.v_token, u.h * p.v_head, 0, lane);
-    const int in_page = (1 << p.page_shift) - 1;
     int pages[2], next[2];  // of the tile's first and second 16 keys
     auto look_up = [&](int tile, int (&pg)[2]) {
 #pragma unroll
@@ -512,11 +517,11 @@ __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, ui
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             const int key = tile * TK + 16 * g;
-            from.load(p, pg[g], key & in_page, u.s.len - key, lds_address(to) + g * (TILE / 2));
+            from.load(p, u, pg[g], key, lds_address(to) + g * (TILE / 2));
         }
     };
     look_up(t, pages);
-    if (t < tl.end) {
+    if (t < u.end) {
         load(k0, t, pages, kw);
         load(v0, t, pages, vw);
     }
@@ -526,20 +531,20 @@ __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, ui
     // (once here, where the compiler sees it: else it waits for q in every turn)
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0
     constexpr int LOADS = TILE / 1024;  // of a tile of keys, or of values
-    for (; t < tl.end; t += WAVES) {
+    for (; t < u.end; t += WAVES) {
         f32x16 st[1] = {f32x16{}};
         wait_loads<LOADS>();  // but for the values'
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) st[0] = E::mfma(read_k<D>(kw, lane & 31, 2 * s + half), q[s], st[0]);
         reads_done();
-        if (t + WAVES < tl.end) load(k0, t + WAVES, next, kw);
+        if (t + WAVES < u.end) load(k0, t + WAVES, next, kw);
         u32x4 pt[2];
         float alpha;
         if (softmax_tile<E, 1>(st, t * TK + 4 * half, x.lo, x.hi, true, c, run, pt, alpha)) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) acc[d] *= alpha;
         }
-        if (t + WAVES < tl.end) wait_loads<LOADS>();  // but for the next keys'
+        if (t + WAVES < u.end) wait_loads<LOADS>();  // but for the next keys'
         else wait_loads<0>();
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
@@ -551,7 +556,7 @@ __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, ui
             }
         }
         reads_done();
-        if (t + WAVES < tl.end) load(v0, t + WAVES, next, vw);
+        if (t + WAVES < u.end) load(v0, t + WAVES, next, vw);
         look_up(t + 2 * WAVES, next);
     }
     run.l = sum_halves(run.l);
@@ -642,9 +647,11 @@ __device__ __forceinline__ void few_piece(const PagedParams& p, int b, bool may_
             u.m = 0;
             u.s = of_lane(x.s, at);
             const uint32_t t = in - u.h * span, stop = min(span, t + (end - cur));
-            const int t0 = tiles_of<FEW>(p, u.s, 0).begin;
-            u.begin = t0 + t;
-            u.end = t0 + min(c, stop);
+            const Tiles all = tiles_of<FEW>(p, u.s, 0);
+            u.lo = all.lo;
+            u.hi = all.hi;
+            u.begin = all.begin + t;
+            u.end = all.begin + min(c, stop);
             u.slot = t == 0 && stop >= c ? -1 : 2 * b + (cur == first ? 0 : 1);
             if (cur != first) __syncthreads();  // the last row tile's join is over
             few_rows<E, D>(p, u, lds, joint);
@@ -700,12 +707,11 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
     const Loader<D, SHARE, false> k0(p.k, p.k_page, p.k_token, u.h * p.k_head, SHARE * wave & 15, lane);
     const Loader<D, SHARE, false> v0(p.v, p.v_page, p.v_token, u.h * p.v_head, SHARE * wave & 15, lane);
     const uint32_t k_lds = lds_address(kt) + wave * (SHARE * D * 2), v_lds = lds_address(vt) + wave * (SHARE * D * 2);
-    const int in_page = (1 << p.page_shift) - 1;
     auto look_up = [&](int t) { return table_entry(p, u.n, ((u.begin + t) * TK + SHARE * wave) >> p.page_shift); };
     auto load = [&](const Loader<D, SHARE, false>& from, int t, int page, uint32_t to) {
         if (t >= count) return;
         const int key = (u.begin + t) * TK + SHARE * wave;
-        from.load(p, page, key & in_page, u.s.len - key, to);
+        from.load(p, u, page, key, to);
     };
     // Table entries of tiles t + 1 and t + 2 as the softmax of t begins.
     int page1 = look_up(0), page2 = look_up(1);

@@ -190,6 +190,27 @@ def test_strided_queries_and_rows(gpu_device):
     assert (o.double().cpu() - want).abs().max() <= _tol(BF16)
 
 
+@pytest.mark.parametrize("T", [1, 5, 150])
+def test_pages_before_the_window_may_be_gone(T, gpu_device):
+    """A window's cache lets pages go once every query is past them: their
+    entries may be -1, or pages that hold anything by now."""
+    dev, page, window = gpu_device, 16, 70
+    lens = [T + 90, T + 333, T + 1000, T + 16]
+    (kc, vc), _, table, ln, gen = make(lens, 2, 128, page, BF16, dev)
+    q = torch.randn(4, T, 8, 128, generator=gen).to(BF16)
+    want, want_lse = oracle.attention(q, kc, vc, table, ln, 0.1, window=window)
+    for n, L in enumerate(lens):
+        gone = max(0, L - T + 1 - window) // page
+        for j in range(gone):
+            kc[int(table[n, j])], vc[int(table[n, j])] = math.nan, math.inf
+            if j % 2:
+                table[n, j] = -1
+    o, lse = paged_attention(q.to(dev), kc.to(dev), vc.to(dev), table.to(dev), ln.to(dev), scale=0.1, window=window,
+                             return_lse=True)
+    assert (o.double().cpu() - want).abs().max() <= _tol(BF16)
+    assert (lse.double().cpu() - want_lse).abs().max() <= 1e-4
+
+
 def test_attention_repeats_its_bits(gpu_device):
     dev = gpu_device
     _, (dk, dv), table, ln, gen = make([3000, 17, 901], 2, 128, 16, BF16, dev)
