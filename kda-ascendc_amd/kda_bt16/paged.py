@@ -262,8 +262,6 @@ def paged_attention(
     if f is None:
         _check_cache(k_cache, v_cache, page_table, seq_lens)
         _check_new("q", q, None, k_cache, page_table, cu_seqlens)
-        _require_gpu(q)
-        f = _fields(k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
     B, T, HQ, D = q.shape
     HKV = k_cache.shape[2]
     if HQ % HKV != 0:
@@ -279,6 +277,9 @@ def paged_attention(
             raise ValueError("window needs causal=True")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise NotImplementedError("paged_attention is forward only: inputs require grad")
+    if f is None:
+        _require_gpu(q)
+        f = _fields(k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
     device = q.device
     o = torch.empty((B, T, HQ, D), dtype=q.dtype, device=device)
     lse = torch.empty((B, T, HQ), dtype=torch.float32, device=device) if return_lse else None
