@@ -281,7 +281,7 @@ def paged_attention(
         _require_gpu(q)
         f = _fields(k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
     device = q.device
-    o = torch.empty((B, T, HQ, D), dtype=q.dtype, device=device)
+    o = torch.empty_like(q) if q.is_contiguous() else torch.empty((B, T, HQ, D), dtype=q.dtype, device=device)
     lse = torch.empty((B, T, HQ), dtype=torch.float32, device=device) if return_lse else None
     (N, T, HQ, HKV, D, dt, P, size, M, cu_dtype, cu, table, table_stride, lens, kp, vp, s0, s1, s2, t0, t1, t2, u0, u1,
      u2) = f
@@ -347,7 +347,7 @@ def _pools(pools) -> list[torch.Tensor]:
             raise ValueError(f"pool {i} dimensions must be positive, got shape {tuple(t.shape)}")
         if t.shape[-4] != P:
             raise ValueError(f"pool {i} must have {P} pages like the first, got {t.shape[-4]}")
-        if t.device != ts[0].device:
+        if i > 0 and t.device != ts[0].device:
             raise ValueError(f"pool {i} device {t.device} must match the first's ({ts[0].device})")
         if t.data_ptr() % 16 or t.stride(-4) * t.element_size() % 16:
             raise ValueError(f"pool {i} must be 16-byte aligned, its pages multiples of 16 bytes")
@@ -357,27 +357,22 @@ def _pools(pools) -> list[torch.Tensor]:
 _NO_POOLS = (0,) * (3 * _hip.PAGED_MAX_POOLS)
 
 
-def _pages_args(P, pools=(), page_table=None, seq_lens=None, page_refs=None, page_size=16, rest=()) -> bytes:
-    """The packed arguments of a call on the pages, up to the workspace;
-    ``rest`` from ``F`` on: F, then src, dst, new_tokens, ok, out_table,
-    out_refs, out_live as tensors or None, as many as there are."""
-    N = M = stride = table = 0
-    if page_table is not None:
-        N, M = page_table.shape
-        table, stride = page_table.data_ptr(), page_table.stride(0) if N > 1 else M
-    arr = _NO_POOLS
-    if pools:
-        arr = []
-        for t in pools:
-            size = t.element_size()
-            page = t.stride(-4) * size
-            arr += (t.data_ptr(), t.numel() * size // (P * page), page)
-        arr += _NO_POOLS[len(arr):]
-    tail = [0 if t is None else t.data_ptr() for t in rest[1:]]
-    tail += [0] * (7 - len(tail))
+def _pool_fields(pools, P) -> tuple:
+    out = ()
+    for t in pools:
+        size = t.element_size()
+        page = t.stride(-4) * size
+        out += (t.data_ptr(), t.numel() * size // (P * page), page)
+    return out + _NO_POOLS[len(out):]
+
+
+def _pack(P, page_size, F, num_pools, pools, table, table_stride=0, N=0, M=0, lens=0, refs=0, src=0, dst=0, more=0, ok=0,
+          out_table=0, out_refs=0, out_live=0) -> bytes:
+    """The packed arguments of a call on the pages, up to the workspace
+    (pointers, 0 for none)."""
     return _hip.PAGES_PACK.pack(
-        _hip.PAGED_ABI_VERSION, N, M, P, page_size, rest[0], len(pools), 0, *arr, table, stride,
-        0 if seq_lens is None else seq_lens.data_ptr(), 0 if page_refs is None else page_refs.data_ptr(), *tail)
+        _hip.PAGED_ABI_VERSION, N, M, P, page_size, F, num_pools, 0, *pools, table, table_stride, lens, refs, src, dst,
+        more, ok, out_table, out_refs, out_live)
 
 
 def _check_refs(page_refs, device) -> None:
@@ -389,25 +384,29 @@ def _check_refs(page_refs, device) -> None:
 
 
 def _check_rows(pairs, device) -> None:
-    dev = device.index
-    if dev is not None:
-        n = pairs[0][1].shape
-        if len(n) == 1 and all(t.shape == n and t.dtype is torch.int32 and t.is_contiguous() and t.get_device() == dev
-                               for _, t in pairs):
-            return
     for name, t in pairs:
         _int32(name, t, 1, device)
         if t.shape[0] != pairs[0][1].shape[0]:
             raise ValueError(f"{name} must have {pairs[0][1].shape[0]} entries like {pairs[0][0]}, got {t.shape[0]}")
 
 
-def _check_counts(page_table, seq_lens, page_refs) -> torch.device:
-    """Table, lengths and counts of one cache; their device."""
-    device = page_table.device
-    if not (page_table.is_cuda and _plain_table(page_table, seq_lens, page_table.get_device())):
-        _check_table(page_table, seq_lens, device)
-    _check_refs(page_refs, device)
-    return device
+def _plain_rows(a, b, dev) -> bool:
+    """Whether these are ordinary int32 rows on GPU ``dev`` that
+    :func:`_check_rows` accepts (as for :func:`_plain_fields`)."""
+    n = a.shape
+    return (len(n) == 1 and b.shape == n and a.dtype is torch.int32 and b.dtype is torch.int32 and a.get_device() == dev
+            and b.get_device() == dev and a.is_contiguous() and b.is_contiguous())
+
+
+def _check_counts(page_table, seq_lens, page_refs) -> int:
+    """Table, lengths and counts of one cache; their GPU, -1 for none."""
+    dev = page_table.get_device()
+    if not (dev >= 0 and _plain_table(page_table, seq_lens, dev) and page_refs.dtype is torch.int32
+            and page_refs.ndim == 1 and page_refs.get_device() == dev and page_refs.is_contiguous()
+            and page_refs.data_ptr() % 16 == 0 and page_refs.shape[0] > 0):
+        _check_table(page_table, seq_lens, page_table.device)
+        _check_refs(page_refs, page_table.device)
+    return dev
 
 
 def paged_reserve(
@@ -424,14 +423,17 @@ def paged_reserve(
     Returns a bool ``[N]``: False for a sequence whose pages cannot all be
     had, or do not fit its row; it keeps what it has.
     """
-    device = _check_counts(page_table, seq_lens, page_refs)
-    _check_rows([("seq_lens", seq_lens), ("new_tokens", new_tokens)], device)
+    dev = _check_counts(page_table, seq_lens, page_refs)
+    if not _plain_rows(seq_lens, new_tokens, dev):
+        _check_rows([("seq_lens", seq_lens), ("new_tokens", new_tokens)], page_table.device)
     _check_page_size(page_size)
     _require_gpu(page_table)
-    ok = torch.empty(seq_lens.shape[0], dtype=torch.bool, device=device)
-    a = _pages_args(page_refs.shape[0], (), page_table, seq_lens, page_refs, page_size,
-                    (0, None, None, new_tokens, ok))
-    _launch("kda_pages_reserve_hip", a + _hip.NO_WORKSPACE, device)
+    ok = seq_lens.new_empty(seq_lens.shape[0], dtype=torch.bool)
+    N, M = page_table.shape
+    _launch("kda_pages_reserve_hip", _pack(
+        page_refs.shape[0], page_size, 0, 0, _NO_POOLS, page_table.data_ptr(), page_table.stride(0) if N > 1 else M, N, M,
+        seq_lens.data_ptr(), page_refs.data_ptr(), 0, 0, new_tokens.data_ptr(), ok.data_ptr()) + _hip.NO_WORKSPACE,
+        page_table.device)
     return ok
 
 
@@ -443,11 +445,15 @@ def paged_free(
 ) -> None:
     """The sequences ``rows`` (int32) end: their pages lose a holder each,
     their entries become -1, their lengths 0."""
-    device = _check_counts(page_table, seq_lens, page_refs)
-    _check_rows([("rows", rows)], device)
+    dev = _check_counts(page_table, seq_lens, page_refs)
+    if not _plain_rows(rows, rows, dev):
+        _check_rows([("rows", rows)], page_table.device)
     _require_gpu(page_table)
-    _launch("kda_pages_free_hip", _pages_args(page_refs.shape[0], (), page_table, seq_lens, page_refs, 16,
-                                              (rows.shape[0], None, rows)) + _hip.NO_WORKSPACE, device)
+    N, M = page_table.shape
+    _launch("kda_pages_free_hip", _pack(
+        page_refs.shape[0], 16, rows.shape[0], 0, _NO_POOLS, page_table.data_ptr(),
+        page_table.stride(0) if N > 1 else M, N, M, seq_lens.data_ptr(), page_refs.data_ptr(), 0, rows.data_ptr())
+        + _hip.NO_WORKSPACE, page_table.device)
 
 
 def paged_fork(
@@ -474,18 +480,23 @@ def paged_fork(
     """
     ts = _pools(pools)
     device = ts[0].device
-    if _check_counts(page_table, seq_lens, page_refs) != device:
+    dev = _check_counts(page_table, seq_lens, page_refs)
+    if dev != ts[0].get_device():
         raise ValueError(f"page_table device {page_table.device} must match ({device})")
-    _check_rows([("src", src), ("dst", dst)], device)
+    if not _plain_rows(src, dst, dev):
+        _check_rows([("src", src), ("dst", dst)], device)
     page_size = ts[0].shape[-3] if page_size is None else page_size
     _check_page_size(page_size)
-    P = ts[0].shape[-4]
+    P, F = ts[0].shape[-4], src.shape[0]
     if page_refs.shape[0] != P:
         raise ValueError(f"page_refs must have one entry a page, {P}, got {page_refs.shape[0]}")
     _require_gpu(ts[0])
-    ok = torch.empty(src.shape[0], dtype=torch.bool, device=device)
-    a = _pages_args(P, ts, page_table, seq_lens, page_refs, page_size, (src.shape[0], src, dst, None, ok))
-    _launch("kda_pages_fork_hip", a + _hip.NO_WORKSPACE, device)
+    ok = src.new_empty(F, dtype=torch.bool)
+    N, M = page_table.shape
+    _launch("kda_pages_fork_hip", _pack(
+        P, page_size, F, len(ts), _pool_fields(ts, P), page_table.data_ptr(), page_table.stride(0) if N > 1 else M, N, M,
+        seq_lens.data_ptr(), page_refs.data_ptr(), src.data_ptr(), dst.data_ptr(), 0, ok.data_ptr()) + _hip.NO_WORKSPACE,
+        device)
     return ok
 
 
@@ -500,10 +511,12 @@ def paged_copy(pools, src: torch.Tensor, dst: torch.Tensor) -> None:
     """
     ts = _pools(pools)
     device = ts[0].device
-    _check_rows([("src", src), ("dst", dst)], device)
+    if not _plain_rows(src, dst, ts[0].get_device()):
+        _check_rows([("src", src), ("dst", dst)], device)
     _require_gpu(ts[0])
-    _launch("kda_pages_copy_hip", _pages_args(ts[0].shape[-4], ts, rest=(src.shape[0], src, dst))
-            + _hip.NO_WORKSPACE, device)
+    P = ts[0].shape[-4]
+    _launch("kda_pages_copy_hip", _pack(P, 16, src.shape[0], len(ts), _pool_fields(ts, P), 0, src=src.data_ptr(),
+                                        dst=dst.data_ptr()) + _hip.NO_WORKSPACE, device)
 
 
 def paged_compact(
@@ -532,9 +545,11 @@ def paged_compact(
     if page_refs.shape[0] != P:
         raise ValueError(f"page_refs must have one entry a page, {P}, got {page_refs.shape[0]}")
     _require_gpu(ts[0])
-    table = torch.empty(page_table.shape, dtype=torch.int32, device=device)
+    N, M = page_table.shape
+    table = torch.empty_like(page_table) if page_table.is_contiguous() else page_table.new_empty((N, M))
     refs = torch.empty_like(page_refs)
-    live = torch.empty(1, dtype=torch.int32, device=device)
-    a = _pages_args(P, ts, page_table, None, page_refs, 16, (0, None, None, None, None, table, refs, live))
-    _launch_in("kda_pages_compact_hip", a, _hip.lib().kda_pages_workspace_bytes(a + _hip.NO_WORKSPACE), device)
+    live = page_refs.new_empty(1)
+    args = _pack(P, 16, 0, len(ts), _pool_fields(ts, P), page_table.data_ptr(), page_table.stride(0) if N > 1 else M, N, M,
+                 0, page_refs.data_ptr(), out_table=table.data_ptr(), out_refs=refs.data_ptr(), out_live=live.data_ptr())
+    _launch_in("kda_pages_compact_hip", args, _hip.lib().kda_pages_workspace_bytes(args + _hip.NO_WORKSPACE), device)
     return table, refs, live
