@@ -210,15 +210,6 @@ __device__ __forceinline__ bool softmax_tile(f32x16 (&st)[NB], int key0, int lo,
 
 // ---- the work and its split ----
 
-__device__ __forceinline__ uint32_t wave_prefix(uint32_t x, int lane) {  // inclusive
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
-    return x;
-}
-
 // Row tile m of (sequence n, kv head h), the keys [lo, hi) that any of its rows
 // sees, and which of their tiles [begin, end); `slot`: its place in the
 // workspace, or -1 where these are all.
@@ -293,7 +284,7 @@ __device__ __forceinline__ Cut few_cut(const PagedParams& p, bool cut, int lane)
             c.first = x;
             c.s0 = s;
         }
-        all += (uint32_t)__builtin_amdgcn_readlane(wave_prefix(x, lane), 63);
+        all += (uint32_t)__builtin_amdgcn_readlane(wave_prefix(x), 63);
         units += __popcll(__ballot(x > 0));
     }
     c.tiles = all * p.HKV;
@@ -316,7 +307,7 @@ __device__ __forceinline__ FewSpans few_spans(const PagedParams& p, const Cut& c
     x.tiles = cut.first;
     if (n0 > 0) x.tiles = few_tiles(p, n0 + lane, x.s);
     x.span = cut.span(x.tiles);
-    x.upto = wave_prefix(x.span * p.HKV, lane);
+    x.upto = wave_prefix(x.span * p.HKV);
     return x;
 }
 
@@ -367,11 +358,11 @@ __device__ __forceinline__ bool many_unit(const PagedParams& p, int id, bool cut
         const int np = cut && w.tiles >= 2 * Shape<MANY>::LEAST
                            ? max(1, min(w.tiles / Shape<MANY>::LEAST, (int)((int64_t)w.tiles * Shape<MANY>::SLOTS / all)))
                            : 1;
-        const uint32_t end = wave_prefix(w.mt * p.HKV * (JOIN ? 1 : np), lane);
-        const uint32_t slot_end = wave_prefix(np > 1 ? w.mt * p.HKV * np : 0, lane);
+        const int end = wave_prefix(w.mt * p.HKV * (JOIN ? 1 : np));
+        const int slot_end = wave_prefix(np > 1 ? w.mt * p.HKV * np : 0);
         const int total = __builtin_amdgcn_readlane(end, 63);
         if (id < total) {
-            const int at = __builtin_ctzll(__ballot((int)end > id));
+            const int at = __builtin_ctzll(__ballot(end > id));
             const int before = at > 0 ? __builtin_amdgcn_readlane(end, at - 1) : 0;
             const int slot0 = slots + (at > 0 ? __builtin_amdgcn_readlane(slot_end, at - 1) : 0);
             const int mt = __builtin_amdgcn_readlane(w.mt, at);

@@ -51,20 +51,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedParams p, int to
 
 // ---- scans ----
 
-__device__ __forceinline__ int wave_scan(int x, int lane) {  // inclusive
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
-    return x;
-}
-
 // Exclusive prefix sum over the work-group's threads, and the total.
 template <int THREADS>
 __device__ __forceinline__ int block_scan(int x, int* lds, int& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int inc = wave_scan(x, lane);
+    const int inc = wave_prefix(x);
     __syncthreads();
     if (lane == 63) lds[wave] = inc;
     __syncthreads();
