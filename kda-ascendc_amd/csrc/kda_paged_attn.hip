@@ -523,31 +523,41 @@ __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, ui
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0
     constexpr int LOADS = TILE / 1024;  // of a tile of keys, or of values
     for (; t < u.end; t += WAVES) {
-        f32x16 st[1] = {f32x16{}};
+        const bool more = t + WAVES < u.end;
+        // All operands of a product are read before it, so that its place is
+        // loaded again while it runs.
         wait_loads<LOADS>();  // but for the values'
+        u32x4 ka[STEPS];
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) st[0] = E::mfma(read_k<D>(kw, lane & 31, 2 * s + half), q[s], st[0]);
+        for (int s = 0; s < STEPS; ++s) ka[s] = read_k<D>(kw, lane & 31, 2 * s + half);
         reads_done();
-        if (t + WAVES < u.end) load(k0, t + WAVES, next, kw);
+        if (more) load(k0, t + WAVES, next, kw);
+        f32x16 st[1] = {f32x16{}};
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) st[0] = E::mfma(ka[s], q[s], st[0]);
+        if (more) wait_loads<LOADS>();  // but for the next keys'
+        else wait_loads<0>();
+        u32x4 va[2][DB];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const u32x2 a = read_v<D>(vw, 16 * k + 4 * half, d, lane);
+                const u32x2 b = read_v<D>(vw, 16 * k + 8 + 4 * half, d, lane);
+                va[k][d] = u32x4{a.x, a.y, b.x, b.y};
+            }
+        reads_done();
+        if (more) load(v0, t + WAVES, next, vw);
         u32x4 pt[2];
         float alpha;
         if (softmax_tile<E, 1>(st, t * TK + 4 * half, x.lo, x.hi, true, c, run, pt, alpha)) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) acc[d] *= alpha;
         }
-        if (t + WAVES < u.end) wait_loads<LOADS>();  // but for the next keys'
-        else wait_loads<0>();
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const u32x2 a = read_v<D>(vw, 16 * k + 4 * half, d, lane);
-                const u32x2 b = read_v<D>(vw, 16 * k + 8 + 4 * half, d, lane);
-                acc[d] = E::mfma(u32x4{a.x, a.y, b.x, b.y}, pt[k], acc[d]);
-            }
-        }
-        reads_done();
-        if (t + WAVES < u.end) load(v0, t + WAVES, next, vw);
+            for (int d = 0; d < DB; ++d) acc[d] = E::mfma(va[k][d], pt[k], acc[d]);
         look_up(t + 2 * WAVES, next);
     }
     run.l = sum_halves(run.l);
