@@ -159,7 +159,8 @@ __device__ __forceinline__ float sum_halves(float x) {
 // (any m does as long as nothing overflows: weights stay at most 2^8, and fp32
 // sums and 16-bit weights keep their relative precision), so that the rescaling
 // of O, 64 multiplications a lane against the softmax's ~130 operations, is
-// rare after the first tiles.
+// rare after the first tiles (a prompt of 8192 tokens: 557 us when m follows
+// every growth, 522 so).
 constexpr float GROWTH = 8.f;
 struct Running {
     float m = -INFINITY;  // -inf: no key seen yet
@@ -258,7 +259,6 @@ __device__ __forceinline__ bool of_kind(const PagedParams& p, const NewTokens& s
 // !cut: row tiles whole, each filled up to a piece of FEW_WHOLE keys, which
 // no row of the table exceeds.
 constexpr int FEW_WHOLE = 24 * Shape<FEW>::TK;
-constexpr uint32_t FEW_UNITS = Shape<FEW>::SLOTS / 4;
 struct Cut {
     uint32_t tiles, size;
     bool filled;
@@ -274,7 +274,9 @@ __device__ __forceinline__ int few_tiles(const PagedParams& p, int n, NewTokens&
     const Tiles t = tiles_of<FEW>(p, s, 0);
     return max(1, t.end - t.begin);
 }
-__device__ __forceinline__ Cut few_cut(const PagedParams& p, bool cut, int lane) {
+// `slots`: the work-groups that run at once (half as many where they have twice
+// the waves).
+__device__ __forceinline__ Cut few_cut(const PagedParams& p, bool cut, uint32_t slots, int lane) {
     Cut c;
     uint32_t all = 0, units = 0;
     for (int n0 = 0; n0 < p.N; n0 += 64) {
@@ -289,8 +291,8 @@ __device__ __forceinline__ Cut few_cut(const PagedParams& p, bool cut, int lane)
     }
     c.tiles = all * p.HKV;
     units *= p.HKV;
-    c.filled = !cut || units <= FEW_UNITS;
-    const uint32_t pieces = c.filled ? Shape<FEW>::SLOTS - units : Shape<FEW>::SLOTS;
+    c.filled = !cut || units <= slots / 4;
+    const uint32_t pieces = c.filled ? slots - units : slots;
     c.size = cut ? max((uint32_t)Shape<FEW>::LEAST, (c.tiles + pieces - 1) / pieces) : FEW_WHOLE / Shape<FEW>::TK;
     c.size = __builtin_amdgcn_readfirstlane(c.size);
     return c;
@@ -324,7 +326,7 @@ struct ManyWork {
 };
 __device__ __forceinline__ ManyWork many_work(const PagedParams& p, int n) {
     constexpr int MT = Shape<MANY>::MT, TK = Shape<MANY>::TK;
-    ManyWork w;
+    ManyWork w = {};
     if (n >= p.N) return w;
     const NewTokens s = new_tokens(p, n);
     if (!of_kind<MANY>(p, s)) return w;
@@ -338,9 +340,27 @@ __device__ __forceinline__ ManyWork many_work(const PagedParams& p, int n) {
     }
     return w;
 }
+// The lanes' sequences in the order of their tiles, most first, so that the
+// longest row tiles do not start last (16 sequences of 512 new tokens after
+// 1000 to 23000: 1027 us in their own order, 987 so): the lane's sequence then.
+__device__ __forceinline__ int longest_first(const PagedParams& p, ManyWork& w, int lane) {
+    int rank = 0;
+    for (int j = 0; j < p.N; ++j) {
+        const int t = __builtin_amdgcn_readlane(w.tiles, j);
+        rank += t > w.tiles || (t == w.tiles && j < lane);
+    }
+    if (lane >= p.N) rank = lane;
+    const int from = __builtin_amdgcn_ds_permute(rank << 2, lane);
+    auto take = [&](int x) { return __builtin_amdgcn_ds_bpermute(from << 2, x); };
+    w.mt = take(w.mt);
+    w.tiles = take(w.tiles);
+    w.s = {take(w.s.first), take(w.s.count), take(w.s.len), take(w.s.pos)};
+    return from;
+}
 // Work-group (JOIN: row tile, its parts' first place and number) `id`'s part.
+// `sort` (up to 64 sequences): the sequences that see the most keys first.
 template <bool JOIN>
-__device__ __forceinline__ bool many_unit(const PagedParams& p, int id, bool cut, int lane, Unit& u, int& parts) {
+__device__ __forceinline__ bool many_unit(const PagedParams& p, int id, bool cut, bool sort, int lane, Unit& u, int& parts) {
     int64_t all = 0;
     if (cut) {
         for (int n0 = 0; n0 < p.N; n0 += 64) {
@@ -354,7 +374,9 @@ __device__ __forceinline__ bool many_unit(const PagedParams& p, int id, bool cut
     }
     int slots = 0;
     for (int n0 = 0; n0 < p.N; n0 += 64) {
-        const ManyWork w = many_work(p, n0 + lane);
+        ManyWork w = many_work(p, n0 + lane);
+        int seq = n0 + lane;
+        if (sort) seq = longest_first(p, w, lane);
         const int np = cut && w.tiles >= 2 * Shape<MANY>::LEAST
                            ? max(1, min(w.tiles / Shape<MANY>::LEAST, (int)((int64_t)w.tiles * Shape<MANY>::SLOTS / all)))
                            : 1;
@@ -367,7 +389,7 @@ __device__ __forceinline__ bool many_unit(const PagedParams& p, int id, bool cut
             const int slot0 = slots + (at > 0 ? __builtin_amdgcn_readlane(slot_end, at - 1) : 0);
             const int mt = __builtin_amdgcn_readlane(w.mt, at);
             parts = __builtin_amdgcn_readlane(np, at);
-            u.n = __builtin_amdgcn_readfirstlane(n0 + at);
+            u.n = __builtin_amdgcn_readlane(seq, at);
             int x = id - before;
             u.h = x % p.HKV;
             x /= p.HKV;
@@ -483,14 +505,14 @@ __device__ __forceinline__ float log_sum(float mc, float l) {
 
 // ---- few rows ----
 
-// Each wave goes over every fourth tile of 32 keys, through LDS of its own:
+// Each wave goes over every WAVES-th tile of 32 keys, through LDS of its own:
 // while it multiplies keys the values arrive, and the other way round.  The
-// four waves' sums are joined at the end, in the same LDS (2 * TILE bytes a
+// waves' sums are joined at the end, in the same LDS (2 * TILE bytes a
 // wave: a tile of keys, one of values; 32 rows of D floats).
-template <class E, int D>
+template <class E, int D, int WAVES>
 __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, uint8_t* kw, uint8_t* vw, int wave,
                                          Running& run, f32x16 (&acc)[D / 32]) {
-    constexpr int STEPS = D / 16, DB = D / 32, TK = Shape<FEW>::TK, WAVES = Shape<FEW>::WAVES;
+    constexpr int STEPS = D / 16, DB = D / 32, TK = Shape<FEW>::TK;
     constexpr int TILE = TK * D * 2;
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const Row x = row_of(p, u, u.m * ROWS + (lane & 31));
@@ -563,16 +585,29 @@ __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, ui
     run.l = sum_halves(run.l);
 }
 
-template <class E, int D>
-__device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, uint8_t* lds, float* joint) {
-    constexpr int DB = D / 32, TILE = Shape<FEW>::TK * D * 2, WAVES = Shape<FEW>::WAVES;
+// A wave's place in LDS: of four waves in one array; of eight, three in either
+// ring of the many rows' kernel and two in an array of their own.
+template <int D, int WAVES>
+struct FewLds {
+    uint8_t *a, *b, *c;
+    __device__ __forceinline__ uint8_t* of(int wave) const {
+        constexpr int EACH = 2 * Shape<FEW>::TK * D * 2;
+        if (WAVES == 4 || wave < 3) return a + wave * EACH;
+        return wave < 6 ? b + (wave - 3) * EACH : c + (wave - 6) * EACH;
+    }
+};
+
+template <class E, int D, int WAVES>
+__device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, const FewLds<D, WAVES>& lds, float* joint) {
+    constexpr int DB = D / 32, TILE = Shape<FEW>::TK * D * 2;
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Running run;
     f32x16 acc[DB];
 #pragma unroll
     for (int i = 0; i < DB; ++i) acc[i] = f32x16{};
-    few_loop<E, D>(p, u, lds + wave * (2 * TILE), lds + wave * (2 * TILE) + TILE, wave, run, acc);
+    uint8_t* mine = lds.of(wave);
+    few_loop<E, D, WAVES>(p, u, mine, mine + TILE, wave, run, acc);
 
     // Join: every wave's m and l, then its O over the tiles' LDS, row by row
     // in pieces of four (the rows' pieces turned by the row, so that the lanes
@@ -583,7 +618,7 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, ui
         joint[wave * 2 * ROWS + ROWS + row] = run.l;
     }
     __syncthreads();
-    float* own = reinterpret_cast<float*>(lds + wave * (2 * TILE));
+    float* own = reinterpret_cast<float*>(mine);
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -594,7 +629,7 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, ui
         }
     __syncthreads();
     float* part = u.slot >= 0 ? Partial<FEW, D>::at(p.ws, u.slot) : nullptr;
-    for (int e = threadIdx.x; e < ROWS * (D / 4); e += 256) {
+    for (int e = threadIdx.x; e < ROWS * (D / 4); e += WAVES * 64) {
         const int r = e / (D / 4), piece = e % (D / 4);
         const Row y = row_of(p, u, u.m * ROWS + r);
         if (!y.live) break;
@@ -608,7 +643,7 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, ui
         for (int w = 0; w < WAVES; ++w) {
             const float f = fast_exp2(joint[w * 2 * ROWS + r] - sub);
             sum = fmaf(f, joint[w * 2 * ROWS + ROWS + r], sum);
-            const float* src = reinterpret_cast<const float*>(lds + w * (2 * TILE));
+            const float* src = reinterpret_cast<const float*>(lds.of(w));
             const f32x4 v = *reinterpret_cast<const f32x4*>(src + r * D + ((piece + r) & (D / 4 - 1)) * 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = fmaf(f, v[i], o[i]);
@@ -629,10 +664,11 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, ui
 }
 
 // Work-group b's piece of the cut, row tile by row tile.
-template <class E, int D>
-__device__ __forceinline__ void few_piece(const PagedParams& p, int b, bool may_cut, uint8_t* lds, float* joint) {
+template <class E, int D, int WAVES>
+__device__ __forceinline__ void few_piece(const PagedParams& p, int b, bool may_cut, uint32_t slots,
+                                          const FewLds<D, WAVES>& lds, float* joint) {
     const int lane = threadIdx.x & 63;
-    const Cut cut = few_cut(p, may_cut, lane);
+    const Cut cut = few_cut(p, may_cut, slots, lane);
     const uint32_t first = b * cut.size, end = first + cut.size;
     uint32_t cur = first, base = 0;
     for (int n0 = 0; n0 < p.N && cur < end; n0 += 64) {
@@ -655,7 +691,7 @@ __device__ __forceinline__ void few_piece(const PagedParams& p, int b, bool may_
             u.end = all.begin + min(c, stop);
             u.slot = t == 0 && stop >= c ? -1 : 2 * b + (cur == first ? 0 : 1);
             if (cur != first) __syncthreads();  // the last row tile's join is over
-            few_rows<E, D>(p, u, lds, joint);
+            few_rows<E, D, WAVES>(p, u, lds, joint);
             cur += stop - t;
         }
         base += total;
@@ -674,8 +710,12 @@ __device__ __forceinline__ void meet() {
 // Eight waves, two on each SIMD, in two groups: while one group's waves form
 // products (phase M: O += V^T P^T of the last tile, S of this one) the other
 // group's do the softmax of theirs (phase S), and they meet after each phase.
-// Left to themselves the two waves of a SIMD fell into step, each pipe idle
-// half of the time (@PINGPONG@).
+// Left to themselves (two work-groups of four waves a CU) the two waves of a
+// SIMD fell into step, the matrix unit busy 48% of the cycles: a prompt of 8192
+// tokens, 32 / 8 heads, 558 us, so 521.  What bounds it now is the rate of the
+// products themselves: with the softmax left out, and with the LDS reads left
+// out too, 470 and 439 us (1.25 PFLOP/s; a bf16 product of 8192^3 reaches 1.15
+// to 1.2 on the same card).
 //   slot     2t             2t + 1         2t + 2
 //   group 0  M(t)           S(t)           M(t + 1)
 //   group 1  S(t - 1)       M(t)           S(t)
@@ -848,16 +888,28 @@ template <class E, int D>
 __global__ __launch_bounds__(256, 2) void paged_few_kernel(PagedParams p, bool cut) {
     __shared__ alignas(1024) uint8_t lds[Shape<FEW>::WAVES * 2 * Shape<FEW>::TK * D * 2];
     __shared__ float joint[Shape<FEW>::WAVES * 2 * ROWS];
-    few_piece<E, D>(p, blockIdx.x, cut, lds, joint);
+    few_piece<E, D, Shape<FEW>::WAVES>(p, blockIdx.x, cut, Shape<FEW>::SLOTS, {lds, nullptr, nullptr}, joint);
 }
 
-template <class E, int D>
-__global__ __launch_bounds__(512, 2) void paged_many_kernel(PagedParams p, bool cut) {
-    __shared__ alignas(1024) uint8_t kt[3 * Shape<MANY>::TK * D * 2];
-    __shared__ alignas(1024) uint8_t vt[3 * Shape<MANY>::TK * D * 2];
+// MIXED: the work-groups from `few_from` on take the sequences of few rows, with
+// as many waves: packed batches of chunks and single tokens in one launch, the
+// few rows on the CUs that the chunks' last row tiles leave (63 sequences of a
+// new token and one of 512: 316 us in two launches, 247 so; 8 sequences of 1 to
+// 1024 new tokens, a window of 4096: 144 and 140).
+template <class E, int D, bool MIXED_KINDS>
+__global__ __launch_bounds__(512, 2) void paged_many_kernel(PagedParams p, bool cut, bool sort, unsigned few_from, bool few_may_cut) {
+    constexpr int WAVES = Shape<MANY>::WAVES, RING = 3 * Shape<MANY>::TK * D * 2;
+    __shared__ alignas(1024) uint8_t kt[RING];
+    __shared__ alignas(1024) uint8_t vt[RING];
+    __shared__ alignas(1024) uint8_t more[MIXED_KINDS ? 2 * 2 * Shape<FEW>::TK * D * 2 : 16];
+    __shared__ float joint[MIXED_KINDS ? WAVES * 2 * ROWS : 1];
+    if (MIXED_KINDS && blockIdx.x >= few_from) {
+        few_piece<E, D, WAVES>(p, blockIdx.x - few_from, few_may_cut, Shape<MANY>::SLOTS, {kt, vt, more}, joint);
+        return;
+    }
     Unit u;
     int parts;
-    if (many_unit<false>(p, blockIdx.x, cut, threadIdx.x & 63, u, parts)) many_rows<E, D>(p, u, kt, vt);
+    if (many_unit<false>(p, blockIdx.x, cut, sort, threadIdx.x & 63, u, parts)) many_rows<E, D>(p, u, kt, vt);
 }
 
 // Joins the partial results of one row tile: four elements of a row a thread,
@@ -928,7 +980,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int few,
     Unit u;
     if (KIND == FEW || (KIND == MIXED && (int)blockIdx.x < few)) {
         const int id = blockIdx.x / few_groups;
-        const Cut cut = few_cut(p, true, lane);
+        const Cut cut = few_cut(p, true, KIND == MIXED ? Shape<MANY>::SLOTS : Shape<FEW>::SLOTS, lane);
         u.n = id / p.HKV;
         u.h = id - u.n * p.HKV;
         u.m = 0;
@@ -958,7 +1010,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int few,
     } else {
         int parts;
         const int x = (int)blockIdx.x - few;
-        if (!many_unit<true>(p, x / many_groups, cut_many, lane, u, parts) || parts == 1) return;
+        if (!many_unit<true>(p, x / many_groups, cut_many, false, lane, u, parts) || parts == 1) return;
         const int items = min(Shape<MANY>::MT, u.s.count * p.G - u.m * Shape<MANY>::MT) * (D / 4);
         for (int group = x % many_groups; group * 256 < items; group += many_groups)
             join<E, D, MANY>(p, u, group, parts, [&](int j) {
@@ -984,8 +1036,10 @@ int64_t many_units(const PagedParams& p) {
 }
 
 // Whether a row tile's keys may go to several work-groups.  Few rows: not where
-// the table's rows hold so few keys that the join costs more (@WHOLE@).  Many
-// rows: row tiles that fill half of SLOTS are taken whole.
+// the table's rows hold so few keys that the join, a launch more, costs more:
+// one sequence of 704 keys 11.9 us whole and 10.4 cut, but the host's part 10.1
+// against 14.1; 64 of 700 keys 32.8 whole and 35.4 cut.  Many rows: row tiles
+// that fill half of SLOTS are taken whole.
 bool may_cut(const PagedParams& p, int kind) {
     const int64_t keys = (int64_t)p.M << p.page_shift;
     if (kind == FEW) return keys > FEW_WHOLE;
@@ -997,10 +1051,15 @@ hipError_t launch(const PagedParams& p, hipStream_t stream) {
     const bool fc = KIND != MANY && may_cut(p, FEW), mc = KIND != FEW && may_cut(p, MANY);
     const int64_t units = KIND == FEW ? 0 : many_units(p);
     // (uncut: one piece a row tile)
-    if (KIND != MANY)
-        paged_few_kernel<E, D><<<dim3((unsigned)(fc ? Shape<FEW>::SLOTS : (int64_t)p.N * p.HKV)), 256, 0, stream>>>(p, fc);
-    if (KIND != FEW)
-        paged_many_kernel<E, D><<<dim3((unsigned)(units + (mc ? Shape<MANY>::SLOTS : 0))), 512, 0, stream>>>(p, mc);
+    const int64_t whole = (int64_t)p.N * p.HKV;
+    if constexpr (KIND == FEW) {
+        paged_few_kernel<E, D><<<dim3((unsigned)(fc ? Shape<FEW>::SLOTS : whole)), 256, 0, stream>>>(p, fc);
+    } else {
+        const int64_t many = units + (mc ? Shape<MANY>::SLOTS : 0);
+        const int64_t few = KIND == MANY ? 0 : (fc ? Shape<MANY>::SLOTS : whole);
+        const bool sort = p.N > 1 && p.N <= 64 && units > Shape<MANY>::SLOTS;
+        paged_many_kernel<E, D, KIND == MIXED><<<dim3((unsigned)(many + few)), 512, 0, stream>>>(p, mc, sort, (unsigned)many, fc);
+    }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !(fc || mc)) return e;
     // work-groups a row tile: one for every 64 fours of what rows there can be, up to 4

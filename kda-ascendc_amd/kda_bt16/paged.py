@@ -286,7 +286,8 @@ def paged_attention(
     (N, T, HQ, HKV, D, dt, P, size, M, cu_dtype, cu, table, table_stride, lens, kp, vp, s0, s1, s2, t0, t1, t2, u0, u1,
      u2) = f
     args = _hip.PAGED_PACK.pack(
-        _hip.PAGED_ABI_VERSION, N, T, HQ, HKV, D, dt, P, size, M, _hip.PAGED_CAUSAL if causal else 0, window or 0, scale,
+        _hip.PAGED_ABI_VERSION, N, T, HQ, HKV, D, dt, P, size, M, _hip.PAGED_CAUSAL if causal else 0,
+        min(window or 0, 1 << 30), scale,
         cu_dtype, cu, table, table_stride, lens, kp, vp, s0, s1, s2, t0, t1, t2, q.data_ptr(), u0, u1, u2, o.data_ptr(),
         0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0)
     nbytes = _hip.lib().kda_paged_attn_workspace_bytes(args + _hip.NO_WORKSPACE)
