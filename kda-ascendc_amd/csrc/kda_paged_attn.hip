@@ -88,6 +88,9 @@ __device__ __forceinline__ int swizzle(int row) {
 // cannot tell the tiles of a ring apart and would wait, before any LDS read,
 // for every such load under way.  So nothing but wait_loads() waits for it;
 // it has no result in registers, and other loads' waits only become longer.
+// The wait states: a buffer load may follow the lane read that wrote its
+// descriptor's registers by 5, which the compiler sees to only for loads it
+// knows.  Nothing else in these kernels uses m0.
 // STREAM: for what is read once, past the caches' lines of other work (the
 // decode step of 64 sequences of 3024 tokens, 32 / 8 heads: 141 us without,
 // 124 us with, 6.4 TB/s; a long chunk's keys, read again by other work-groups,
@@ -95,11 +98,11 @@ __device__ __forceinline__ int swizzle(int row) {
 template <bool STREAM>
 __device__ __forceinline__ void load_lds(u32x4 rsrc, int off, uint32_t lds) {
     if constexpr (STREAM)
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds" ::"v"(off), "s"(rsrc),
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds" ::"v"(off), "s"(rsrc),
                      "s"(lds)
                      : "memory");
     else
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc),
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc),
                      "s"(lds)
                      : "memory");
 }

@@ -196,7 +196,8 @@ int kda_paged_append_hip(const KdaPagedArgs* args, void* stream) {
         !strides_ok(args->nv_row, args->nv_token, args->nv_head))
         return KDA_BT16_EINVAL;
     const int64_t tokens = args->cu_seqlens ? args->T : (int64_t)args->N * args->T;
-    if (tokens * args->HKV > I32_MAX / 4) return KDA_BT16_EUNSUPPORTED;
+    // one thread for each 16 bytes of a token's keys
+    if (tokens > I32_MAX / 16 / args->HKV) return KDA_BT16_EUNSUPPORTED;
     p.nk = static_cast<const uint16_t*>(args->new_k);
     p.nv = static_cast<const uint16_t*>(args->new_v);
     p.nk_row = args->nk_row;

@@ -470,7 +470,6 @@ __global__ __launch_bounds__(256) void pages_move_kernel(PagesParams p) {
 hipError_t launch_paged_append(const PagedParams& p, int D, hipStream_t stream) {
     const int64_t tokens = p.cu_seqlens ? p.T : (int64_t)p.N * p.T;
     const int64_t total = tokens * p.HKV * (D / 8);
-    if (total > 0x7fffffff) return hipErrorInvalidValue;
     const dim3 grid((unsigned)((total + 255) / 256));
     if (D == 128) paged_append_kernel<128><<<grid, 256, 0, stream>>>(p, (int)total);
     else paged_append_kernel<64><<<grid, 256, 0, stream>>>(p, (int)total);
