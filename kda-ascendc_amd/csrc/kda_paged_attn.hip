@@ -715,10 +715,15 @@ __device__ __forceinline__ void meet() {
 // group's do the softmax of theirs (phase S), and they meet after each phase.
 // Left to themselves (two work-groups of four waves a CU) the two waves of a
 // SIMD fell into step, the matrix unit busy 48% of the cycles: a prompt of 8192
-// tokens, 32 / 8 heads, 558 us, so 521.  What bounds it now is the rate of the
-// products themselves: with the softmax left out, and with the LDS reads left
-// out too, 470 and 439 us (1.25 PFLOP/s; a bf16 product of 8192^3 reaches 1.15
-// to 1.2 on the same card).
+// tokens, 32 / 8 heads, 558 us, so 521 (1.06 PFLOP/s; a bf16 product of 8192^3
+// reaches 1.15 to 1.2 on the same card).  What bounds it now is that both phases
+// are longer than their matrix ops, 1024 cycles of a slot's 2190 (the matrix unit
+// is busy 47%, the vector unit 44%).  In M four waves read an operand of 1 KB for
+// each matrix op of 32 cycles, 128 bytes a cycle, all that LDS gives: without the
+// softmax 424 us.  S is 32 exponentials of 16 cycles and some 120 further vector
+// and 90 scalar operations: without the LDS reads 417 us.  One straight block of
+// both products, and the loads begun between its matrix ops, 540 (515 beside it).
+// Fewer LDS reads take 64 rows a wave, more registers than two waves a SIMD have.
 //   slot     2t             2t + 1         2t + 2
 //   group 0  M(t)           S(t)           M(t + 1)
 //   group 1  S(t - 1)       M(t)           S(t)
