@@ -277,9 +277,10 @@ __device__ __forceinline__ int few_tiles(const PagedParams& p, int n, NewTokens&
     const Tiles t = tiles_of<FEW>(p, s, 0);
     return max(1, t.end - t.begin);
 }
-// `slots`: the work-groups that run at once (half as many where they have twice
-// the waves).
-__device__ __forceinline__ Cut few_cut(const PagedParams& p, bool cut, uint32_t slots, int lane) {
+// Of work-groups with twice the waves half as many run at once.
+constexpr uint32_t few_slots(int waves) { return Shape<FEW>::SLOTS * Shape<FEW>::WAVES / waves; }
+__device__ __forceinline__ Cut few_cut(const PagedParams& p, bool cut, int waves, int lane) {
+    const uint32_t slots = few_slots(waves);
     Cut c;
     uint32_t all = 0, units = 0;
     for (int n0 = 0; n0 < p.N; n0 += 64) {
@@ -588,8 +589,8 @@ __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, ui
     run.l = sum_halves(run.l);
 }
 
-// A wave's place in LDS: of four waves in one array; of eight, three in either
-// ring of the many rows' kernel and two in an array of their own.
+// A wave's place in LDS: of four waves in one array; of eight, three in each of
+// two and two in a third (the many rows' kernel: its rings, and an array more).
 template <int D, int WAVES>
 struct FewLds {
     uint8_t *a, *b, *c;
@@ -668,10 +669,9 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, co
 
 // Work-group b's piece of the cut, row tile by row tile.
 template <class E, int D, int WAVES>
-__device__ __forceinline__ void few_piece(const PagedParams& p, int b, bool may_cut, uint32_t slots,
-                                          const FewLds<D, WAVES>& lds, float* joint) {
+__device__ __forceinline__ void few_piece(const PagedParams& p, int b, bool may_cut, const FewLds<D, WAVES>& lds, float* joint) {
     const int lane = threadIdx.x & 63;
-    const Cut cut = few_cut(p, may_cut, slots, lane);
+    const Cut cut = few_cut(p, may_cut, WAVES, lane);
     const uint32_t first = b * cut.size, end = first + cut.size;
     uint32_t cur = first, base = 0;
     for (int n0 = 0; n0 < p.N && cur < end; n0 += 64) {
@@ -892,11 +892,12 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
 
 // ---- kernels ----
 
-template <class E, int D>
-__global__ __launch_bounds__(256, 2) void paged_few_kernel(PagedParams p, bool cut) {
-    __shared__ alignas(1024) uint8_t lds[Shape<FEW>::WAVES * 2 * Shape<FEW>::TK * D * 2];
-    __shared__ float joint[Shape<FEW>::WAVES * 2 * ROWS];
-    few_piece<E, D, Shape<FEW>::WAVES>(p, blockIdx.x, cut, Shape<FEW>::SLOTS, {lds, nullptr, nullptr}, joint);
+template <class E, int D, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void paged_few_kernel(PagedParams p, bool cut) {
+    constexpr int EACH = 2 * Shape<FEW>::TK * D * 2;
+    __shared__ alignas(1024) uint8_t lds[WAVES * EACH];
+    __shared__ float joint[WAVES * 2 * ROWS];
+    few_piece<E, D, WAVES>(p, blockIdx.x, cut, {lds, lds + 3 * EACH, lds + 6 * EACH}, joint);
 }
 
 // MIXED: the work-groups from `few_from` on take the sequences of few rows, with
@@ -912,7 +913,7 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(PagedParams p, bool 
     __shared__ alignas(1024) uint8_t more[MIXED_KINDS ? 2 * 2 * Shape<FEW>::TK * D * 2 : 16];
     __shared__ float joint[MIXED_KINDS ? WAVES * 2 * ROWS : 1];
     if (MIXED_KINDS && blockIdx.x >= few_from) {
-        few_piece<E, D, WAVES>(p, blockIdx.x - few_from, few_may_cut, Shape<MANY>::SLOTS, {kt, vt, more}, joint);
+        few_piece<E, D, WAVES>(p, blockIdx.x - few_from, few_may_cut, {kt, vt, more}, joint);
         return;
     }
     Unit u;
@@ -988,7 +989,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int few,
     Unit u;
     if (KIND == FEW || (KIND == MIXED && (int)blockIdx.x < few)) {
         const int id = blockIdx.x / few_groups;
-        const Cut cut = few_cut(p, true, KIND == MIXED ? Shape<MANY>::SLOTS : Shape<FEW>::SLOTS, lane);
+        const Cut cut = few_cut(p, true, Shape<KIND == MIXED ? MANY : FEW>::WAVES, lane);
         u.n = id / p.HKV;
         u.h = id - u.n * p.HKV;
         u.m = 0;
@@ -1045,13 +1046,24 @@ int64_t many_units(const PagedParams& p) {
 
 // Whether a row tile's keys may go to several work-groups.  Few rows: not where
 // the table's rows hold so few keys that the join, a launch more, costs more:
-// one sequence of 704 keys 11.9 us whole and 10.4 cut, but the host's part 10.1
+// one sequence of 704 keys 10.5 us whole and 9.9 cut, but the host's part 10.1
 // against 14.1; 64 of 700 keys 32.8 whole and 35.4 cut.  Many rows: row tiles
 // that fill half of SLOTS are taken whole.
 bool may_cut(const PagedParams& p, int kind) {
     const int64_t keys = (int64_t)p.M << p.page_shift;
     if (kind == FEW) return keys > FEW_WHOLE;
     return keys >= 2 * Shape<MANY>::LEAST * Shape<MANY>::TK && many_units(p) <= Shape<MANY>::SLOTS / 2;
+}
+// The waves of a work-group of few rows, in a call of their kind alone: twice as
+// many where the row tiles are taken whole and all run at once so, and may be of
+// more than two tiles a wave (one sequence of 700 keys, 8 heads, on the GPU
+// 11.7 -> 10.5 us, 16 drafts of 5 over 700 10.3 -> 9.1; of up to 128 keys the
+// join of more waves costs 0.4 to 0.7).
+int few_waves(const PagedParams& p) {
+    constexpr int ONCE = Shape<FEW>::WAVES;
+    const int64_t keys = (int64_t)p.M << p.page_shift;
+    const bool more = !may_cut(p, FEW) && keys > 2 * ONCE * Shape<FEW>::TK && (int64_t)p.N * p.HKV <= few_slots(2 * ONCE);
+    return more ? 2 * ONCE : ONCE;
 }
 
 template <class E, int D, int KIND>
@@ -1061,7 +1073,11 @@ hipError_t launch(const PagedParams& p, hipStream_t stream) {
     // (uncut: one piece a row tile)
     const int64_t whole = (int64_t)p.N * p.HKV;
     if constexpr (KIND == FEW) {
-        paged_few_kernel<E, D><<<dim3((unsigned)(fc ? Shape<FEW>::SLOTS : whole)), 256, 0, stream>>>(p, fc);
+        constexpr int ONCE = Shape<FEW>::WAVES, TWICE = 2 * ONCE;
+        if (few_waves(p) == TWICE)
+            paged_few_kernel<E, D, TWICE><<<dim3((unsigned)whole), TWICE * 64, 0, stream>>>(p, false);
+        else
+            paged_few_kernel<E, D, ONCE><<<dim3((unsigned)(fc ? Shape<FEW>::SLOTS : whole)), ONCE * 64, 0, stream>>>(p, fc);
     } else {
         const int64_t many = units + (mc ? Shape<MANY>::SLOTS : 0);
         const int64_t few = KIND == MANY ? 0 : (fc ? Shape<MANY>::SLOTS : whole);
