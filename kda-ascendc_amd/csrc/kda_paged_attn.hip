@@ -716,14 +716,16 @@ __device__ __forceinline__ void meet() {
 // Left to themselves (two work-groups of four waves a CU) the two waves of a
 // SIMD fell into step, the matrix unit busy 48% of the cycles: a prompt of 8192
 // tokens, 32 / 8 heads, 558 us, so 521 (1.06 PFLOP/s; a bf16 product of 8192^3
-// reaches 1.15 to 1.2 on the same card).  What bounds it now is that both phases
-// are longer than their matrix ops, 1024 cycles of a slot's 2190 (the matrix unit
-// is busy 47%, the vector unit 44%).  In M four waves read an operand of 1 KB for
-// each matrix op of 32 cycles, 128 bytes a cycle, all that LDS gives: without the
-// softmax 424 us.  S is 32 exponentials of 16 cycles and some 120 further vector
-// and 90 scalar operations: without the LDS reads 417 us.  One straight block of
-// both products, and the loads begun between its matrix ops, 540 (515 beside it).
-// Fewer LDS reads take 64 rows a wave, more registers than two waves a SIMD have.
+// reaches 1.15 to 1.2 on the same card).  What bounds it now is that a slot takes
+// 1.06 us where its 32 matrix ops take 0.54 (17 ns each, in a loop of nothing
+// else): the matrix unit is busy 47% of the cycles, the vector unit 44%.  S is
+// some 120 vector operations at the 2.5 ns that one wave of a SIMD issues them,
+// 32 exponentials at 6.8 and 90 scalar operations: 0.7 us; and the phases hold
+// each other up (64 multiply-adds take 160 ns, 8 matrix ops 140, both at once
+// 190).  Without S the prompt takes 424 us, without M's LDS reads 417 (they are
+// 0.29 us of a slot at the 560 and 380 bytes a ns that a CU reads so).  Two or
+// three groups of operands ahead instead of one, both products in one straight
+// block, or the loads begun between matrix ops: 523 and 540 to 555 us.
 //   slot     2t             2t + 1         2t + 2
 //   group 0  M(t)           S(t)           M(t + 1)
 //   group 1  S(t - 1)       M(t)           S(t)
