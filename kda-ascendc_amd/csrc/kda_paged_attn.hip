@@ -459,6 +459,15 @@ __device__ __forceinline__ void load_q(const PagedParams& p, const Unit& u, cons
     for (int s = 0; s < D / 16; ++s) q[s] = *reinterpret_cast<const u32x4*>(at + 16 * s + 8 * half);
 }
 
+// Keys (or values) in memory: the address of the first, and their bytes.
+struct Place {
+    uint32_t lo, hi, bytes;
+};
+__device__ __forceinline__ Place of_lane(const Place& x, int at) {
+    return {(uint32_t)__builtin_amdgcn_readlane(x.lo, at), (uint32_t)__builtin_amdgcn_readlane(x.hi, at),
+            (uint32_t)__builtin_amdgcn_readlane(x.bytes, at)};
+}
+
 // What a wave loads of a tile: NROWS keys (or values) of one head, all of one
 // page, 1 KiB a load.
 template <int D, int NROWS, bool STREAM>
@@ -476,16 +485,20 @@ struct Loader {
             off[j] = row * (int)token_bytes + (((lane & (PIECES - 1)) ^ swizzle<D>(row0 + row)) << 4);
         }
     }
-    // Keys `key` on, of a page (an entry of the table), to LDS.  Keys past the
+    // Keys `key` on, of a page (an entry of the table).  In LDS, keys past the
     // last that the row tile sees become zeros (the descriptor ends with it),
     // and so do all where it sees none of them or there is no page: whatever
     // pages hold beyond a sequence, or had before its window, does not reach
     // the products.
-    __device__ __forceinline__ void load(const PagedParams& p, const Unit& u, int page, int key, uint32_t lds) const {
+    __device__ __forceinline__ Place place(const PagedParams& p, const Unit& u, int page, int key) const {
         const int n = is_page(p, page) && key + NROWS > u.lo ? min(u.hi - key, NROWS) : 0;
         const int in = key & ((1 << p.page_shift) - 1);
         const uint64_t at = head + (uint64_t)(n > 0 ? (uint32_t)page : 0u) * page_bytes + (uint32_t)in * token_bytes;
-        const u32x4 rsrc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, n > 0 ? (n - 1) * token_bytes + D * 2 : 0u, BUF_RAW};
+        return {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, n > 0 ? (n - 1) * token_bytes + D * 2 : 0u};
+    }
+    // (the place the same in all lanes)
+    __device__ __forceinline__ void load(const Place& x, uint32_t lds) const {
+        const u32x4 rsrc = {x.lo, x.hi, x.bytes, BUF_RAW};
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) load_lds<STREAM>(rsrc, off[j], lds + j * 1024);
     }
@@ -534,7 +547,7 @@ __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, ui
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             const int key = tile * TK + 16 * g;
-            from.load(p, u, pg[g], key, lds_address(to) + g * (TILE / 2));
+            from.load(from.place(p, u, pg[g], key), lds_address(to) + g * (TILE / 2));
         }
     };
     look_up(t, pages);
@@ -714,18 +727,18 @@ __device__ __forceinline__ void meet() {
 // products (phase M: O += V^T P^T of the last tile, S of this one) the other
 // group's do the softmax of theirs (phase S), and they meet after each phase.
 // Left to themselves (two work-groups of four waves a CU) the two waves of a
-// SIMD fell into step, the matrix unit busy 48% of the cycles: a prompt of 8192
-// tokens, 32 / 8 heads, 558 us, so 521 (1.06 PFLOP/s; a bf16 product of 8192^3
-// reaches 1.15 to 1.2 on the same card).  What bounds it now is that a slot takes
-// 1.06 us where its 32 matrix ops take 0.54 (17 ns each, in a loop of nothing
-// else): the matrix unit is busy 47% of the cycles, the vector unit 44%.  S is
-// some 120 vector operations at the 2.5 ns that one wave of a SIMD issues them,
-// 32 exponentials at 6.8 and 90 scalar operations: 0.7 us; and the phases hold
-// each other up (64 multiply-adds take 160 ns, 8 matrix ops 140, both at once
-// 190).  Without S the prompt takes 424 us, without M's LDS reads 417 (they are
-// 0.29 us of a slot at the 560 and 380 bytes a ns that a CU reads so).  Two or
-// three groups of operands ahead instead of one, both products in one straight
-// block, or the loads begun between matrix ops: 523 and 540 to 555 us.
+// SIMD fell into step: a prompt of 8192 tokens, 32 / 8 heads, 558 us, so 521, and
+// 502 with a tile's places found for 64 tiles at once (1.1 PFLOP/s; a bf16
+// product of 8192^3 reaches 1.15 to 1.2 on the same card).  What bounds it now is
+// that a slot takes 1 us where its 32 matrix ops take 0.54 (17 ns each, in a loop
+// of nothing else).  S is some 120 vector operations at the 2.5 ns that one wave
+// of a SIMD issues them, 32 exponentials at 6.8 and the loads: 0.6 us; and the
+// phases hold each other up (64 multiply-adds take 160 ns, 8 matrix ops 140, both
+// at once 190).  On the way there, of 521 us: without S 424, without M's LDS
+// reads 417 (0.29 us of a slot at the 560 and 380 bytes a ns that a CU reads so);
+// now, without the loads 462.  Two or three groups of operands ahead instead of
+// one, both products in one straight block, or the loads begun between matrix
+// ops: 15 to 35 us more.
 //   slot     2t             2t + 1         2t + 2
 //   group 0  M(t)           S(t)           M(t + 1)
 //   group 1  S(t - 1)       M(t)           S(t)
@@ -758,19 +771,19 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
     const Loader<D, SHARE, false> k0(p.k, p.k_page, p.k_token, u.h * p.k_head, SHARE * wave & 15, lane);
     const Loader<D, SHARE, false> v0(p.v, p.v_page, p.v_token, u.h * p.v_head, SHARE * wave & 15, lane);
     const uint32_t k_lds = lds_address(kt) + wave * (SHARE * D * 2), v_lds = lds_address(vt) + wave * (SHARE * D * 2);
-    auto look_up = [&](int t) { return table_entry(p, u.n, ((u.begin + t) * TK + SHARE * wave) >> p.page_shift); };
-    auto load = [&](const Loader<D, SHARE, false>& from, int t, int page, uint32_t to) {
-        if (t >= count) return;
-        const int key = (u.begin + t) * TK + SHARE * wave;
-        from.load(p, u, page, key, to);
+    // Where this wave's keys of 64 tiles lie, a tile a lane: a tile's loads then
+    // need no more than lane reads (a table entry and an address for each, by
+    // scalar operations, took a fifth of a slot).  Past the last tile: nothing,
+    // zeros.
+    auto places = [&](const Loader<D, SHARE, false>& of, int t) {
+        const int key = (u.begin + max(min(t + lane, count - 1), 0)) * TK + SHARE * wave;
+        const int at = min(key >> p.page_shift, p.M - 1);
+        return of.place(p, u, t + lane < count ? p.page_table[u.n * p.table_stride + at] : -1, key);
     };
-    // Table entries of tiles t + 1 and t + 2 as the softmax of t begins.
-    int page1 = look_up(0), page2 = look_up(1);
-    load(k0, 0, page1, k_lds);
-    load(k0, 1, page2, k_lds + TILE);
-    load(v0, 0, page1, v_lds);
-    page1 = page2;
-    page2 = look_up(2);
+    Place k_of = places(k0, 0), v_of = places(v0, 0);
+    k0.load(of_lane(k_of, 0), k_lds);
+    k0.load(of_lane(k_of, 1), k_lds + TILE);
+    v0.load(of_lane(v_of, 0), v_lds);
     u32x4 q[STEPS];
     load_q<D>(p, u, x, half, q);
 
@@ -779,15 +792,10 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
         return t0 < any_hi && t0 + TK > any_lo;
     };
     auto begin_loads = [&](int t, int kbuf, int vbuf) {
-        load(k0, t + 2, page2, k_lds + kbuf * TILE);
-        load(v0, t + 1, page1, v_lds + vbuf * TILE);
-        page1 = page2;
-        page2 = look_up(t + 3);
-    };
-    // K(t + 1) and V(t) have arrived: what was begun after them may be under way.
-    auto arrived = [&](int t) {
-        if (t + 2 < count) wait_loads<2 * LOADS>();
-        else wait_loads<0>();
+        if (((t + 2) & 63) == 0) k_of = places(k0, t + 2);
+        if (((t + 1) & 63) == 0) v_of = places(v0, t + 1);
+        k0.load(of_lane(k_of, (t + 2) & 63), k_lds + kbuf * TILE);
+        v0.load(of_lane(v_of, (t + 1) & 63), v_lds + vbuf * TILE);
     };
     // The products' operands are read one group of matrix ops ahead of their
     // use, a read between two matrix ops: an LDS read takes several of them.
@@ -848,7 +856,7 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
         meet();
         begin_loads(t, (I + 2) % 3, (I + 1) % 3);
         softmax(t);
-        if (!second) arrived(t);
+        if (!second) wait_loads<2 * LOADS>();  // but for what was begun just now: K(t + 1) and V(t) have arrived
         meet();
     };
     if (count > 0) {
@@ -864,6 +872,7 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
         if (sees(count - 1)) outputs(vt + (count - 1) % 3 * TILE);
         if (!second) meet();
     }
+    wait_loads<0>();  // (past the last tile)
 
     const float l = sum_halves(run.l);
     if (!x.live) return;
