@@ -106,6 +106,20 @@ __device__ __forceinline__ void load_lds(u32x4 rsrc, int off, uint32_t lds) {
                      "s"(lds)
                      : "memory");
 }
+// One or two such loads at `AT` past `lds`, the second 1 KiB on.
+template <int AT, int LOADS>
+__device__ __forceinline__ void load_lds_at(u32x4 rsrc, const int (&off)[LOADS], uint32_t lds) {
+    static_assert(LOADS <= 2, "one instruction each below");
+    if constexpr (LOADS == 1)
+        asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off[0]), "s"(rsrc),
+                     "s"(lds), "i"(AT)
+                     : "memory", "scc");
+    else
+        asm volatile("s_add_u32 m0, %3, %4\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds\n\t"
+                     "s_add_u32 m0, %3, %5\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"v"(off[0]),
+                     "v"(off[LOADS - 1]), "s"(rsrc), "s"(lds), "i"(AT), "i"(AT + 1024)
+                     : "memory", "scc");
+}
 // All but the last `n` of this wave's loads have arrived.
 template <int N>
 __device__ __forceinline__ void wait_loads() {
@@ -502,6 +516,10 @@ struct Loader {
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) load_lds<STREAM>(rsrc, off[j], lds + j * 1024);
     }
+    template <int AT>
+    __device__ __forceinline__ void load_at(const Place& x, uint32_t lds) const {
+        load_lds_at<AT, LOADS>(u32x4{x.lo, x.hi, x.bytes, BUF_RAW}, off, lds);
+    }
 };
 
 // This wave's LDS reads have returned: what they read may be loaded over.
@@ -728,8 +746,9 @@ __device__ __forceinline__ void meet() {
 // group's do the softmax of theirs (phase S), and they meet after each phase.
 // Left to themselves (two work-groups of four waves a CU) the two waves of a
 // SIMD fell into step: a prompt of 8192 tokens, 32 / 8 heads, 558 us, so 521, and
-// 502 with a tile's places found for 64 tiles at once (1.1 PFLOP/s; a bf16
-// product of 8192^3 reaches 1.15 to 1.2 on the same card).  What bounds it now is
+// 502 with a tile's places found for 64 tiles at once and 489 with fewer scalar
+// operations about them (1.1 PFLOP/s; a bf16 product of 8192^3 reaches 1.15 to
+// 1.2 on the same card).  What bounds it now is
 // that a slot takes 1 us where its 32 matrix ops take 0.54 (17 ns each, in a loop
 // of nothing else).  S is some 120 vector operations at the 2.5 ns that one wave
 // of a SIMD issues them, 32 exponentials at 6.8 and the loads: 0.6 us; and the
@@ -757,10 +776,14 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
     const int row = wave * ROWS + (lane & 31);
     const Row x = row_of(p, u, u.m * MT + row);
     const int count = u.end - u.begin;
-    // the keys that every row of this wave sees, and those that any does
+    // the keys that every row of this wave sees, and those that any does; the
+    // tiles of u.begin on that are among the first, and that have some of the others
     const int all_lo = __builtin_amdgcn_readlane(x.lo, 31), all_hi = __builtin_amdgcn_readlane(x.hi, 0);
     const int any_lo = __builtin_amdgcn_readlane(x.lo, 0);
     const int any_hi = u.m * MT + wave * ROWS < u.s.count * p.G ? __builtin_amdgcn_readlane(x.hi, 31) : 0;
+    const int all0 = (int)(((unsigned)all_lo + TK - 1) / TK) - u.begin, any0 = max(any_lo / TK - u.begin, 0);
+    const unsigned all_tiles = max(all_hi / TK - u.begin - all0, 0);
+    const unsigned any_tiles = max((int)(((unsigned)any_hi + TK - 1) / TK) - u.begin - any0, 0);
     const float c = p.scale * LOG2E;
     Running run;
     f32x16 acc[DB], st[2];
@@ -787,15 +810,12 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
     u32x4 q[STEPS];
     load_q<D>(p, u, x, half, q);
 
-    auto sees = [&](int t) {
-        const int t0 = (u.begin + t) * TK;
-        return t0 < any_hi && t0 + TK > any_lo;
-    };
-    auto begin_loads = [&](int t, int kbuf, int vbuf) {
+    auto sees = [&](int t) { return (unsigned)(t - any0) < any_tiles; };
+    auto begin_loads = [&](int t, auto I) {
         if (((t + 2) & 63) == 0) k_of = places(k0, t + 2);
         if (((t + 1) & 63) == 0) v_of = places(v0, t + 1);
-        k0.load(of_lane(k_of, (t + 2) & 63), k_lds + kbuf * TILE);
-        v0.load(of_lane(v_of, (t + 1) & 63), v_lds + vbuf * TILE);
+        k0.template load_at<(I + 2) % 3 * TILE>(of_lane(k_of, (t + 2) & 63), k_lds);
+        v0.template load_at<(I + 1) % 3 * TILE>(of_lane(v_of, (t + 1) & 63), v_lds);
     };
     // The products' operands are read one group of matrix ops ahead of their
     // use, a read between two matrix ops: an LDS read takes several of them.
@@ -836,25 +856,25 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
     };
     auto products = [&](int t, const uint8_t* ks, const uint8_t* vs) {
         __builtin_amdgcn_s_setprio(1);
-        if (t > 0 && sees(t - 1)) outputs(vs);
+        if (sees(t - 1)) outputs(vs);
         if (sees(t)) scores(ks);
         __builtin_amdgcn_s_setprio(0);
     };
     auto softmax = [&](int t) {
         if (!sees(t)) return;
-        const int t0 = (u.begin + t) * TK;
         float alpha;
-        if (softmax_tile<E, 2>(st, t0 + 4 * half, x.lo, x.hi, t0 < all_lo || t0 + TK > all_hi, c, run, pt, alpha)) {
+        if (softmax_tile<E, 2>(st, (u.begin + t) * TK + 4 * half, x.lo, x.hi, (unsigned)(t - all0) >= all_tiles, c, run, pt,
+                               alpha)) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) acc[d] *= alpha;
         }
     };
     // Tile t, in place I = t % 3 of the rings.
-    auto step = [&](int t, int I) {
+    auto step = [&](int t, auto I) {
         products(t, kt + I * TILE, vt + (I + 2) % 3 * TILE);
         if (second) wait_loads<0>();
         meet();
-        begin_loads(t, (I + 2) % 3, (I + 1) % 3);
+        begin_loads(t, I);
         softmax(t);
         if (!second) wait_loads<2 * LOADS>();  // but for what was begun just now: K(t + 1) and V(t) have arrived
         meet();
@@ -865,9 +885,9 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
         meet();
         if (second) meet();
         for (int t = 0; t < count; t += 3) {
-            step(t, 0);
-            if (t + 1 < count) step(t + 1, 1);
-            if (t + 2 < count) step(t + 2, 2);
+            step(t, std::integral_constant<int, 0>{});
+            if (t + 1 < count) step(t + 1, std::integral_constant<int, 1>{});
+            if (t + 2 < count) step(t + 2, std::integral_constant<int, 2>{});
         }
         if (sees(count - 1)) outputs(vt + (count - 1) % 3 * TILE);
         if (!second) meet();
