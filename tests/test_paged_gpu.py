@@ -157,6 +157,15 @@ def test_long_context(T, gpu_device):
     check([5000, 3001], T, 4, 2, 128, 32, BF16, gpu_device)
 
 
+@pytest.mark.parametrize("causal, window", [(True, None), (True, 4200), (False, None)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_contexts_taken_whole(D, causal, window, gpu_device):
+    """More row tiles than half the work-groups that run at once: each goes
+    over all of its keys, more than 64 tiles of them, in one piece."""
+    lens = [9000, 4099, 8192] + [5 + 3 * n % 60 for n in range(130)]
+    check(lens, 5, 8, 1, D, 16, BF16, gpu_device, causal=causal, window=window)
+
+
 @pytest.mark.parametrize("T", [1, 16, 140])
 def test_large_scores(T, gpu_device):
     """Scores of some hundreds: the running maximum moves far, most weights
