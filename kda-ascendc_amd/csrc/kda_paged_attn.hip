@@ -745,19 +745,16 @@ __device__ __forceinline__ void meet() {
 // products (phase M: O += V^T P^T of the last tile, S of this one) the other
 // group's do the softmax of theirs (phase S), and they meet after each phase.
 // Left to themselves (two work-groups of four waves a CU) the two waves of a
-// SIMD fell into step: a prompt of 8192 tokens, 32 / 8 heads, 558 us, so 521, and
-// 502 with a tile's places found for 64 tiles at once and 489 with fewer scalar
-// operations about them (1.1 PFLOP/s; a bf16 product of 8192^3 reaches 1.15 to
-// 1.2 on the same card).  What bounds it now is
-// that a slot takes 1 us where its 32 matrix ops take 0.54 (17 ns each, in a loop
-// of nothing else).  S is some 120 vector operations at the 2.5 ns that one wave
-// of a SIMD issues them, 32 exponentials at 6.8 and the loads: 0.6 us; and the
-// phases hold each other up (64 multiply-adds take 160 ns, 8 matrix ops 140, both
-// at once 190).  On the way there, of 521 us: without S 424, without M's LDS
-// reads 417 (0.29 us of a slot at the 560 and 380 bytes a ns that a CU reads so);
-// now, without the loads 462.  Two or three groups of operands ahead instead of
-// one, both products in one straight block, or the loads begun between matrix
-// ops: 15 to 35 us more.
+// SIMD fell into step: a prompt of 8192 tokens, 32 / 8 heads, 558 us, so 521.
+// S was then the longer phase (a lone wave issues a vector operation every 2.5 ns
+// and an exponential every 6.8, and the loads' addresses took 80 scalar ones);
+// with the places of 64 tiles found at once the prompt takes 970 kilocycles
+// instead of 1137 and 489 to 508 us (1.1 PFLOP/s; a bf16 product of 8192^3
+// reaches 1.15 to 1.2 on the same card), the matrix unit 54% busy.  What bounds
+// it now is the card's power: the clock, 2.08 GHz before, went down to 1.90.
+// No gain from: two or three groups of operands ahead instead of one, both
+// products in one straight block (540), the loads begun between matrix ops (540
+// to 553), other orders of the softmax's operations.
 //   slot     2t             2t + 1         2t + 2
 //   group 0  M(t)           S(t)           M(t + 1)
 //   group 1  S(t - 1)       M(t)           S(t)
