@@ -546,7 +546,7 @@ __device__ __forceinline__ float log_sum(float mc, float l) {
 // wave: a tile of keys, one of values; 32 rows of D floats).  Where there is
 // much to read HBM bounds it (64 sequences of 100 to 16000 tokens, 32 / 8 heads,
 // 765 MB in 137 us, 5.6 TB/s; a large read reaches 6.3), with little the chain
-// of lengths, table entry, keys, values: 6 us, and 1.3 more for each further
+// of lengths, table entry, keys, values: 6 us, and 1.9 more for each further
 // tile of a wave.
 template <class E, int D, int WAVES>
 __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, uint8_t* kw, uint8_t* vw, int wave,
@@ -555,6 +555,8 @@ __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, ui
     constexpr int TILE = TK * D * 2;
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const Row x = row_of(p, u, u.m * ROWS + (lane & 31));
+    // the keys that every row sees
+    const int all_lo = __builtin_amdgcn_readlane(x.lo, 31), all_hi = __builtin_amdgcn_readlane(x.hi, 0);
     const float c = p.scale * LOG2E;
 
     int t = u.begin + wave;
@@ -611,7 +613,7 @@ __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, ui
         if (more) load(v0, t + WAVES, next, vw);
         u32x4 pt[2];
         float alpha;
-        if (softmax_tile<E, 1>(st, t * TK + 4 * half, x.lo, x.hi, true, c, run, pt, alpha)) {
+        if (softmax_tile<E, 1>(st, t * TK + 4 * half, x.lo, x.hi, t * TK < all_lo || t * TK + TK > all_hi, c, run, pt, alpha)) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) acc[d] *= alpha;
         }
@@ -1079,7 +1081,7 @@ int64_t many_units(const PagedParams& p) {
 
 // Whether a row tile's keys may go to several work-groups.  Few rows: not where
 // the table's rows hold so few keys that the join, a launch more, costs more:
-// one sequence of 704 keys 10.5 us whole and 9.9 cut, but the host's part 10.1
+// one sequence of 704 keys 10.0 us whole and 9.7 cut, but the host's part 10.1
 // against 14.1; 64 of 700 keys 32.8 whole and 35.4 cut.  Many rows: row tiles
 // that fill half of SLOTS are taken whole.
 bool may_cut(const PagedParams& p, int kind) {
