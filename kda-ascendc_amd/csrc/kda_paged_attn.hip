@@ -545,7 +545,7 @@ __device__ __forceinline__ float log_sum(float mc, float l) {
 // waves' sums are joined at the end, in the same LDS (2 * TILE bytes a
 // wave: a tile of keys, one of values; 32 rows of D floats).  Where there is
 // much to read HBM bounds it (64 sequences of 100 to 16000 tokens, 32 / 8 heads,
-// 765 MB in 137 us, 5.6 TB/s; a large read reaches 6.3), with little the chain
+// 765 MB in 132 us, 5.8 TB/s; a large read reaches 6.3), with little the chain
 // of lengths, table entry, keys, values: 6 us, and 1.9 more for each further
 // tile of a wave.
 template <class E, int D, int WAVES>
@@ -755,7 +755,7 @@ __device__ __forceinline__ void meet() {
 // S was then the longer phase (a lone wave issues a vector operation every 2.5 ns
 // and an exponential every 6.8, and the loads' addresses took 80 scalar ones);
 // with the places of 64 tiles found at once the prompt takes 970 kilocycles
-// instead of 1137 and 489 to 508 us (1.1 PFLOP/s; a bf16 product of 8192^3
+// instead of 1137 and 489 to 516 us (1.1 PFLOP/s; a bf16 product of 8192^3
 // reaches 1.15 to 1.2 on the same card), the matrix unit 54% busy.  What bounds
 // it now is the card's power: the clock, 2.08 GHz before, went down to 1.90.
 // No gain from: two or three groups of operands ahead instead of one, both
