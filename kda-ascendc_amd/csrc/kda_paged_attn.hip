@@ -131,20 +131,41 @@ __device__ __forceinline__ uint32_t lds_address(const uint8_t* p) {
 
 // Operand of the first product: rows lane & 31, elements 16 * s + 8 * (lane >> 5) .. +7.
 template <int D>
+__device__ __forceinline__ const uint8_t* k_place(const uint8_t* lds, int row, int piece) {
+    return lds + row * (D * 2) + ((piece ^ swizzle<D>(row)) << 4);
+}
+__device__ __forceinline__ u32x4 load_operand(uint32_t at) {
+    typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+    return *reinterpret_cast<lds_u32x4*>(at);
+}
+template <int D>
 __device__ __forceinline__ u32x4 read_k(const uint8_t* lds, int row, int piece) {
-    return *reinterpret_cast<const u32x4*>(lds + row * (D * 2) + ((piece ^ swizzle<D>(row)) << 4));
+    return *reinterpret_cast<const u32x4*>(k_place<D>(lds, row, piece));
 }
 
 // Half an operand of the second product: lane's column d = 32 * db + (lane & 31)
 // of rows key .. key + 3.  In each group of 16 lanes, lane n receives as item i
 // element n % 4 of the 8 bytes that lane 4 * i + n / 4 points at.
 template <int D>
-__device__ __forceinline__ u32x2 read_v(const uint8_t* lds, int key, int db, int lane) {
-    typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+__device__ __forceinline__ const uint8_t* v_place(const uint8_t* lds, int key, int db, int lane) {
     const int row = key + ((lane & 15) >> 2);
     const int d = 32 * db + (lane & 16) + 4 * (lane & 3);
-    const uint8_t* at = lds + row * (D * 2) + (((d >> 3) ^ swizzle<D>(row)) << 4) + (d & 4) * 2;
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at));
+    return lds + row * (D * 2) + (((d >> 3) ^ swizzle<D>(row)) << 4) + (d & 4) * 2;
+}
+__device__ __forceinline__ u32x2 load_transposed(uint32_t at) {
+    typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_i16x4*>(at)));
+}
+template <int D>
+__device__ __forceinline__ u32x2 read_v(const uint8_t* lds, int key, int db, int lane) {
+    return load_transposed(lds_address(v_place<D>(lds, key, db, lane)));
+}
+// A number that the compiler takes as it is, where it stands: else it keeps, all
+// along, whatever a kernel's addresses are made of, in more registers than there
+// are.
+__device__ __forceinline__ uint32_t hide(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
 }
 
 // Maximum and sum of x and the value of lane ^ 32: the swap exchanges the upper
@@ -545,56 +566,64 @@ __device__ __forceinline__ float log_sum(float mc, float l) {
 // waves' sums are joined at the end, in the same LDS (2 * TILE bytes a
 // wave: a tile of keys, one of values; 32 rows of D floats).  Where there is
 // much to read HBM bounds it (64 sequences of 100 to 16000 tokens, 32 / 8 heads,
-// 765 MB in 132 us, 5.8 TB/s; a large read reaches 6.3), with little the chain
-// of lengths, table entry, keys, values: 6 us, and 1.9 more for each further
+// 765 MB in 130 us, 5.9 TB/s; a large read reaches 6.3), with little the chain
+// of lengths, table entry, keys, values: 6 us, and 1.8 more for each further
 // tile of a wave.
 template <class E, int D, int WAVES>
-__device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, uint8_t* kw, uint8_t* vw, int wave,
-                                         Running& run, f32x16 (&acc)[D / 32]) {
+__device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, uint8_t* lds, int wave, Running& run,
+                                         f32x16 (&acc)[D / 32]) {
     constexpr int STEPS = D / 16, DB = D / 32, TK = Shape<FEW>::TK;
-    constexpr int TILE = TK * D * 2;
-    const int lane = threadIdx.x & 63, half = lane >> 5;
+    constexpr int TILE = TK * D * 2, LOADS = TILE / 1024;  // loads of a tile of keys, or of values
+    const int lane = (int)hide(threadIdx.x & 63), half = lane >> 5;
     const Row x = row_of(p, u, u.m * ROWS + (lane & 31));
     // the keys that every row sees
     const int all_lo = __builtin_amdgcn_readlane(x.lo, 31), all_hi = __builtin_amdgcn_readlane(x.hi, 0);
     const float c = p.scale * LOG2E;
-
-    int t = u.begin + wave;
-    const Loader<D, 16, true> k0(p.k, p.k_page, p.k_token, u.h * p.k_head, 0, lane);
-    const Loader<D, 16, true> v0(p.v, p.v_page, p.v_token, u.h * p.v_head, 0, lane);
-    int pages[2], next[2];  // of the tile's first and second 16 keys
-    auto look_up = [&](int tile, int (&pg)[2]) {
-#pragma unroll
-        for (int g = 0; g < 2; ++g) pg[g] = table_entry(p, u.n, (tile * TK + 16 * g) >> p.page_shift);
-    };
-    auto load = [&](const Loader<D, 16, true>& from, int tile, const int (&pg)[2], uint8_t* to) {
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            const int key = tile * TK + 16 * g;
-            from.load(from.place(p, u, pg[g], key), lds_address(to) + g * (TILE / 2));
-        }
-    };
-    look_up(t, pages);
-    if (t < u.end) {
-        load(k0, t, pages, kw);
-        load(v0, t, pages, vw);
-    }
-    look_up(t + WAVES, next);
     u32x4 q[STEPS];
     load_q<D>(p, u, x, half, q);
-    // (once here, where the compiler sees it: else it waits for q in every turn)
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0
-    constexpr int LOADS = TILE / 1024;  // of a tile of keys, or of values
-    for (; t < u.end; t += WAVES) {
-        const bool more = t + WAVES < u.end;
+
+    // The wave's tiles are first, first + WAVES and so on, `count` of them.  Where
+    // 32 of them lie, 16 keys a lane: a tile's loads then need no more than lane
+    // reads (found tile by tile with scalar operations, one sequence of 700 keys
+    // took 10.4 us instead of 9.8, 64 sequences 132 instead of 130).
+    const int first = u.begin + wave, count = (u.end - first + WAVES - 1) / WAVES;
+    if (count <= 0) return;
+    const Loader<D, 16, true> k0(p.k, p.k_page, p.k_token, u.h * p.k_head, 0, lane);
+    const Loader<D, 16, true> v0(p.v, p.v_page, p.v_token, u.h * p.v_head, 0, lane);
+    Place k_of, v_of;
+    auto places = [&](int j) {
+        const int mine = j + (lane >> 1);
+        const int key = (first + min(mine, count - 1) * WAVES) * TK + 16 * (lane & 1);
+        const int at = min(key >> p.page_shift, p.M - 1);
+        const int page = mine < count ? p.page_table[u.n * p.table_stride + at] : -1;
+        k_of = k0.place(p, u, page, key);
+        v_of = v0.place(p, u, page, key);
+    };
+    auto load = [&](const Loader<D, 16, true>& from, const Place& at, int j, uint8_t* to) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) from.load(of_lane(at, 2 * (j & 31) + g), lds_address(to) + g * (TILE / 2));
+    };
+    uint32_t k_at[STEPS], v_at[DB][2];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) k_at[s] = lds_address(k_place<D>(lds, lane & 31, 2 * s + half));
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) v_at[d][i] = lds_address(v_place<D>(lds + TILE, 8 * i + 4 * half, d, lane));
+    places(0);
+    load(k0, k_of, 0, lds);
+    load(v0, v_of, 0, lds + TILE);
+    for (int j = 0; j < count; ++j) {
+        const bool more = j + 1 < count;
+        if (((j + 1) & 31) == 0) places(j + 1);
         // All operands of a product are read before it, so that its place is
         // loaded again while it runs.
         wait_loads<LOADS>();  // but for the values'
         u32x4 ka[STEPS];
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) ka[s] = read_k<D>(kw, lane & 31, 2 * s + half);
+        for (int s = 0; s < STEPS; ++s) ka[s] = load_operand(k_at[s]);
         reads_done();
-        if (more) load(k0, t + WAVES, next, kw);
+        if (more) load(k0, k_of, j + 1, lds);
         f32x16 st[1] = {f32x16{}};
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) st[0] = E::mfma(ka[s], q[s], st[0]);
@@ -605,15 +634,16 @@ __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, ui
         for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                const u32x2 a = read_v<D>(vw, 16 * k + 4 * half, d, lane);
-                const u32x2 b = read_v<D>(vw, 16 * k + 8 + 4 * half, d, lane);
+                const u32x2 a = load_transposed(v_at[d][0] + 16 * k * D * 2);
+                const u32x2 b = load_transposed(v_at[d][1] + 16 * k * D * 2);
                 va[k][d] = u32x4{a.x, a.y, b.x, b.y};
             }
         reads_done();
-        if (more) load(v0, t + WAVES, next, vw);
+        if (more) load(v0, v_of, j + 1, lds + TILE);
         u32x4 pt[2];
         float alpha;
-        if (softmax_tile<E, 1>(st, t * TK + 4 * half, x.lo, x.hi, t * TK < all_lo || t * TK + TK > all_hi, c, run, pt, alpha)) {
+        const int key = (first + j * WAVES) * TK;
+        if (softmax_tile<E, 1>(st, key + 4 * half, x.lo, x.hi, key < all_lo || key + TK > all_hi, c, run, pt, alpha)) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) acc[d] *= alpha;
         }
@@ -621,7 +651,6 @@ __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, ui
         for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int d = 0; d < DB; ++d) acc[d] = E::mfma(va[k][d], pt[k], acc[d]);
-        look_up(t + 2 * WAVES, next);
     }
     run.l = sum_halves(run.l);
 }
@@ -630,9 +659,9 @@ __device__ __forceinline__ void few_loop(const PagedParams& p, const Unit& u, ui
 // two and two in a third (the many rows' kernel: its rings, and an array more).
 template <int D, int WAVES>
 struct FewLds {
+    static constexpr int EACH = 2 * Shape<FEW>::TK * D * 2;
     uint8_t *a, *b, *c;
     __device__ __forceinline__ uint8_t* of(int wave) const {
-        constexpr int EACH = 2 * Shape<FEW>::TK * D * 2;
         if (WAVES == 4 || wave < 3) return a + wave * EACH;
         return wave < 6 ? b + (wave - 3) * EACH : c + (wave - 6) * EACH;
     }
@@ -640,7 +669,7 @@ struct FewLds {
 
 template <class E, int D, int WAVES>
 __device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, const FewLds<D, WAVES>& lds, float* joint) {
-    constexpr int DB = D / 32, TILE = Shape<FEW>::TK * D * 2;
+    constexpr int DB = D / 32;
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Running run;
@@ -648,7 +677,7 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, co
 #pragma unroll
     for (int i = 0; i < DB; ++i) acc[i] = f32x16{};
     uint8_t* mine = lds.of(wave);
-    few_loop<E, D, WAVES>(p, u, mine, mine + TILE, wave, run, acc);
+    few_loop<E, D, WAVES>(p, u, mine, wave, run, acc);
 
     // Join: every wave's m and l, then its O over the tiles' LDS, row by row
     // in pieces of four (the rows' pieces turned by the row, so that the lanes
@@ -706,7 +735,8 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Unit& u, co
 
 // Work-group b's piece of the cut, row tile by row tile.
 template <class E, int D, int WAVES>
-__device__ __forceinline__ void few_piece(const PagedParams& p, int b, bool may_cut, const FewLds<D, WAVES>& lds, float* joint) {
+__device__ __forceinline__ void few_piece(const PagedParams& p, int b, bool may_cut, const FewLds<D, WAVES>& lds,
+                                          float* joint) {
     const int lane = threadIdx.x & 63;
     const Cut cut = few_cut(p, may_cut, WAVES, lane);
     const uint32_t first = b * cut.size, end = first + cut.size;
@@ -928,10 +958,10 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const Unit& u, u
 
 template <class E, int D, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void paged_few_kernel(PagedParams p, bool cut) {
-    constexpr int EACH = 2 * Shape<FEW>::TK * D * 2;
-    __shared__ alignas(1024) uint8_t lds[WAVES * EACH];
+    typedef FewLds<D, WAVES> Lds;
+    __shared__ alignas(1024) uint8_t lds[WAVES * Lds::EACH];
     __shared__ float joint[WAVES * 2 * ROWS];
-    few_piece<E, D, WAVES>(p, blockIdx.x, cut, {lds, lds + 3 * EACH, lds + 6 * EACH}, joint);
+    few_piece<E, D>(p, blockIdx.x, cut, Lds{lds, lds + 3 * Lds::EACH, lds + 6 * Lds::EACH}, joint);
 }
 
 // MIXED: the work-groups from `few_from` on take the sequences of few rows, with
@@ -947,7 +977,7 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(PagedParams p, bool 
     __shared__ alignas(1024) uint8_t more[MIXED_KINDS ? 2 * 2 * Shape<FEW>::TK * D * 2 : 16];
     __shared__ float joint[MIXED_KINDS ? WAVES * 2 * ROWS : 1];
     if (MIXED_KINDS && blockIdx.x >= few_from) {
-        few_piece<E, D, WAVES>(p, blockIdx.x - few_from, few_may_cut, {kt, vt, more}, joint);
+        few_piece<E, D>(p, blockIdx.x - few_from, few_may_cut, FewLds<D, WAVES>{kt, vt, more}, joint);
         return;
     }
     Unit u;
@@ -1081,7 +1111,7 @@ int64_t many_units(const PagedParams& p) {
 
 // Whether a row tile's keys may go to several work-groups.  Few rows: not where
 // the table's rows hold so few keys that the join, a launch more, costs more:
-// one sequence of 704 keys 10.0 us whole and 9.7 cut, but the host's part 10.1
+// one sequence of 704 keys 9.5 us whole and 9.2 cut, but the host's part 10.1
 // against 14.1; 64 of 700 keys 32.8 whole and 35.4 cut.  Many rows: row tiles
 // that fill half of SLOTS are taken whole.
 bool may_cut(const PagedParams& p, int kind) {
