@@ -86,9 +86,10 @@ typedef struct KdaPagedArgs {
 
 /* o = softmax(scale * q k^T) v over the cached keys each query sees, query
  * head h reading the cache's head h / (HQ / HKV); lse = log of the sum of
- * the exponentials.  A query that sees no key has o = 0 and lse = -inf.  What
- * the pages hold at and beyond seq_lens is not read into the result, whatever
- * it is; the keys and values before it have to be finite. */
+ * the exponentials.  A query that sees no key has o = 0 and lse = -inf; one
+ * with a score of NaN or +inf has NaN in both, and the other queries' results
+ * stay as they are.  What the pages hold at and beyond seq_lens is not read into the
+ * result, whatever it is; the keys and values before it have to be finite. */
 size_t kda_paged_attn_workspace_bytes(const KdaPagedArgs* args);
 int kda_paged_attn_hip(const KdaPagedArgs* args, void* stream);
 

@@ -555,8 +555,9 @@ template <class E, int D>
 __device__ __forceinline__ void store_o(const PagedParams& p, int64_t out, int d, float a, float b, float c, float e) {
     *reinterpret_cast<u32x2*>(p.o + out * D + d) = u32x2{E::pack(a, b), E::pack(c, e)};
 }
+// (l is 0 only where no key is seen; NaN, of scores that are not finite, stays)
 __device__ __forceinline__ float log_sum(float mc, float l) {
-    return l > 0.f ? (mc + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+    return l == 0.f ? -INFINITY : (mc + __builtin_amdgcn_logf(l)) * LN2;
 }
 
 // ---- few rows ----

@@ -254,8 +254,9 @@ def paged_attention(
 
     Returns ``o`` in q's shape and type, with ``return_lse`` also the log of
     the sum of the exponentials, fp32 ``[N, T, HQ]``.  A query that sees no
-    key (an empty sequence) has o = 0 and -inf.  What the pages hold beyond
-    ``seq_lens`` does not matter; keys and values before it have to be finite.
+    key (an empty sequence) has o = 0 and -inf, one with a score of NaN or +inf
+    NaN in both.  What the pages hold beyond ``seq_lens`` does not matter; keys and
+    values before it have to be finite.
     Forward only: raises if q requires a gradient.
     """
     f = _plain_fields(k_cache, v_cache, page_table, seq_lens, q, 0, cu_seqlens)
