@@ -138,8 +138,8 @@ size_t kda_pages_workspace_bytes(const KdaPagesArgs* args);
 /* Room for new_tokens[n] more tokens of every sequence n: the lowest free
  * pages, in the sequences' order, until they run out; seq_lens grows by as
  * many.  A sequence whose pages cannot all be had, or do not fit its row,
- * keeps what it has and its ok is 0 (then also every later one that needs a
- * page the earlier ones left none for). */
+ * keeps what it has and its ok is 0.  Once pages could not all be had, so is
+ * every later one's that needs a page. */
 int kda_pages_reserve_hip(const KdaPagesArgs* args, void* stream);
 
 /* Rows dst[0..F) become empty: their pages lose one holder each, their

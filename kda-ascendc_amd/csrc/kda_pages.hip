@@ -123,6 +123,8 @@ __device__ __forceinline__ int find_free(const PagesParams& p, int from, int wan
 // to the entry that its rank falls to, a thread a rank.  One, because each
 // sequence's pages follow from what the earlier ones take; bound by its chain of
 // loads, sums and barriers: 4.6 us for 32 sequences, 5.4 for 64.
+// Once the pages have run out no later sequence gets any, not even those that
+// the one they ran out in gives back: else it would depend on SEQS who does.
 constexpr int SEQS = 4096, RANKS = 4096;
 __global__ __launch_bounds__(1024) void pages_reserve_kernel(PagesParams p) {
     __shared__ int lds[16];
@@ -139,6 +141,7 @@ __global__ __launch_bounds__(1024) void pages_reserve_kernel(PagesParams p) {
         return max(0, pages_for((int)want, p.page_shift) - have);
     };
     int from = 0;
+    bool out = false;  // the pages have run out
     for (int n0 = 0; n0 < p.N; n0 += SEQS) {
         const int count = min(SEQS, p.N - n0);
         int needed = 0;
@@ -153,7 +156,7 @@ __global__ __launch_bounds__(1024) void pages_reserve_kernel(PagesParams p) {
             needed += total;
         }
         int found = 0;
-        for (int base = 0; base < needed && found == base; base += RANKS) {
+        for (int base = 0; !out && base < needed && found == base; base += RANKS) {
             int next;
             const int got = find_free<1024>(p, from, min(RANKS, needed - base), lds, next,
                                             [&](int rank, int page) { list[rank] = page; });
@@ -174,6 +177,7 @@ __global__ __launch_bounds__(1024) void pages_reserve_kernel(PagesParams p) {
             found += got;
             __syncthreads();
         }
+        out |= found < needed;
         for (int i = tid; i < count; i += 1024) {
             int have;
             const int n = n0 + i, need = need_of(n, have);

@@ -423,7 +423,8 @@ def paged_reserve(
     out; ``seq_lens`` grows by as many.
 
     Returns a bool ``[N]``: False for a sequence whose pages cannot all be
-    had, or do not fit its row; it keeps what it has.
+    had, or do not fit its row; it keeps what it has.  Once pages could not all
+    be had, later sequences get none.
     """
     dev = _check_counts(page_table, seq_lens, page_refs)
     if not _plain_rows(seq_lens, new_tokens, dev):
