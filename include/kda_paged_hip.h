@@ -111,7 +111,7 @@ typedef struct KdaPagesArgs {
     int32_t abi_version;  /* KDA_PAGED_ABI_VERSION */
     int32_t N;            /* rows of the page table */
     int32_t M;            /* entries a row */
-    int32_t P;            /* pages (rows of the pools) */
+    int32_t P;            /* pages (rows of the pools); with page_refs below 2^31 - 2^16 */
     int32_t page_size;    /* tokens a page, a power of two, 16 to 1024 */
     int32_t F;            /* rows to free or fork, pages to copy */
     int32_t num_pools;

@@ -139,6 +139,8 @@ int pages_params(const KdaPagesArgs* a, PagesParams& p, unsigned need) {
     }
     if (need & REFS) {
         if (!a->page_refs || misaligned(a->page_refs, 16)) return KDA_BT16_EINVAL;
+        // (the steps over the counts form numbers up to 2^15 past the last page)
+        if (a->P > I32_MAX - (1 << 16)) return KDA_BT16_EUNSUPPORTED;
         p.refs = a->page_refs;
     }
     if ((need & SRC) && a->F > 0 && (!a->src || misaligned(a->src, 4))) return KDA_BT16_EINVAL;
