@@ -87,6 +87,17 @@ __device__ __forceinline__ uint32_t wave_prefix(uint32_t x) {
     return x;
 }
 
+// The same with sums above `most` (below 2^31, as is every x) taken as `most`.
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t x, uint32_t most) {
+    x = min(x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false), most);
+    x = min(x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false), most);
+    x = min(x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false), most);
+    x = min(x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false), most);
+    x = min(x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false), most);
+    x = min(x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false), most);
+    return x;
+}
+
 // Pools and counts of a call on the pages (kda_paged_hip.h).
 struct PagesParams {
     int N, M, P, F, page_shift;

@@ -73,6 +73,27 @@ __device__ __forceinline__ int block_scan(int x, int* lds, int& total) {
     return before + inc - x;
 }
 
+// Exclusive prefix sum over the work-group's threads, and the total, of numbers
+// up to `most` (below 2^31), sums above it taken as `most`.
+template <int THREADS>
+__device__ __forceinline__ uint32_t block_scan_upto(uint32_t x, uint32_t most, int* lds, uint32_t& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t inc = wave_prefix(x, most);
+    __syncthreads();
+    if (lane == 63) lds[wave] = (int)inc;
+    __syncthreads();
+    uint32_t before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+        if (w == wave) before = total;
+        total = min(total + (uint32_t)lds[w], most);
+    }
+    // (the lane before's: a sum that was cut off says nothing about its parts)
+    const uint32_t last = __shfl_up(inc, 1);
+    return min(before + (lane == 0 ? 0u : last), most);
+}
+
 __device__ __forceinline__ int pages_for(int tokens, int shift) {
     return tokens <= 0 ? 0 : (int)(((int64_t)tokens + (1 << shift) - 1) >> shift);
 }
@@ -132,6 +153,8 @@ __global__ __launch_bounds__(1024) void pages_reserve_kernel(PagesParams p) {
     __shared__ int list[RANKS];
     const int tid = threadIdx.x;
     const int64_t most = (int64_t)p.M << p.page_shift;
+    // More than there are: what sums of needs stop at (they may pass 32 bits).
+    const uint32_t beyond = (uint32_t)p.P + 1;
     // pages that sequence n needs beyond those it has; -1: more than a row holds
     auto need_of = [&](int n, int& have) {
         const int len = max(0, p.lens[n]);
@@ -144,17 +167,19 @@ __global__ __launch_bounds__(1024) void pages_reserve_kernel(PagesParams p) {
     bool out = false;  // the pages have run out
     for (int n0 = 0; n0 < p.N; n0 += SEQS) {
         const int count = min(SEQS, p.N - n0);
-        int needed = 0;
+        uint32_t sum = 0;
         for (int i0 = 0; i0 < count; i0 += 1024) {
-            int have = 0, total;
-            const int need = i0 + tid < count ? max(0, need_of(n0 + i0 + tid, have)) : 0;
-            const int before = block_scan<1024>(need, lds, total);
+            int have = 0;
+            uint32_t total;
+            const uint32_t need = i0 + tid < count ? max(0, need_of(n0 + i0 + tid, have)) : 0;
+            const uint32_t before = block_scan_upto<1024>(min(need, beyond), beyond, lds, total);
             if (i0 + tid < count) {
-                start[i0 + tid] = needed + before;
+                start[i0 + tid] = (int)min(sum + before, beyond);
                 had[i0 + tid] = have;
             }
-            needed += total;
+            sum = min(sum + total, beyond);
         }
+        const int needed = (int)sum;
         int found = 0;
         for (int base = 0; !out && base < needed && found == base; base += RANKS) {
             int next;
@@ -181,12 +206,12 @@ __global__ __launch_bounds__(1024) void pages_reserve_kernel(PagesParams p) {
         for (int i = tid; i < count; i += 1024) {
             int have;
             const int n = n0 + i, need = need_of(n, have);
-            const bool ok = need == 0 || (need > 0 && start[i] + need <= found);
+            const bool ok = need == 0 || (need > 0 && need <= found - start[i]);
             if (ok) {
                 p.lens[n] = max(0, p.lens[n]) + max(0, p.more[n]);
             } else if (need > 0) {
                 // pages ran out inside it: what it got goes back
-                for (int j = 0; start[i] + j < found; ++j) {
+                for (int j = 0; j < found - start[i]; ++j) {
                     int32_t* entry = p.table + n * p.table_stride + have + j;
                     p.refs[*entry] = 0;
                     *entry = -1;

@@ -50,3 +50,25 @@ def test_thousands_of_sequences(N, P, seed, gpu_device):
 def test_more_than_4096_pages_for_few_sequences(P, gpu_device):
     s = pages(5, 5000, P, 7, gpu_device, used=0.4)
     reserve(s, [16 * 1000, 3, 16 * 3000 + 5, 16 * 4100, 1])
+
+
+# Tables of 11 GB and 19 GB; requests for more than 2^31 pages in all, and for more than 2^32.
+@pytest.mark.parametrize("N,M", [(4096, 5 << 17), (70, (1 << 26) - 1)])
+def test_requests_past_32_bits(N, M, gpu_device):
+    """More pages wanted than 32 bits count: the first two rows get theirs, the
+    third what is left and gives it back, the others none."""
+    P, size, dev = 100, 16, gpu_device
+    table = torch.full((N, M), -1, dtype=torch.int32, device=dev)
+    lens = torch.zeros(N, dtype=torch.int32, device=dev)
+    refs = torch.zeros(P, dtype=torch.int32, device=dev)
+    refs[::2] = 1
+    more = torch.full((N,), M * size, dtype=torch.int32, device=dev)
+    more[:2] = torch.tensor([1, 33], dtype=torch.int32)
+    more[-2:] = torch.tensor([0, 8 * size], dtype=torch.int32)
+    ok = paged_reserve(table, lens, refs, more, size)
+    assert ok.tolist() == [True, True] + [False] * (N - 4) + [True, False]
+    assert lens.tolist() == [1, 33] + [0] * (N - 2)
+    assert refs.tolist() == [int(p % 2 == 0 or p < 8) for p in range(P)]
+    assert table[0, :2].tolist() == [1, -1] and table[1, :4].tolist() == [3, 5, 7, -1]
+    held = [n for n in range(N) if bool((table[n] >= 0).any())]
+    assert held == [0, 1]
