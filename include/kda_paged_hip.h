@@ -15,8 +15,9 @@
  *                                       tokens; page, token and head strides
  *                                       are given in elements, multiples of
  *                                       8, a token's stride at least D
- *   page_table  [N, M] int32            the pages of each sequence in order
- *                                       (row stride given), -1: none
+ *   page_table  [N, M] int32            the pages of each sequence in order,
+ *                                       from the first entry on (row stride
+ *                                       given), -1: none
  *   seq_lens    [N] int32               cached tokens of each sequence, those
  *                                       of the call included
  *   page_refs   [P] int32               how many sequences hold each page; 0:
@@ -24,7 +25,10 @@
  * The new tokens of a call are [N, T, heads, D], or with cu_seqlens ([N + 1]
  * int32 or int64, from 0 to T, non-decreasing) T tokens of N sequences packed
  * one after another.  Sequence n's new tokens are its last ones: token i of
- * T_n sits at position seq_lens[n] - T_n + i.
+ * T_n sits at position seq_lens[n] - T_n + i.  Lowering seq_lens[n] takes the
+ * last tokens back, those of a rejected draft: the pages behind the new length
+ * stay the row's until it grows into them or ends.  It must not become shorter
+ * than what it shares with a fork, whose page its next tokens would go into.
  *
  * Table entries outside [0, P), lengths beyond M * page_size, offsets outside
  * [0, T] and row numbers outside [0, N) give unspecified results but never an
@@ -135,9 +139,9 @@ typedef struct KdaPagesArgs {
 /* Workspace of kda_pages_compact_hip (P read). */
 size_t kda_pages_workspace_bytes(const KdaPagesArgs* args);
 
-/* Room for new_tokens[n] more tokens of every sequence n: the lowest free
- * pages, in the sequences' order, until they run out; seq_lens grows by as
- * many.  A sequence whose pages cannot all be had, or do not fit its row,
+/* Room for new_tokens[n] more tokens of every sequence n: first the held pages
+ * that follow its tokens' in its row, then the lowest free pages, in the
+ * sequences' order, until they run out; seq_lens grows by as many.  A sequence whose pages cannot all be had, or do not fit its row,
  * keeps what it has and its ok is 0.  Once pages could not all be had, so is
  * every later one's that needs a page. */
 int kda_pages_reserve_hip(const KdaPagesArgs* args, void* stream);
@@ -146,7 +150,7 @@ int kda_pages_reserve_hip(const KdaPagesArgs* args, void* stream);
  * entries become -1, their lengths 0.  A row named twice is freed once. */
 int kda_pages_free_hip(const KdaPagesArgs* args, void* stream);
 
-/* Row dst[i] (empty, named once) becomes a copy of row src[i]: whole pages
+/* Row dst[i] (new or freed, named once) becomes a copy of row src[i]: whole pages
  * are shared, the tokens of a last partial page are copied, in every pool, to
  * the lowest free page not taken by an earlier fork.  Without a free page the
  * row stays empty and ok[i] is 0.  No row is in src and in dst. */

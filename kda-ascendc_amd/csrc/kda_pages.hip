@@ -144,6 +144,8 @@ __device__ __forceinline__ int find_free(const PagesParams& p, int from, int wan
 // to the entry that its rank falls to, a thread a rank.  One, because each
 // sequence's pages follow from what the earlier ones take; bound by its chain of
 // loads, sums and barriers: 4.6 us for 32 sequences, 5.4 for 64.
+// A row's entries past its tokens are looked at one by one, but only where
+// tokens need more pages: one entry each unless its length was lowered.
 // Once the pages have run out no later sequence gets any, not even those that
 // the one they ran out in gives back: else it would depend on SEQS who does.
 constexpr int SEQS = 4096, RANKS = 4096;
@@ -155,13 +157,23 @@ __global__ __launch_bounds__(1024) void pages_reserve_kernel(PagesParams p) {
     const int64_t most = (int64_t)p.M << p.page_shift;
     // More than there are: what sums of needs stop at (they may pass 32 bits).
     const uint32_t beyond = (uint32_t)p.P + 1;
-    // pages that sequence n needs beyond those it has; -1: more than a row holds
-    auto need_of = [&](int n, int& have) {
-        const int len = max(0, p.lens[n]);
-        have = pages_for(len, p.page_shift);
+    // pages that sequence n holds in all once it has its tokens; -1: more than
+    // a row holds
+    auto pages_of = [&](int n, int& len) {
+        len = max(0, p.lens[n]);
         const int64_t want = (int64_t)len + max(0, p.more[n]);
-        if (want > most) return -1;
-        return max(0, pages_for((int)want, p.page_shift) - have);
+        return want > most ? -1 : pages_for((int)want, p.page_shift);
+    };
+    // pages that it has: those of its tokens, and any that follow them in its
+    // row (its length was lowered: the tokens of a rejected draft)
+    auto pages_had = [&](int n, int len, int want) {
+        const int32_t* row = p.table + n * p.table_stride;
+        int have = pages_for(len, p.page_shift);
+        for (; have < want; ++have) {
+            const uint32_t page = (uint32_t)row[have];
+            if (page >= (uint32_t)p.P || p.refs[page] == 0) break;
+        }
+        return have;
     };
     int from = 0;
     bool out = false;  // the pages have run out
@@ -169,9 +181,14 @@ __global__ __launch_bounds__(1024) void pages_reserve_kernel(PagesParams p) {
         const int count = min(SEQS, p.N - n0);
         uint32_t sum = 0;
         for (int i0 = 0; i0 < count; i0 += 1024) {
-            int have = 0;
+            int have = 0, want = 0;
             uint32_t total;
-            const uint32_t need = i0 + tid < count ? max(0, need_of(n0 + i0 + tid, have)) : 0;
+            if (i0 + tid < count) {
+                int len;
+                want = pages_of(n0 + i0 + tid, len);
+                have = pages_had(n0 + i0 + tid, len, want);
+            }
+            const uint32_t need = max(0, want - have);
             const uint32_t before = block_scan_upto<1024>(min(need, beyond), beyond, lds, total);
             if (i0 + tid < count) {
                 start[i0 + tid] = (int)min(sum + before, beyond);
@@ -204,12 +221,12 @@ __global__ __launch_bounds__(1024) void pages_reserve_kernel(PagesParams p) {
         }
         out |= found < needed;
         for (int i = tid; i < count; i += 1024) {
-            int have;
-            const int n = n0 + i, need = need_of(n, have);
-            const bool ok = need == 0 || (need > 0 && need <= found - start[i]);
+            int len;
+            const int n = n0 + i, want = pages_of(n, len), have = had[i];
+            const bool fits = want >= 0, ok = fits && (want <= have || want - have <= found - start[i]);
             if (ok) {
-                p.lens[n] = max(0, p.lens[n]) + max(0, p.more[n]);
-            } else if (need > 0) {
+                p.lens[n] = len + max(0, p.more[n]);
+            } else if (fits) {
                 // pages ran out inside it: what it got goes back
                 for (int j = 0; j < found - start[i]; ++j) {
                     int32_t* entry = p.table + n * p.table_stride + have + j;

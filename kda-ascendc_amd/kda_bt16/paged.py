@@ -11,7 +11,8 @@ The cache of a layer is a pool of pages for its keys and one for its values,
 contiguous (tokens of a head together, ``[P, HKV, page_size, D]`` transposed,
 read in longer pieces).  One table serves all layers:
 
-* ``page_table`` ``[N, M]`` int32: the pages of each sequence, -1 for none;
+* ``page_table`` ``[N, M]`` int32: the pages of each sequence, from the first
+  entry on, -1 for none;
 * ``seq_lens`` ``[N]`` int32: its cached tokens, those of the call included;
 * ``page_refs`` ``[P]`` int32: the sequences that hold each page, 0 if it is
   free.
@@ -25,7 +26,13 @@ length on the host.  A step of a serving loop::
         o = paged_attention(q, layer.k_cache, layer.v_cache, page_table, seq_lens)
 
 The new tokens of a sequence are its last ones: token i of T sits at position
-``seq_lens - T + i``.  Entries outside ``[0, P)``, lengths beyond the table's
+``seq_lens - T + i``.  Lowering ``seq_lens`` takes a sequence's last tokens
+back, those of a rejected draft; the pages behind its new length stay its own
+until it grows into them (:func:`paged_reserve`) or ends.  It must not become
+shorter than what it shares with a fork: its next tokens go into the page that
+it then ends in.
+
+Entries outside ``[0, P)``, lengths beyond the table's
 rows and row numbers outside ``[0, N)`` give unspecified results but never an
 access outside the tensors.
 """
@@ -419,8 +426,9 @@ def paged_reserve(
     page_size: int,
 ) -> torch.Tensor:
     """Room for ``new_tokens[n]`` (int32 ``[N]``) more tokens of every
-    sequence: the lowest free pages, in the sequences' order, until they run
-    out; ``seq_lens`` grows by as many.
+    sequence: first the pages that its row holds past its length, then the
+    lowest free ones, in the sequences' order, until they run out;
+    ``seq_lens`` grows by as many.
 
     Returns a bool ``[N]``: False for a sequence whose pages cannot all be
     had, or do not fit its row; it keeps what it has.  Once pages could not all
@@ -469,7 +477,7 @@ def paged_fork(
     *,
     page_size: int | None = None,
 ) -> torch.Tensor:
-    """Row ``dst[i]`` (empty) becomes a copy of row ``src[i]`` (int32): whole
+    """Row ``dst[i]`` (new or freed) becomes a copy of row ``src[i]`` (int32): whole
     pages are shared, the tokens of a last partial page copied, in every pool,
     to the lowest free page not taken by an earlier fork.
 
