@@ -32,9 +32,10 @@ until it grows into them (:func:`paged_reserve`) or ends.  It must not become
 shorter than what it shares with a fork: its next tokens go into the page that
 it then ends in.
 
-Entries outside ``[0, P)``, lengths beyond the table's
-rows and row numbers outside ``[0, N)`` give unspecified results but never an
-access outside the tensors.
+Entries outside ``[0, P)``, lengths beyond the table's rows and row numbers
+outside ``[0, N)`` give unspecified results but never an access outside the
+tensors.  Forward only: where gradients are recorded, keys,
+values, queries, caches and pools that require one are refused.
 """
 
 from __future__ import annotations
@@ -213,6 +214,14 @@ def _fields(k, v, table, lens, x, cu_seqlens) -> tuple:
             *_strides(x))
 
 
+def _forward_only(name: str, *tensors: torch.Tensor) -> None:
+    """The launches are outside of autograd: a gradient would be lost."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise NotImplementedError(f"{name} is forward only: inputs require grad")
+
+
 def _launch(name: str, args: bytes, device: torch.device) -> None:
     """The entry point on the tensors' device and its current stream."""
     if torch._C._cuda_getDevice() == device.index:
@@ -264,7 +273,6 @@ def paged_attention(
     key (an empty sequence) has o = 0 and -inf, one with a score of NaN or +inf
     NaN in both.  What the pages hold beyond ``seq_lens`` does not matter; keys and
     values before it have to be finite.
-    Forward only: raises if q requires a gradient.
     """
     f = _plain_fields(k_cache, v_cache, page_table, seq_lens, q, 0, cu_seqlens)
     if f is None:
@@ -283,8 +291,7 @@ def paged_attention(
             raise ValueError(f"window must be at least 1, got {window}")
         if not causal:
             raise ValueError("window needs causal=True")
-    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
-        raise NotImplementedError("paged_attention is forward only: inputs require grad")
+    _forward_only("paged_attention", q, k_cache, v_cache)
     if f is None:
         _require_gpu(q)
         f = _fields(k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
@@ -331,6 +338,8 @@ def paged_append(
             _check_new(name, t, k_cache.shape[2], k_cache, page_table, cu_seqlens)
         if v.shape != k.shape:
             raise ValueError(f"v.shape {tuple(v.shape)} must match k {tuple(k.shape)}")
+    _forward_only("paged_append", k, v, k_cache, v_cache)
+    if f is None:
         _require_gpu(k)
         f = _fields(k_cache, v_cache, page_table, seq_lens, k, cu_seqlens) + _strides(v)
     (N, T, HQ, HKV, D, dt, P, size, M, cu_dtype, cu, table, table_stride, lens, kp, vp, s0, s1, s2, t0, t1, t2, u0, u1,
@@ -501,6 +510,7 @@ def paged_fork(
     P, F = ts[0].shape[-4], src.shape[0]
     if page_refs.shape[0] != P:
         raise ValueError(f"page_refs must have one entry a page, {P}, got {page_refs.shape[0]}")
+    _forward_only("paged_fork", *ts)
     _require_gpu(ts[0])
     ok = src.new_empty(F, dtype=torch.bool)
     N, M = page_table.shape
@@ -524,6 +534,7 @@ def paged_copy(pools, src: torch.Tensor, dst: torch.Tensor) -> None:
     device = ts[0].device
     if not _plain_rows(src, dst, ts[0].get_device()):
         _check_rows([("src", src), ("dst", dst)], device)
+    _forward_only("paged_copy", *ts)
     _require_gpu(ts[0])
     P = ts[0].shape[-4]
     _launch("kda_pages_copy_hip", _pack(P, 16, src.shape[0], len(ts), _pool_fields(ts, P), 0, src=src.data_ptr(),
@@ -555,6 +566,7 @@ def paged_compact(
     _check_refs(page_refs, device)
     if page_refs.shape[0] != P:
         raise ValueError(f"page_refs must have one entry a page, {P}, got {page_refs.shape[0]}")
+    _forward_only("paged_compact", *ts)
     _require_gpu(ts[0])
     N, M = page_table.shape
     table = torch.empty_like(page_table) if page_table.is_contiguous() else page_table.new_empty((N, M))
