@@ -787,8 +787,9 @@ __device__ __forceinline__ void meet() {
 // and an exponential every 6.8, and the loads' addresses took 80 scalar ones);
 // with the places of 64 tiles found at once the prompt takes 970 kilocycles
 // instead of 1137 and 489 to 516 us (1.1 PFLOP/s; a bf16 product of 8192^3
-// reaches 1.15 to 1.2 on the same card), the matrix unit 54% busy.  What bounds
-// it now is the card's power: the clock, 2.08 GHz before, went down to 1.90.
+// reaches 1.15 to 1.2 on the same card), the matrix unit 54% busy.  15% fewer
+// cycles were 6% less time: the clock (cycles over time) went from 2.08 to 1.90
+// GHz, which looks like the card's power; no reading of it was taken.
 // No gain from: two or three groups of operands ahead instead of one, both
 // products in one straight block (540), the loads begun between matrix ops (540
 // to 553), other orders of the softmax's operations.
@@ -967,9 +968,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void paged_few_kernel(PagedParams p,
 
 // MIXED: the work-groups from `few_from` on take the sequences of few rows, with
 // as many waves: packed batches of chunks and single tokens in one launch, the
-// few rows on the CUs that the chunks' last row tiles leave (63 sequences of a
-// new token and one of 512: 316 us in two launches, 247 so; 8 sequences of 1 to
-// 1024 new tokens, a window of 4096: 144 and 140).
+// few rows on the CUs that the chunks' last row tiles leave (32 / 8 heads, 63
+// sequences of a new token and 256 to 16384 keys and one of 512 after 5488: 316
+// us in two launches, 240 to 247 so; 8 sequences of 1 to 1024 new tokens, a
+// window of 4096: 144 and 140).
 template <class E, int D, bool MIXED_KINDS>
 __global__ __launch_bounds__(512, 2) void paged_many_kernel(PagedParams p, bool cut, bool sort, unsigned few_from, bool few_may_cut) {
     constexpr int WAVES = Shape<MANY>::WAVES, RING = 3 * Shape<MANY>::TK * D * 2;

@@ -143,7 +143,8 @@ __device__ __forceinline__ int find_free(const PagesParams& p, int from, int wan
 // pages that are needed; then, RANKS at a time, the free pages in order, each
 // to the entry that its rank falls to, a thread a rank.  One, because each
 // sequence's pages follow from what the earlier ones take; bound by its chain of
-// loads, sums and barriers: 4.6 us for 32 sequences, 5.4 for 64.
+// loads, sums and barriers: 5.4 us for 32 sequences, 6.2 for 64 (0.8 of it the
+// look into the row and sums that stop in time).
 // A row's entries past its tokens are looked at one by one, but only where
 // tokens need more pages: one entry each unless its length was lowered.
 // Once the pages have run out no later sequence gets any, not even those that
