@@ -101,6 +101,24 @@ int kda_paged_attn_hip(const KdaPagedArgs* args, void* stream);
  * negative positions, beyond the table or on no page are left out. */
 int kda_paged_append_hip(const KdaPagedArgs* args, void* stream);
 
+/* The append with the position rotation on the way, and the queries' with it. */
+typedef struct KdaPagedRotaryArgs {
+    KdaPagedArgs paged;     /* as for the append; q and its strides: the queries, HQ heads (any number) */
+    const float* inv_freq;  /* [rotary_dim / 2] fp32: angle per position of each pair */
+    int32_t rotary_dim;     /* elements of a head that are turned, the first: a multiple of 16, 16 to D */
+    int32_t interleaved;    /* 0: pairs (i, i + rotary_dim / 2); else (2 i, 2 i + 1) */
+    void* q_out;            /* [N, T, HQ, D] by the strides below; q itself (with q's strides) or apart from it */
+    int64_t out_row, out_token, out_head;
+} KdaPagedRotaryArgs;
+
+/* A pair (a, b) of the token at position p becomes (a cos x - b sin x,
+ * b cos x + a sin x), x = p * inv_freq of the pair, in every head of the
+ * queries (to q_out) and of the new keys (into their places in the pages); the
+ * values go into theirs as they are.  Tokens that the append leaves out have
+ * their queries turned all the same, by their positions; tokens of no sequence
+ * (packed, before the first offset or behind the last) are left as they are. */
+int kda_paged_append_rotary_hip(const KdaPagedRotaryArgs* args, void* stream);
+
 #define KDA_PAGED_MAX_POOLS 8
 
 /* A pool: [lead, P, ...] contiguous, `page_bytes` a page (a multiple of 16),

@@ -67,6 +67,17 @@ __device__ __forceinline__ NewTokens new_tokens(const PagedParams& p, int n) {
     return s;
 }
 
+// The sequence of packed token t: the largest n with cu[n] <= t.
+__device__ __forceinline__ int sequence_of(const PagedParams& p, int t) {
+    int lo = 0, hi = p.N - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (paged_cu(p, mid) <= t) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
 // Entry i of sequence n's row of the page table: the last one for any i past
 // it.  A page only if is_page().
 __device__ __forceinline__ int table_entry(const PagedParams& p, int n, int i) {
@@ -117,9 +128,19 @@ struct PagesParams {
     int32_t* ws;
 };
 
+// The append with the position rotation (kda_paged_hip.h).
+struct RotaryParams : PagedParams {
+    const float* inv_freq;
+    int units;  // of 16 turned elements
+    int interleaved;
+    uint16_t* q_out;
+    int64_t out_row, out_token, out_head;
+};
+
 size_t paged_attn_workspace(const PagedParams& p, int D);
 hipError_t launch_paged_attn(const PagedParams& p, int D, hipStream_t stream);
 hipError_t launch_paged_append(const PagedParams& p, int D, hipStream_t stream);
+hipError_t launch_paged_append_rotary(const RotaryParams& p, int D, hipStream_t stream);
 hipError_t launch_pages_reserve(const PagesParams& p, hipStream_t stream);
 hipError_t launch_pages_free(const PagesParams& p, hipStream_t stream);
 hipError_t launch_pages_fork(const PagesParams& p, hipStream_t stream);

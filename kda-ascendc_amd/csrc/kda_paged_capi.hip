@@ -110,6 +110,26 @@ int attn_params(const KdaPagedArgs* a, PagedParams& p) {
     return KDA_BT16_OK;
 }
 
+int append_params(const KdaPagedArgs* a, PagedParams& p) {
+    const int rc = paged_params(a, p);
+    if (rc != KDA_BT16_OK) return rc;
+    if (!a->new_k || !a->new_v || misaligned(a->new_k, 16) || misaligned(a->new_v, 16)) return KDA_BT16_EINVAL;
+    if (!strides_ok(a->nk_row, a->nk_token, a->nk_head) || !strides_ok(a->nv_row, a->nv_token, a->nv_head))
+        return KDA_BT16_EINVAL;
+    const int64_t tokens = a->cu_seqlens ? a->T : (int64_t)a->N * a->T;
+    // one thread for each 16 bytes of a token's keys
+    if (tokens > I32_MAX / 16 / a->HKV) return KDA_BT16_EUNSUPPORTED;
+    p.nk = static_cast<const uint16_t*>(a->new_k);
+    p.nv = static_cast<const uint16_t*>(a->new_v);
+    p.nk_row = a->nk_row;
+    p.nk_token = a->nk_token;
+    p.nk_head = a->nk_head;
+    p.nv_row = a->nv_row;
+    p.nv_token = a->nv_token;
+    p.nv_head = a->nv_head;
+    return KDA_BT16_OK;
+}
+
 enum Need { POOLS = 1, TABLE = 2, REFS = 4, SRC = 8, DST = 16, WS = 32 };
 
 int pages_params(const KdaPagesArgs* a, PagesParams& p, unsigned need) {
@@ -190,25 +210,38 @@ int kda_paged_attn_hip(const KdaPagedArgs* args, void* stream) {
 
 int kda_paged_append_hip(const KdaPagedArgs* args, void* stream) {
     PagedParams p;
-    const int rc = paged_params(args, p);
+    const int rc = append_params(args, p);
     if (rc != KDA_BT16_OK) return rc;
-    if (!args->new_k || !args->new_v || misaligned(args->new_k, 16) || misaligned(args->new_v, 16))
-        return KDA_BT16_EINVAL;
-    if (!strides_ok(args->nk_row, args->nk_token, args->nk_head) ||
-        !strides_ok(args->nv_row, args->nv_token, args->nv_head))
-        return KDA_BT16_EINVAL;
-    const int64_t tokens = args->cu_seqlens ? args->T : (int64_t)args->N * args->T;
-    // one thread for each 16 bytes of a token's keys
-    if (tokens > I32_MAX / 16 / args->HKV) return KDA_BT16_EUNSUPPORTED;
-    p.nk = static_cast<const uint16_t*>(args->new_k);
-    p.nv = static_cast<const uint16_t*>(args->new_v);
-    p.nk_row = args->nk_row;
-    p.nk_token = args->nk_token;
-    p.nk_head = args->nk_head;
-    p.nv_row = args->nv_row;
-    p.nv_token = args->nv_token;
-    p.nv_head = args->nv_head;
     return launched(kda::launch_paged_append(p, args->D, static_cast<hipStream_t>(stream)));
+}
+
+int kda_paged_append_rotary_hip(const KdaPagedRotaryArgs* args, void* stream) {
+    if (args == nullptr) return KDA_BT16_EINVAL;
+    const KdaPagedArgs* a = &args->paged;
+    kda::RotaryParams p{};
+    const int rc = append_params(a, p);
+    if (rc != KDA_BT16_OK) return rc;
+    if (a->HQ <= 0 || !a->q || !args->q_out || !args->inv_freq) return KDA_BT16_EINVAL;
+    if (misaligned(a->q, 16) || misaligned(args->q_out, 16) || misaligned(args->inv_freq, 4)) return KDA_BT16_EINVAL;
+    if (!strides_ok(a->q_row, a->q_token, a->q_head) ||
+        !strides_ok(args->out_row, args->out_token, args->out_head))
+        return KDA_BT16_EINVAL;
+    if (args->rotary_dim < 16 || args->rotary_dim > a->D || args->rotary_dim % 16 != 0) return KDA_BT16_EUNSUPPORTED;
+    const int64_t tokens = a->cu_seqlens ? a->T : (int64_t)a->N * a->T;
+    // one thread for each 16 elements of a token
+    if (((int64_t)a->HQ + 2 * (int64_t)a->HKV) > I32_MAX / 16 / tokens) return KDA_BT16_EUNSUPPORTED;
+    p.q = static_cast<const uint16_t*>(a->q);
+    p.q_row = a->q_row;
+    p.q_token = a->q_token;
+    p.q_head = a->q_head;
+    p.inv_freq = args->inv_freq;
+    p.units = args->rotary_dim / 16;
+    p.interleaved = args->interleaved;
+    p.q_out = static_cast<uint16_t*>(args->q_out);
+    p.out_row = args->out_row;
+    p.out_token = args->out_token;
+    p.out_head = args->out_head;
+    return launched(kda::launch_paged_append_rotary(p, a->D, static_cast<hipStream_t>(stream)));
 }
 
 size_t kda_pages_workspace_bytes(const KdaPagesArgs* args) {

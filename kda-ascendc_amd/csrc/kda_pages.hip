@@ -15,17 +15,6 @@ namespace {
 
 // ---- append ----
 
-// The sequence of packed token t: the largest n with cu[n] <= t.
-__device__ __forceinline__ int sequence_of(const PagedParams& p, int t) {
-    int lo = 0, hi = p.N - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (paged_cu(p, mid) <= t) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
-}
-
 // One thread moves 16 bytes of a token's keys and the same of its values: as
 // many threads as there are pieces, since what bounds it is the chain of loads
 // before them (sequence, length, table entry).  128 tokens of 8 heads 3.2 us on

@@ -32,6 +32,7 @@ from .kernels import (
 )
 from .paged import (
     paged_append,
+    paged_append_rotary,
     paged_attention,
     paged_compact,
     paged_copy,
@@ -56,6 +57,7 @@ __all__ = [
     "dispatch",
     "paged_attention",
     "paged_append",
+    "paged_append_rotary",
     "paged_reserve",
     "paged_free",
     "paged_fork",

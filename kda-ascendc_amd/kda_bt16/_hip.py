@@ -68,6 +68,7 @@ PAGED_SYMBOLS = (
     "kda_paged_attn_workspace_bytes",
     "kda_paged_attn_hip",
     "kda_paged_append_hip",
+    "kda_paged_append_rotary_hip",
     "kda_pages_workspace_bytes",
     "kda_pages_reserve_hip",
     "kda_pages_free_hip",
@@ -189,6 +190,21 @@ class KdaPagedArgs(ctypes.Structure):
     ]
 
 
+class KdaPagedRotaryArgs(ctypes.Structure):
+    """Mirror of ``struct KdaPagedRotaryArgs``."""
+
+    _fields_ = [
+        ("paged", KdaPagedArgs),
+        ("inv_freq", ctypes.c_void_p),
+        ("rotary_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("q_out", ctypes.c_void_p),
+        ("out_row", ctypes.c_int64),
+        ("out_token", ctypes.c_int64),
+        ("out_head", ctypes.c_int64),
+    ]
+
+
 class KdaPagePool(ctypes.Structure):
     """Mirror of ``struct KdaPagePool``."""
 
@@ -247,6 +263,8 @@ def _packer(fields) -> struct.Struct:
 PAGED_PACK = _packer(KdaPagedArgs._fields_[:-2])
 PAGES_PACK = _packer(KdaPagesArgs._fields_[:-2])
 WORKSPACE_PACK = _packer(KdaPagedArgs._fields_[-2:])
+# What follows the paged arguments in the structs that begin with them.
+ROTARY_PACK = _packer(KdaPagedRotaryArgs._fields_[1:])
 NO_WORKSPACE = WORKSPACE_PACK.pack(0, 0)
 
 

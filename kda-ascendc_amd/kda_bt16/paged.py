@@ -111,6 +111,15 @@ def _check_cache(k_cache, v_cache, page_table, seq_lens) -> None:
     _check_table(page_table, seq_lens, k_cache.device)
 
 
+def _check_written(name: str, t: torch.Tensor) -> None:
+    """No element of a strided output is another's."""
+    need = t.shape[-1]
+    for stride, n in sorted((t.stride(i), t.shape[i]) for i in range(t.ndim - 1) if t.shape[i] > 1):
+        if stride < need:
+            raise ValueError(f"{name}'s elements must not overlap, got strides {t.stride()}")
+        need = stride * n
+
+
 def _check_new(name: str, t: torch.Tensor, heads: int | None, k_cache, page_table, cu_seqlens) -> None:
     """Tensors of the new tokens: [N, T, heads, D], or [1, T, heads, D] packed."""
     if t.ndim != 4:
@@ -348,6 +357,77 @@ def paged_append(
         _hip.PAGED_ABI_VERSION, N, T, HQ, HKV, D, dt, P, size, M, 0, 0, 1.0, cu_dtype, cu, table, table_stride, lens, kp,
         vp, s0, s1, s2, t0, t1, t2, 0, 0, 0, 0, 0, 0, k.data_ptr(), v.data_ptr(), u0, u1, u2, *w) + _hip.NO_WORKSPACE,
         k.device)
+
+
+def paged_append_rotary(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    page_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    inv_freq: torch.Tensor,
+    *,
+    interleaved: bool = False,
+    cu_seqlens: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`paged_append` with the position rotation on the way: the new
+    tokens' queries and keys are turned by their positions, the keys and values
+    go into their places in the pages, the turned queries are returned.
+
+    ``q`` is ``[N, T, HQ, D]`` (any HQ) or packed ``[1, total, HQ, D]``, ``k``
+    and ``v`` as for the append; all may be views (slices of a fused
+    projection).  ``inv_freq`` (fp32 ``[R / 2]``, R a multiple of 16 up to D)
+    is the angle per position of each pair of the first R elements of a head:
+    ``base ** (-2 j / R)`` as it is or scaled.  Pairs are elements j and
+    j + R / 2, or with ``interleaved`` 2 j and 2 j + 1; elements from R on stay
+    as they are.  Angles are formed in 64 bits, the rotation in fp32, rounded
+    once.
+
+    ``out`` is where the turned queries go, in q's shape and type: ``q`` itself
+    (turned in place) or a tensor of other storage; by default a new one.
+    Queries of tokens that the append leaves out are turned all the same;
+    packed tokens of no sequence (behind the last offset) are not written.
+    """
+    shape = q.shape
+    if k.ndim == 4 and v.ndim == 4 and (k.shape[:2] != shape[:2] or v.shape != k.shape):
+        raise ValueError(f"q, k and v must have the same tokens and k and v the same heads, got shapes {tuple(shape)}, "
+                         f"{tuple(k.shape)} and {tuple(v.shape)}")
+    _check_cache(k_cache, v_cache, page_table, seq_lens)
+    for name, t, heads in (("q", q, None), ("k", k, k_cache.shape[2]), ("v", v, k_cache.shape[2])):
+        _check_new(name, t, heads, k_cache, page_table, cu_seqlens)
+    D = shape[-1]
+    if inv_freq.ndim != 1 or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
+        raise ValueError(f"inv_freq must be contiguous 1D float32, got {inv_freq.dtype} with shape {tuple(inv_freq.shape)}")
+    if inv_freq.device != q.device:
+        raise ValueError(f"inv_freq device {inv_freq.device} must match q ({q.device})")
+    R = 2 * inv_freq.shape[0]
+    if R < 16 or R > D or R % 16:
+        raise ValueError(f"twice inv_freq's entries must be a multiple of 16 from 16 to the head size {D}, got {R}")
+    _forward_only("paged_append_rotary", q, k, v, k_cache, v_cache, inv_freq)
+    if out is None:
+        _require_gpu(q)
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    else:
+        _check_new("out", out, shape[2], k_cache, page_table, cu_seqlens)
+        if out.shape != shape:
+            raise ValueError(f"out.shape {tuple(out.shape)} must match q {tuple(shape)}")
+        _check_written("out", out)
+        _forward_only("paged_append_rotary", out)
+        if (out.data_ptr() != q.data_ptr() or out.stride() != q.stride()) and out.untyped_storage().data_ptr() in {
+                t.untyped_storage().data_ptr() for t in (q, k, v, k_cache, v_cache)}:
+            raise ValueError("out must be q itself or of other storage than the inputs")
+    _require_gpu(q)
+    (N, T, _, HKV, D, dt, P, size, M, cu_dtype, cu, table, table_stride, lens, kp, vp, s0, s1, s2, t0, t1, t2, u0, u1,
+     u2) = _fields(k_cache, v_cache, page_table, seq_lens, k, cu_seqlens)
+    _launch("kda_paged_append_rotary_hip", _hip.PAGED_PACK.pack(
+        _hip.PAGED_ABI_VERSION, N, T, shape[2], HKV, D, dt, P, size, M, 0, 0, 1.0, cu_dtype, cu, table, table_stride, lens,
+        kp, vp, s0, s1, s2, t0, t1, t2, q.data_ptr(), *_strides(q), 0, 0, k.data_ptr(), v.data_ptr(), u0, u1, u2,
+        *_strides(v)) + _hip.NO_WORKSPACE + _hip.ROTARY_PACK.pack(
+            inv_freq.data_ptr(), R, interleaved, out.data_ptr(), *_strides(out)), q.device)
+    return out
 
 
 def _pools(pools) -> list[torch.Tensor]:
