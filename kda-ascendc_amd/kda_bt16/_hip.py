@@ -263,8 +263,7 @@ def _packer(fields) -> struct.Struct:
 PAGED_PACK = _packer(KdaPagedArgs._fields_[:-2])
 PAGES_PACK = _packer(KdaPagesArgs._fields_[:-2])
 WORKSPACE_PACK = _packer(KdaPagedArgs._fields_[-2:])
-# What follows the paged arguments in the structs that begin with them.
-ROTARY_PACK = _packer(KdaPagedRotaryArgs._fields_[1:])
+PAGED_ROTARY_PACK = _packer(KdaPagedArgs._fields_ + KdaPagedRotaryArgs._fields_[1:])
 NO_WORKSPACE = WORKSPACE_PACK.pack(0, 0)
 
 

@@ -392,24 +392,13 @@ def paged_append_rotary(
     packed tokens of no sequence (behind the last offset) are not written.
     """
     shape = q.shape
-    if k.ndim == 4 and v.ndim == 4 and (k.shape[:2] != shape[:2] or v.shape != k.shape):
-        raise ValueError(f"q, k and v must have the same tokens and k and v the same heads, got shapes {tuple(shape)}, "
-                         f"{tuple(k.shape)} and {tuple(v.shape)}")
-    _check_cache(k_cache, v_cache, page_table, seq_lens)
-    for name, t, heads in (("q", q, None), ("k", k, k_cache.shape[2]), ("v", v, k_cache.shape[2])):
-        _check_new(name, t, heads, k_cache, page_table, cu_seqlens)
-    D = shape[-1]
-    if inv_freq.ndim != 1 or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
-        raise ValueError(f"inv_freq must be contiguous 1D float32, got {inv_freq.dtype} with shape {tuple(inv_freq.shape)}")
-    if inv_freq.device != q.device:
-        raise ValueError(f"inv_freq device {inv_freq.device} must match q ({q.device})")
-    R = 2 * inv_freq.shape[0]
-    if R < 16 or R > D or R % 16:
-        raise ValueError(f"twice inv_freq's entries must be a multiple of 16 from 16 to the head size {D}, got {R}")
+    f = _plain_rotary(q, k, v, k_cache, v_cache, page_table, seq_lens, inv_freq, cu_seqlens)
+    if f is None:
+        f = _checked_rotary(q, k, v, k_cache, v_cache, page_table, seq_lens, inv_freq, cu_seqlens)
     _forward_only("paged_append_rotary", q, k, v, k_cache, v_cache, inv_freq)
     if out is None:
         _require_gpu(q)
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check_new("out", out, shape[2], k_cache, page_table, cu_seqlens)
         if out.shape != shape:
@@ -419,15 +408,54 @@ def paged_append_rotary(
         if (out.data_ptr() != q.data_ptr() or out.stride() != q.stride()) and out.untyped_storage().data_ptr() in {
                 t.untyped_storage().data_ptr() for t in (q, k, v, k_cache, v_cache)}:
             raise ValueError("out must be q itself or of other storage than the inputs")
-    _require_gpu(q)
-    (N, T, _, HKV, D, dt, P, size, M, cu_dtype, cu, table, table_stride, lens, kp, vp, s0, s1, s2, t0, t1, t2, u0, u1,
-     u2) = _fields(k_cache, v_cache, page_table, seq_lens, k, cu_seqlens)
-    _launch("kda_paged_append_rotary_hip", _hip.PAGED_PACK.pack(
-        _hip.PAGED_ABI_VERSION, N, T, shape[2], HKV, D, dt, P, size, M, 0, 0, 1.0, cu_dtype, cu, table, table_stride, lens,
-        kp, vp, s0, s1, s2, t0, t1, t2, q.data_ptr(), *_strides(q), 0, 0, k.data_ptr(), v.data_ptr(), u0, u1, u2,
-        *_strides(v)) + _hip.NO_WORKSPACE + _hip.ROTARY_PACK.pack(
-            inv_freq.data_ptr(), R, interleaved, out.data_ptr(), *_strides(out)), q.device)
+        _require_gpu(q)
+    (N, T, HQ, HKV, D, dt, P, size, M, cu_dtype, cu, table, table_stride, lens, kp, vp, s0, s1, s2, t0, t1, t2, u0, u1,
+     u2, w0, w1, w2, x0, x1, x2) = f
+    _launch("kda_paged_append_rotary_hip", _hip.PAGED_ROTARY_PACK.pack(
+        _hip.PAGED_ABI_VERSION, N, T, HQ, HKV, D, dt, P, size, M, 0, 0, 1.0, cu_dtype, cu, table, table_stride, lens,
+        kp, vp, s0, s1, s2, t0, t1, t2, q.data_ptr(), u0, u1, u2, 0, 0, k.data_ptr(), v.data_ptr(), w0, w1, w2, x0, x1, x2,
+        0, 0, inv_freq.data_ptr(), 2 * inv_freq.shape[0], interleaved, out.data_ptr(), *_strides(out)), q.device)
     return out
+
+
+def _plain_rotary(q, k, v, k_cache, v_cache, table, lens, inv_freq, cu) -> tuple | None:
+    """:func:`_plain_fields` of an ordinary append with rotation: the strides
+    of q, k and v last."""
+    f = _plain_fields(k_cache, v_cache, table, lens, q, 0, cu)
+    n = k.shape
+    if f is None or v.shape != n or len(n) != 4:
+        return None
+    w0, w1, w2, w3 = k.stride()
+    x0, x1, x2, x3 = v.stride()
+    dev, R = q.get_device(), 2 * inv_freq.shape[0] if inv_freq.ndim == 1 else 0
+    if not (
+        n[:2] == q.shape[:2] and n[2] == f[3] and n[3] == f[4] and k.dtype is q.dtype and v.dtype is q.dtype
+        and w3 == 1 and x3 == 1 and (w0 | w1 | w2 | x0 | x1 | x2) % 8 == 0 and (k.data_ptr() | v.data_ptr()) % 16 == 0
+        and k.get_device() == dev and v.get_device() == dev and inv_freq.get_device() == dev
+        and inv_freq.dtype is torch.float32 and inv_freq.is_contiguous() and 16 <= R <= f[4] and R % 16 == 0
+    ):
+        return None
+    return f + (w0, w1, w2, x0, x1, x2)
+
+
+def _checked_rotary(q, k, v, k_cache, v_cache, table, lens, inv_freq, cu) -> tuple:
+    """:func:`_plain_rotary` of any call, whose arguments are looked at in the
+    order of their messages."""
+    if k.ndim == 4 and v.ndim == 4 and (k.shape[:2] != q.shape[:2] or v.shape != k.shape):
+        raise ValueError(f"q, k and v must have the same tokens and k and v the same heads, got shapes {tuple(q.shape)}, "
+                         f"{tuple(k.shape)} and {tuple(v.shape)}")
+    _check_cache(k_cache, v_cache, table, lens)
+    for name, t, heads in (("q", q, None), ("k", k, k_cache.shape[2]), ("v", v, k_cache.shape[2])):
+        _check_new(name, t, heads, k_cache, table, cu)
+    D = q.shape[-1]
+    if inv_freq.ndim != 1 or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
+        raise ValueError(f"inv_freq must be contiguous 1D float32, got {inv_freq.dtype} with shape {tuple(inv_freq.shape)}")
+    if inv_freq.device != q.device:
+        raise ValueError(f"inv_freq device {inv_freq.device} must match q ({q.device})")
+    R = 2 * inv_freq.shape[0]
+    if R < 16 or R > D or R % 16:
+        raise ValueError(f"twice inv_freq's entries must be a multiple of 16 from 16 to the head size {D}, got {R}")
+    return _fields(k_cache, v_cache, table, lens, q, cu) + _strides(k) + _strides(v)
 
 
 def _pools(pools) -> list[torch.Tensor]:

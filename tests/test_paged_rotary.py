@@ -113,7 +113,8 @@ def test_c_compiler_sees_the_same_layout(tmp_path):
 def test_packed_arguments_are_the_struct():
     base = paged()
     tail = dict(inv_freq=11, rotary_dim=64, interleaved=1, q_out=12, out_row=13, out_token=14, out_head=15)
-    assert bytes(base) + _hip.ROTARY_PACK.pack(*tail.values()) == bytes(_hip.KdaPagedRotaryArgs(base, *tail.values()))
+    flat = [getattr(base, f) or 0 for f, _ in base._fields_]
+    assert _hip.PAGED_ROTARY_PACK.pack(*flat, *tail.values()) == bytes(_hip.KdaPagedRotaryArgs(base, *tail.values()))
 
 
 def rotary(base=None, **change):
