@@ -97,6 +97,17 @@ typedef struct KdaPagedArgs {
 size_t kda_paged_attn_workspace_bytes(const KdaPagedArgs* args);
 int kda_paged_attn_hip(const KdaPagedArgs* args, void* stream);
 
+/* The same with a window (which has to be given, and the causal flag) and the
+ * first `sinks` tokens of every sequence visible outside of it too: a query at
+ * position p sees the keys j <= p with j > p - window or j < sinks. */
+typedef struct KdaPagedSinksArgs {
+    KdaPagedArgs paged;
+    int32_t sinks;  /* 0 or more */
+    int32_t reserved;
+} KdaPagedSinksArgs;
+size_t kda_paged_attn_sinks_workspace_bytes(const KdaPagedSinksArgs* args);
+int kda_paged_attn_sinks_hip(const KdaPagedSinksArgs* args, void* stream);
+
 /* The new tokens' keys and values into their places in the pages.  Tokens at
  * negative positions, beyond the table or on no page are left out. */
 int kda_paged_append_hip(const KdaPagedArgs* args, void* stream);

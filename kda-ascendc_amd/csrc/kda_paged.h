@@ -128,6 +128,11 @@ struct PagesParams {
     int32_t* ws;
 };
 
+// Attention with a window and first tokens that stay visible (kda_paged_hip.h).
+struct SinkParams : PagedParams {
+    int sinks;
+};
+
 // The append with the position rotation (kda_paged_hip.h).
 struct RotaryParams : PagedParams {
     const float* inv_freq;
@@ -139,6 +144,8 @@ struct RotaryParams : PagedParams {
 
 size_t paged_attn_workspace(const PagedParams& p, int D);
 hipError_t launch_paged_attn(const PagedParams& p, int D, hipStream_t stream);
+size_t paged_attn_workspace(const SinkParams& p, int D);
+hipError_t launch_paged_attn(const SinkParams& p, int D, hipStream_t stream);
 hipError_t launch_paged_append(const PagedParams& p, int D, hipStream_t stream);
 hipError_t launch_paged_append_rotary(const RotaryParams& p, int D, hipStream_t stream);
 hipError_t launch_pages_reserve(const PagesParams& p, hipStream_t stream);

@@ -8,6 +8,7 @@ namespace {
 
 using kda::PagedParams;
 using kda::PagesParams;
+using kda::SinkParams;
 
 constexpr int64_t I32_MAX = 0x7fffffffLL;
 
@@ -184,7 +185,27 @@ int pages_lens(const KdaPagesArgs* a, PagesParams& p) {
     return KDA_BT16_OK;
 }
 
+int sink_params(const KdaPagedSinksArgs* a, SinkParams& p) {
+    if (a == nullptr) return KDA_BT16_EINVAL;
+    const int rc = attn_params(&a->paged, p);
+    if (rc != KDA_BT16_OK) return rc;
+    if (a->sinks < 0) return KDA_BT16_EINVAL;
+    if (p.window == 0) return KDA_BT16_EUNSUPPORTED;  // (without one every key is visible)
+    p.sinks = a->sinks < I32_MAX / 2 ? a->sinks : (int32_t)(I32_MAX / 2);
+    return KDA_BT16_OK;
+}
+
 int launched(hipError_t e) { return e == hipSuccess ? KDA_BT16_OK : KDA_BT16_ELAUNCH; }
+
+template <class P>
+int attn_launch(const KdaPagedArgs* a, P& p, void* stream) {
+    const size_t need = kda::paged_attn_workspace(p, a->D);
+    if (need > 0) {
+        if (!a->workspace || misaligned(a->workspace, 256) || a->workspace_bytes < need) return KDA_BT16_EWORKSPACE;
+        p.ws = static_cast<float*>(a->workspace);
+    }
+    return launched(kda::launch_paged_attn(p, a->D, static_cast<hipStream_t>(stream)));
+}
 
 }  // namespace
 
@@ -198,14 +219,18 @@ size_t kda_paged_attn_workspace_bytes(const KdaPagedArgs* args) {
 int kda_paged_attn_hip(const KdaPagedArgs* args, void* stream) {
     PagedParams p;
     const int rc = attn_params(args, p);
-    if (rc != KDA_BT16_OK) return rc;
-    const size_t need = kda::paged_attn_workspace(p, args->D);
-    if (need > 0) {
-        if (!args->workspace || misaligned(args->workspace, 256) || args->workspace_bytes < need)
-            return KDA_BT16_EWORKSPACE;
-        p.ws = static_cast<float*>(args->workspace);
-    }
-    return launched(kda::launch_paged_attn(p, args->D, static_cast<hipStream_t>(stream)));
+    return rc == KDA_BT16_OK ? attn_launch(args, p, stream) : rc;
+}
+
+size_t kda_paged_attn_sinks_workspace_bytes(const KdaPagedSinksArgs* args) {
+    SinkParams p{};
+    return sink_params(args, p) == KDA_BT16_OK ? kda::paged_attn_workspace(p, args->paged.D) : 0;
+}
+
+int kda_paged_attn_sinks_hip(const KdaPagedSinksArgs* args, void* stream) {
+    SinkParams p{};
+    const int rc = sink_params(args, p);
+    return rc == KDA_BT16_OK ? attn_launch(&args->paged, p, stream) : rc;
 }
 
 int kda_paged_append_hip(const KdaPagedArgs* args, void* stream) {

@@ -67,6 +67,8 @@ PAGED_MAX_POOLS = 8
 PAGED_SYMBOLS = (
     "kda_paged_attn_workspace_bytes",
     "kda_paged_attn_hip",
+    "kda_paged_attn_sinks_workspace_bytes",
+    "kda_paged_attn_sinks_hip",
     "kda_paged_append_hip",
     "kda_paged_append_rotary_hip",
     "kda_pages_workspace_bytes",
@@ -190,6 +192,16 @@ class KdaPagedArgs(ctypes.Structure):
     ]
 
 
+class KdaPagedSinksArgs(ctypes.Structure):
+    """Mirror of ``struct KdaPagedSinksArgs``."""
+
+    _fields_ = [
+        ("paged", KdaPagedArgs),
+        ("sinks", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 class KdaPagedRotaryArgs(ctypes.Structure):
     """Mirror of ``struct KdaPagedRotaryArgs``."""
 
@@ -263,6 +275,7 @@ def _packer(fields) -> struct.Struct:
 PAGED_PACK = _packer(KdaPagedArgs._fields_[:-2])
 PAGES_PACK = _packer(KdaPagesArgs._fields_[:-2])
 WORKSPACE_PACK = _packer(KdaPagedArgs._fields_[-2:])
+SINKS_PACK = _packer(KdaPagedSinksArgs._fields_[1:])
 PAGED_ROTARY_PACK = _packer(KdaPagedArgs._fields_ + KdaPagedRotaryArgs._fields_[1:])
 NO_WORKSPACE = WORKSPACE_PACK.pack(0, 0)
 

@@ -240,14 +240,14 @@ def _launch(name: str, args: bytes, device: torch.device) -> None:
         _hip.call_packed(name, args, _raw_stream(device))
 
 
-def _launch_in(name: str, args: bytes, nbytes: int, device: torch.device) -> None:
+def _launch_in(name: str, args: bytes, nbytes: int, device: torch.device, more: bytes = b"") -> None:
     """:func:`_launch` with a workspace of ``nbytes``, the caller's stream's
-    again once the launches are queued."""
+    again once the launches are queued; ``more``: the arguments behind it."""
     if nbytes == 0:
-        _launch(name, args + _hip.NO_WORKSPACE, device)
+        _launch(name, args + _hip.NO_WORKSPACE + more, device)
         return
     ws = workspace.scratch(device, nbytes)
-    _launch(name, args + _hip.WORKSPACE_PACK.pack(ws.data_ptr(), nbytes), device)
+    _launch(name, args + _hip.WORKSPACE_PACK.pack(ws.data_ptr(), nbytes) + more, device)
 
 
 def paged_attention(
@@ -260,6 +260,7 @@ def paged_attention(
     scale: float | None = None,
     causal: bool = True,
     window: int | None = None,
+    sinks: int = 0,
     cu_seqlens: torch.Tensor | None = None,
     return_lse: bool = False,
 ):
@@ -273,7 +274,10 @@ def paged_attention(
     ``q`` may be a view (a slice of a fused projection).
 
     A query at position p sees the keys up to p (``causal``; else all), with
-    ``window`` those above ``p - window`` only.  ``scale`` (above 0) is
+    ``window`` those above ``p - window`` only, and with ``sinks`` besides it
+    the sequence's first ``sinks`` ones (a stream's first tokens, which keep
+    their weight however far the window has gone; the pages between them and
+    the window may be given away).  ``scale`` (above 0) is
     ``D ** -0.5`` by default.  Sums and the softmax are held in fp32; the
     exponentials are rounded to q's type for the product with the values.
 
@@ -300,6 +304,11 @@ def paged_attention(
             raise ValueError(f"window must be at least 1, got {window}")
         if not causal:
             raise ValueError("window needs causal=True")
+    if sinks:
+        if sinks < 0:
+            raise ValueError(f"sinks must not be negative, got {sinks}")
+        if window is None:
+            raise ValueError("sinks needs a window")
     _forward_only("paged_attention", q, k_cache, v_cache)
     if f is None:
         _require_gpu(q)
@@ -314,8 +323,13 @@ def paged_attention(
         min(window or 0, 1 << 30), scale,
         cu_dtype, cu, table, table_stride, lens, kp, vp, s0, s1, s2, t0, t1, t2, q.data_ptr(), u0, u1, u2, o.data_ptr(),
         0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0)
-    nbytes = _hip.lib().kda_paged_attn_workspace_bytes(args + _hip.NO_WORKSPACE)
-    _launch_in("kda_paged_attn_hip", args, nbytes, device)
+    if sinks:
+        more = _hip.SINKS_PACK.pack(min(sinks, 1 << 30), 0)
+        nbytes = _hip.lib().kda_paged_attn_sinks_workspace_bytes(args + _hip.NO_WORKSPACE + more)
+        _launch_in("kda_paged_attn_sinks_hip", args, nbytes, device, more)
+    else:
+        nbytes = _hip.lib().kda_paged_attn_workspace_bytes(args + _hip.NO_WORKSPACE)
+        _launch_in("kda_paged_attn_hip", args, nbytes, device)
     return (o, lse) if return_lse else o
 
 
