@@ -31,8 +31,8 @@
  * than what it shares with a fork, whose page its next tokens would go into.
  *
  * Table entries outside [0, P), lengths beyond M * page_size, offsets outside
- * [0, T] and row numbers outside [0, N) give unspecified results but never an
- * access outside the tensors.
+ * [0, T] and row numbers outside [0, N), or offsets that decrease, give
+ * unspecified results but never an access outside the tensors.
  */
 #ifndef KDA_PAGED_HIP_H
 #define KDA_PAGED_HIP_H
@@ -107,6 +107,25 @@ typedef struct KdaPagedSinksArgs {
 } KdaPagedSinksArgs;
 size_t kda_paged_attn_sinks_workspace_bytes(const KdaPagedSinksArgs* args);
 int kda_paged_attn_sinks_hip(const KdaPagedSinksArgs* args, void* stream);
+
+/* kda_paged_attn_hip (causal, no window) for sequences in groups that share
+ * their first tokens, which are read and worked on once for a group: rows
+ * cu_groups[g] to cu_groups[g + 1] - 1 of the table hold the same keys and values
+ * in their first shared_lens[g] tokens, in the same pages (as kda_pages_fork_hip
+ * leaves them) or in copies; one row's are read.  Which one, and how sums are
+ * rounded, depends on the groups, nothing else does.  A sequence whose new tokens
+ * do not all come behind the shared ones (an ended one's) takes part by itself,
+ * and so do rows of no group, and all rows of a group one of whose sequences has
+ * new tokens for a row tile of its own (T_n * HQ / HKV at least 256). */
+typedef struct KdaPagedSharedArgs {
+    KdaPagedArgs paged;
+    const int32_t* cu_groups;   /* [num_groups + 1], from 0 to N, non-decreasing */
+    const int32_t* shared_lens; /* [num_groups] */
+    int32_t num_groups;
+    int32_t reserved;
+} KdaPagedSharedArgs;
+size_t kda_paged_attn_shared_workspace_bytes(const KdaPagedSharedArgs* args);
+int kda_paged_attn_shared_hip(const KdaPagedSharedArgs* args, void* stream);
 
 /* The new tokens' keys and values into their places in the pages.  Tokens at
  * negative positions, beyond the table or on no page are left out. */

@@ -133,6 +133,15 @@ struct SinkParams : PagedParams {
     int sinks;
 };
 
+// Attention of sequences in groups that share their first tokens
+// (kda_paged_hip.h).
+struct SharedParams : PagedParams {
+    int NG;
+    const int32_t* cu_groups;
+    const int32_t* shared_lens;
+    int32_t* plan;
+};
+
 // The append with the position rotation (kda_paged_hip.h).
 struct RotaryParams : PagedParams {
     const float* inv_freq;
@@ -146,6 +155,10 @@ size_t paged_attn_workspace(const PagedParams& p, int D);
 hipError_t launch_paged_attn(const PagedParams& p, int D, hipStream_t stream);
 size_t paged_attn_workspace(const SinkParams& p, int D);
 hipError_t launch_paged_attn(const SinkParams& p, int D, hipStream_t stream);
+
+
+size_t paged_attn_workspace(const SharedParams& p, int D);
+hipError_t launch_paged_attn(const SharedParams& p, int D, hipStream_t stream);
 hipError_t launch_paged_append(const PagedParams& p, int D, hipStream_t stream);
 hipError_t launch_paged_append_rotary(const RotaryParams& p, int D, hipStream_t stream);
 hipError_t launch_pages_reserve(const PagesParams& p, hipStream_t stream);

@@ -39,9 +39,11 @@ constexpr float LN2 = 0.6931471805599453f;
 constexpr int BUF_RAW = 0x00020000;
 
 // What a call's parameters are of: PagedParams, or with first tokens that stay
-// visible outside of the window.
+// visible outside of the window, or with groups of sequences that share theirs.
 template <class P>
 constexpr bool SINKS = std::is_same<P, SinkParams>::value;
+template <class P>
+constexpr bool SHARED = std::is_same<P, SharedParams>::value;
 template <class P>
 __device__ __forceinline__ int sinks_of(const P& p) {
     if constexpr (SINKS<P>) return p.sinks;
@@ -270,6 +272,10 @@ struct Unit {
     int n, h, m, lo, hi, begin, end, slot;
     NewTokens s;
     int split, gap;
+    // With groups: n is a row of the table, s.first a token of all, and the
+    // partial results are those of `rows` rows, from float `place` on (none: -1).
+    int rows;
+    int64_t place;
 };
 
 // The keys that rows [m * MT, m * MT + MT) of a sequence see, and their tiles.
@@ -498,6 +504,21 @@ struct Partial {
     static constexpr int64_t FLOATS = MT * (D + 2);
     static __device__ __forceinline__ float* at(float* ws, int slot) { return ws + slot * FLOATS; }
 };
+// Whether a unit's results are partial ones, where they go, and the rows that
+// they are of.
+template <class P>
+__device__ __forceinline__ bool is_partial(const Unit& u) {
+    return SHARED<P> ? u.place >= 0 : u.slot >= 0;
+}
+template <int KIND, int D, class P>
+__device__ __forceinline__ float* partial_of(const P& p, const Unit& u, int64_t before) {
+    if constexpr (SHARED<P>) return p.ws + u.place;
+    return Partial<KIND, D>::at(p.ws + before, u.slot);
+}
+template <int KIND, class P>
+__device__ __forceinline__ int partial_rows(const Unit& u) {
+    return SHARED<P> ? u.rows : Shape<KIND>::MT;
+}
 // Floats of the workspace before the parts of kind MANY.
 template <int D>
 constexpr int64_t few_floats() { return Shape<FEW>::PLACES * Partial<FEW, D>::FLOATS; }
@@ -517,18 +538,24 @@ __device__ __forceinline__ Row row_of(const P& p, const Unit& u, int r) {
     x.head = u.h * p.G + (rc - x.tok * p.G);
     const int pos = u.s.pos + x.tok;
     x.hi = p.causal ? max(0, min(pos + 1, u.s.len)) : u.s.len;
-    x.lo = p.window ? max(0, pos + 1 - p.window) : 0;
+    x.lo = SHARED<P> ? u.lo : (p.window ? max(0, pos + 1 - p.window) : 0);
     return x;
 }
 
 template <class P>
 __device__ __forceinline__ int64_t out_row(const P& p, const Unit& u, const Row& x) {
-    return (p.cu_seqlens ? (int64_t)u.s.first + x.tok : (int64_t)u.n * p.T + x.tok) * p.HQ + x.head;
+    return (p.cu_seqlens || SHARED<P> ? (int64_t)u.s.first + x.tok : (int64_t)u.n * p.T + x.tok) * p.HQ + x.head;
 }
 
 template <int D, class P>
 __device__ __forceinline__ void load_q(const P& p, const Unit& u, const Row& x, int half, u32x4 (&q)[D / 16]) {
-    const uint16_t* at = p.q + (p.cu_seqlens ? u.s.first * p.q_token : u.n * p.q_row) + x.tok * p.q_token + x.head * p.q_head;
+    const uint16_t* at;
+    if (SHARED<P> && !p.cu_seqlens) {
+        const int t = u.s.first + x.tok, n = t / p.T;
+        at = p.q + n * p.q_row + (t - n * p.T) * p.q_token + x.head * p.q_head;
+    } else {
+        at = p.q + (p.cu_seqlens ? u.s.first * p.q_token : u.n * p.q_row) + x.tok * p.q_token + x.head * p.q_head;
+    }
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) q[s] = *reinterpret_cast<const u32x4*>(at + 16 * s + 8 * half);
 }
@@ -743,7 +770,8 @@ __device__ __forceinline__ void few_rows(const P& p, const Unit& u, const FewLds
                 f32x4{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
         }
     __syncthreads();
-    float* part = u.slot >= 0 ? Partial<FEW, D>::at(p.ws, u.slot) : nullptr;
+    float* part = is_partial<P>(u) ? partial_of<FEW, D>(p, u, 0) : nullptr;
+    const int R = partial_rows<FEW, P>(u);
     for (int e = threadIdx.x; e < ROWS * (D / 4); e += WAVES * 64) {
         const int r = e / (D / 4), piece = e % (D / 4);
         const Row y = row_of(p, u, u.m * ROWS + r);
@@ -764,10 +792,10 @@ __device__ __forceinline__ void few_rows(const P& p, const Unit& u, const FewLds
             for (int i = 0; i < 4; ++i) o[i] = fmaf(f, v[i], o[i]);
         }
         if (part) {
-            *reinterpret_cast<f32x4*>(part + 2 * ROWS + r * D + piece * 4) = o;
+            *reinterpret_cast<f32x4*>(part + 2 * R + r * D + piece * 4) = o;
             if (piece == 0) {
                 part[r] = mx;
-                part[ROWS + r] = sum;
+                part[R + r] = sum;
             }
         } else {
             const float inv = sum > 0.f ? 1.f / sum : 0.f;
@@ -988,17 +1016,18 @@ __device__ __forceinline__ void many_rows(const P& p, const Unit& u, uint8_t* kt
 
     const float l = sum_halves(run.l);
     if (!x.live) return;
-    if (u.slot >= 0) {
-        float* part = Partial<MANY, D>::at(p.ws + few_floats<D>(), u.slot);
+    if (is_partial<P>(u)) {
+        float* part = partial_of<MANY, D>(p, u, few_floats<D>());
+        const int R = partial_rows<MANY, P>(u);
         if (half == 0) {
             part[row] = run.log2_max();
-            part[MT + row] = l;
+            part[R + row] = l;
         }
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<f32x4*>(part + 2 * MT + row * D + 32 * d + 2 * i + 4 * half) =
+                *reinterpret_cast<f32x4*>(part + 2 * R + row * D + 32 * d + 2 * i + 4 * half) =
                     f32x4{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
         return;
     }
@@ -1157,13 +1186,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(P p, int few, int few_g
 
 // What a call's kinds are from what the host knows: packed sequences may be of
 // both, unless their tokens cannot be of many rows.
-int kind_of(const PagedParams& p) {
+inline int kind_of(const PagedParams& p) {
     if ((int64_t)p.T * p.G <= ROWS) return FEW;
     return p.cu_seqlens ? MIXED : MANY;
 }
 
 // Row tiles of many rows at most (packed sequences each leave one unfilled).
-int64_t many_units(const PagedParams& p) {
+inline int64_t many_units(const PagedParams& p) {
     constexpr int MT = Shape<MANY>::MT;
     const int64_t rows = (int64_t)p.T * p.G;
     return (p.cu_seqlens ? rows / MT + p.N : p.N * ((rows + MT - 1) / MT)) * p.HKV;
@@ -1175,8 +1204,8 @@ int64_t many_units(const PagedParams& p) {
 // against 14.1; 64 of 700 keys 32.8 whole and 35.4 cut.  Many rows: row tiles
 // that fill half of SLOTS are taken whole.
 // (what a sequence of few rows can see at most, its first and last tiles whole)
-int64_t few_keys(const PagedParams& p) { return (int64_t)p.M << p.page_shift; }
-int64_t few_keys(const SinkParams& p) {
+inline int64_t few_keys(const PagedParams& p) { return (int64_t)p.M << p.page_shift; }
+inline int64_t few_keys(const SinkParams& p) {
     return std::min((int64_t)p.M << p.page_shift, (int64_t)p.window + p.sinks + ROWS + 3 * Shape<FEW>::TK);
 }
 template <class P>

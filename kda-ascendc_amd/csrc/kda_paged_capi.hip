@@ -8,6 +8,7 @@ namespace {
 
 using kda::PagedParams;
 using kda::PagesParams;
+using kda::SharedParams;
 using kda::SinkParams;
 
 constexpr int64_t I32_MAX = 0x7fffffffLL;
@@ -195,6 +196,20 @@ int sink_params(const KdaPagedSinksArgs* a, SinkParams& p) {
     return KDA_BT16_OK;
 }
 
+int shared_params(const KdaPagedSharedArgs* a, SharedParams& p) {
+    if (a == nullptr) return KDA_BT16_EINVAL;
+    const int rc = attn_params(&a->paged, p);
+    if (rc != KDA_BT16_OK) return rc;
+    if (!p.causal || p.window != 0) return KDA_BT16_EUNSUPPORTED;
+    if (a->num_groups <= 0 || !a->cu_groups || !a->shared_lens || misaligned(a->cu_groups, 4) ||
+        misaligned(a->shared_lens, 4))
+        return KDA_BT16_EINVAL;
+    p.NG = a->num_groups;
+    p.cu_groups = a->cu_groups;
+    p.shared_lens = a->shared_lens;
+    return KDA_BT16_OK;
+}
+
 int launched(hipError_t e) { return e == hipSuccess ? KDA_BT16_OK : KDA_BT16_ELAUNCH; }
 
 template <class P>
@@ -230,6 +245,17 @@ size_t kda_paged_attn_sinks_workspace_bytes(const KdaPagedSinksArgs* args) {
 int kda_paged_attn_sinks_hip(const KdaPagedSinksArgs* args, void* stream) {
     SinkParams p{};
     const int rc = sink_params(args, p);
+    return rc == KDA_BT16_OK ? attn_launch(&args->paged, p, stream) : rc;
+}
+
+size_t kda_paged_attn_shared_workspace_bytes(const KdaPagedSharedArgs* args) {
+    SharedParams p{};
+    return shared_params(args, p) == KDA_BT16_OK ? kda::paged_attn_workspace(p, args->paged.D) : 0;
+}
+
+int kda_paged_attn_shared_hip(const KdaPagedSharedArgs* args, void* stream) {
+    SharedParams p{};
+    const int rc = shared_params(args, p);
     return rc == KDA_BT16_OK ? attn_launch(&args->paged, p, stream) : rc;
 }
 

@@ -34,6 +34,7 @@ from .paged import (
     paged_append,
     paged_append_rotary,
     paged_attention,
+    paged_attention_shared,
     paged_compact,
     paged_copy,
     paged_fork,
@@ -56,6 +57,7 @@ __all__ = [
     "fused_recurrent_kda",
     "dispatch",
     "paged_attention",
+    "paged_attention_shared",
     "paged_append",
     "paged_append_rotary",
     "paged_reserve",

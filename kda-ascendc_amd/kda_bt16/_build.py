@@ -20,7 +20,8 @@ LIB_NAME = "libkda_bt16_hip.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 SOURCES = ["kda_capi.hip", "kda_k1.hip", "kda_k2.hip", "kda_k2w.hip", "kda_fused.hip",
            "kda_recurrent.hip", "kda_bwd.hip", "kda_paged_capi.hip", "kda_paged_attn.hip", "kda_pages.hip",
-           "kda_paged_rotary.hip", "kda_paged_sinks.hip"]
+           "kda_paged_rotary.hip", "kda_paged_sinks.hip",
+           "kda_paged_shared.hip"]
 HEADERS = ["kda_common.h", "kda_k2_shared.h", "kda_k1_chunk.h", "kda_k2w_step.h",
            "kda_paged.h", "kda_paged_attn.h"]
 

@@ -69,6 +69,8 @@ PAGED_SYMBOLS = (
     "kda_paged_attn_hip",
     "kda_paged_attn_sinks_workspace_bytes",
     "kda_paged_attn_sinks_hip",
+    "kda_paged_attn_shared_workspace_bytes",
+    "kda_paged_attn_shared_hip",
     "kda_paged_append_hip",
     "kda_paged_append_rotary_hip",
     "kda_pages_workspace_bytes",
@@ -202,6 +204,18 @@ class KdaPagedSinksArgs(ctypes.Structure):
     ]
 
 
+class KdaPagedSharedArgs(ctypes.Structure):
+    """Mirror of ``struct KdaPagedSharedArgs``."""
+
+    _fields_ = [
+        ("paged", KdaPagedArgs),
+        ("cu_groups", ctypes.c_void_p),
+        ("shared_lens", ctypes.c_void_p),
+        ("num_groups", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 class KdaPagedRotaryArgs(ctypes.Structure):
     """Mirror of ``struct KdaPagedRotaryArgs``."""
 
@@ -276,6 +290,7 @@ PAGED_PACK = _packer(KdaPagedArgs._fields_[:-2])
 PAGES_PACK = _packer(KdaPagesArgs._fields_[:-2])
 WORKSPACE_PACK = _packer(KdaPagedArgs._fields_[-2:])
 SINKS_PACK = _packer(KdaPagedSinksArgs._fields_[1:])
+SHARED_PACK = _packer(KdaPagedSharedArgs._fields_[1:])
 PAGED_ROTARY_PACK = _packer(KdaPagedArgs._fields_ + KdaPagedRotaryArgs._fields_[1:])
 NO_WORKSPACE = WORKSPACE_PACK.pack(0, 0)
 

@@ -287,6 +287,52 @@ def paged_attention(
     NaN in both.  What the pages hold beyond ``seq_lens`` does not matter; keys and
     values before it have to be finite.
     """
+    return _attention("paged_attention", q, k_cache, v_cache, page_table, seq_lens, scale, causal, window, sinks, cu_seqlens,
+                      return_lse, None)
+
+
+def paged_attention_shared(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    page_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    cu_groups: torch.Tensor,
+    shared_lens: torch.Tensor,
+    *,
+    scale: float | None = None,
+    cu_seqlens: torch.Tensor | None = None,
+    return_lse: bool = False,
+):
+    """:func:`paged_attention` (causal) of sequences in groups that share their
+    first tokens (answers forked from one prompt, prompts behind one document):
+    the shared keys and values are read and worked on once for the whole group.
+
+    Rows ``cu_groups[g]`` to ``cu_groups[g + 1] - 1`` of the table (int32 ``[G +
+    1]``, from 0 to N) hold the same first ``shared_lens[g]`` (int32 ``[G]``)
+    tokens, in the same pages or in copies of them: what :func:`paged_fork`
+    leaves, its copied last page included.  One row's are read for all.
+
+    Same result as :func:`paged_attention`'s but for the order of fp32 sums.  A
+    sequence whose new tokens do not all come behind the shared ones (a freed
+    row) is worked on by itself, and so are rows of no group.  Sequences with new
+    tokens for a whole row tile of their own (256 rows, T * HQ / HKV) gain
+    nothing: one in a group, and the whole group is worked on one by one; give
+    it a group of its own.
+    """
+    device = k_cache.device
+    for name, t in (("cu_groups", cu_groups), ("shared_lens", shared_lens)):
+        _int32(name, t, 1, device)
+    if shared_lens.shape[0] < 1 or cu_groups.shape[0] != shared_lens.shape[0] + 1:
+        raise ValueError(f"cu_groups must have one entry more than shared_lens, of one at least, got {cu_groups.shape[0]} and "
+                         f"{shared_lens.shape[0]}")
+    return _attention("paged_attention_shared", q, k_cache, v_cache, page_table, seq_lens, scale, True, None, 0, cu_seqlens,
+                      return_lse, (cu_groups, shared_lens))
+
+
+def _attention(name, q, k_cache, v_cache, page_table, seq_lens, scale, causal, window, sinks, cu_seqlens, return_lse, groups):
+    """The attention calls, their arguments as in :func:`paged_attention`;
+    ``groups``: the groups' offsets and shared tokens."""
     f = _plain_fields(k_cache, v_cache, page_table, seq_lens, q, 0, cu_seqlens)
     if f is None:
         _check_cache(k_cache, v_cache, page_table, seq_lens)
@@ -309,7 +355,7 @@ def paged_attention(
             raise ValueError(f"sinks must not be negative, got {sinks}")
         if window is None:
             raise ValueError("sinks needs a window")
-    _forward_only("paged_attention", q, k_cache, v_cache)
+    _forward_only(name, q, k_cache, v_cache)
     if f is None:
         _require_gpu(q)
         f = _fields(k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
@@ -323,7 +369,11 @@ def paged_attention(
         min(window or 0, 1 << 30), scale,
         cu_dtype, cu, table, table_stride, lens, kp, vp, s0, s1, s2, t0, t1, t2, q.data_ptr(), u0, u1, u2, o.data_ptr(),
         0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0)
-    if sinks:
+    if groups is not None:
+        more = _hip.SHARED_PACK.pack(groups[0].data_ptr(), groups[1].data_ptr(), groups[1].shape[0], 0)
+        nbytes = _hip.lib().kda_paged_attn_shared_workspace_bytes(args + _hip.NO_WORKSPACE + more)
+        _launch_in("kda_paged_attn_shared_hip", args, nbytes, device, more)
+    elif sinks:
         more = _hip.SINKS_PACK.pack(min(sinks, 1 << 30), 0)
         nbytes = _hip.lib().kda_paged_attn_sinks_workspace_bytes(args + _hip.NO_WORKSPACE + more)
         _launch_in("kda_paged_attn_sinks_hip", args, nbytes, device, more)
