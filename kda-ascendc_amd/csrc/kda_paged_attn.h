@@ -739,8 +739,11 @@ struct FewLds {
     }
 };
 
+// The waves' sums to LDS: every wave's m and l to `joint`, then its O over its
+// tiles, row by row in pieces of four (the rows' pieces turned by the row, so
+// that the lanes of a half, one row each, write different banks).
 template <class E, int D, int WAVES, class P>
-__device__ __forceinline__ void few_rows(const P& p, const Unit& u, const FewLds<D, WAVES>& lds, float* joint) {
+__device__ __forceinline__ void few_sums(const P& p, const Unit& u, const FewLds<D, WAVES>& lds, float* joint) {
     constexpr int DB = D / 32;
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -751,9 +754,6 @@ __device__ __forceinline__ void few_rows(const P& p, const Unit& u, const FewLds
     uint8_t* mine = lds.of(wave);
     few_loop<E, D, WAVES>(p, u, mine, wave, run, acc);
 
-    // Join: every wave's m and l, then its O over the tiles' LDS, row by row
-    // in pieces of four (the rows' pieces turned by the row, so that the lanes
-    // of a half, one row each, write different banks).
     const int row = lane & 31;
     if (half == 0) {
         joint[wave * 2 * ROWS + row] = run.log2_max();
@@ -770,27 +770,43 @@ __device__ __forceinline__ void few_rows(const P& p, const Unit& u, const FewLds
                 f32x4{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
         }
     __syncthreads();
+}
+
+// The waves' sums of four elements from 4 * piece on of row r: m, l, O.
+struct Sums {
+    float mx, sum;
+    f32x4 o;
+};
+template <int D, int WAVES>
+__device__ __forceinline__ Sums few_sum(const FewLds<D, WAVES>& lds, const float* joint, int r, int piece) {
+    Sums s = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s.mx = fmaxf(s.mx, joint[w * 2 * ROWS + r]);
+    const float sub = s.mx == -INFINITY ? 0.f : s.mx;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        const float f = fast_exp2(joint[w * 2 * ROWS + r] - sub);
+        s.sum = fmaf(f, joint[w * 2 * ROWS + ROWS + r], s.sum);
+        const float* src = reinterpret_cast<const float*>(lds.of(w));
+        const f32x4 v = *reinterpret_cast<const f32x4*>(src + r * D + ((piece + r) & (D / 4 - 1)) * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s.o[i] = fmaf(f, v[i], s.o[i]);
+    }
+    return s;
+}
+
+template <class E, int D, int WAVES, class P>
+__device__ __forceinline__ void few_rows(const P& p, const Unit& u, const FewLds<D, WAVES>& lds, float* joint) {
+    few_sums<E, D, WAVES>(p, u, lds, joint);
     float* part = is_partial<P>(u) ? partial_of<FEW, D>(p, u, 0) : nullptr;
     const int R = partial_rows<FEW, P>(u);
     for (int e = threadIdx.x; e < ROWS * (D / 4); e += WAVES * 64) {
         const int r = e / (D / 4), piece = e % (D / 4);
         const Row y = row_of(p, u, u.m * ROWS + r);
         if (!y.live) break;
-        float mx = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) mx = fmaxf(mx, joint[w * 2 * ROWS + r]);
-        const float sub = mx == -INFINITY ? 0.f : mx;
-        float sum = 0.f;
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            const float f = fast_exp2(joint[w * 2 * ROWS + r] - sub);
-            sum = fmaf(f, joint[w * 2 * ROWS + ROWS + r], sum);
-            const float* src = reinterpret_cast<const float*>(lds.of(w));
-            const f32x4 v = *reinterpret_cast<const f32x4*>(src + r * D + ((piece + r) & (D / 4 - 1)) * 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = fmaf(f, v[i], o[i]);
-        }
+        const Sums s = few_sum<D, WAVES>(lds, joint, r, piece);
+        const float mx = s.mx, sum = s.sum;
+        const f32x4 o = s.o;
         if (part) {
             *reinterpret_cast<f32x4*>(part + 2 * R + r * D + piece * 4) = o;
             if (piece == 0) {

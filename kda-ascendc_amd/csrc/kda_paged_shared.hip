@@ -57,53 +57,47 @@ int64_t plan_bytes(const SharedParams& p) {
 // Rows of a tile of partial results: a multiple of 4.
 __host__ __device__ inline int padded(int rows) { return (rows + 3) & ~3; }
 
-// Inclusive prefix sums of three numbers over the work-group's threads.
+// Three numbers, and their sums up to a thread (its own included) and over all
+// of the work-group's; c and its sums no more than LIMIT.
 struct Three {
-    int a, b, c;
+    uint32_t a, b, c;
 };
+constexpr uint32_t LIMIT = 0x7fffffff;
 template <int THREADS>
-__device__ __forceinline__ Three scan(Three x, int (&lds)[3][16]) {
+__device__ __forceinline__ Three scan(Three x, uint32_t (&lds)[3][16], Three& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    Three s = {(int)wave_prefix(x.a), (int)wave_prefix(x.b), (int)wave_prefix(x.c)};
-    __syncthreads();
+    Three s = {wave_prefix(x.a), wave_prefix(x.b), wave_prefix(x.c, LIMIT)};
     if (lane == 63) {
         lds[0][wave] = s.a;
         lds[1][wave] = s.b;
         lds[2][wave] = s.c;
     }
     __syncthreads();
+    all = {0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w)
-        if (w < wave) {
-            s.a += lds[0][w];
-            s.b += lds[1][w];
-            s.c += lds[2][w];
-        }
+    for (int w = 0; w < THREADS / 64; ++w) {
+        if (w == wave) s = {s.a + all.a, s.b + all.b, min(s.c + all.c, LIMIT)};
+        all = {all.a + lds[0][w], all.b + lds[1][w], min(all.c + lds[2][w], LIMIT)};
+    }
     return s;
 }
-// Sums over the work-group's threads.
-template <int THREADS>
-__device__ __forceinline__ int64_t sum(int64_t x, int64_t (&lds)[16]) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
-    __syncthreads();
-    int64_t all = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) all += lds[w];
-    return all;
-}
 
-// One work-group.  `waves`: those of a work-group of few rows; `room`: of the
-// partial results, in 4 rows.
+// Of sequences that share, those with few rows and up to this many tiles of keys
+// of their own have them worked on in the join.
+constexpr int IN_JOIN = 16;
+// Rounds of parts of many rows at most, on 256 CUs each.
+constexpr int ROUNDS = 3;
+
+// One work-group.  `waves`: those of a work-group of few rows; `rounds`: of parts
+// of many rows, at most; `room`: of the partial results, in 4 rows.
 template <int THREADS>
-__global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams p, int waves, int room) {
+__global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams p, int waves, int rounds, int room) {
+    constexpr bool ONE = THREADS < 1024;  // a record a thread
     __shared__ int cu[MOST + 1], least[MOST], sharing[MOST], shared_of[MOST];
-    __shared__ int lds3[3][16];
-    __shared__ int64_t lds[16];
+    __shared__ uint32_t lds[2][3][16];
     constexpr int BIG = 1 << 20;
-    const int tid = threadIdx.x, V = p.NG + p.N, each = (V + THREADS - 1) / THREADS;  // records a thread
+    const int tid = threadIdx.x, V = p.NG + p.N;
+    const int each = ONE ? 1 : (V + THREADS - 1) / THREADS, v0 = tid * each, v1 = min(V, v0 + each);
     const int64_t most = (int64_t)p.M << p.page_shift;
     for (int g = tid; g <= p.NG; g += THREADS) {
         cu[g] = min(max(p.cu_groups[g], 0), p.N);
@@ -114,6 +108,9 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
             sharing[g] = 0;
         }
     }
+    NewTokens mine = {};  // (a record a thread: its sequence's)
+    if (ONE && v0 >= p.NG && v0 < V) mine = new_tokens(p, v0 - p.NG);
+    auto tokens = [&](int v) { return ONE ? mine : new_tokens(p, v - p.NG); };
     __syncthreads();
     // The group of sequence n, -1 for none.
     auto group_of = [&](int n) {
@@ -127,11 +124,11 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
     };
     // A sequence shares if its new tokens all come behind the group's shared ones.
     auto shares = [&](const NewTokens& s, int g) { return g >= 0 && s.count > 0 && shared_of[g] > 0 && s.pos >= shared_of[g]; };
-    for (int n = tid; n < p.N; n += THREADS) {
-        const NewTokens s = new_tokens(p, n);
-        const int g = group_of(n);
+    for (int v = max(v0, p.NG); v < v1; ++v) {
+        const NewTokens s = tokens(v);
+        const int g = group_of(v - p.NG);
         if (shares(s, g)) {
-            atomicMin(&least[g], n);
+            atomicMin(&least[g], v - p.NG);
             atomicAdd(&sharing[g], 1);
         }
         // (a sequence that fills a row tile by itself: nothing to gain for it)
@@ -140,15 +137,15 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
     __syncthreads();
     auto active = [&](int g) { return sharing[g] >= 2 && sharing[g] < BIG; };
 
-    // What there is to work on, and how much of each kind.
     const Plan plan = plan_of(p);
-    int64_t few_all = 0, many_all = 0, many_tiles = 0;
-    for (int v = tid * each; v < min(V, (tid + 1) * each); ++v) {
+    // Record v, but for its parts and their place.
+    auto record = [&](int v) {
         Work w = {};
-        w.group = -1;
+        w.group = NONE;
+        w.place = NONE;
         if (v >= p.NG) {
             const int n = v - p.NG;
-            const NewTokens s = new_tokens(p, n);
+            const NewTokens s = tokens(v);
             w.first = p.cu_seqlens ? s.first : n * p.T;
             w.count = s.count;
             w.len = s.len;
@@ -166,65 +163,84 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
             w.len = w.pos = shared_of[v];
             w.row = least[v];
         }
-        if (w.count > 0) {
-            w.few = (int64_t)w.count * p.G <= ROWS;
-            const int TK = w.few ? Shape<FEW>::TK : Shape<MANY>::TK, MT = w.few ? Shape<FEW>::MT : Shape<MANY>::MT;
-            w.mt = (int)(((int64_t)w.count * p.G + MT - 1) / MT);
-            w.tiles = max(1, (w.len + TK - 1) / TK - w.from / TK);
-            if (w.few) {
-                few_all += w.tiles;
-            } else {
-                many_all += w.mt;
-                many_tiles += (int64_t)w.mt * w.tiles;
-            }
+        w.few = (int64_t)w.count * p.G <= ROWS;
+        const int shift = w.few ? 5 : 6, MT = w.few ? Shape<FEW>::MT : Shape<MANY>::MT;
+        static_assert(Shape<FEW>::TK == 32 && Shape<MANY>::TK == 64, "keys a tile");
+        w.mt = (int)(((int64_t)w.count * p.G + MT - 1) / MT);
+        w.tiles = max(1, (int)(((uint32_t)w.len + (1u << shift) - 1) >> shift) - (w.from >> shift));
+        return w;
+    };
+    // Whether the join works on a record's keys.
+    auto in_join = [&](const Work& w) { return w.few && w.group >= 0 && w.tiles <= IN_JOIN; };
+    Work w;
+    Three x = {0, 0, 0}, all;
+    for (int v = v0; v < v1; ++v) {
+        w = record(v);
+        if (w.count > 0 && !in_join(w)) {
+            if (w.few) x.a += w.tiles * p.HKV;
+            else x = {x.a, x.b + w.mt * p.HKV, (uint32_t)min((int64_t)x.c + (int64_t)w.mt * p.HKV * w.tiles, (int64_t)LIMIT)};
         }
-        plan.work[v] = w;
+        if (!ONE) plan.work[v] = w;
     }
-    few_all = sum<THREADS>(few_all, lds) * p.HKV;
-    many_all = sum<THREADS>(many_all, lds) * p.HKV;
-    many_tiles = sum<THREADS>(many_tiles, lds) * p.HKV;
-    const int slots = few_slots(waves);
-    const int64_t size = max((int64_t)waves, (few_all + slots - 1) / slots);
-    const bool cut = many_all <= Shape<MANY>::SLOTS / 2;
-    // Units of few and of many rows, and the room that a record's results need.
+    scan<THREADS>(x, lds[0], all);
+    // Few rows: parts of `size` tiles, at most as many of them as run at once.
+    const uint32_t slots = few_slots(waves), size = max((uint32_t)waves, (all.a + slots - 1) / slots);
+    // Many rows: with all.b row tiles of all.c tiles of keys together, `share` parts
+    // of equal size if they can be had, in 1 to 3 rounds: the fewest tiles one after
+    // the other, 4 more a round for its beginning and end.  (Of LIMIT tiles, which
+    // are hours of work, none is cut.)
+    uint32_t share = 0;
+    float best = 3.4e38f;
+    for (int r = 1; r <= rounds && all.c < LIMIT; ++r) {
+        const uint32_t k = all.b > 0 ? (uint32_t)(r * Shape<MANY>::SLOTS) / all.b : 0;
+        const float cost = k > 0 ? r * ((float)all.c / (float)(all.b * k) + 4.f) : best;
+        if (cost < best) {
+            best = cost;
+            share = r * Shape<MANY>::SLOTS;
+        }
+    }
+    // A record's parts; units of few and of many rows, and the room of its results.
     auto needs = [&](Work& w, int v) {
         Three x = {0, 0, 0};
-        if (w.count == 0) return x;
+        if (w.count == 0 || in_join(w)) return x;
         if (w.few) {
             w.parts = (int)((w.tiles + size - 1) / size);
             x.a = w.parts * p.HKV;
         } else {
             w.parts = 1;
-            if (cut) {
-                const int64_t parts = (int64_t)w.tiles * Shape<MANY>::SLOTS / many_tiles;
-                w.parts = (int)max((int64_t)1, min((int64_t)w.tiles / Shape<MANY>::LEAST, parts));
+            if (share > 0) {
+                // (exact: the quotient of 32 bits by 32 is no nearer to a whole number than 2^-32)
+                const uint32_t parts = (uint32_t)((double)w.tiles * (double)share / (double)all.c);
+                w.parts = (int)max(1u, min((uint32_t)w.tiles / Shape<MANY>::LEAST, parts));
             }
             x.b = w.mt * w.parts * p.HKV;
         }
-        w.place = NONE;
-        if (w.parts > 1 || v < p.NG || w.group >= 0) x.c = padded(w.count * p.G) / 4 * w.parts * p.HKV;
+        if (w.parts > 1 || v < p.NG || w.group >= 0)
+            x.c = (uint32_t)min((int64_t)(padded(w.count * p.G) / 4) * w.parts * p.HKV, (int64_t)LIMIT);
         return x;
     };
-    Three mine = {0, 0, 0};
-    for (int v = tid * each; v < min(V, (tid + 1) * each); ++v) {
-        Work w = plan.work[v];
-        const Three x = needs(w, v);
-        mine = {mine.a + x.a, mine.b + x.b, mine.c + x.c};
+    Three mine3 = {0, 0, 0};
+    for (int v = v0; v < v1; ++v) {
+        if (!ONE) w = plan.work[v];
+        x = needs(w, v);
+        mine3 = {mine3.a + x.a, mine3.b + x.b, min(mine3.c + x.c, LIMIT)};
     }
-    const Three upto = scan<THREADS>(mine, lds3);
-    Three at = {upto.a - mine.a, upto.b - mine.b, upto.c - mine.c};
-    for (int v = tid * each; v < min(V, (tid + 1) * each); ++v) {
-        Work w = plan.work[v];
-        const Three x = needs(w, v);
-        if (x.c > 0) w.place = at.c + x.c <= room ? at.c : OVER;
-        at = {at.a + x.a, at.b + x.b, at.c + x.c};
+    const Three upto = scan<THREADS>(mine3, lds[1], all);
+    Three at = {upto.a - mine3.a, upto.b - mine3.b, upto.c - mine3.c};  // (room is below LIMIT)
+    for (int v = v0; v < v1; ++v) {
+        if (!ONE) {
+            w = plan.work[v];
+            x = needs(w, v);
+        }
+        if (x.c > 0) w.place = upto.c < LIMIT && at.c + x.c <= (uint32_t)room ? (int)at.c : OVER;
+        at = {at.a + x.a, at.b + x.b, min(at.c + x.c, LIMIT)};
         plan.few_end[v] = at.a;
         plan.many_end[v] = at.b;
         plan.work[v] = w;
     }
     if (tid == THREADS - 1) {
-        plan.head[0] = upto.a;
-        plan.head[1] = upto.b;
+        plan.head[0] = all.a;
+        plan.head[1] = all.b;
     }
 }
 
@@ -326,80 +342,113 @@ __global__ __launch_bounds__(KIND == FEW ? 256 : 512, 2) void paged_shared_kerne
     }
 }
 
-// Joins the parts of (sequence n, kv head h): its own and those of its group's
-// shared tokens, four elements of a row a thread, SLICES threads' parts in turn.
+// Where the partial results of a row are: `parts` of them, `step` floats apart,
+// each of R rows with this one the r-th.
+struct Parts {
+    const float* first;
+    int64_t step;
+    int parts, R, r;
+    __device__ __forceinline__ const float* at(int j) const { return first + j * step; }
+};
+template <int D>
+__device__ __forceinline__ Parts parts_of(const SharedParams& p, const Work& w, int h, int row) {
+    constexpr int MT = Shape<MANY>::MT;
+    Parts x;
+    const int m = w.few ? 0 : row / MT;
+    x.r = row - m * MT;
+    x.R = w.few ? tile_rows<ROWS>(p, w, 0) : tile_rows<MT>(p, w, m);
+    x.first = p.ws + (w.few ? place_of<D, ROWS>(p, w, 0, h, 0, x.R) : place_of<D, MT>(p, w, m, h, 0, x.R));
+    x.step = (x.R / 4) * FOUR<D>;
+    x.parts = w.parts;
+    return x;
+}
+__device__ __forceinline__ void add(Sums& s, float mx, float sum, const f32x4& o) {
+    const float top = fmaxf(s.mx, mx), sub = top == -INFINITY ? 0.f : top;
+    const float f0 = fast_exp2(s.mx - sub), f = fast_exp2(mx - sub);
+    s.mx = top;
+    s.sum = fmaf(f, sum, s.sum * f0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s.o[i] = fmaf(f, o[i], s.o[i] * f0);
+}
+// Parts from, from + by and so on of four elements of a row, in one pass, so that
+// no load waits for another.
+__device__ __forceinline__ void add_parts(Sums& s, const Parts& x, int piece, int D, int from, int by) {
+#pragma unroll 8
+    for (int j = from; j < x.parts; j += by) {
+        const float* part = x.at(j);
+        add(s, part[x.r], part[x.R + x.r], *reinterpret_cast<const f32x4*>(part + 2 * x.R + x.r * D + piece * 4));
+    }
+}
+
+// Joins the parts of (sequence n, kv head h): those of its group's shared tokens
+// and its own, or its own keys worked on here where they are few (work-group 0 of
+// `groups`).  Four elements of a row a thread; where rows are few, several
+// threads' parts in turn.
 template <class E, int D>
-__global__ __launch_bounds__(256) void paged_shared_join_kernel(SharedParams p, int groups) {
-    __shared__ float lds[6 * 256];
+__global__ __launch_bounds__(256, 2) void paged_shared_join_kernel(SharedParams p, int groups) {
+    constexpr int WAVES = Shape<FEW>::WAVES;
+    typedef FewLds<D, WAVES> Lds;
+    __shared__ alignas(1024) uint8_t lds[WAVES * Lds::EACH];
+    __shared__ float joint[WAVES * 2 * ROWS];
+    __shared__ float sums[6 * 256];
     const Plan plan = plan_of(p);
     const int id = blockIdx.x / groups, n = id / p.HKV, h = id - n * p.HKV;
     const Work w = load_work(plan, p.NG + n);
-    if (w.count == 0 || w.place < 0) return;
+    const bool here = w.parts == 0;
+    if (w.count == 0 || (here ? (int)blockIdx.x % groups > 0 : w.place < 0)) return;
     Work g = {};
     if (w.group >= 0) g = load_work(plan, w.group);
     if (g.place == OVER) return;
-    const int rows = w.count * p.G, rows_g = g.count * p.G;
-    const bool w_few = w.few, g_few = g.few;
-    const int slice = threadIdx.x >> 6;
-    for (int group = blockIdx.x % groups; group * 64 < rows * (D / 4); group += groups) {
-        const int e = group * 64 + (threadIdx.x & 63), r = e / (D / 4), piece = e % (D / 4);
+    const Lds tiles = {lds, lds, lds};
+    if (here) {
+        Unit u;
+        u.n = w.row;
+        u.h = h;
+        u.m = 0;
+        u.s = NewTokens{w.first, w.count, w.len, w.pos};
+        u.lo = w.from;
+        u.hi = w.len;
+        u.begin = w.from / Shape<FEW>::TK;
+        u.end = (w.len + Shape<FEW>::TK - 1) / Shape<FEW>::TK;
+        few_sums<E, D, WAVES>(p, u, tiles, joint);
+    }
+    const int rows = w.count * p.G, items = rows * (D / 4);
+    // threads an item, at most 4, that divide the work-group
+    const int shift = items > 128 ? 0 : (items > 64 ? 1 : 2), per = 256 >> shift;
+    const int slice = threadIdx.x / per, item = threadIdx.x % per;
+    // (work-group 0 has all of its own)
+    const int group0 = here ? 0 : blockIdx.x % groups, by = here ? 1 : groups;
+    for (int group = group0; group * per < items; group += by) {
+        const int e = group * per + item, r = e / (D / 4), piece = e % (D / 4);
         const bool live = r < rows;
-        // its place in the group's rows
-        const int rg = (w.first - g.first) * p.G + r;
-        const int shared_parts = w.group >= 0 && rg >= 0 && rg < rows_g ? g.parts : 0;
-        float mx = -INFINITY, total = 0.f;
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        Sums s = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
         if (live) {
-            const int m = w_few ? 0 : r / Shape<MANY>::MT, mg = g_few ? 0 : rg / Shape<MANY>::MT;
-            const int R = w_few ? tile_rows<ROWS>(p, w, 0) : tile_rows<Shape<MANY>::MT>(p, w, m);
-            const int RG = g_few ? tile_rows<ROWS>(p, g, 0) : tile_rows<Shape<MANY>::MT>(p, g, mg);
-            const float* own = p.ws + (w_few ? place_of<D, ROWS>(p, w, 0, h, 0, R) : place_of<D, Shape<MANY>::MT>(p, w, m, h, 0, R));
-            const float* theirs = p.ws + (g_few ? place_of<D, ROWS>(p, g, 0, h, 0, RG) : place_of<D, Shape<MANY>::MT>(p, g, mg, h, 0, RG));
-            const int r_own = r - m * Shape<MANY>::MT, r_theirs = rg - mg * Shape<MANY>::MT;
-#pragma unroll 4
-            for (int j = slice; j < shared_parts + w.parts; j += SLICES) {
-                const bool s = j < shared_parts;
-                const float* part = s ? theirs + (int64_t)j * (RG / 4) * FOUR<D> : own + (int64_t)(j - shared_parts) * (R / 4) * FOUR<D>;
-                const int rr = s ? r_theirs : r_own, RR = s ? RG : R;
-                const float mj = part[rr], lj = part[RR + rr];
-                const f32x4 v = *reinterpret_cast<const f32x4*>(part + 2 * RR + rr * D + piece * 4);
-                const float top = fmaxf(mx, mj), sub = top == -INFINITY ? 0.f : top;
-                const float f0 = fast_exp2(mx - sub), f = fast_exp2(mj - sub);
-                mx = top;
-                total = fmaf(f, lj, total * f0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] = fmaf(f, v[i], o[i] * f0);
-            }
+            if (here && slice == 0) s = few_sum<D, WAVES>(tiles, joint, r, piece);
+            const int rg = (w.first - g.first) * p.G + r;  // its place in the group's rows
+            if (w.group >= 0 && rg >= 0 && rg < g.count * p.G) add_parts(s, parts_of<D>(p, g, h, rg), piece, D, slice, 1 << shift);
+            if (!here) add_parts(s, parts_of<D>(p, w, h, r), piece, D, slice, 1 << shift);
         }
-        const int t = threadIdx.x;
-        lds[t] = mx;
-        lds[256 + t] = total;
+        if (shift > 0) {
+            const int t = threadIdx.x;
+            sums[t] = s.mx;
+            sums[256 + t] = s.sum;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) lds[(2 + i) * 256 + t] = o[i];
-        __syncthreads();
-        if (slice == 0 && live) {
-            float top = mx;
-#pragma unroll
-            for (int k = 1; k < SLICES; ++k) top = fmaxf(top, lds[k * 64 + t]);
-            const float sub = top == -INFINITY ? 0.f : top;
-            float f = fast_exp2(mx - sub);
-            total *= f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] *= f;
-#pragma unroll
-            for (int k = 1; k < SLICES; ++k) {
-                f = fast_exp2(lds[k * 64 + t] - sub);
-                total = fmaf(f, lds[256 + k * 64 + t], total);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] = fmaf(f, lds[(2 + i) * 256 + k * 64 + t], o[i]);
-            }
-            const float inv = total > 0.f ? 1.f / total : 0.f;
+            for (int i = 0; i < 4; ++i) sums[(2 + i) * 256 + t] = s.o[i];
+            __syncthreads();
+            if (slice == 0)
+                for (int k = 1; k < 1 << shift; ++k) {
+                    const int j = k * per + item;
+                    add(s, sums[j], sums[256 + j], f32x4{sums[512 + j], sums[768 + j], sums[1024 + j], sums[1280 + j]});
+                }
+            __syncthreads();
+        }
+        if (live && slice == 0) {
+            const float inv = s.sum > 0.f ? 1.f / s.sum : 0.f;
             const int tok = r / p.G;
             const int64_t out = ((int64_t)w.first + tok) * p.HQ + h * p.G + (r - tok * p.G);
-            store_o<E, D>(p, out, piece * 4, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-            if (p.lse && piece == 0) p.lse[out] = log_sum(top, total);
+            store_o<E, D>(p, out, piece * 4, s.o[0] * inv, s.o[1] * inv, s.o[2] * inv, s.o[3] * inv);
+            if (p.lse && piece == 0) p.lse[out] = log_sum(s.mx, s.sum);
         }
-        __syncthreads();
     }
 }
 
@@ -413,6 +462,21 @@ bool together(const SharedParams& p) {
 int64_t tokens_of(const SharedParams& p) { return p.cu_seqlens ? p.T : (int64_t)p.N * p.T; }
 bool few_only(const SharedParams& p) { return tokens_of(p) * p.G <= ROWS; }
 
+// Row tiles of many rows at most.  Records of many rows have more than ROWS.
+int64_t row_tiles(const SharedParams& p) {
+    if (few_only(p)) return 0;
+    const int64_t rows = tokens_of(p) * p.G;
+    const bool members = p.cu_seqlens || (int64_t)p.T * p.G > ROWS;
+    const int64_t records = std::min(std::min(p.NG, p.N / 2) + (members ? p.N : 0), (int)std::min((members ? 2 : 1) * rows / ROWS, (int64_t)MOST * 2));
+    return (records + (members ? 2 : 1) * rows / Shape<MANY>::MT) * p.HKV;
+}
+// Rounds of parts of many rows (two and more only with more than half as many row
+// tiles as CUs: fewer are cut well in one).
+int rounds_of(const SharedParams& p) {
+    const int64_t tiles = row_tiles(p);
+    return tiles == 0 ? 0 : tiles <= Shape<MANY>::SLOTS / 2 ? 1 : ROUNDS;
+}
+
 // Room of the partial results, in 4 rows: twice the rows that may be worked on
 // together (a group's and the sequences', each filled up to 4), and the parts
 // that keys are cut into.
@@ -420,30 +484,25 @@ int64_t room_of(const SharedParams& p) {
     const int64_t sharing = std::min(tokens_of(p), (int64_t)p.N * (Shape<MANY>::MT / p.G + 1));
     const int64_t rows = (2 * sharing * p.G + 3 * (int64_t)(p.N + p.NG)) * p.HKV;
     const int64_t few = 2 * (int64_t)few_slots(Shape<FEW>::WAVES) * ROWS;
-    const int64_t many = few_only(p) ? 0 : (int64_t)Shape<MANY>::SLOTS * Shape<MANY>::MT;
+    const int64_t many = (int64_t)rounds_of(p) * Shape<MANY>::SLOTS * Shape<MANY>::MT;
     return (rows + few + many + 3) / 4;
 }
 
 // Units at most: a record's heads and row tiles, and the parts more that keys
-// are cut into.  Records of many rows have more than ROWS of them.
+// are cut into.
 int64_t units_of(const SharedParams& p, int waves) {
-    const int64_t rows = tokens_of(p) * p.G;
-    const int64_t groups = std::min(p.NG, p.N / 2), all = p.N + groups;
-    const int64_t few = all * p.HKV + few_slots(waves);
-    if (few_only(p)) return few;
-    const bool members = p.cu_seqlens || (int64_t)p.T * p.G > ROWS;
-    const int64_t records = std::min(groups + (members ? p.N : 0), (members ? 2 : 1) * rows / ROWS);
-    return few + (records + (members ? 2 : 1) * rows / Shape<MANY>::MT) * p.HKV + Shape<MANY>::SLOTS;
+    const int64_t few = ((int64_t)p.N + std::min(p.NG, p.N / 2)) * p.HKV + few_slots(waves);
+    return few + row_tiles(p) + rounds_of(p) * Shape<MANY>::SLOTS;
 }
 
 template <class E, int D>
 hipError_t launch_shared(SharedParams p, hipStream_t stream) {
     p.plan = reinterpret_cast<int32_t*>(p.ws + 4 * (D + 2) * room_of(p));
-    const int V = p.NG + p.N, room = (int)std::min(room_of(p), (int64_t)0x7fffffff);
+    const int V = p.NG + p.N, room = (int)std::min(room_of(p), (int64_t)LIMIT - 1);
     const bool only = few_only(p);
     const int waves = Shape<FEW>::WAVES * (only ? 1 : 2);
-    if (V <= 256) paged_shared_plan_kernel<256><<<1, 256, 0, stream>>>(p, waves, room);
-    else paged_shared_plan_kernel<1024><<<1, 1024, 0, stream>>>(p, waves, room);
+    if (V <= 256) paged_shared_plan_kernel<256><<<1, 256, 0, stream>>>(p, waves, rounds_of(p), room);
+    else paged_shared_plan_kernel<1024><<<1, 1024, 0, stream>>>(p, waves, rounds_of(p), room);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const dim3 grid((unsigned)units_of(p, waves));
@@ -451,9 +510,12 @@ hipError_t launch_shared(SharedParams p, hipStream_t stream) {
     else paged_shared_kernel<E, D, MIXED><<<grid, 512, 0, stream>>>(p);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const int64_t rows = p.cu_seqlens ? ROWS : std::min((int64_t)p.T * p.G, (int64_t)ROWS);
-    const int groups = (int)std::min((rows * (D / 4) + 63) / 64, (int64_t)4);
-    paged_shared_join_kernel<E, D><<<dim3((unsigned)(p.N * p.HKV * groups)), 256, 0, stream>>>(p, groups);
+    // work-groups a (sequence, head): one for every 256 fours of its rows, as many
+    // as there is some use for
+    const int64_t pairs = (int64_t)p.N * p.HKV;
+    const int64_t rows = std::min((int64_t)p.T * p.G, p.cu_seqlens ? (int64_t)1 << 20 : (int64_t)Shape<MANY>::MT);
+    const int groups = (int)std::max((int64_t)1, std::min((rows * (D / 4) + 255) / 256, 4096 / pairs));
+    paged_shared_join_kernel<E, D><<<dim3((unsigned)(pairs * groups)), 256, 0, stream>>>(p, groups);
     return hipGetLastError();
 }
 
