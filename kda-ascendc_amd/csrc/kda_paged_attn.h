@@ -858,6 +858,49 @@ __device__ __forceinline__ void few_piece(const P& p, int b, bool may_cut, const
 
 // ---- many rows ----
 
+// The products of a wave's 32 rows and a tile of 64 keys at `ks`, or values at
+// `vs`.  Their operands are read one group of matrix ops ahead of their use, a
+// read between two matrix ops: an LDS read takes several of them.
+template <class E, int D>
+__device__ __forceinline__ void tile_scores(const uint8_t* ks, const u32x4 (&q)[D / 16], f32x16 (&st)[2], int lane) {
+    constexpr int STEPS = D / 16;
+    const int half = lane >> 5;
+    u32x4 a[2][4];
+    auto read = [&](int g, int i) { return read_k<D>(ks, 32 * (i & 1) + (lane & 31), 2 * (2 * g + (i >> 1)) + half); };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[0][i] = read(0, i);
+    st[0] = st[1] = f32x16{};
+#pragma unroll
+    for (int g = 0; g < STEPS / 2; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (g + 1 < STEPS / 2) a[(g + 1) & 1][i] = read(g + 1, i);
+            st[i & 1] = E::mfma(a[g & 1][i], q[2 * g + (i >> 1)], st[i & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+}
+template <class E, int D>
+__device__ __forceinline__ void tile_outputs(const uint8_t* vs, const u32x4 (&pt)[4], f32x16 (&acc)[D / 32], int lane) {
+    constexpr int DB = D / 32;
+    const int half = lane >> 5;
+    u32x4 a[2][DB];
+    auto read = [&](int k, int d) {
+        const u32x2 v0 = read_v<D>(vs, 16 * k + 4 * half, d, lane);
+        const u32x2 v1 = read_v<D>(vs, 16 * k + 8 + 4 * half, d, lane);
+        return u32x4{v0.x, v0.y, v1.x, v1.y};
+    };
+#pragma unroll
+    for (int d = 0; d < DB; ++d) a[0][d] = read(0, d);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            if (k + 1 < 4) a[(k + 1) & 1][d] = read(k + 1, d);
+            acc[d] = E::mfma(a[k & 1][d], pt[k], acc[d]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+}
+
 // The work-group meets; the wave's LDS reads have returned.  The clobber keeps
 // LDS accesses on their side.
 __device__ __forceinline__ void meet() {
@@ -953,47 +996,10 @@ __device__ __forceinline__ void many_rows(const P& p, const Unit& u, uint8_t* kt
         k0.template load_at<(I + 2) % 3 * TILE>(of_lane(k_of, (t + 2) & 63), k_lds);
         v0.template load_at<(I + 1) % 3 * TILE>(of_lane(v_of, (t + 1) & 63), v_lds);
     };
-    // The products' operands are read one group of matrix ops ahead of their
-    // use, a read between two matrix ops: an LDS read takes several of them.
-    auto scores = [&](const uint8_t* ks) {
-        u32x4 a[2][4];
-        auto read = [&](int g, int i) {
-            return read_k<D>(ks, 32 * (i & 1) + (lane & 31), 2 * (2 * g + (i >> 1)) + half);
-        };
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a[0][i] = read(0, i);
-        st[0] = st[1] = f32x16{};
-#pragma unroll
-        for (int g = 0; g < STEPS / 2; ++g)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (g + 1 < STEPS / 2) a[(g + 1) & 1][i] = read(g + 1, i);
-                st[i & 1] = E::mfma(a[g & 1][i], q[2 * g + (i >> 1)], st[i & 1]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-    };
-    auto outputs = [&](const uint8_t* vs) {
-        u32x4 a[2][DB];
-        auto read = [&](int k, int d) {
-            const u32x2 v0 = read_v<D>(vs, 16 * k + 4 * half, d, lane);
-            const u32x2 v1 = read_v<D>(vs, 16 * k + 8 + 4 * half, d, lane);
-            return u32x4{v0.x, v0.y, v1.x, v1.y};
-        };
-#pragma unroll
-        for (int d = 0; d < DB; ++d) a[0][d] = read(0, d);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                if (k + 1 < 4) a[(k + 1) & 1][d] = read(k + 1, d);
-                acc[d] = E::mfma(a[k & 1][d], pt[k], acc[d]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-    };
     auto products = [&](int t, const uint8_t* ks, const uint8_t* vs) {
         __builtin_amdgcn_s_setprio(1);
-        if (sees(t - 1)) outputs(vs);
-        if (sees(t)) scores(ks);
+        if (sees(t - 1)) tile_outputs<E, D>(vs, pt, acc, lane);
+        if (sees(t)) tile_scores<E, D>(ks, q, st, lane);
         __builtin_amdgcn_s_setprio(0);
     };
     auto softmax = [&](int t) {
@@ -1025,7 +1031,7 @@ __device__ __forceinline__ void many_rows(const P& p, const Unit& u, uint8_t* kt
             if (t + 1 < count) step(t + 1, std::integral_constant<int, 1>{});
             if (t + 2 < count) step(t + 2, std::integral_constant<int, 2>{});
         }
-        if (sees(count - 1)) outputs(vt + (count - 1) % 3 * TILE);
+        if (sees(count - 1)) tile_outputs<E, D>(vt + (count - 1) % 3 * TILE, pt, acc, lane);
         if (!second) meet();
     }
     wait_loads<0>();  // (past the last tile)

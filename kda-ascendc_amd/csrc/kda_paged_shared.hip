@@ -19,6 +19,16 @@
 namespace kda {
 namespace {
 
+// Rows of a tile: fewer than a work-group's waves have, whose two groups of four
+// have the same rows and go over keys of their own, every other tile.  A part then
+// leaves half the partial results of one with 256 rows, which is what its time
+// goes to where a prefix is cut for the whole card: 64 sequences of 4 heads a kv
+// head behind 16000 tokens are 256 parts of 8 tiles of 256 rows, whose results
+// (34 MB) took 7 us to write and as long to read.
+constexpr int MT = 128;
+template <int KIND>
+constexpr int rows_of() { return KIND == FEW ? ROWS : MT; }
+
 // Sequences and groups that a plan has room for.
 constexpr int MOST = 2048;
 
@@ -132,7 +142,7 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
             atomicAdd(&sharing[g], 1);
         }
         // (a sequence that fills a row tile by itself: nothing to gain for it)
-        if (g >= 0 && (int64_t)s.count * p.G >= Shape<MANY>::MT) atomicOr(&sharing[g], BIG);
+        if (g >= 0 && (int64_t)s.count * p.G >= MT) atomicOr(&sharing[g], BIG);
     }
     __syncthreads();
     auto active = [&](int g) { return sharing[g] >= 2 && sharing[g] < BIG; };
@@ -164,9 +174,9 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
             w.row = least[v];
         }
         w.few = (int64_t)w.count * p.G <= ROWS;
-        const int shift = w.few ? 5 : 6, MT = w.few ? Shape<FEW>::MT : Shape<MANY>::MT;
+        const int shift = w.few ? 5 : 6, rows = w.few ? ROWS : MT;
         static_assert(Shape<FEW>::TK == 32 && Shape<MANY>::TK == 64, "keys a tile");
-        w.mt = (int)(((int64_t)w.count * p.G + MT - 1) / MT);
+        w.mt = (int)(((int64_t)w.count * p.G + rows - 1) / rows);
         w.tiles = max(1, (int)(((uint32_t)w.len + (1u << shift) - 1) >> shift) - (w.from >> shift));
         return w;
     };
@@ -249,13 +259,13 @@ template <int D>
 constexpr int64_t FOUR = 4 * (D + 2);
 
 // Where the part-th part of row tile m of (w, kv head h) is, of `rows` rows.
-template <int D, int MT>
+template <int D, int ROWS_A_TILE>
 __device__ __forceinline__ int64_t place_of(const SharedParams& p, const Work& w, int m, int h, int part, int rows) {
-    return FOUR<D> * (w.place + (int64_t)m * (MT / 4) * p.HKV * w.parts + (h * w.parts + part) * (rows / 4));
+    return FOUR<D> * (w.place + (int64_t)m * (ROWS_A_TILE / 4) * p.HKV * w.parts + (h * w.parts + part) * (rows / 4));
 }
-template <int MT>
+template <int ROWS_A_TILE>
 __device__ __forceinline__ int tile_rows(const SharedParams& p, const Work& w, int m) {
-    return padded(min(MT, w.count * p.G - m * MT));
+    return padded(min(ROWS_A_TILE, w.count * p.G - m * ROWS_A_TILE));
 }
 
 __device__ __forceinline__ Work load_work(const Plan& plan, int v) {
@@ -276,10 +286,163 @@ __device__ __forceinline__ Work load_work(const Plan& plan, int v) {
     return w;
 }
 
+// ---- many rows ----
+
+// The two groups' products and softmax alternate as in many_rows(), and so do
+// their tiles: group g's are g, g + 2 and so on.
+//   slot     t (even)                        t + 1
+//   group 0  products: V(t - 2), K(t)        loads K(t + 3), V(t + 1); softmax(t)
+//   group 1  loads K(t + 2), V(t); softmax(t - 1)   products: V(t - 1), K(t + 1)
+// The group that does the softmax loads for the other: a tile is waited for by
+// its loader at the end of the next slot and read in the one after that.  So a
+// tile needs its place for three slots, and the tiles of either parity have two
+// places each: 4 tiles of keys, 4 of values.
+template <class E, int D>
+__device__ __forceinline__ void split_rows(const SharedParams& p, const Unit& u, uint8_t* kt, uint8_t* vt, float* joint) {
+    constexpr int STEPS = D / 16, DB = D / 32, TK = Shape<MANY>::TK;
+    constexpr int TILE = TK * D * 2, SHARE = TK / 4;  // keys that a wave loads of a tile
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = wave >> 2, in = wave & 3;
+    const int row = in * ROWS + (lane & 31);
+    const Row x = row_of(p, u, u.m * MT + row);
+    const int count = u.end - u.begin;
+    // the keys that every row of this wave sees, and those that any does
+    const int all_hi = __builtin_amdgcn_readlane(x.hi, 0);
+    const int any_hi = u.m * MT + in * ROWS < u.s.count * p.G ? __builtin_amdgcn_readlane(x.hi, 31) : 0;
+    const float c = p.scale * LOG2E;
+    Running run;
+    f32x16 acc[DB], st[2];
+    u32x4 pt[4];
+#pragma unroll
+    for (int i = 0; i < DB; ++i) acc[i] = f32x16{};
+
+    const Loader<D, SHARE, false> k0(p.k, p.k_page, p.k_token, u.h * p.k_head, 0, lane);
+    const Loader<D, SHARE, false> v0(p.v, p.v_page, p.v_token, u.h * p.v_head, 0, lane);
+    // Where this wave's keys lie of 64 tiles of the other group's, j on (the tile
+    // 2 j + 1 - g is its j-th).  Past the last: nothing, zeros.
+    Place k_of, v_of;
+    auto places = [&](int j) {
+        const int t = 2 * (j + lane) + 1 - g;
+        const int key = (u.begin + min(t, count)) * TK + SHARE * in;
+        const int at = min(key >> p.page_shift, p.M - 1);
+        const int page = t < count ? p.page_table[u.n * p.table_stride + at] : -1;
+        k_of = k0.place(p, u, page, key);
+        v_of = v0.place(p, u, page, key);
+    };
+    // places of tile t: parity, then every other
+    auto place = [&](uint8_t* ring, int t) { return lds_address(ring) + ((t & 1) * 2 + ((t >> 1) & 1)) * TILE + in * (SHARE * D * 2); };
+    auto load = [&](const Loader<D, SHARE, false>& of, const Place& at, int j, uint8_t* ring, int t) {
+        of.load(of_lane(at, j & 63), place(ring, t));
+    };
+    // The loads in slot t: keys of tile t + 2 and values of tile t, the other group's.
+    auto begin_loads = [&](int t) {
+        const int j = (t - 1 + g) >> 1;
+        // (the values' places of 64 tiles are the keys' before the next ones are found)
+        load(v0, v_of, j, vt, t);
+        if (((j + 1) & 63) == 0) places(j + 1);
+        load(k0, k_of, j + 1, kt, t + 2);
+    };
+    places(0);
+    load(k0, k_of, 0, kt, 1 - g);
+    u32x4 q[STEPS];
+    load_q<D>(p, u, x, half, q);
+
+    auto key_of = [&](int t) { return (u.begin + t) * TK; };
+    auto sees = [&](int t) { return (unsigned)t < (unsigned)count && key_of(t) < any_hi; };
+    auto softmax = [&](int t) {
+        if (!sees(t)) return;
+        float alpha;
+        const int key = key_of(t);
+        if (softmax_tile<E, false>(st, key + 4 * half, x.lo, x.hi, 0, key < u.lo || key + TK > all_hi, c, run, pt, alpha)) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d) acc[d] *= alpha;
+        }
+    };
+    const uint8_t *kg = kt + g * 2 * TILE, *vg = vt + g * 2 * TILE;
+    const int steps = (count + 1) / 2;
+    // This group's s-th tile, in place I = s % 2.
+    auto step = [&](int s, auto I) {
+        const int t = 2 * s + g;
+        __builtin_amdgcn_s_setprio(1);
+        if (s > 0 && sees(t - 2)) tile_outputs<E, D>(vg + (1 - I) * TILE, pt, acc, lane);
+        if (sees(t)) tile_scores<E, D>(kg + I * TILE, q, st, lane);
+        __builtin_amdgcn_s_setprio(0);
+        wait_loads<0>();
+        meet();
+        begin_loads(t + 1);
+        softmax(t);
+        if (g == 0 || s + 1 < steps) meet();
+    };
+    if (count > 0) {
+        // (where the compiler sees it: else it waits for q in every turn)
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0
+        meet();
+        if (g == 1) {
+            begin_loads(0);
+            meet();
+        }
+        for (int s = 0; s < steps; s += 2) {
+            step(s, std::integral_constant<int, 0>{});
+            if (s + 1 < steps) step(s + 1, std::integral_constant<int, 1>{});
+        }
+        wait_loads<0>();
+        meet();
+        const int last = 2 * (steps - 1) + g;
+        if (sees(last)) tile_outputs<E, D>(vg + ((steps - 1) & 1) * TILE, pt, acc, lane);
+    }
+    // Join: the second group's sums through LDS, each lane's to the lane with the
+    // same row and elements.
+    run.l = sum_halves(run.l);
+    __syncthreads();  // (all have read their values)
+    f32x4* o = reinterpret_cast<f32x4*>(kt) + in * 64 + lane;
+    if (g == 1) {
+        if (half == 0) {
+            joint[row] = run.log2_max();
+            joint[MT + row] = run.l;
+        }
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                o[(4 * d + i) * 256] = f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+    }
+    __syncthreads();
+    if (g == 1 || !x.live) return;
+    const float m0 = run.log2_max(), m1 = joint[row], top = fmaxf(m0, m1), sub = top == -INFINITY ? 0.f : top;
+    const float f0 = fast_exp2(m0 - sub), f1 = fast_exp2(m1 - sub);
+    const float l = fmaf(f1, joint[MT + row], run.l * f0);
+    float* part = is_partial<SharedParams>(u) ? p.ws + u.place : nullptr;
+    const float inv = part ? 1.f : (l > 0.f ? 1.f / l : 0.f);
+    const int64_t out = out_row(p, u, x);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 theirs = o[(4 * d + i) * 256];
+            f32x4 sum;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] = fmaf(f1, theirs[e], acc[d][4 * i + e] * f0) * inv;
+            const int at = 32 * d + 8 * i + 4 * half;
+            if (part) *reinterpret_cast<f32x4*>(part + 2 * u.rows + row * D + at) = sum;
+            else store_o<E, D>(p, out, at, sum[0], sum[1], sum[2], sum[3]);
+        }
+    if (half == 0) {
+        if (part) {
+            part[row] = top;
+            part[u.rows + row] = l;
+        } else if (p.lse) {
+            p.lse[out] = log_sum(top, l);
+        }
+    }
+}
+
+// ---- parts ----
+
 // Unit x of kind KIND; false where its results have no room.
 template <int KIND, int D>
 __device__ __forceinline__ bool unit_of(const SharedParams& p, const Plan& plan, int x, int lane, Unit& u) {
-    constexpr int TK = Shape<KIND>::TK, MT = Shape<KIND>::MT;
+    constexpr int TK = Shape<KIND>::TK, MT = rows_of<KIND>();
     const int32_t* ends = KIND == FEW ? plan.few_end : plan.many_end;
     const int V = p.NG + p.N;
     int v = 0, before = 0;
@@ -323,10 +486,8 @@ template <class E, int D, int KIND>
 __global__ __launch_bounds__(KIND == FEW ? 256 : 512, 2) void paged_shared_kernel(SharedParams p) {
     constexpr int WAVES = Shape<KIND == FEW ? FEW : MANY>::WAVES;
     typedef FewLds<D, WAVES> Lds;
-    constexpr int RING = KIND == FEW ? 16 : 3 * Shape<MANY>::TK * D * 2;
-    __shared__ alignas(1024) uint8_t kt[KIND == FEW ? WAVES * Lds::EACH : RING];
-    __shared__ alignas(1024) uint8_t vt[RING];
-    __shared__ alignas(1024) uint8_t more[KIND == FEW ? 16 : 2 * Lds::EACH];
+    __shared__ alignas(1024) uint8_t lds[WAVES * Lds::EACH];
+    static_assert(WAVES == 4 || sizeof(lds) == 8 * Shape<MANY>::TK * D * 2, "four tiles of keys, four of values");
     __shared__ float joint[WAVES * 2 * ROWS];
     const int lane = threadIdx.x & 63, id = blockIdx.x;
     const Plan plan = plan_of(p);
@@ -336,9 +497,9 @@ __global__ __launch_bounds__(KIND == FEW ? 256 : 512, 2) void paged_shared_kerne
     Unit u;
     if (KIND == FEW || id >= many) {
         if (unit_of<FEW, D>(p, plan, id - many, lane, u))
-            few_rows<E, D, WAVES>(p, u, KIND == FEW ? Lds{kt, kt, kt} : Lds{kt, vt, more}, joint);
+            few_rows<E, D, WAVES>(p, u, Lds{lds, lds + 3 * Lds::EACH, lds + 6 * Lds::EACH}, joint);
     } else if constexpr (KIND != FEW) {
-        if (unit_of<MANY, D>(p, plan, id, lane, u)) many_rows<E, D>(p, u, kt, vt);
+        if (unit_of<MANY, D>(p, plan, id, lane, u)) split_rows<E, D>(p, u, lds, lds + sizeof(lds) / 2, joint);
     }
 }
 
@@ -352,7 +513,6 @@ struct Parts {
 };
 template <int D>
 __device__ __forceinline__ Parts parts_of(const SharedParams& p, const Work& w, int h, int row) {
-    constexpr int MT = Shape<MANY>::MT;
     Parts x;
     const int m = w.few ? 0 : row / MT;
     x.r = row - m * MT;
@@ -454,10 +614,14 @@ __global__ __launch_bounds__(256, 2) void paged_shared_join_kernel(SharedParams 
 
 // ---- launches ----
 
+// Rows of a sequence from which on it is no different from others without a
+// prefix to share: a row tile of the ordinary kernels'.
+constexpr int WHOLE = Shape<MANY>::MT;
+
 // Whether sequences are worked on together at all: not where each fills row
 // tiles by itself, nor where there are more than a plan has room for.
 bool together(const SharedParams& p) {
-    return p.N >= 2 && p.N <= MOST && p.NG <= MOST && (p.cu_seqlens || (int64_t)p.T * p.G < Shape<MANY>::MT);
+    return p.N >= 2 && p.N <= MOST && p.NG <= MOST && (p.cu_seqlens || (int64_t)p.T * p.G < WHOLE);
 }
 int64_t tokens_of(const SharedParams& p) { return p.cu_seqlens ? p.T : (int64_t)p.N * p.T; }
 bool few_only(const SharedParams& p) { return tokens_of(p) * p.G <= ROWS; }
@@ -468,7 +632,7 @@ int64_t row_tiles(const SharedParams& p) {
     const int64_t rows = tokens_of(p) * p.G;
     const bool members = p.cu_seqlens || (int64_t)p.T * p.G > ROWS;
     const int64_t records = std::min(std::min(p.NG, p.N / 2) + (members ? p.N : 0), (int)std::min((members ? 2 : 1) * rows / ROWS, (int64_t)MOST * 2));
-    return (records + (members ? 2 : 1) * rows / Shape<MANY>::MT) * p.HKV;
+    return (records + (members ? 2 : 1) * rows / MT) * p.HKV;
 }
 // Rounds of parts of many rows (two and more only with more than half as many row
 // tiles as CUs: fewer are cut well in one).
@@ -481,10 +645,10 @@ int rounds_of(const SharedParams& p) {
 // together (a group's and the sequences', each filled up to 4), and the parts
 // that keys are cut into.
 int64_t room_of(const SharedParams& p) {
-    const int64_t sharing = std::min(tokens_of(p), (int64_t)p.N * (Shape<MANY>::MT / p.G + 1));
+    const int64_t sharing = std::min(tokens_of(p), (int64_t)p.N * (MT / p.G + 1));
     const int64_t rows = (2 * sharing * p.G + 3 * (int64_t)(p.N + p.NG)) * p.HKV;
     const int64_t few = 2 * (int64_t)few_slots(Shape<FEW>::WAVES) * ROWS;
-    const int64_t many = (int64_t)rounds_of(p) * Shape<MANY>::SLOTS * Shape<MANY>::MT;
+    const int64_t many = (int64_t)rounds_of(p) * Shape<MANY>::SLOTS * MT;
     return (rows + few + many + 3) / 4;
 }
 
@@ -513,7 +677,7 @@ hipError_t launch_shared(SharedParams p, hipStream_t stream) {
     // work-groups a (sequence, head): one for every 256 fours of its rows, as many
     // as there is some use for
     const int64_t pairs = (int64_t)p.N * p.HKV;
-    const int64_t rows = std::min((int64_t)p.T * p.G, p.cu_seqlens ? (int64_t)1 << 20 : (int64_t)Shape<MANY>::MT);
+    const int64_t rows = std::min((int64_t)p.T * p.G, p.cu_seqlens ? (int64_t)1 << 20 : (int64_t)WHOLE);
     const int groups = (int)std::max((int64_t)1, std::min((rows * (D / 4) + 255) / 256, 4096 / pairs));
     paged_shared_join_kernel<E, D><<<dim3((unsigned)(pairs * groups)), 256, 0, stream>>>(p, groups);
     return hipGetLastError();
