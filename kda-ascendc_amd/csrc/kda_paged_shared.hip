@@ -35,33 +35,29 @@ constexpr int MOST = 2048;
 // What is worked on together: the queries of a group over its shared tokens, or
 // those of a sequence over its own.  Records of all groups, then of all
 // sequences.
-struct Work {
+struct alignas(16) Work {
     int first, count, len, pos;  // as NewTokens, `first` a token of all
     int from, row;               // the first key, a row of the table
     int parts, mt;               // parts of a row tile's keys; row tiles
     int place;                   // of the partial results, in 4 rows; NONE, or OVER where there is no room
     int group;                   // a sequence's record of shared tokens, -1: none
     int few, tiles;              // of few rows; tiles of keys
+    int few_end, many_end;       // the units of few and of many rows up to this record's
+    int pad[2];
 };
 constexpr int NONE = -1, OVER = -2;
 
-// The plan in the workspace: a head, the ends of every record's units of few
-// and of many rows, the records.
+// The plan in the workspace: a head, the records.
 constexpr int HEAD = 16;
 struct Plan {
     int32_t* head;  // units of few rows, of many
-    int32_t* few_end;
-    int32_t* many_end;
     Work* work;
 };
-__host__ __device__ inline int round16(int x) { return (x + 15) & ~15; }
 __device__ __forceinline__ Plan plan_of(const SharedParams& p) {
-    const int V = round16(p.NG + p.N);
-    return {p.plan, p.plan + HEAD, p.plan + HEAD + V, reinterpret_cast<Work*>(p.plan + HEAD + 2 * V)};
+    return {p.plan, reinterpret_cast<Work*>(p.plan + HEAD)};
 }
 int64_t plan_bytes(const SharedParams& p) {
-    const int64_t V = round16(p.NG + p.N);
-    return (HEAD + 2 * V + V * (int64_t)(sizeof(Work) / 4)) * 4;
+    return HEAD * 4 + ((int64_t)p.NG + p.N) * (int64_t)sizeof(Work);
 }
 
 // Rows of a tile of partial results: a multiple of 4.
@@ -93,7 +89,10 @@ __device__ __forceinline__ Three scan(Three x, uint32_t (&lds)[3][16], Three& al
 }
 
 // Of sequences that share, those with few rows and up to this many tiles of keys
-// of their own have them worked on in the join.
+// of their own have them worked on in the join: not in parts that would only
+// begin when those of the prefixes are over (64 sequences with 10 to 500 tokens of
+// their own behind 16000: 47 us, with up to 8 or 12 tiles 51, with 4 54; drafts
+// with up to 700 tokens 36.9, 36.0 and 35.2).
 constexpr int IN_JOIN = 16;
 // Rounds of parts of many rows at most, on 256 CUs each.
 constexpr int ROUNDS = 3;
@@ -202,11 +201,11 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
     uint32_t share = 0;
     float best = 3.4e38f;
     for (int r = 1; r <= rounds && all.c < LIMIT; ++r) {
-        const uint32_t k = all.b > 0 ? (uint32_t)(r * Shape<MANY>::SLOTS) / all.b : 0;
+        const uint32_t most = r * Shape<MANY>::SLOTS, k = all.b > 0 ? most / all.b : 0;
         const float cost = k > 0 ? r * ((float)all.c / (float)(all.b * k) + 4.f) : best;
         if (cost < best) {
             best = cost;
-            share = r * Shape<MANY>::SLOTS;
+            share = most;
         }
     }
     // A record's parts; units of few and of many rows, and the room of its results.
@@ -244,8 +243,8 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
         }
         if (x.c > 0) w.place = upto.c < LIMIT && at.c + x.c <= (uint32_t)room ? (int)at.c : OVER;
         at = {at.a + x.a, at.b + x.b, min(at.c + x.c, LIMIT)};
-        plan.few_end[v] = at.a;
-        plan.many_end[v] = at.b;
+        w.few_end = at.a;
+        w.many_end = at.b;
         plan.work[v] = w;
     }
     if (tid == THREADS - 1) {
@@ -439,26 +438,35 @@ __device__ __forceinline__ void split_rows(const SharedParams& p, const Unit& u,
 
 // ---- parts ----
 
-// Unit x of kind KIND; false where its results have no room.
+// Unit x of kind KIND; false where its results have no room.  Every lane has a
+// record: no load waits for another (but for every 64 records more).
 template <int KIND, int D>
 __device__ __forceinline__ bool unit_of(const SharedParams& p, const Plan& plan, int x, int lane, Unit& u) {
     constexpr int TK = Shape<KIND>::TK, MT = rows_of<KIND>();
-    const int32_t* ends = KIND == FEW ? plan.few_end : plan.many_end;
     const int V = p.NG + p.N;
-    int v = 0, before = 0;
+    Work w = {};
+    int before = 0;
     for (int v0 = 0; v0 < V; v0 += 64) {
-        const int end = v0 + lane < V ? ends[v0 + lane] : 0x7fffffff;
+        const Work mine = plan.work[min(v0 + lane, V - 1)];
+        const int end = KIND == FEW ? mine.few_end : mine.many_end;
         const uint64_t past = __ballot(end > x);
         if (past) {
             const int at = __builtin_ctzll(past);
-            v = v0 + at;
             if (at > 0) before = __builtin_amdgcn_readlane(end, at - 1);
+            auto take = [&](int y) { return __builtin_amdgcn_readlane(y, at); };
+            w.first = take(mine.first);
+            w.count = take(mine.count);
+            w.len = take(mine.len);
+            w.pos = take(mine.pos);
+            w.from = take(mine.from);
+            w.row = take(mine.row);
+            w.parts = take(mine.parts);
+            w.mt = take(mine.mt);
+            w.place = take(mine.place);
             break;
         }
         before = __builtin_amdgcn_readlane(end, 63);
     }
-    v = __builtin_amdgcn_readfirstlane(v);
-    const Work w = load_work(plan, v);
     if (w.place == OVER || w.count == 0) return false;
     x -= before;
     // heads innermost, as the XCDs go round; row tiles that see the most keys first
@@ -541,9 +549,9 @@ __device__ __forceinline__ void add_parts(Sums& s, const Parts& x, int piece, in
 }
 
 // Joins the parts of (sequence n, kv head h): those of its group's shared tokens
-// and its own, or its own keys worked on here where they are few (work-group 0 of
-// `groups`).  Four elements of a row a thread; where rows are few, several
-// threads' parts in turn.
+// and its own, or its own keys worked on here where they are few (by each of its
+// `groups` work-groups, which divide the joining).  Four elements of a row a
+// thread; where rows are few, several threads' parts in turn.
 template <class E, int D>
 __global__ __launch_bounds__(256, 2) void paged_shared_join_kernel(SharedParams p, int groups) {
     constexpr int WAVES = Shape<FEW>::WAVES;
@@ -555,7 +563,8 @@ __global__ __launch_bounds__(256, 2) void paged_shared_join_kernel(SharedParams 
     const int id = blockIdx.x / groups, n = id / p.HKV, h = id - n * p.HKV;
     const Work w = load_work(plan, p.NG + n);
     const bool here = w.parts == 0;
-    if (w.count == 0 || (here ? (int)blockIdx.x % groups > 0 : w.place < 0)) return;
+    const int rows = w.count * p.G, items = rows * (D / 4), group0 = blockIdx.x % groups;
+    if (w.count == 0 || group0 * 64 >= items || (!here && w.place < 0)) return;
     Work g = {};
     if (w.group >= 0) g = load_work(plan, w.group);
     if (g.place == OVER) return;
@@ -572,13 +581,10 @@ __global__ __launch_bounds__(256, 2) void paged_shared_join_kernel(SharedParams 
         u.end = (w.len + Shape<FEW>::TK - 1) / Shape<FEW>::TK;
         few_sums<E, D, WAVES>(p, u, tiles, joint);
     }
-    const int rows = w.count * p.G, items = rows * (D / 4);
-    // threads an item, at most 4, that divide the work-group
-    const int shift = items > 128 ? 0 : (items > 64 ? 1 : 2), per = 256 >> shift;
+    // threads an item: 1, 2 or 4
+    const int shift = items > 128 * groups ? 0 : (items > 64 * groups ? 1 : 2), per = 256 >> shift;
     const int slice = threadIdx.x / per, item = threadIdx.x % per;
-    // (work-group 0 has all of its own)
-    const int group0 = here ? 0 : blockIdx.x % groups, by = here ? 1 : groups;
-    for (int group = group0; group * per < items; group += by) {
+    for (int group = group0; group * per < items; group += groups) {
         const int e = group * per + item, r = e / (D / 4), piece = e % (D / 4);
         const bool live = r < rows;
         Sums s = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
@@ -620,10 +626,21 @@ constexpr int WHOLE = Shape<MANY>::MT;
 
 // Whether sequences are worked on together at all: not where each fills row
 // tiles by itself, nor where there are more than a plan has room for.
-bool together(const SharedParams& p) {
-    return p.N >= 2 && p.N <= MOST && p.NG <= MOST && (p.cu_seqlens || (int64_t)p.T * p.G < WHOLE);
-}
+//
+// Nor where the table is so small that reading the shared keys again for each
+// sequence costs less than the plan and the longer join, 15 us for 9: by the bytes
+// that its rows hold, whose second reading is from the caches. Decode of 8
+// sequences, 32 / 8 heads: 67 MB 15.3 us one by one and 17.9 so, 131 MB 21.3 and
+// 19.4; 2 sequences: 66 MB 18.9 and 22.1, 131 MB 29.0 and 26.5.  Drafts of 5, 24 /
+// 4 heads of 64 (30 rows: their row tiles are full one by one too): 131 MB 24.4
+// and 27.8, 262 MB 35.9 and 33.5.
 int64_t tokens_of(const SharedParams& p) { return p.cu_seqlens ? p.T : (int64_t)p.N * p.T; }
+bool together(const SharedParams& p, int D) {
+    if (p.N < 2 || p.N > MOST || p.NG > MOST || (!p.cu_seqlens && (int64_t)p.T * p.G >= WHOLE)) return false;
+    const int64_t row = ((int64_t)p.M << p.page_shift) * p.HKV * D * 4;
+    const int64_t least = tokens_of(p) * p.G <= (int64_t)p.N * (ROWS / 2) ? 112 << 20 : 224 << 20;
+    return row >= least / p.N;
+}
 bool few_only(const SharedParams& p) { return tokens_of(p) * p.G <= ROWS; }
 
 // Row tiles of many rows at most.  Records of many rows have more than ROWS.
@@ -674,11 +691,14 @@ hipError_t launch_shared(SharedParams p, hipStream_t stream) {
     else paged_shared_kernel<E, D, MIXED><<<grid, 512, 0, stream>>>(p);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // work-groups a (sequence, head): one for every 256 fours of its rows, as many
-    // as there is some use for
+    // work-groups a (sequence, head): one for every 128 fours of its rows (with one
+    // for every 64, 8 sequences of 4 rows behind 2000 tokens took 18.2 us instead of
+    // 16.8: each works on the own keys), as many as run at once, of many rows
+    // (whose own keys are not worked on there) eight times as many
     const int64_t pairs = (int64_t)p.N * p.HKV;
     const int64_t rows = std::min((int64_t)p.T * p.G, p.cu_seqlens ? (int64_t)1 << 20 : (int64_t)WHOLE);
-    const int groups = (int)std::max((int64_t)1, std::min((rows * (D / 4) + 255) / 256, 4096 / pairs));
+    const int64_t most = rows > ROWS ? 8 * Shape<FEW>::SLOTS : Shape<FEW>::SLOTS;
+    const int groups = (int)std::max((int64_t)1, std::min((rows * (D / 4) + 127) / 128, most / pairs));
     paged_shared_join_kernel<E, D><<<dim3((unsigned)(pairs * groups)), 256, 0, stream>>>(p, groups);
     return hipGetLastError();
 }
@@ -686,12 +706,12 @@ hipError_t launch_shared(SharedParams p, hipStream_t stream) {
 }  // namespace
 
 size_t paged_attn_workspace(const SharedParams& p, int D) {
-    if (!together(p)) return paged_attn_workspace(static_cast<const PagedParams&>(p), D);
+    if (!together(p, D)) return paged_attn_workspace(static_cast<const PagedParams&>(p), D);
     return (size_t)(4 * (D + 2) * room_of(p) * 4 + plan_bytes(p));
 }
 
 hipError_t launch_paged_attn(const SharedParams& p, int D, hipStream_t stream) {
-    if (!together(p)) return launch_paged_attn(static_cast<const PagedParams&>(p), D, stream);
+    if (!together(p, D)) return launch_paged_attn(static_cast<const PagedParams&>(p), D, stream);
     if (D == 128) return p.fp16 ? launch_shared<FP16, 128>(p, stream) : launch_shared<BF16, 128>(p, stream);
     return p.fp16 ? launch_shared<FP16, 64>(p, stream) : launch_shared<BF16, 64>(p, stream);
 }

@@ -94,16 +94,22 @@ def test_packed_arguments_are_the_struct():
 def test_workspace_sizes():
     f, plain = _hip.lib().kda_paged_attn_shared_workspace_bytes, _hip.lib().kda_paged_attn_workspace_bytes
     assert f(None) == 0
-    # one sequence, whole row tiles, more sequences than a plan holds: as without groups
-    for base in (dict(N=1), dict(T=128), dict(N=2049)):
+    # one sequence, whole row tiles, more sequences than a plan holds, rows of few keys
+    # (112 MB of keys and values together, 224 with more than 16 rows a sequence):
+    # as without groups
+    wide = dict(M=8000, table_stride=8000)
+    for base in (dict(N=1, **wide), dict(T=128, **wide), dict(N=2049, **wide), dict(), dict(M=3583, table_stride=3583),
+                 dict(T=16, M=6000, table_stride=6000)):
         a = shared(base)
         assert f(ctypes.byref(a)) == plain(ctypes.byref(a.paged)), base
-    assert f(ctypes.byref(shared(dict(N=2048)))) > 0 and f(ctypes.byref(shared(dict(T=127)))) > 0
+    for base in (dict(N=2048), dict(T=127, **wide), dict(M=3584, table_stride=3584), dict(T=16, **wide)):
+        a = shared(base)
+        assert f(ctypes.byref(a)) != plain(ctypes.byref(a.paged)), base
     # 8 sequences of a token, 8 / 2 heads: rows of both kinds (2 * 32 * 2, and 3 for each of 10 records and
-    # head), 1024 places of 32 rows, in rows of D + 2 floats; the plan of 16 records
+    # head), 1024 places of 32 rows, in rows of D + 2 floats; the plan of 10 records
     rows = 2 * 8 * 4 * 2 + 3 * 10 * 2 + 2 * 512 * 32
-    got = f(ctypes.byref(shared(dict(N=8, HQ=8, q_row=1024, q_token=1024))))
-    assert got == (rows + 3) // 4 * 4 * 130 * 4 + (16 + 2 * 16 + 16 * 12) * 4
+    got = f(ctypes.byref(shared(dict(N=8, HQ=8, q_row=1024, q_token=1024, **wide))))
+    assert got == (rows + 3) // 4 * 4 * 130 * 4 + (16 + 10 * 16) * 4
 
 
 @fake_pointers

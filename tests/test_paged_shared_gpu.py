@@ -23,10 +23,12 @@ pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
 
 
-def make(groups, own, page, HKV, D, dtype, gen, layout="token", before=0, after=0, width=0):
+def make(groups, own, page, HKV, D, dtype, gen, layout="token", before=0, after=0, wide=True):
     """``groups``: (shared tokens, sequences) each; ``own(n)``: sequence n's
     tokens behind them; ``before`` and ``after``: rows of no group at the ends.
-    Table, lengths, caches and the groups' tensors, on the CPU."""
+    ``wide``: a table whose rows have room for 256 MB of keys and values (those of
+    less are worked on one by one).  Caches, table, lengths and the groups'
+    tensors, on the CPU."""
     lens, starts, shared, members = [], [before], [], []
     lens += [own(n) for n in range(before)]
     for tokens, count in groups:
@@ -35,7 +37,7 @@ def make(groups, own, page, HKV, D, dtype, gen, layout="token", before=0, after=
         starts.append(len(lens))
         shared.append(tokens)
     lens += [own(len(lens) + i) for i in range(after)]
-    table, P = tables(lens, page, gen, width)
+    table, P = tables(lens, page, gen, -(-(256 << 20) // (len(lens) * HKV * D * 4 * page)) if wide else 0)
     for (tokens, _), rows in zip(groups, members):
         for n in rows:
             table[n, :tokens // page] = table[rows[0], :tokens // page]
@@ -64,11 +66,11 @@ def compare(dev, q, kc, vc, table, lens, starts, shared, cu=None, want=None):
 
 
 def check(dev, groups, own=None, T=1, HQ=4, HKV=2, D=128, page=16, dtype=BF16, layout="token", new=None, before=0, after=0,
-          seed=0, width=0, cu_dtype=torch.int32):
+          seed=0, wide=True, cu_dtype=torch.int32):
     gen = torch.Generator().manual_seed(seed)
     new_of = (lambda n: T) if new is None else (lambda n: new[n])
     own = own or (lambda n: new_of(n) + (37 * n) % 61)
-    kc, vc, table, lens, starts, shared = make(groups, own, page, HKV, D, dtype, gen, layout, before, after, width)
+    kc, vc, table, lens, starts, shared = make(groups, own, page, HKV, D, dtype, gen, layout, before, after, wide)
     cu = None if new is None else torch.tensor([0] + new).cumsum(0).to(cu_dtype)
     q = torch.randn(*((len(lens), T) if new is None else (1, sum(new))), HQ, D, generator=gen).to(dtype)
     return compare(dev, q, kc, vc, table, lens, starts, shared, cu)
@@ -105,6 +107,11 @@ def test_new_tokens(T, gpu_device):
 def test_pages(page, layout, gpu_device):
     check(gpu_device, [(1500, 4), (1024, 3), (17, 2)], page=page, layout=layout)
     check(gpu_device, [(1500, 4), (1024, 3), (17, 2)], page=page, layout=layout, T=20)
+
+
+def test_narrow_tables(gpu_device):
+    for T in (1, 20):
+        check(gpu_device, [(300, 4), (90, 3)], T=T, wide=False, after=1)
 
 
 def test_several_groups_and_rows_of_none(gpu_device):
@@ -246,7 +253,8 @@ def test_answers_forked_from_a_prompt(gpu_device):
     N, page, P, HKV, G, D, L = 6, 16, 60, 2, 4, 64, 150
     pool = torch.randn(2, P, page, HKV, D, generator=gen).to(BF16).to(d)
     i32 = dict(dtype=torch.int32, device=d)
-    table, lens, refs = torch.full((N, 20), -1, **i32), torch.zeros(N, **i32), torch.zeros(P, **i32)
+    # (a wide table: the shared keys are worked on together)
+    table, lens, refs = torch.full((N, 6000), -1, **i32), torch.zeros(N, **i32), torch.zeros(P, **i32)
     assert bool(paged_reserve(table, lens, refs, torch.tensor([L] + [0] * 5, **i32), page)[0])
     rows = torch.arange(1, N, **i32)
     assert bool(paged_fork(pool, table, lens, refs, torch.zeros_like(rows), rows).all())
