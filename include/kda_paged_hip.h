@@ -114,9 +114,9 @@ int kda_paged_attn_sinks_hip(const KdaPagedSinksArgs* args, void* stream);
  * in their first shared_lens[g] tokens, in the same pages (as kda_pages_fork_hip
  * leaves them) or in copies; one row's are read.  Which one, and how sums are
  * rounded, depends on the groups, nothing else does.  A sequence whose new tokens
- * do not all come behind the shared ones (an ended one's) takes part by itself,
- * and so do rows of no group, and all rows of a group one of whose sequences has
- * new tokens for a row tile of its own (T_n * HQ / HKV at least 256). */
+ * do not all come behind the shared ones (an ended one's) is worked on by itself,
+ * and so are rows of no group, and sequences whose new tokens fill a row tile
+ * (T_n * HQ / HKV at least 128), which have nothing to gain. */
 typedef struct KdaPagedSharedArgs {
     KdaPagedArgs paged;
     const int32_t* cu_groups;   /* [num_groups + 1], from 0 to N, non-decreasing */

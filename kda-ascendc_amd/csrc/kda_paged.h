@@ -140,6 +140,8 @@ struct SharedParams : PagedParams {
     const int32_t* cu_groups;
     const int32_t* shared_lens;
     int32_t* plan;
+    int32_t* map;  // the tokens that share
+    int map_size;
 };
 
 // The append with the position rotation (kda_paged_hip.h).

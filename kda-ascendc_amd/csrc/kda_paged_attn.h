@@ -272,10 +272,12 @@ struct Unit {
     int n, h, m, lo, hi, begin, end, slot;
     NewTokens s;
     int split, gap;
-    // With groups: n is a row of the table, s.first a token of all, and the
-    // partial results are those of `rows` rows, from float `place` on (none: -1).
+    // With groups: n is a row of the table, s.first a token of all (mapped: of
+    // those that share), and the partial results are those of `rows` rows, from
+    // float `place` on (none: -1).
     int rows;
     int64_t place;
+    bool mapped;
 };
 
 // The keys that rows [m * MT, m * MT + MT) of a sequence see, and their tiles.
@@ -550,8 +552,10 @@ __device__ __forceinline__ int64_t out_row(const P& p, const Unit& u, const Row&
 template <int D, class P>
 __device__ __forceinline__ void load_q(const P& p, const Unit& u, const Row& x, int half, u32x4 (&q)[D / 16]) {
     const uint16_t* at;
-    if (SHARED<P> && !p.cu_seqlens) {
-        const int t = u.s.first + x.tok, n = t / p.T;
+    if constexpr (SHARED<P>) {
+        int t = u.s.first + x.tok, n = 0;
+        if (u.mapped) t = p.map[min(t, p.map_size - 1)];
+        if (!p.cu_seqlens) n = t / p.T;
         at = p.q + n * p.q_row + (t - n * p.T) * p.q_token + x.head * p.q_head;
     } else {
         at = p.q + (p.cu_seqlens ? u.s.first * p.q_token : u.n * p.q_row) + x.tok * p.q_token + x.head * p.q_head;

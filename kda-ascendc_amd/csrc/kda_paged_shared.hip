@@ -36,18 +36,20 @@ constexpr int MOST = 2048;
 // those of a sequence over its own.  Records of all groups, then of all
 // sequences.
 struct alignas(16) Work {
-    int first, count, len, pos;  // as NewTokens, `first` a token of all
+    int first, count, len, pos;  // as NewTokens, `first` a token of all, or a group's of those that share
     int from, row;               // the first key, a row of the table
     int parts, mt;               // parts of a row tile's keys; row tiles
     int place;                   // of the partial results, in 4 rows; NONE, or OVER where there is no room
     int group;                   // a sequence's record of shared tokens, -1: none
     int few, tiles;              // of few rows; tiles of keys
     int few_end, many_end;       // the units of few and of many rows up to this record's
-    int pad[2];
+    int sharer;                  // the first of its tokens among those that share
+    int pad;
 };
 constexpr int NONE = -1, OVER = -2;
 
-// The plan in the workspace: a head, the records.
+// The plan in the workspace: a head, the records, and the tokens that share (of
+// each group one after the other: sequences that do not are left out).
 constexpr int HEAD = 16;
 struct Plan {
     int32_t* head;  // units of few rows, of many
@@ -56,37 +58,48 @@ struct Plan {
 __device__ __forceinline__ Plan plan_of(const SharedParams& p) {
     return {p.plan, reinterpret_cast<Work*>(p.plan + HEAD)};
 }
+int64_t tokens_of(const SharedParams& p) { return p.cu_seqlens ? p.T : (int64_t)p.N * p.T; }
+// Tokens that share at most: of each sequence fewer than fill a row tile.
+int64_t sharing_tokens(const SharedParams& p) { return std::min(tokens_of(p), (int64_t)p.N * (MT / p.G + 1)); }
 int64_t plan_bytes(const SharedParams& p) {
-    return HEAD * 4 + ((int64_t)p.NG + p.N) * (int64_t)sizeof(Work);
+    return HEAD * 4 + ((int64_t)p.NG + p.N) * (int64_t)sizeof(Work) + 4 * sharing_tokens(p);
 }
 
 // Rows of a tile of partial results: a multiple of 4.
 __host__ __device__ inline int padded(int rows) { return (rows + 3) & ~3; }
 
-// Three numbers, and their sums up to a thread (its own included) and over all
-// of the work-group's; c and its sums no more than LIMIT.
-struct Three {
-    uint32_t a, b, c;
+// Numbers of a thread, and their sums up to it (its own included) and over all of
+// the work-group's; the last and its sums no more than LIMIT.
+template <int K>
+struct Numbers {
+    uint32_t x[K] = {};
 };
 constexpr uint32_t LIMIT = 0x7fffffff;
-template <int THREADS>
-__device__ __forceinline__ Three scan(Three x, uint32_t (&lds)[3][16], Three& all) {
+template <int THREADS, int K>
+__device__ __forceinline__ Numbers<K> scan(const Numbers<K>& x, uint32_t (&lds)[K][16], Numbers<K>& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    Three s = {wave_prefix(x.a), wave_prefix(x.b), wave_prefix(x.c, LIMIT)};
-    if (lane == 63) {
-        lds[0][wave] = s.a;
-        lds[1][wave] = s.b;
-        lds[2][wave] = s.c;
+    Numbers<K> s;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        s.x[k] = k < K - 1 ? wave_prefix(x.x[k]) : wave_prefix(x.x[k], LIMIT);
+        if (lane == 63) lds[k][wave] = s.x[k];
     }
     __syncthreads();
-    all = {0, 0, 0};
+    all = {};
 #pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) {
-        if (w == wave) s = {s.a + all.a, s.b + all.b, min(s.c + all.c, LIMIT)};
-        all = {all.a + lds[0][w], all.b + lds[1][w], min(all.c + lds[2][w], LIMIT)};
-    }
+    for (int w = 0; w < THREADS / 64; ++w)
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (w == wave) s.x[k] += all.x[k];
+            all.x[k] += lds[k][w];
+            if (k == K - 1) {
+                s.x[k] = min(s.x[k], LIMIT);
+                all.x[k] = min(all.x[k], LIMIT);
+            }
+        }
     return s;
 }
+__device__ __forceinline__ uint32_t limited(int64_t x) { return (uint32_t)min(x, (int64_t)LIMIT); }
 
 // Of sequences that share, those with few rows and up to this many tiles of keys
 // of their own have them worked on in the join: not in parts that would only
@@ -102,9 +115,10 @@ constexpr int ROUNDS = 3;
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams p, int waves, int rounds, int room) {
     constexpr bool ONE = THREADS < 1024;  // a record a thread
-    __shared__ int cu[MOST + 1], least[MOST], sharing[MOST], shared_of[MOST];
-    __shared__ uint32_t lds[2][3][16];
-    constexpr int BIG = 1 << 20;
+    // (of the groups: their sequences' offsets, the first that shares, how many do,
+    // with how many tokens; the shared ones.  Sharing tokens before each sequence.)
+    __shared__ int cu[MOST + 1], least[MOST], sharing[MOST], tokens_of[MOST], shared_of[MOST], before[MOST + 1];
+    __shared__ uint32_t lds5[5][16], lds3[3][16];
     const int tid = threadIdx.x, V = p.NG + p.N;
     const int each = ONE ? 1 : (V + THREADS - 1) / THREADS, v0 = tid * each, v1 = min(V, v0 + each);
     const int64_t most = (int64_t)p.M << p.page_shift;
@@ -114,40 +128,38 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
             const int len = p.shared_lens[g];
             shared_of[g] = len < 0 ? 0 : ((int64_t)len > most ? (int)most : len);
             least[g] = p.N;
-            sharing[g] = 0;
+            sharing[g] = tokens_of[g] = 0;
         }
     }
     NewTokens mine = {};  // (a record a thread: its sequence's)
     if (ONE && v0 >= p.NG && v0 < V) mine = new_tokens(p, v0 - p.NG);
     auto tokens = [&](int v) { return ONE ? mine : new_tokens(p, v - p.NG); };
     __syncthreads();
-    // The group of sequence n, -1 for none.
-    auto group_of = [&](int n) {
+    // The group that sequence n shares with, -1 for none: if its new tokens all come
+    // behind the group's shared ones, and do not fill a row tile by themselves (which
+    // then has nothing to gain).
+    auto group_of = [&](int n, const NewTokens& s) {
         int lo = 0, hi = p.NG - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
             if (cu[mid] <= n) lo = mid;
             else hi = mid - 1;
         }
-        return cu[lo] <= n && n < cu[lo + 1] ? lo : -1;
+        const bool in = cu[lo] <= n && n < cu[lo + 1] && shared_of[lo] > 0 && s.pos >= shared_of[lo];
+        return in && s.count > 0 && (int64_t)s.count * p.G < MT ? lo : -1;
     };
-    // A sequence shares if its new tokens all come behind the group's shared ones.
-    auto shares = [&](const NewTokens& s, int g) { return g >= 0 && s.count > 0 && shared_of[g] > 0 && s.pos >= shared_of[g]; };
     for (int v = max(v0, p.NG); v < v1; ++v) {
         const NewTokens s = tokens(v);
-        const int g = group_of(v - p.NG);
-        if (shares(s, g)) {
-            atomicMin(&least[g], v - p.NG);
-            atomicAdd(&sharing[g], 1);
-        }
-        // (a sequence that fills a row tile by itself: nothing to gain for it)
-        if (g >= 0 && (int64_t)s.count * p.G >= MT) atomicOr(&sharing[g], BIG);
+        const int g = group_of(v - p.NG, s);
+        if (g < 0) continue;
+        atomicMin(&least[g], v - p.NG);
+        atomicAdd(&sharing[g], 1);
+        atomicAdd(&tokens_of[g], s.count);
     }
     __syncthreads();
-    auto active = [&](int g) { return sharing[g] >= 2 && sharing[g] < BIG; };
 
     const Plan plan = plan_of(p);
-    // Record v, but for its parts and their place.
+    // Record v, but for its parts, their place and where its group's rows begin.
     auto record = [&](int v) {
         Work w = {};
         w.group = NONE;
@@ -160,15 +172,13 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
             w.len = s.len;
             w.pos = s.pos;
             w.row = n;
-            const int g = group_of(n);
-            if (shares(s, g) && active(g)) {
+            const int g = group_of(n, s);
+            if (g >= 0 && sharing[g] >= 2) {
                 w.group = g;
                 w.from = shared_of[g];
             }
-        } else if (active(v)) {
-            const int n0 = cu[v], n1 = max(n0, cu[v + 1]);
-            w.first = p.cu_seqlens ? paged_cu(p, n0) : n0 * p.T;
-            w.count = max(0, (p.cu_seqlens ? paged_cu(p, n1) : n1 * p.T) - w.first);
+        } else if (sharing[v] >= 2) {
+            w.count = tokens_of[v];
             w.len = w.pos = shared_of[v];
             w.row = least[v];
         }
@@ -182,27 +192,37 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
     // Whether the join works on a record's keys.
     auto in_join = [&](const Work& w) { return w.few && w.group >= 0 && w.tiles <= IN_JOIN; };
     Work w;
-    Three x = {0, 0, 0}, all;
+    // tiles and records of few rows, tokens that share, row tiles and tiles of many
+    Numbers<5> x, all;
     for (int v = v0; v < v1; ++v) {
         w = record(v);
+        if (w.group >= 0) x.x[2] += w.count;
         if (w.count > 0 && !in_join(w)) {
-            if (w.few) x.a += w.tiles * p.HKV;
-            else x = {x.a, x.b + w.mt * p.HKV, (uint32_t)min((int64_t)x.c + (int64_t)w.mt * p.HKV * w.tiles, (int64_t)LIMIT)};
+            if (w.few) {
+                x.x[0] += w.tiles * p.HKV;
+                x.x[1] += p.HKV;
+            } else {
+                x.x[3] += w.mt * p.HKV;
+                x.x[4] = limited(x.x[4] + (int64_t)w.mt * p.HKV * w.tiles);
+            }
         }
         if (!ONE) plan.work[v] = w;
     }
-    scan<THREADS>(x, lds[0], all);
+    const Numbers<5> upto5 = scan<THREADS>(x, lds5, all);
     // Few rows: parts of `size` tiles, at most as many of them as run at once.
-    const uint32_t slots = few_slots(waves), size = max((uint32_t)waves, (all.a + slots - 1) / slots);
-    // Many rows: with all.b row tiles of all.c tiles of keys together, `share` parts
-    // of equal size if they can be had, in 1 to 3 rounds: the fewest tiles one after
-    // the other, 4 more a round for its beginning and end.  (Of LIMIT tiles, which
-    // are hours of work, none is cut.)
+    const uint32_t slots = few_slots(waves), size = max((uint32_t)waves, (all.x[0] + slots - 1) / slots);
+    // Many rows: with `units` row tiles of `tiles` tiles of keys together, `share`
+    // parts of equal size if they can be had, in 1 to 3 rounds: the fewest tiles one
+    // after the other, 7 more a round for its beginning and end (a tile of 128 rows
+    // takes 1 us).  A few parts of few rows run in the first round too.  (Of LIMIT
+    // tiles, which are hours of work, none is cut.)
+    const uint32_t units = all.x[3], tiles = all.x[4], beside = all.x[0] / size + all.x[1];
     uint32_t share = 0;
     float best = 3.4e38f;
-    for (int r = 1; r <= rounds && all.c < LIMIT; ++r) {
-        const uint32_t most = r * Shape<MANY>::SLOTS, k = all.b > 0 ? most / all.b : 0;
-        const float cost = k > 0 ? r * ((float)all.c / (float)(all.b * k) + 4.f) : best;
+    for (int r = 1; r <= rounds && tiles < LIMIT; ++r) {
+        const uint32_t most = r * Shape<MANY>::SLOTS - (beside <= Shape<MANY>::SLOTS / 4 ? beside : 0);
+        const uint32_t k = units > 0 ? most / units : 0;
+        const float cost = k > 0 ? r * ((float)tiles / (float)(units * k) + 7.f) : best;
         if (cost < best) {
             best = cost;
             share = most;
@@ -210,46 +230,63 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
     }
     // A record's parts; units of few and of many rows, and the room of its results.
     auto needs = [&](Work& w, int v) {
-        Three x = {0, 0, 0};
+        Numbers<3> x;
         if (w.count == 0 || in_join(w)) return x;
         if (w.few) {
             w.parts = (int)((w.tiles + size - 1) / size);
-            x.a = w.parts * p.HKV;
+            x.x[0] = w.parts * p.HKV;
         } else {
             w.parts = 1;
             if (share > 0) {
                 // (exact: the quotient of 32 bits by 32 is no nearer to a whole number than 2^-32)
-                const uint32_t parts = (uint32_t)((double)w.tiles * (double)share / (double)all.c);
+                const uint32_t parts = (uint32_t)((double)w.tiles * (double)share / (double)tiles);
                 w.parts = (int)max(1u, min((uint32_t)w.tiles / Shape<MANY>::LEAST, parts));
             }
-            x.b = w.mt * w.parts * p.HKV;
+            x.x[1] = w.mt * w.parts * p.HKV;
         }
-        if (w.parts > 1 || v < p.NG || w.group >= 0)
-            x.c = (uint32_t)min((int64_t)(padded(w.count * p.G) / 4) * w.parts * p.HKV, (int64_t)LIMIT);
+        if (w.parts > 1 || v < p.NG || w.group >= 0) x.x[2] = limited((int64_t)(padded(w.count * p.G) / 4) * w.parts * p.HKV);
         return x;
     };
-    Three mine3 = {0, 0, 0};
+    Numbers<3> mine3, x3, all3;
+    int sharers = upto5.x[2] - x.x[2];
     for (int v = v0; v < v1; ++v) {
         if (!ONE) w = plan.work[v];
-        x = needs(w, v);
-        mine3 = {mine3.a + x.a, mine3.b + x.b, min(mine3.c + x.c, LIMIT)};
+        x3 = needs(w, v);
+        mine3.x[0] += x3.x[0];
+        mine3.x[1] += x3.x[1];
+        mine3.x[2] = limited((int64_t)mine3.x[2] + x3.x[2]);
+        if (v >= p.NG) {
+            before[v - p.NG] = sharers;
+            if (w.group >= 0) sharers += w.count;
+        }
     }
-    const Three upto = scan<THREADS>(mine3, lds[1], all);
-    Three at = {upto.a - mine3.a, upto.b - mine3.b, upto.c - mine3.c};  // (room is below LIMIT)
+    if (tid == 0) before[p.N] = all.x[2];
+    const Numbers<3> upto = scan<THREADS>(mine3, lds3, all3);  // (which waits for all of `before`)
+    Numbers<3> at;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) at.x[k] = upto.x[k] - mine3.x[k];
     for (int v = v0; v < v1; ++v) {
         if (!ONE) {
             w = plan.work[v];
-            x = needs(w, v);
+            x3 = needs(w, v);
         }
-        if (x.c > 0) w.place = upto.c < LIMIT && at.c + x.c <= (uint32_t)room ? (int)at.c : OVER;
-        at = {at.a + x.a, at.b + x.b, min(at.c + x.c, LIMIT)};
-        w.few_end = at.a;
-        w.many_end = at.b;
+        if (x3.x[2] > 0) w.place = upto.x[2] < LIMIT && at.x[2] + x3.x[2] <= (uint32_t)room ? (int)at.x[2] : OVER;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) at.x[k] += x3.x[k];
+        w.few_end = at.x[0];
+        w.many_end = at.x[1];
+        if (v < p.NG) {
+            w.first = w.sharer = before[cu[v]];
+        } else {
+            w.sharer = before[v - p.NG];
+            if (w.group >= 0)
+                for (int i = 0; i < w.count && w.sharer + i < p.map_size; ++i) p.map[w.sharer + i] = w.first + i;
+        }
         plan.work[v] = w;
     }
     if (tid == THREADS - 1) {
-        plan.head[0] = all.a;
-        plan.head[1] = all.b;
+        plan.head[0] = all3.x[0];
+        plan.head[1] = all3.x[1];
     }
 }
 
@@ -282,6 +319,7 @@ __device__ __forceinline__ Work load_work(const Plan& plan, int v) {
     w.place = at[8];
     w.group = at[9];
     w.few = at[10];
+    w.sharer = at[14];
     return w;
 }
 
@@ -463,6 +501,7 @@ __device__ __forceinline__ bool unit_of(const SharedParams& p, const Plan& plan,
             w.parts = take(mine.parts);
             w.mt = take(mine.mt);
             w.place = take(mine.place);
+            u.mapped = v0 + at < p.NG;
             break;
         }
         before = __builtin_amdgcn_readlane(end, 63);
@@ -575,6 +614,7 @@ __global__ __launch_bounds__(256, 2) void paged_shared_join_kernel(SharedParams 
         u.h = h;
         u.m = 0;
         u.s = NewTokens{w.first, w.count, w.len, w.pos};
+        u.mapped = false;
         u.lo = w.from;
         u.hi = w.len;
         u.begin = w.from / Shape<FEW>::TK;
@@ -590,7 +630,7 @@ __global__ __launch_bounds__(256, 2) void paged_shared_join_kernel(SharedParams 
         Sums s = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
         if (live) {
             if (here && slice == 0) s = few_sum<D, WAVES>(tiles, joint, r, piece);
-            const int rg = (w.first - g.first) * p.G + r;  // its place in the group's rows
+            const int rg = (w.sharer - g.sharer) * p.G + r;  // its place in the group's rows
             if (w.group >= 0 && rg >= 0 && rg < g.count * p.G) add_parts(s, parts_of<D>(p, g, h, rg), piece, D, slice, 1 << shift);
             if (!here) add_parts(s, parts_of<D>(p, w, h, r), piece, D, slice, 1 << shift);
         }
@@ -634,7 +674,6 @@ constexpr int WHOLE = Shape<MANY>::MT;
 // 19.4; 2 sequences: 66 MB 18.9 and 22.1, 131 MB 29.0 and 26.5.  Drafts of 5, 24 /
 // 4 heads of 64 (30 rows: their row tiles are full one by one too): 131 MB 24.4
 // and 27.8, 262 MB 35.9 and 33.5.
-int64_t tokens_of(const SharedParams& p) { return p.cu_seqlens ? p.T : (int64_t)p.N * p.T; }
 bool together(const SharedParams& p, int D) {
     if (p.N < 2 || p.N > MOST || p.NG > MOST || (!p.cu_seqlens && (int64_t)p.T * p.G >= WHOLE)) return false;
     const int64_t row = ((int64_t)p.M << p.page_shift) * p.HKV * D * 4;
@@ -662,8 +701,7 @@ int rounds_of(const SharedParams& p) {
 // together (a group's and the sequences', each filled up to 4), and the parts
 // that keys are cut into.
 int64_t room_of(const SharedParams& p) {
-    const int64_t sharing = std::min(tokens_of(p), (int64_t)p.N * (MT / p.G + 1));
-    const int64_t rows = (2 * sharing * p.G + 3 * (int64_t)(p.N + p.NG)) * p.HKV;
+    const int64_t rows = (2 * sharing_tokens(p) * p.G + 3 * (int64_t)(p.N + p.NG)) * p.HKV;
     const int64_t few = 2 * (int64_t)few_slots(Shape<FEW>::WAVES) * ROWS;
     const int64_t many = (int64_t)rounds_of(p) * Shape<MANY>::SLOTS * MT;
     return (rows + few + many + 3) / 4;
@@ -679,6 +717,8 @@ int64_t units_of(const SharedParams& p, int waves) {
 template <class E, int D>
 hipError_t launch_shared(SharedParams p, hipStream_t stream) {
     p.plan = reinterpret_cast<int32_t*>(p.ws + 4 * (D + 2) * room_of(p));
+    p.map_size = (int)sharing_tokens(p);
+    p.map = p.plan + HEAD + ((int64_t)p.NG + p.N) * (int64_t)(sizeof(Work) / 4);
     const int V = p.NG + p.N, room = (int)std::min(room_of(p), (int64_t)LIMIT - 1);
     const bool only = few_only(p);
     const int waves = Shape<FEW>::WAVES * (only ? 1 : 2);

@@ -315,10 +315,11 @@ def paged_attention_shared(
 
     Same result as :func:`paged_attention`'s but for the order of fp32 sums.  A
     sequence whose new tokens do not all come behind the shared ones (a freed
-    row) is worked on by itself, and so are rows of no group.  Sequences with new
-    tokens for a whole row tile of their own (256 rows, T * HQ / HKV) gain
-    nothing: one in a group, and the whole group is worked on one by one; give
-    it a group of its own.
+    row) is worked on by itself, and so are rows of no group and sequences whose
+    new tokens fill a row tile (T * HQ / HKV at least 128), which have nothing to
+    gain.  Where the table has room for few keys only (112 MB of keys and values
+    in all rows together; 224 MB with more than 16 rows, T * HQ / HKV, a sequence
+    on average) all are worked on one by one, which is faster then.
     """
     device = k_cache.device
     for name, t in (("cu_groups", cu_groups), ("shared_lens", shared_lens)):

@@ -106,10 +106,10 @@ def test_workspace_sizes():
         a = shared(base)
         assert f(ctypes.byref(a)) != plain(ctypes.byref(a.paged)), base
     # 8 sequences of a token, 8 / 2 heads: rows of both kinds (2 * 32 * 2, and 3 for each of 10 records and
-    # head), 1024 places of 32 rows, in rows of D + 2 floats; the plan of 10 records
+    # head), 1024 places of 32 rows, in rows of D + 2 floats; the plan of 10 records and 8 tokens
     rows = 2 * 8 * 4 * 2 + 3 * 10 * 2 + 2 * 512 * 32
     got = f(ctypes.byref(shared(dict(N=8, HQ=8, q_row=1024, q_token=1024, **wide))))
-    assert got == (rows + 3) // 4 * 4 * 130 * 4 + (16 + 10 * 16) * 4
+    assert got == (rows + 3) // 4 * 4 * 130 * 4 + (16 + 10 * 16 + 8) * 4
 
 
 @fake_pointers
