@@ -456,7 +456,6 @@ def paged_append_rotary(
     Queries of tokens that the append leaves out are turned all the same;
     packed tokens of no sequence (behind the last offset) are not written.
     """
-    shape = q.shape
     f = _plain_rotary(q, k, v, k_cache, v_cache, page_table, seq_lens, inv_freq, cu_seqlens)
     if f is None:
         f = _checked_rotary(q, k, v, k_cache, v_cache, page_table, seq_lens, inv_freq, cu_seqlens)
@@ -464,22 +463,25 @@ def paged_append_rotary(
     if out is None:
         _require_gpu(q)
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        token = f[2] * f[4]
+        to = (f[1] * token, token, f[4])
     else:
-        _check_new("out", out, shape[2], k_cache, page_table, cu_seqlens)
-        if out.shape != shape:
-            raise ValueError(f"out.shape {tuple(out.shape)} must match q {tuple(shape)}")
+        _check_new("out", out, q.shape[2], k_cache, page_table, cu_seqlens)
+        if out.shape != q.shape:
+            raise ValueError(f"out.shape {tuple(out.shape)} must match q {tuple(q.shape)}")
         _check_written("out", out)
         _forward_only("paged_append_rotary", out)
         if (out.data_ptr() != q.data_ptr() or out.stride() != q.stride()) and out.untyped_storage().data_ptr() in {
                 t.untyped_storage().data_ptr() for t in (q, k, v, k_cache, v_cache)}:
             raise ValueError("out must be q itself or of other storage than the inputs")
         _require_gpu(q)
+        to = _strides(out)
     (N, T, HQ, HKV, D, dt, P, size, M, cu_dtype, cu, table, table_stride, lens, kp, vp, s0, s1, s2, t0, t1, t2, u0, u1,
      u2, w0, w1, w2, x0, x1, x2) = f
     _launch("kda_paged_append_rotary_hip", _hip.PAGED_ROTARY_PACK.pack(
         _hip.PAGED_ABI_VERSION, N, T, HQ, HKV, D, dt, P, size, M, 0, 0, 1.0, cu_dtype, cu, table, table_stride, lens,
         kp, vp, s0, s1, s2, t0, t1, t2, q.data_ptr(), u0, u1, u2, 0, 0, k.data_ptr(), v.data_ptr(), w0, w1, w2, x0, x1, x2,
-        0, 0, inv_freq.data_ptr(), 2 * inv_freq.shape[0], interleaved, out.data_ptr(), *_strides(out)), q.device)
+        0, 0, inv_freq.data_ptr(), 2 * inv_freq.shape[0], interleaved, out.data_ptr(), *to), q.device)
     return out
 
 
@@ -492,11 +494,12 @@ def _plain_rotary(q, k, v, k_cache, v_cache, table, lens, inv_freq, cu) -> tuple
         return None
     w0, w1, w2, w3 = k.stride()
     x0, x1, x2, x3 = v.stride()
-    dev, R = q.get_device(), 2 * inv_freq.shape[0] if inv_freq.ndim == 1 else 0
+    dev, dt, r = q.get_device(), q.dtype, inv_freq.shape
+    R = 2 * r[0] if len(r) == 1 else 0
     if not (
-        n[:2] == q.shape[:2] and n[2] == f[3] and n[3] == f[4] and k.dtype is q.dtype and v.dtype is q.dtype
-        and w3 == 1 and x3 == 1 and (w0 | w1 | w2 | x0 | x1 | x2) % 8 == 0 and (k.data_ptr() | v.data_ptr()) % 16 == 0
-        and k.get_device() == dev and v.get_device() == dev and inv_freq.get_device() == dev
+        n[0] == (f[0] if cu is None else 1) and n[1] == f[1] and n[2] == f[3] and n[3] == f[4] and k.dtype is dt
+        and v.dtype is dt and w3 == 1 and x3 == 1 and (w0 | w1 | w2 | x0 | x1 | x2) % 8 == 0
+        and (k.data_ptr() | v.data_ptr()) % 16 == 0 and k.get_device() == dev and v.get_device() == dev and inv_freq.get_device() == dev
         and inv_freq.dtype is torch.float32 and inv_freq.is_contiguous() and 16 <= R <= f[4] and R % 16 == 0
     ):
         return None

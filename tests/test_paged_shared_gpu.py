@@ -89,7 +89,7 @@ def test_group_sizes(count, T, gpu_device):
     check(gpu_device, [(333, count)], T=T)
 
 
-@pytest.mark.parametrize("HQ,HKV", [(1, 1), (3, 1), (10, 2), (32, 8), (40, 1), (16, 16), (70, 2)])
+@pytest.mark.parametrize("HQ,HKV", [(1, 1), (3, 1), (10, 2), (32, 8), (40, 1), (16, 16), (70, 2), (127, 1), (130, 1)])
 @pytest.mark.parametrize("T", [1, 4])
 def test_heads(HQ, HKV, T, gpu_device):
     check(gpu_device, [(200, 6), (75, 3)], T=T, HQ=HQ, HKV=HKV)
