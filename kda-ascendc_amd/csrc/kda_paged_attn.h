@@ -511,20 +511,16 @@ struct Partial {
     static constexpr int64_t FLOATS = MT * (D + 2);
     static __device__ __forceinline__ float* at(float* ws, int slot) { return ws + slot * FLOATS; }
 };
-// Whether a unit's results are partial ones, where they go, and the rows that
-// they are of.
+// Where a unit of few rows' partial results go (nullptr: it has all there is),
+// and the rows that they are of.
+template <int D, class P>
+__device__ __forceinline__ float* few_partial(const P& p, const Unit& u) {
+    if constexpr (SHARED<P>) return u.place >= 0 ? p.ws + u.place : nullptr;
+    return u.slot >= 0 ? Partial<FEW, D>::at(p.ws, u.slot) : nullptr;
+}
 template <class P>
-__device__ __forceinline__ bool is_partial(const Unit& u) {
-    return SHARED<P> ? u.place >= 0 : u.slot >= 0;
-}
-template <int KIND, int D, class P>
-__device__ __forceinline__ float* partial_of(const P& p, const Unit& u, int64_t before) {
-    if constexpr (SHARED<P>) return p.ws + u.place;
-    return Partial<KIND, D>::at(p.ws + before, u.slot);
-}
-template <int KIND, class P>
-__device__ __forceinline__ int partial_rows(const Unit& u) {
-    return SHARED<P> ? u.rows : Shape<KIND>::MT;
+__device__ __forceinline__ int few_partial_rows(const Unit& u) {
+    return SHARED<P> ? u.rows : ROWS;
 }
 // Floats of the workspace before the parts of kind MANY.
 template <int D>
@@ -807,8 +803,8 @@ __device__ __forceinline__ Sums few_sum(const FewLds<D, WAVES>& lds, const float
 template <class E, int D, int WAVES, class P>
 __device__ __forceinline__ void few_rows(const P& p, const Unit& u, const FewLds<D, WAVES>& lds, float* joint) {
     few_sums<E, D, WAVES>(p, u, lds, joint);
-    float* part = is_partial<P>(u) ? partial_of<FEW, D>(p, u, 0) : nullptr;
-    const int R = partial_rows<FEW, P>(u);
+    float* part = few_partial<D>(p, u);
+    const int R = few_partial_rows<P>(u);
     for (int e = threadIdx.x; e < ROWS * (D / 4); e += WAVES * 64) {
         const int r = e / (D / 4), piece = e % (D / 4);
         const Row y = row_of(p, u, u.m * ROWS + r);
@@ -1047,18 +1043,17 @@ __device__ __forceinline__ void many_rows(const P& p, const Unit& u, uint8_t* kt
 
     const float l = sum_halves(run.l);
     if (!x.live) return;
-    if (is_partial<P>(u)) {
-        float* part = partial_of<MANY, D>(p, u, few_floats<D>());
-        const int R = partial_rows<MANY, P>(u);
+    if (u.slot >= 0) {
+        float* part = Partial<MANY, D>::at(p.ws + few_floats<D>(), u.slot);
         if (half == 0) {
             part[row] = run.log2_max();
-            part[R + row] = l;
+            part[MT + row] = l;
         }
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<f32x4*>(part + 2 * R + row * D + 32 * d + 2 * i + 4 * half) =
+                *reinterpret_cast<f32x4*>(part + 2 * MT + row * D + 32 * d + 2 * i + 4 * half) =
                     f32x4{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
         return;
     }

@@ -85,9 +85,9 @@ __device__ __forceinline__ int sequence_in_wave(const PagedParams& p, int t, int
 // turned units both pieces of 8 belong to the same 8 pairs: elements 8 u and
 // rotary_dim / 2 + 8 u on, or, interleaved, 16 u and 16 u + 8 on.
 // Few tokens are bound by the chain of loads (offsets, length, table entry),
-// many by HBM: on the GPU one token of 32 + 8 + 8 heads 2.6 us, 128 3.3, 16 packed
-// prompts of 1500 tokens together (24 + 4 + 4 heads of 64, 19 MB) 5.5, 8192 tokens
-// 35.9 (201 MB, 5.6 TB/s; a large copy reaches 4.8).  Two or four heads a thread,
+// many by HBM: on the GPU one token of 32 + 8 + 8 heads 2.5 us, 128 3.1, 16 packed
+// prompts of 2311 tokens together (24 + 4 + 4 heads of 64, 19 MB) 6.2, 8192 tokens
+// 36.2 (201 MB, 5.6 TB/s; a large copy reaches 5.2).  Two or four heads a thread,
 // which need the angles once, were slower (single tokens 3.0 and 3.8 us, 8192 the
 // same): the angles are not what bounds it.  Stores past the caches' lines:
 // 8192 tokens 37.9 us without; with the attention that reads what was stored

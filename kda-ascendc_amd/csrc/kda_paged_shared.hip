@@ -13,18 +13,26 @@
 // Three launches.  A plan, by one work-group: what there is to work on (for each
 // group its shared tokens, for each sequence what is its own), into how many
 // parts its keys are cut, where the partial results go.  The parts, a work-group
-// each.  The join.
+// each.  The join, which also works on the own keys of sequences that have few.
+//
+// 64 answers with 10 to 500 tokens of their own behind 16000, 32 / 8 heads: 47 us
+// (400 one by one), where the keys read once at 5.2 TB/s are 19 and the products at
+// 1.4 PFLOP/s 12.  The plan takes 4.5: its loads, three sums over the work-group.
+// The parts 29: 1.8 until a work-group has its unit, 3 until its first keys, 16.5
+// for 8 times two tiles (the matrix unit and the softmax in turn, as in
+// many_rows()), 3 for the groups' join and the stores, the rest the kernel's
+// beginning and end.  The join 14: 1 until it has its records, 11 for the longest
+// own keys (4 tiles a wave one after the other; 5 in the middle), 2 for 16 parts.
 #include "kda_paged_attn.h"
 
 namespace kda {
 namespace {
 
 // Rows of a tile: fewer than a work-group's waves have, whose two groups of four
-// have the same rows and go over keys of their own, every other tile.  A part then
-// leaves half the partial results of one with 256 rows, which is what its time
-// goes to where a prefix is cut for the whole card: 64 sequences of 4 heads a kv
-// head behind 16000 tokens are 256 parts of 8 tiles of 256 rows, whose results
-// (34 MB) took 7 us to write and as long to read.
+// have the same rows and go over keys of their own, every other tile.  Where a
+// prefix is cut for the whole card the parts then leave half the partial results
+// that they would with 256 rows (64 sequences of 4 heads a kv head behind 16000
+// tokens: 17 MB instead of 34, 46 us instead of 50).
 constexpr int MT = 128;
 template <int KIND>
 constexpr int rows_of() { return KIND == FEW ? ROWS : MT; }
@@ -449,7 +457,7 @@ __device__ __forceinline__ void split_rows(const SharedParams& p, const Unit& u,
     const float m0 = run.log2_max(), m1 = joint[row], top = fmaxf(m0, m1), sub = top == -INFINITY ? 0.f : top;
     const float f0 = fast_exp2(m0 - sub), f1 = fast_exp2(m1 - sub);
     const float l = fmaf(f1, joint[MT + row], run.l * f0);
-    float* part = is_partial<SharedParams>(u) ? p.ws + u.place : nullptr;
+    float* part = u.place >= 0 ? p.ws + u.place : nullptr;
     const float inv = part ? 1.f : (l > 0.f ? 1.f / l : 0.f);
     const int64_t out = out_row(p, u, x);
 #pragma unroll
