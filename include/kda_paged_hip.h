@@ -1,7 +1,8 @@
 /*
  * kda_paged_hip.h -- C ABI of libkda_bt16_hip.so for a paged cache of keys
  * and values: attention of new tokens over it, the append of their keys and
- * values, and the work on its pages (reserve, free, fork, compact, copy).
+ * values (with the position rotation), and the work on its pages (reserve,
+ * free, fork, compact, copy).
  *
  * For models that alternate KDA layers with softmax-attention layers: the
  * KDA layers keep a state of fixed size, the attention layers this cache.

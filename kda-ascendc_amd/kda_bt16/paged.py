@@ -1,5 +1,5 @@
 """A paged cache of keys and values on MI355X: attention of new tokens over
-it, their append, and the work on its pages.
+it, their append (with the position rotation), and the work on its pages.
 
 For models that alternate KDA layers with softmax-attention layers: the KDA
 layers keep a state of fixed size (:func:`kda_bt16.kda_decode_step`), the
@@ -24,6 +24,10 @@ length on the host.  A step of a serving loop::
     for layer in layers:
         paged_append(k, v, layer.k_cache, layer.v_cache, page_table, seq_lens)
         o = paged_attention(q, layer.k_cache, layer.v_cache, page_table, seq_lens)
+
+With positions, :func:`paged_append_rotary` turns the new queries and keys on
+the way into the pages.  Rows forked from one prompt (:func:`paged_fork`) that
+stand next to each other share its keys in :func:`paged_attention_shared`.
 
 The new tokens of a sequence are its last ones: token i of T sits at position
 ``seq_lens - T + i``.  Lowering ``seq_lens`` takes a sequence's last tokens
