@@ -414,8 +414,8 @@ __device__ __forceinline__ FewSpans few_spans(const P& p, const Cut& cut, int n0
 // Under a window of up to a third of the new tokens first first: most row tiles
 // see the same number of keys, and the few that see less, begun first, keep the
 // others from beginning all at once, round by round (a prompt of 8192 tokens, a
-// window of 2048 285 -> 269 us, of 512 134 -> 127; 2700 331 -> 325, 3300 366 and
-// 371, 4096 412 and 430).
+// window of 2048 265 -> 254 us, of 512 119 -> 113; 2700 312 -> 305, 3300 347 and
+// 350, 4096 390 and 407).
 struct ManyWork {
     int mt = 0, tiles = 0;  // row tiles, and tiles of keys that one sees at most
     NewTokens s;

@@ -112,8 +112,8 @@ __device__ __forceinline__ uint32_t limited(int64_t x) { return (uint32_t)min(x,
 // Of sequences that share, those with few rows and up to this many tiles of keys
 // of their own have them worked on in the join: not in parts that would only
 // begin when those of the prefixes are over (64 sequences with 10 to 500 tokens of
-// their own behind 16000: 47 us, with up to 8 or 12 tiles 51, with 4 54; drafts
-// with up to 700 tokens 36.9, 36.0 and 35.2).
+// their own behind 16000: 47 us, with up to 8 or 12 tiles 52; drafts with up to 700
+// tokens 31.6, with up to 24 tiles 33.6).
 constexpr int IN_JOIN = 16;
 // Rounds of parts of many rows at most, on 256 CUs each.
 constexpr int ROUNDS = 3;
