@@ -549,6 +549,8 @@ __global__ __launch_bounds__(KIND == FEW ? 256 : 512, 2) void paged_shared_kerne
     typedef __attribute__((address_space(4))) const int32_t c_i32;
     const int few = ((c_i32*)plan.head)[0], many = ((c_i32*)plan.head)[1];
     if (id >= few + many) return;
+    // (of few rows only there are no others, unless the offsets are none)
+    if (KIND == FEW && id < many) return;
     Unit u;
     if (KIND == FEW || id >= many) {
         if (unit_of<FEW, D>(p, plan, id - many, lane, u))
@@ -610,8 +612,12 @@ __global__ __launch_bounds__(256, 2) void paged_shared_join_kernel(SharedParams 
     const int id = blockIdx.x / groups, n = id / p.HKV, h = id - n * p.HKV;
     const Work w = load_work(plan, p.NG + n);
     const bool here = w.parts == 0;
+    // work-groups that there is some use for: where each works on the own keys, one
+    // for every 128 fours (with one for every 64, 8 sequences of 4 rows behind 2000
+    // tokens took 18.2 us instead of 16.8), else for every 64
     const int rows = w.count * p.G, items = rows * (D / 4), group0 = blockIdx.x % groups;
-    if (w.count == 0 || group0 * 64 >= items || (!here && w.place < 0)) return;
+    const int used = min(groups, here ? (items + 127) / 128 : (items + 63) / 64);
+    if (group0 >= used || (!here && w.place < 0)) return;
     Work g = {};
     if (w.group >= 0) g = load_work(plan, w.group);
     if (g.place == OVER) return;
@@ -630,9 +636,9 @@ __global__ __launch_bounds__(256, 2) void paged_shared_join_kernel(SharedParams 
         few_sums<E, D, WAVES>(p, u, tiles, joint);
     }
     // threads an item: 1, 2 or 4
-    const int shift = items > 128 * groups ? 0 : (items > 64 * groups ? 1 : 2), per = 256 >> shift;
+    const int shift = items > 128 * used ? 0 : (items > 64 * used ? 1 : 2), per = 256 >> shift;
     const int slice = threadIdx.x / per, item = threadIdx.x % per;
-    for (int group = group0; group * per < items; group += groups) {
+    for (int group = group0; group * per < items; group += used) {
         const int e = group * per + item, r = e / (D / 4), piece = e % (D / 4);
         const bool live = r < rows;
         Sums s = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
@@ -739,14 +745,13 @@ hipError_t launch_shared(SharedParams p, hipStream_t stream) {
     else paged_shared_kernel<E, D, MIXED><<<grid, 512, 0, stream>>>(p);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // work-groups a (sequence, head): one for every 128 fours of its rows (with one
-    // for every 64, 8 sequences of 4 rows behind 2000 tokens took 18.2 us instead of
-    // 16.8: each works on the own keys), as many as run at once, of many rows
-    // (whose own keys are not worked on there) eight times as many
+    // work-groups a (sequence, head): one for every 64 fours of its rows, together as
+    // many as run at once, where there may be many rows (whose own keys are not
+    // worked on there) eight times as many
     const int64_t pairs = (int64_t)p.N * p.HKV;
     const int64_t rows = std::min((int64_t)p.T * p.G, p.cu_seqlens ? (int64_t)1 << 20 : (int64_t)WHOLE);
     const int64_t most = rows > ROWS ? 8 * Shape<FEW>::SLOTS : Shape<FEW>::SLOTS;
-    const int groups = (int)std::max((int64_t)1, std::min((rows * (D / 4) + 127) / 128, most / pairs));
+    const int groups = (int)std::max((int64_t)1, std::min((rows * (D / 4) + 63) / 64, most / pairs));
     paged_shared_join_kernel<E, D><<<dim3((unsigned)(pairs * groups)), 256, 0, stream>>>(p, groups);
     return hipGetLastError();
 }

@@ -201,6 +201,23 @@ def test_offsets_that_are_none_stay_inside(gpu_device):
                            cu_seqlens=cu)
     torch.cuda.synchronize()
     compare(gpu_device, q, kc, vc, table, lens, starts, shared)
+    # a sequence of all 8 tokens several times over: more rows in a group than there are
+    kc, vc, table, lens, starts, shared = make([(40, 8)], lambda n: 60 + n, 16, 2, 64, BF16, gen)
+    args = [t.to(gpu_device) for t in (q.view(1, 8, 4, 64), kc, vc, table, lens, starts, shared)]
+    paged_attention_shared(*args, cu_seqlens=cu)
+    torch.cuda.synchronize()
+    compare(gpu_device, q, kc, vc, table, lens, starts, shared)
+
+
+def test_packed_single_tokens_equal_batch_rows(gpu_device):
+    gen = torch.Generator().manual_seed(16)
+    kc, vc, table, lens, starts, shared = make([(333, 9), (100, 30)], lambda n: 1 + 9 * n, 16, 4, 128, BF16, gen)
+    q = torch.randn(39, 1, 16, 128, generator=gen).to(BF16).to(gpu_device)
+    args = [t.to(gpu_device) for t in (kc, vc, table, lens, starts, shared)]
+    cu = torch.arange(40, dtype=torch.int32, device=gpu_device)
+    want = paged_attention_shared(q, *args, return_lse=True)
+    o, lse = paged_attention_shared(q.view(1, 39, 16, 128), *args, cu_seqlens=cu, return_lse=True)
+    assert torch.equal(o.view_as(q), want[0]) and torch.equal(lse.view_as(want[1]), want[1])
 
 
 @pytest.mark.parametrize("T", [1, 8, 40])
@@ -230,18 +247,20 @@ def test_strided_queries(gpu_device):
     assert torch.equal(o, want) and torch.equal(lse, want_lse)
 
 
-def test_scores_that_are_not_finite(gpu_device):
+@pytest.mark.parametrize("T", [1, 20])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_scores_that_are_not_finite(T, bad, gpu_device):
     """An infinite query makes its own results NaN and no other's."""
     gen = torch.Generator().manual_seed(13)
-    kc, vc, table, lens, starts, shared = make([(90, 4)], lambda n: 3 + n, 16, 2, 64, BF16, gen)
+    kc, vc, table, lens, starts, shared = make([(300, 4)], lambda n: T + 2 + n, 16, 2, 64, BF16, gen)
     d = gpu_device
-    q = torch.randn(4, 1, 4, 64, generator=gen).to(BF16).to(d)
+    q = torch.randn(4, T, 4, 64, generator=gen).to(BF16).to(d)
     args = (kc.to(d), vc.to(d), table.to(d), lens.to(d), starts.to(d), shared.to(d))
     want, want_lse = paged_attention_shared(q, *args, return_lse=True)
-    q[2, 0, 1, 0] = float("inf")
+    q[2, 0, 1, 0] = bad
     o, lse = paged_attention_shared(q, *args, return_lse=True)
     assert o[2, 0, 1].isnan().all() and lse[2, 0, 1].isnan()
-    keep = torch.ones(4, 1, 4, dtype=torch.bool, device=d)
+    keep = torch.ones(4, T, 4, dtype=torch.bool, device=d)
     keep[2, 0, 1] = False
     assert torch.equal(o[keep], want[keep]) and torch.equal(lse[keep], want_lse[keep])
 
