@@ -599,24 +599,27 @@ __device__ __forceinline__ void add_parts(Sums& s, const Parts& x, int piece, in
 
 // Joins the parts of (sequence n, kv head h): those of its group's shared tokens
 // and its own, or its own keys worked on here where they are few (by each of its
-// `groups` work-groups, which divide the joining).  Four elements of a row a
+// up to `groups` work-groups, which divide the joining).  Four elements of a row a
 // thread; where rows are few, several threads' parts in turn.
 template <class E, int D>
-__global__ __launch_bounds__(256, 2) void paged_shared_join_kernel(SharedParams p, int groups) {
+__global__ __launch_bounds__(256, 2) void paged_shared_join_kernel(SharedParams p, int groups, int fours) {
     constexpr int WAVES = Shape<FEW>::WAVES;
     typedef FewLds<D, WAVES> Lds;
     __shared__ alignas(1024) uint8_t lds[WAVES * Lds::EACH];
     __shared__ float joint[WAVES * 2 * ROWS];
     __shared__ float sums[6 * 256];
     const Plan plan = plan_of(p);
-    const int id = blockIdx.x / groups, n = id / p.HKV, h = id - n * p.HKV;
+    // (the first work-groups of all first, as of the others many have nothing to do:
+    // 64 packed single tokens behind 16000 47.5 us, with each one's together 90.9)
+    const int pairs = p.N * p.HKV, group0 = blockIdx.x / pairs, id = blockIdx.x - group0 * pairs;
+    const int n = id / p.HKV, h = id - n * p.HKV;
     const Work w = load_work(plan, p.NG + n);
     const bool here = w.parts == 0;
-    // work-groups that there is some use for: where each works on the own keys, one
-    // for every 128 fours (with one for every 64, 8 sequences of 4 rows behind 2000
-    // tokens took 18.2 us instead of 16.8), else for every 64
-    const int rows = w.count * p.G, items = rows * (D / 4), group0 = blockIdx.x % groups;
-    const int used = min(groups, here ? (items + 127) / 128 : (items + 63) / 64);
+    // work-groups that there is some use for: one for every `fours` fours, for 128 at
+    // least where each works on the own keys (with one for every 64, 8 sequences of
+    // 4 rows behind 2000 tokens took 18.2 us instead of 16.8)
+    const int rows = w.count * p.G, items = rows * (D / 4);
+    const int each = here ? max(128, fours) : fours, used = min(groups, (items + each - 1) / each);
     if (group0 >= used || (!here && w.place < 0)) return;
     Work g = {};
     if (w.group >= 0) g = load_work(plan, w.group);
@@ -745,14 +748,19 @@ hipError_t launch_shared(SharedParams p, hipStream_t stream) {
     else paged_shared_kernel<E, D, MIXED><<<grid, 512, 0, stream>>>(p);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // work-groups a (sequence, head): one for every 64 fours of its rows, together as
-    // many as run at once, where there may be many rows (whose own keys are not
-    // worked on there) eight times as many
+    // Work-groups a (sequence, head): one for every 64 fours of its rows; where there
+    // may be many rows, for so many fours that all rows together fill the card once
+    // (8 tokens of each of 64 packed sequences behind 16000 tokens: 163 us, with one
+    // for every 64 fours 276).  The grid has room for eight times as many, so that a
+    // chunk among single tokens is divided too: 63 of them and a chunk of 300
+    // tokens 175 us, with room for as many as run at once 412; the rest end at once.
     const int64_t pairs = (int64_t)p.N * p.HKV;
     const int64_t rows = std::min((int64_t)p.T * p.G, p.cu_seqlens ? (int64_t)1 << 20 : (int64_t)WHOLE);
-    const int64_t most = rows > ROWS ? 8 * Shape<FEW>::SLOTS : Shape<FEW>::SLOTS;
-    const int groups = (int)std::max((int64_t)1, std::min((rows * (D / 4) + 63) / 64, most / pairs));
-    paged_shared_join_kernel<E, D><<<dim3((unsigned)(pairs * groups)), 256, 0, stream>>>(p, groups);
+    const bool many = rows > ROWS;
+    const int64_t most = (many ? 8 : 1) * Shape<FEW>::SLOTS, all = tokens_of(p) * p.HQ * (D / 4);
+    const int fours = (int)std::max((int64_t)64, many ? all / Shape<FEW>::SLOTS : 0);
+    const int groups = (int)std::max((int64_t)1, std::min((rows * (D / 4) + fours - 1) / fours, most / pairs));
+    paged_shared_join_kernel<E, D><<<dim3((unsigned)(pairs * groups)), 256, 0, stream>>>(p, groups, fours);
     return hipGetLastError();
 }
 

@@ -133,6 +133,13 @@ def test_packed_with_a_chunk_in_a_group(gpu_device):
     check(gpu_device, [(200, 2), (150, 1), (200, 3)], new=new)
 
 
+@pytest.mark.parametrize("new", [[1] * 63 + [60], [60] + [1] * 63, [8] * 64, [63] + [1] * 20 + [200] + [1] * 42])
+def test_packed_uneven_rows_are_joined(new, gpu_device):
+    """A few sequences with most of the rows, and rows enough for every
+    work-group of the join to take more than one pass."""
+    check(gpu_device, [(400, 64)], new=new, HQ=32, HKV=8, own=lambda n: new[n] + 20)
+
+
 @pytest.mark.parametrize("N", [2, 64, 65, 255, 256, 300, 1500])
 def test_many_groups(N, gpu_device):
     """Plans of one and of several records a thread."""
