@@ -157,8 +157,6 @@ size_t paged_attn_workspace(const PagedParams& p, int D);
 hipError_t launch_paged_attn(const PagedParams& p, int D, hipStream_t stream);
 size_t paged_attn_workspace(const SinkParams& p, int D);
 hipError_t launch_paged_attn(const SinkParams& p, int D, hipStream_t stream);
-
-
 size_t paged_attn_workspace(const SharedParams& p, int D);
 hipError_t launch_paged_attn(const SharedParams& p, int D, hipStream_t stream);
 hipError_t launch_paged_append(const PagedParams& p, int D, hipStream_t stream);

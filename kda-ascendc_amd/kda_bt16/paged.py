@@ -124,6 +124,27 @@ def _check_written(name: str, t: torch.Tensor) -> None:
         need = stride * n
 
 
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of new tokens (the same ones) lie apart: in other
+    memory, or side by side in every row or every token of one tensor, as slices
+    of a fused projection do.  Other ways of lying apart are not seen."""
+    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+        return True
+    if a.storage_offset() > b.storage_offset():
+        a, b = b, a
+    gap = b.storage_offset() - a.storage_offset()
+    (N, T), (u0, u1), (w0, w1) = a.shape[:2], a.stride()[:2], b.stride()[:2]
+
+    def end(t: torch.Tensor, dim: int) -> int:
+        return 1 + sum((n - 1) * s for n, s in zip(t.shape[dim:], t.stride()[dim:]))
+
+    if gap >= end(a, 0):
+        return True
+    if N > 1 and u0 == w0 and end(a, 1) <= gap <= u0 - end(b, 1):
+        return True
+    return T > 1 and u1 == w1 and end(a, 2) <= gap <= u1 - end(b, 2) and (N == 1 or (u0 == w0 and T * u1 <= u0))
+
+
 def _check_new(name: str, t: torch.Tensor, heads: int | None, k_cache, page_table, cu_seqlens) -> None:
     """Tensors of the new tokens: [N, T, heads, D], or [1, T, heads, D] packed."""
     if t.ndim != 4:
@@ -456,7 +477,8 @@ def paged_append_rotary(
     once.
 
     ``out`` is where the turned queries go, in q's shape and type: ``q`` itself
-    (turned in place) or a tensor of other storage; by default a new one.
+    (turned in place; ``k`` and ``v`` lie apart from it, or side by side with it as
+    slices of one tensor) or a tensor of other storage; by default a new one.
     Queries of tokens that the append leaves out are turned all the same;
     packed tokens of no sequence (behind the last offset) are not written.
     """
@@ -478,6 +500,8 @@ def paged_append_rotary(
         if (out.data_ptr() != q.data_ptr() or out.stride() != q.stride()) and out.untyped_storage().data_ptr() in {
                 t.untyped_storage().data_ptr() for t in (q, k, v, k_cache, v_cache)}:
             raise ValueError("out must be q itself or of other storage than the inputs")
+        if out.data_ptr() == q.data_ptr() and not (_apart(q, k) and _apart(q, v)):
+            raise ValueError("q is turned in place: k and v must lie apart from it, or side by side with it in one tensor")
         _require_gpu(q)
         to = _strides(out)
     (N, T, HQ, HKV, D, dt, P, size, M, cu_dtype, cu, table, table_stride, lens, kp, vp, s0, s1, s2, t0, t1, t2, u0, u1,

@@ -12,6 +12,7 @@ import pytest
 import torch
 
 from kda_bt16 import _hip, paged_append_rotary
+from kda_bt16.paged import _apart
 from test_paged_capi import FAKE, HEADER, _text, fake_pointers, paged
 
 BF16 = torch.bfloat16
@@ -74,6 +75,44 @@ def test_in_place_on_a_broadcast_input_is_refused():
     q = torch.zeros(2, 1, 4, 64, dtype=BF16).expand(2, 3, 4, 64)
     with pytest.raises(ValueError, match="must not overlap"):
         call(q=q, out=q)
+
+
+@pytest.mark.parametrize("k,v", [(slice(0, 2), slice(6, 8)), (slice(4, 6), slice(3, 5)), (slice(2, 4), slice(2, 4))])
+def test_in_place_on_keys_or_values_is_refused(k, v):
+    q = _BUF[:, :, :4]
+    with pytest.raises(ValueError, match="k and v must lie apart"):
+        call(q=q, out=q, k=_BUF[:, :, k], v=_BUF[:, :, v])
+
+
+@pytest.mark.parametrize("shape,order", [((2, 3, 8, 64), (0, 1, 2, 3)), ((2, 8, 3, 64), (0, 2, 1, 3)), ((8, 2, 3, 64), (1, 2, 0, 3)),
+                                         ((2, 3, 8, 64), None)])
+def test_in_place_beside_keys_and_values(shape, order):
+    """Slices of one projection, tokens or heads outside, and tensors of their
+    own, go on to the launch."""
+    buf = torch.zeros(shape, dtype=BF16)
+    buf = buf if order is None else buf.permute(order)
+    for parts in ((slice(0, 4), slice(4, 6), slice(6, 8)), (slice(2, 6), slice(0, 2), slice(6, 8)), (slice(4, 8), slice(0, 2), slice(2, 4))):
+        q, k, v = (buf[:, :, x] if order else buf[:, :, x].contiguous() for x in parts)
+        with pytest.raises(ValueError, match="runs on a ROCm GPU"):
+            call(q=q, out=q, k=k, v=v)
+
+
+def test_apart_means_no_element_in_common():
+    gen = torch.Generator().manual_seed(0)
+
+    def draw(*choices):
+        return choices[int(torch.randint(len(choices), (1,), generator=gen))]
+
+    buf, seen = torch.arange(600), {True: 0, False: 0}
+    for _ in range(4000):
+        N, T = draw(1, 2, 3), draw(1, 2, 3)
+        rows, tokens = draw(12, 24, 30, 36, 72), draw(4, 8, 10, 12, 24)
+        a, b = (buf.as_strided((N, T, draw(1, 2), 2), (draw(rows, rows, rows, 18), draw(tokens, tokens, tokens, 6), draw(2, 4, 12), 1),
+                               draw(0, 2, 4, 6, 8, 12, 36, 72, 200)) for _ in range(2))
+        apart = _apart(a, b)
+        assert not apart or not set(a.flatten().tolist()) & set(b.flatten().tolist()), (a.shape, a.stride(), b.shape, b.stride())
+        seen[apart] += 1
+    assert min(seen.values()) > 400, seen
 
 
 @pytest.mark.parametrize("name", ["q", "k", "v", "k_cache", "v_cache", "inv_freq", "out"])
