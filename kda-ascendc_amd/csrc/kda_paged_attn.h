@@ -1051,17 +1051,18 @@ __device__ __forceinline__ void many_rows(const P& p, const Unit& u, uint8_t* kt
 
     const float l = sum_halves(run.l);
     if (!x.live) return;
-    if (u.slot >= 0) {
-        float* part = Partial<MANY, D>::at(p.ws + few_floats<D>(), u.slot);
+    if (SHARED<P> ? u.place >= 0 : u.slot >= 0) {
+        float* part = SHARED<P> ? p.ws + u.place : Partial<MANY, D>::at(p.ws + few_floats<D>(), u.slot);
+        const int rows = SHARED<P> ? u.rows : MT;  // of the partial result
         if (half == 0) {
             part[row] = run.log2_max();
-            part[MT + row] = l;
+            part[rows + row] = l;
         }
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<f32x4*>(part + 2 * MT + row * D + 32 * d + 2 * i + 4 * half) =
+                *reinterpret_cast<f32x4*>(part + 2 * rows + row * D + 32 * d + 2 * i + 4 * half) =
                     f32x4{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
         return;
     }

@@ -34,8 +34,13 @@ namespace {
 // that they would with 256 rows (64 sequences of 4 heads a kv head behind 16000
 // tokens: 17 MB instead of 34, 46 us instead of 50).
 constexpr int MT = 128;
-template <int KIND>
-constexpr int rows_of() { return KIND == FEW ? ROWS : MT; }
+// Rows of a sequence's own tiles (but for a last one of up to MT) where there are
+// enough of them for some rounds: as without groups, half as many beginnings and
+// ends.  WIDE row tiles of MT rows, which 256 CUs work on in three rounds: 8 chunks
+// of up to 2048 tokens behind 12000 771 -> 701 us (690 one by one), 2 of up to 4000
+// behind 30000 1965 -> 1856 (1802).  With fewer the parts are coarser: 8 of up to
+// 512 behind 12000 take 251 us so instead of 196, 4 of up to 300 158 instead of 137.
+constexpr int WIDE_MT = Shape<MANY>::MT, WIDE = 3 * Shape<MANY>::SLOTS;
 
 // Sequences and groups that a plan has room for.
 constexpr int MOST = 2048;
@@ -52,7 +57,7 @@ struct alignas(16) Work {
     int few, tiles;              // of few rows; tiles of keys
     int few_end, many_end;       // the units of few and of many rows up to this record's
     int sharer;                  // the first of its tokens among those that share
-    int pad;
+    int tile;                    // rows of a row tile
 };
 constexpr int NONE = -1, OVER = -2;
 
@@ -191,9 +196,10 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
             w.row = least[v];
         }
         w.few = (int64_t)w.count * p.G <= ROWS;
-        const int shift = w.few ? 5 : 6, rows = w.few ? ROWS : MT;
+        const int shift = w.few ? 5 : 6;
         static_assert(Shape<FEW>::TK == 32 && Shape<MANY>::TK == 64, "keys a tile");
-        w.mt = (int)(((int64_t)w.count * p.G + rows - 1) / rows);
+        w.tile = w.few ? ROWS : MT;
+        w.mt = (int)(((int64_t)w.count * p.G + w.tile - 1) / w.tile);
         w.tiles = max(1, (int)(((uint32_t)w.len + (1u << shift) - 1) >> shift) - (w.from >> shift));
         return w;
     };
@@ -224,7 +230,8 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
     // after the other, 7 more a round for its beginning and end (a tile of 128 rows
     // takes 1 us).  A few parts of few rows run in the first round too.  (Of LIMIT
     // tiles, which are hours of work, none is cut.)
-    const uint32_t units = all.x[3], tiles = all.x[4], beside = all.x[0] / size + all.x[1];
+    const bool wide = all.x[3] >= WIDE;
+    const uint32_t units = wide ? all.x[3] / 2 : all.x[3], tiles = all.x[4], beside = all.x[0] / size + all.x[1];
     uint32_t share = 0;
     float best = 3.4e38f;
     for (int r = 1; r <= rounds && tiles < LIMIT; ++r) {
@@ -245,9 +252,17 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
             x.x[0] = w.parts * p.HKV;
         } else {
             w.parts = 1;
+            uint32_t own = share;
+            if (wide && v >= p.NG) {
+                // (a row tile of twice the rows has twice the parts)
+                const uint32_t narrow = (uint32_t)(((int64_t)w.count * p.G + MT - 1) / MT), mt = (narrow + 1) / 2;
+                own = 2 * share - (narrow & 1 ? (share + mt - 1) / mt : 0);
+                w.tile = WIDE_MT;
+                w.mt = mt;
+            }
             if (share > 0) {
                 // (exact: the quotient of 32 bits by 32 is no nearer to a whole number than 2^-32)
-                const uint32_t parts = (uint32_t)((double)w.tiles * (double)share / (double)tiles);
+                const uint32_t parts = (uint32_t)((double)w.tiles * (double)own / (double)tiles);
                 w.parts = (int)max(1u, min((uint32_t)w.tiles / Shape<MANY>::LEAST, parts));
             }
             x.x[1] = w.mt * w.parts * p.HKV;
@@ -303,13 +318,12 @@ template <int D>
 constexpr int64_t FOUR = 4 * (D + 2);
 
 // Where the part-th part of row tile m of (w, kv head h) is, of `rows` rows.
-template <int D, int ROWS_A_TILE>
+template <int D>
 __device__ __forceinline__ int64_t place_of(const SharedParams& p, const Work& w, int m, int h, int part, int rows) {
-    return FOUR<D> * (w.place + (int64_t)m * (ROWS_A_TILE / 4) * p.HKV * w.parts + (h * w.parts + part) * (rows / 4));
+    return FOUR<D> * (w.place + (int64_t)m * (w.tile / 4) * p.HKV * w.parts + (h * w.parts + part) * (rows / 4));
 }
-template <int ROWS_A_TILE>
 __device__ __forceinline__ int tile_rows(const SharedParams& p, const Work& w, int m) {
-    return padded(min(ROWS_A_TILE, w.count * p.G - m * ROWS_A_TILE));
+    return padded(min(w.tile, w.count * p.G - m * w.tile));
 }
 
 __device__ __forceinline__ Work load_work(const Plan& plan, int v) {
@@ -328,6 +342,7 @@ __device__ __forceinline__ Work load_work(const Plan& plan, int v) {
     w.group = at[9];
     w.few = at[10];
     w.sharer = at[14];
+    w.tile = at[15];
     return w;
 }
 
@@ -488,7 +503,7 @@ __device__ __forceinline__ void split_rows(const SharedParams& p, const Unit& u,
 // record: no load waits for another (but for every 64 records more).
 template <int KIND, int D>
 __device__ __forceinline__ bool unit_of(const SharedParams& p, const Plan& plan, int x, int lane, Unit& u) {
-    constexpr int TK = Shape<KIND>::TK, MT = rows_of<KIND>();
+    constexpr int TK = Shape<KIND>::TK;
     const int V = p.NG + p.N;
     Work w = {};
     int before = 0;
@@ -509,6 +524,7 @@ __device__ __forceinline__ bool unit_of(const SharedParams& p, const Plan& plan,
             w.parts = take(mine.parts);
             w.mt = take(mine.mt);
             w.place = take(mine.place);
+            w.tile = take(mine.tile);
             u.mapped = v0 + at < p.NG;
             break;
         }
@@ -523,21 +539,24 @@ __device__ __forceinline__ bool unit_of(const SharedParams& p, const Plan& plan,
     const int part = x % w.parts;
     u.m = w.mt - 1 - x / w.parts;
     u.s = NewTokens{w.first, w.count, w.len, w.pos};
-    const int last = (min(w.count * p.G, u.m * MT + MT) - 1) / p.G;
+    const int last = (min(w.count * p.G, u.m * w.tile + w.tile) - 1) / p.G;
     u.lo = w.from;
     u.hi = max(w.from, min(w.pos + last + 1, w.len));
     const int t0 = u.lo / TK;
     const int64_t tiles = max(t0, (u.hi + TK - 1) / TK) - t0;
     u.begin = t0 + (int)(tiles * part / w.parts);
     u.end = t0 + (int)(tiles * (part + 1) / w.parts);
-    u.rows = tile_rows<MT>(p, w, u.m);
-    u.place = w.place == NONE ? -1 : place_of<D, MT>(p, w, u.m, u.h, part, u.rows);
+    u.rows = tile_rows(p, w, u.m);
+    u.place = w.place == NONE ? -1 : place_of<D>(p, w, u.m, u.h, part, u.rows);
+    if (KIND == MANY && u.rows <= MT) u.m *= w.tile / MT;  // (as split_rows counts)
     return true;
 }
 
 // A part a work-group, those of many rows first (the grid is what the host knows
-// that there can be at most).
-template <class E, int D, int KIND>
+// that there can be at most).  LONG: where there may be WIDE row tiles (in the
+// others' kernel their code costs 1 %: 8 packed questions behind 12000 196 -> 198
+// us, 16 chunks of up to 16 tokens 97.7 -> 99.2).
+template <class E, int D, int KIND, bool LONG>
 __global__ __launch_bounds__(KIND == FEW ? 256 : 512, 2) void paged_shared_kernel(SharedParams p) {
     constexpr int WAVES = Shape<KIND == FEW ? FEW : MANY>::WAVES;
     typedef FewLds<D, WAVES> Lds;
@@ -556,7 +575,14 @@ __global__ __launch_bounds__(KIND == FEW ? 256 : 512, 2) void paged_shared_kerne
         if (unit_of<FEW, D>(p, plan, id - many, lane, u))
             few_rows<E, D, WAVES>(p, u, Lds{lds, lds + 3 * Lds::EACH, lds + 6 * Lds::EACH}, joint);
     } else if constexpr (KIND != FEW) {
-        if (unit_of<MANY, D>(p, plan, id, lane, u)) split_rows<E, D>(p, u, lds, lds + sizeof(lds) / 2, joint);
+        if (!unit_of<MANY, D>(p, plan, id, lane, u)) return;
+        if constexpr (LONG) {
+            if (u.rows > MT) {
+                many_rows<E, D>(p, u, lds, lds + sizeof(lds) / 2);
+                return;
+            }
+        }
+        split_rows<E, D>(p, u, lds, lds + sizeof(lds) / 2, joint);
     }
 }
 
@@ -571,10 +597,10 @@ struct Parts {
 template <int D>
 __device__ __forceinline__ Parts parts_of(const SharedParams& p, const Work& w, int h, int row) {
     Parts x;
-    const int m = w.few ? 0 : row / MT;
-    x.r = row - m * MT;
-    x.R = w.few ? tile_rows<ROWS>(p, w, 0) : tile_rows<MT>(p, w, m);
-    x.first = p.ws + (w.few ? place_of<D, ROWS>(p, w, 0, h, 0, x.R) : place_of<D, MT>(p, w, m, h, 0, x.R));
+    const int m = row / w.tile;
+    x.r = row - m * w.tile;
+    x.R = tile_rows(p, w, m);
+    x.first = p.ws + place_of<D>(p, w, m, h, 0, x.R);
     x.step = (x.R / 4) * FOUR<D>;
     x.parts = w.parts;
     return x;
@@ -707,6 +733,8 @@ int64_t row_tiles(const SharedParams& p) {
     const int64_t records = std::min(std::min(p.NG, p.N / 2) + (members ? p.N : 0), (int)std::min((members ? 2 : 1) * rows / ROWS, (int64_t)MOST * 2));
     return (records + (members ? 2 : 1) * rows / MT) * p.HKV;
 }
+// Whether there may be WIDE row tiles.
+bool may_be_wide(const SharedParams& p) { return row_tiles(p) >= WIDE; }
 // Rounds of parts of many rows (two and more only with more than half as many row
 // tiles as CUs: fewer are cut well in one).
 int rounds_of(const SharedParams& p) {
@@ -720,7 +748,7 @@ int rounds_of(const SharedParams& p) {
 int64_t room_of(const SharedParams& p) {
     const int64_t rows = (2 * sharing_tokens(p) * p.G + 3 * (int64_t)(p.N + p.NG)) * p.HKV;
     const int64_t few = 2 * (int64_t)few_slots(Shape<FEW>::WAVES) * ROWS;
-    const int64_t many = (int64_t)rounds_of(p) * Shape<MANY>::SLOTS * MT;
+    const int64_t many = (int64_t)rounds_of(p) * Shape<MANY>::SLOTS * (may_be_wide(p) ? WIDE_MT : MT);
     return (rows + few + many + 3) / 4;
 }
 
@@ -744,8 +772,9 @@ hipError_t launch_shared(SharedParams p, hipStream_t stream) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const dim3 grid((unsigned)units_of(p, waves));
-    if (only) paged_shared_kernel<E, D, FEW><<<grid, 256, 0, stream>>>(p);
-    else paged_shared_kernel<E, D, MIXED><<<grid, 512, 0, stream>>>(p);
+    if (only) paged_shared_kernel<E, D, FEW, false><<<grid, 256, 0, stream>>>(p);
+    else if (may_be_wide(p)) paged_shared_kernel<E, D, MIXED, true><<<grid, 512, 0, stream>>>(p);
+    else paged_shared_kernel<E, D, MIXED, false><<<grid, 512, 0, stream>>>(p);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
     // Work-groups a (sequence, head): one for every 64 fours of its rows; where there

@@ -140,6 +140,16 @@ def test_packed_uneven_rows_are_joined(new, gpu_device):
     check(gpu_device, [(400, 64)], new=new, HQ=32, HKV=8, own=lambda n: new[n] + 20)
 
 
+@pytest.mark.parametrize("dtype,D,HQ,HKV", [(FP16, 64, 128, 32), (BF16, 128, 128, 32), (BF16, 64, 96, 16)])
+@pytest.mark.parametrize("own", [20, 3000])
+def test_packed_long_chunks_beside_a_group(own, dtype, D, HQ, HKV, gpu_device):
+    """Row tiles enough for several rounds: chunks in row tiles of 256, whose
+    last may be of few rows, whole and (those of one far longer sequence) cut."""
+    new = [400, 1, 60, 33, 1, 290, 64, 1, 257]
+    check(gpu_device, [(200, 5), (70, 2)], new=new, HQ=HQ, HKV=HKV, D=D, dtype=dtype, before=1, after=1,
+          own=lambda n: new[n] + (own if n == 5 else 20 + n))
+
+
 @pytest.mark.parametrize("N", [2, 64, 65, 255, 256, 300, 1500])
 def test_many_groups(N, gpu_device):
     """Plans of one and of several records a thread."""
