@@ -82,19 +82,19 @@ int64_t plan_bytes(const SharedParams& p) {
 __host__ __device__ inline int padded(int rows) { return (rows + 3) & ~3; }
 
 // Numbers of a thread, and their sums up to it (its own included) and over all of
-// the work-group's; the last and its sums no more than LIMIT.
+// the work-group's; those from PLAIN on and their sums no more than LIMIT.
 template <int K>
 struct Numbers {
     uint32_t x[K] = {};
 };
 constexpr uint32_t LIMIT = 0x7fffffff;
-template <int THREADS, int K>
+template <int THREADS, int PLAIN, int K>
 __device__ __forceinline__ Numbers<K> scan(const Numbers<K>& x, uint32_t (&lds)[K][16], Numbers<K>& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     Numbers<K> s;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        s.x[k] = k < K - 1 ? wave_prefix(x.x[k]) : wave_prefix(x.x[k], LIMIT);
+        s.x[k] = k < PLAIN ? wave_prefix(x.x[k]) : wave_prefix(x.x[k], LIMIT);
         if (lane == 63) lds[k][wave] = s.x[k];
     }
     __syncthreads();
@@ -105,7 +105,7 @@ __device__ __forceinline__ Numbers<K> scan(const Numbers<K>& x, uint32_t (&lds)[
         for (int k = 0; k < K; ++k) {
             if (w == wave) s.x[k] += all.x[k];
             all.x[k] += lds[k][w];
-            if (k == K - 1) {
+            if (k >= PLAIN) {
                 s.x[k] = min(s.x[k], LIMIT);
                 all.x[k] = min(all.x[k], LIMIT);
             }
@@ -123,10 +123,20 @@ constexpr int IN_JOIN = 16;
 // Rounds of parts of many rows at most, on 256 CUs each.
 constexpr int ROUNDS = 3;
 
-// One work-group.  `waves`: those of a work-group of few rows; `rounds`: of parts
-// of many rows, at most; `room`: of the partial results, in 4 rows.
+// Parts that keys of few rows are cut into at most, two to four rounds of them: as
+// many as run at once, or more that still have 4 tiles a wave (8 of head size 64, of
+// half the bytes), as lengths are uneven and a round waits for its longest.  Decode,
+// 32 / 8 heads: 32 pairs behind 8000 to 16000 tokens 335 -> 299 us, 16 fours behind 2000
+// to 4000 72.5 -> 64.0, 4 groups of 16 behind 100 to 200 with up to 8000 of their own 165
+// -> 146 (one by one 533, 145, 142); by 6 or 8 tiles a wave the fours take 72.5 again,
+// with 1024 parts in any case 78.7.
+constexpr int FEW_PARTS = 1024;
+
+// One work-group.  `waves`: those of a work-group of few rows; `fine`: tiles of their
+// parts where they are more than run at once; `rounds`: of parts of many rows, at most; `room`: of the partial results,
+// in 4 rows.
 template <int THREADS>
-__global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams p, int waves, int rounds, int room) {
+__global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams p, int waves, int fine, int rounds, int room) {
     constexpr bool ONE = THREADS < 1024;  // a record a thread
     // (of the groups: their sequences' offsets, the first that shares, how many do,
     // with how many tokens; the shared ones.  Sharing tokens before each sequence.)
@@ -206,32 +216,36 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
     // Whether the join works on a record's keys.
     auto in_join = [&](const Work& w) { return w.few && w.group >= 0 && w.tiles <= IN_JOIN; };
     Work w;
-    // tiles and records of few rows, tokens that share, row tiles and tiles of many
+    // records of few rows, tokens that share, row tiles of many; tiles of few, of many
     Numbers<5> x, all;
     for (int v = v0; v < v1; ++v) {
         w = record(v);
-        if (w.group >= 0) x.x[2] += w.count;
+        if (w.group >= 0) x.x[1] += w.count;
         if (w.count > 0 && !in_join(w)) {
             if (w.few) {
-                x.x[0] += w.tiles * p.HKV;
-                x.x[1] += p.HKV;
+                x.x[0] += p.HKV;
+                x.x[3] = limited(x.x[3] + (int64_t)w.tiles * p.HKV);
             } else {
-                x.x[3] += w.mt * p.HKV;
+                x.x[2] += w.mt * p.HKV;
                 x.x[4] = limited(x.x[4] + (int64_t)w.mt * p.HKV * w.tiles);
             }
         }
         if (!ONE) plan.work[v] = w;
     }
-    const Numbers<5> upto5 = scan<THREADS>(x, lds5, all);
-    // Few rows: parts of `size` tiles, at most as many of them as run at once.
-    const uint32_t slots = few_slots(waves), size = max((uint32_t)waves, (all.x[0] + slots - 1) / slots);
+    const Numbers<5> upto5 = scan<THREADS, 3>(x, lds5, all);
+    // Few rows: parts of `size` tiles, as many as run at once, or up to FEW_PARTS that
+    // are still of `fine` tiles.  (Of LIMIT tiles, which are seconds of work, none
+    // is cut.)
+    const uint32_t slots = few_slots(waves), once = (all.x[3] + slots - 1) / slots;
+    const uint32_t finer = max((all.x[3] + FEW_PARTS - 1) / FEW_PARTS, min(once, (uint32_t)fine));
+    const uint32_t size = all.x[3] < LIMIT ? max((uint32_t)waves, finer) : LIMIT;
     // Many rows: with `units` row tiles of `tiles` tiles of keys together, `share`
     // parts of equal size if they can be had, in 1 to 3 rounds: the fewest tiles one
     // after the other, 7 more a round for its beginning and end (a tile of 128 rows
     // takes 1 us).  A few parts of few rows run in the first round too.  (Of LIMIT
     // tiles, which are hours of work, none is cut.)
-    const bool wide = all.x[3] >= WIDE;
-    const uint32_t units = wide ? all.x[3] / 2 : all.x[3], tiles = all.x[4], beside = all.x[0] / size + all.x[1];
+    const bool wide = all.x[2] >= WIDE;
+    const uint32_t units = wide ? all.x[2] / 2 : all.x[2], tiles = all.x[4], beside = all.x[3] / size + all.x[0];
     uint32_t share = 0;
     float best = 3.4e38f;
     for (int r = 1; r <= rounds && tiles < LIMIT; ++r) {
@@ -271,7 +285,7 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
         return x;
     };
     Numbers<3> mine3, x3, all3;
-    int sharers = upto5.x[2] - x.x[2];
+    int sharers = upto5.x[1] - x.x[1];
     for (int v = v0; v < v1; ++v) {
         if (!ONE) w = plan.work[v];
         x3 = needs(w, v);
@@ -283,8 +297,8 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
             if (w.group >= 0) sharers += w.count;
         }
     }
-    if (tid == 0) before[p.N] = all.x[2];
-    const Numbers<3> upto = scan<THREADS>(mine3, lds3, all3);  // (which waits for all of `before`)
+    if (tid == 0) before[p.N] = all.x[1];
+    const Numbers<3> upto = scan<THREADS, 2>(mine3, lds3, all3);  // (which waits for all of `before`)
     Numbers<3> at;
 #pragma unroll
     for (int k = 0; k < 3; ++k) at.x[k] = upto.x[k] - mine3.x[k];
@@ -747,15 +761,15 @@ int rounds_of(const SharedParams& p) {
 // that keys are cut into.
 int64_t room_of(const SharedParams& p) {
     const int64_t rows = (2 * sharing_tokens(p) * p.G + 3 * (int64_t)(p.N + p.NG)) * p.HKV;
-    const int64_t few = 2 * (int64_t)few_slots(Shape<FEW>::WAVES) * ROWS;
+    const int64_t few = (int64_t)FEW_PARTS * ROWS;
     const int64_t many = (int64_t)rounds_of(p) * Shape<MANY>::SLOTS * (may_be_wide(p) ? WIDE_MT : MT);
     return (rows + few + many + 3) / 4;
 }
 
 // Units at most: a record's heads and row tiles, and the parts more that keys
 // are cut into.
-int64_t units_of(const SharedParams& p, int waves) {
-    const int64_t few = ((int64_t)p.N + std::min(p.NG, p.N / 2)) * p.HKV + few_slots(waves);
+int64_t units_of(const SharedParams& p) {
+    const int64_t few = ((int64_t)p.N + std::min(p.NG, p.N / 2)) * p.HKV + FEW_PARTS;
     return few + row_tiles(p) + rounds_of(p) * Shape<MANY>::SLOTS;
 }
 
@@ -766,12 +780,12 @@ hipError_t launch_shared(SharedParams p, hipStream_t stream) {
     p.map = p.plan + HEAD + ((int64_t)p.NG + p.N) * (int64_t)(sizeof(Work) / 4);
     const int V = p.NG + p.N, room = (int)std::min(room_of(p), (int64_t)LIMIT - 1);
     const bool only = few_only(p);
-    const int waves = Shape<FEW>::WAVES * (only ? 1 : 2);
-    if (V <= 256) paged_shared_plan_kernel<256><<<1, 256, 0, stream>>>(p, waves, rounds_of(p), room);
-    else paged_shared_plan_kernel<1024><<<1, 1024, 0, stream>>>(p, waves, rounds_of(p), room);
+    const int waves = Shape<FEW>::WAVES * (only ? 1 : 2), fine = 4 * waves * (128 / D);
+    if (V <= 256) paged_shared_plan_kernel<256><<<1, 256, 0, stream>>>(p, waves, fine, rounds_of(p), room);
+    else paged_shared_plan_kernel<1024><<<1, 1024, 0, stream>>>(p, waves, fine, rounds_of(p), room);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const dim3 grid((unsigned)units_of(p, waves));
+    const dim3 grid((unsigned)units_of(p));
     if (only) paged_shared_kernel<E, D, FEW, false><<<grid, 256, 0, stream>>>(p);
     else if (may_be_wide(p)) paged_shared_kernel<E, D, MIXED, true><<<grid, 512, 0, stream>>>(p);
     else paged_shared_kernel<E, D, MIXED, false><<<grid, 512, 0, stream>>>(p);
