@@ -117,32 +117,31 @@ def _check_cache(k_cache, v_cache, page_table, seq_lens) -> None:
 
 def _check_written(name: str, t: torch.Tensor) -> None:
     """No element of a strided output is another's."""
-    need = t.shape[-1]
-    for stride, n in sorted((t.stride(i), t.shape[i]) for i in range(t.ndim - 1) if t.shape[i] > 1):
+    (_, T, H, D), (s0, s1, s2, _) = t.shape, t.stride()
+    if s2 >= D and s1 >= H * s2 and s0 >= T * s1:
+        return
+    need = D
+    for stride, n in sorted((t.stride(i), t.shape[i]) for i in range(3) if t.shape[i] > 1):
         if stride < need:
             raise ValueError(f"{name}'s elements must not overlap, got strides {t.stride()}")
         need = stride * n
 
 
 def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two tensors of new tokens (the same ones) lie apart: in other
-    memory, or side by side in every row or every token of one tensor, as slices
-    of a fused projection do.  Other ways of lying apart are not seen."""
-    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+    """Whether two tensors of new tokens (the same ones) lie apart: side by side
+    in every token or every row, as slices of a fused projection do, or one
+    behind the other.  Other ways of lying apart are not seen."""
+    gap = b.data_ptr() - a.data_ptr()
+    if gap < 0:
+        a, b, gap = b, a, -gap
+    gap //= a.element_size()
+    (N, T, H, D), (a0, a1, a2, _), (b0, b1, b2, _) = a.shape, a.stride(), b.stride()
+    # from the first element of a token's (a row's) to behind its last
+    a_token, b_token = (H - 1) * a2 + D, (b.shape[2] - 1) * b2 + D
+    if T > 1 and a1 == b1 and a_token <= gap <= a1 - b_token and (N == 1 or (a0 == b0 and T * a1 <= a0)):
         return True
-    if a.storage_offset() > b.storage_offset():
-        a, b = b, a
-    gap = b.storage_offset() - a.storage_offset()
-    (N, T), (u0, u1), (w0, w1) = a.shape[:2], a.stride()[:2], b.stride()[:2]
-
-    def end(t: torch.Tensor, dim: int) -> int:
-        return 1 + sum((n - 1) * s for n, s in zip(t.shape[dim:], t.stride()[dim:]))
-
-    if gap >= end(a, 0):
-        return True
-    if N > 1 and u0 == w0 and end(a, 1) <= gap <= u0 - end(b, 1):
-        return True
-    return T > 1 and u1 == w1 and end(a, 2) <= gap <= u1 - end(b, 2) and (N == 1 or (u0 == w0 and T * u1 <= u0))
+    a_row, b_row = (T - 1) * a1 + a_token, (T - 1) * b1 + b_token
+    return (N > 1 and a0 == b0 and a_row <= gap <= a0 - b_row) or gap >= (N - 1) * a0 + a_row
 
 
 def _check_new(name: str, t: torch.Tensor, heads: int | None, k_cache, page_table, cu_seqlens) -> None:
@@ -492,15 +491,16 @@ def paged_append_rotary(
         token = f[2] * f[4]
         to = (f[1] * token, token, f[4])
     else:
-        _check_new("out", out, q.shape[2], k_cache, page_table, cu_seqlens)
-        if out.shape != q.shape:
-            raise ValueError(f"out.shape {tuple(out.shape)} must match q {tuple(q.shape)}")
+        if out is not q:
+            _check_new("out", out, q.shape[2], k_cache, page_table, cu_seqlens)
+            if out.shape != q.shape:
+                raise ValueError(f"out.shape {tuple(out.shape)} must match q {tuple(q.shape)}")
+            _forward_only("paged_append_rotary", out)
         _check_written("out", out)
-        _forward_only("paged_append_rotary", out)
-        if (out.data_ptr() != q.data_ptr() or out.stride() != q.stride()) and out.untyped_storage().data_ptr() in {
-                t.untyped_storage().data_ptr() for t in (q, k, v, k_cache, v_cache)}:
-            raise ValueError("out must be q itself or of other storage than the inputs")
-        if out.data_ptr() == q.data_ptr() and not (_apart(q, k) and _apart(q, v)):
+        if out.data_ptr() != q.data_ptr() or out.stride() != q.stride():
+            if out.untyped_storage().data_ptr() in {t.untyped_storage().data_ptr() for t in (q, k, v, k_cache, v_cache)}:
+                raise ValueError("out must be q itself or of other storage than the inputs")
+        elif not (_apart(q, k) and _apart(q, v)):
             raise ValueError("q is turned in place: k and v must lie apart from it, or side by side with it in one tensor")
         _require_gpu(q)
         to = _strides(out)
