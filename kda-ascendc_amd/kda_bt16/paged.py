@@ -128,20 +128,39 @@ def _check_written(name: str, t: torch.Tensor) -> None:
 
 
 def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two tensors of new tokens (the same ones) lie apart: side by side
-    in every token or every row, as slices of a fused projection do, or one
-    behind the other.  Other ways of lying apart are not seen."""
+    """Whether two tensors of new tokens (the same ones) lie apart: one behind
+    the other, or side by side in every head, token or row, as slices of a fused
+    projection do in any order of its dimensions.  Other ways of lying apart are
+    not seen."""
     gap = b.data_ptr() - a.data_ptr()
     if gap < 0:
         a, b, gap = b, a, -gap
     gap //= a.element_size()
     (N, T, H, D), (a0, a1, a2, _), (b0, b1, b2, _) = a.shape, a.stride(), b.stride()
+    H2 = b.shape[2]
     # from the first element of a token's (a row's) to behind its last
-    a_token, b_token = (H - 1) * a2 + D, (b.shape[2] - 1) * b2 + D
-    if T > 1 and a1 == b1 and a_token <= gap <= a1 - b_token and (N == 1 or (a0 == b0 and T * a1 <= a0)):
-        return True
+    a_token, b_token = (H - 1) * a2 + D, (H2 - 1) * b2 + D
     a_row, b_row = (T - 1) * a1 + a_token, (T - 1) * b1 + b_token
-    return (N > 1 and a0 == b0 and a_row <= gap <= a0 - b_row) or gap >= (N - 1) * a0 + a_row
+    # One behind the other, or slices of tokens or rows in their order (what most
+    # calls have: a small call's time is the host's).
+    if (gap >= (N - 1) * a0 + a_row or (N > 1 and a0 == b0 and a_row <= gap <= a0 - b_row)
+            or (T > 1 and a1 == b1 and a_token <= gap <= a1 - b_token and (N == 1 or (a0 == b0 and T * a1 <= a0)))):
+        return True
+    dims = [x for x in ((a0, b0, N, N), (a1, b1, T, T), (a2, b2, H, H2)) if max(x[2:]) > 1]
+
+    def span(i, inner):  # of a (0) or b (1), in these dimensions
+        return sum(x[i] * (x[2 + i] - 1) for x in inner) + D
+
+    # Side by side in every step of `period`: what is inside of a step in both
+    # tensors ends within it, and the steps of one size do not reach into those of
+    # the next.
+    for period in {s for s, u, _, _ in dims if s == u}:
+        outer = sorted((s, max(n, m)) for s, u, n, m in dims if s == u and s >= period)
+        inner = [x for x in dims if x[0] != x[1] or x[0] < period]
+        if (span(0, inner) <= gap <= period - span(1, inner)
+                and all(s * n <= t for (s, n), (t, _) in zip(outer, outer[1:]))):
+            return True
+    return False
 
 
 def _check_new(name: str, t: torch.Tensor, heads: int | None, k_cache, page_table, cu_seqlens) -> None:

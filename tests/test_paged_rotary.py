@@ -97,6 +97,47 @@ def test_in_place_beside_keys_and_values(shape, order):
             call(q=q, out=q, k=k, v=v)
 
 
+@pytest.mark.parametrize("shape,order,at", [
+    ((3, 2, 8, 64), (1, 0, 2, 3), 2), ((8, 3, 2, 64), (2, 1, 0, 3), 2), ((3, 8, 2, 64), (2, 0, 1, 3), 2),
+    ((2, 3, 2, 3, 64), None, 3), ((3, 2, 2, 3, 64), (1, 0, 2, 3, 4), 3), ((2, 3, 3, 2, 64), None, 2)])
+def test_in_place_beside_keys_and_values_in_any_order(shape, order, at):
+    """Slices of one projection whose tokens stand outside of the rows (time
+    first), or of whose heads each has its query, key and value side by side."""
+    buf = torch.zeros(shape, dtype=BF16)
+    buf = buf if order is None else buf.permute(order)
+    if buf.ndim == 4:
+        q, k, v = buf.split([4, 2, 2], at)
+    else:
+        q, k, v = buf.unbind(at)
+    assert q.shape[:2] == (2, 3)
+    for x, y, z in ((q, k, v), (q, v, k)) + (((k, q, v), (v, k, q)) if buf.ndim == 5 else ()):
+        with pytest.raises(ValueError, match="runs on a ROCm GPU"):
+            call(q=x, out=x, k=y, v=z)
+        with pytest.raises(ValueError, match="k and v must lie apart"):
+            call(q=x, out=x, k=y, v=x[:, :, :2])
+
+
+def test_apart_sees_every_order_of_a_projection():
+    """Of random slices of one tensor in any order of its dimensions: the same as
+    by their elements."""
+    gen = torch.Generator().manual_seed(1)
+    seen = {True: 0, False: 0}
+    for _ in range(3000):
+        N, T, H, third = (int(x) for x in torch.randint(1, 4, (4,), generator=gen))
+        order = torch.randperm(4, generator=gen).tolist()
+        buf = torch.arange(N * T * H * third * 2).view(*[(N, T, H, third)[i] for i in order], 2)
+        buf = buf.permute(*[order.index(i) for i in range(4)], 4)
+        if third > 1:
+            a, b = (buf[:, :, :, int(i)] for i in torch.randint(third, (2,), generator=gen))
+        else:
+            (i, j), (k, l) = (sorted(torch.randint(H, (2,), generator=gen).tolist()) for _ in range(2))
+            a, b = buf[:, :, i:j + 1, 0], buf[:, :, k:l + 1, 0]
+        common = bool(set(a.flatten().tolist()) & set(b.flatten().tolist()))
+        assert _apart(a, b) != common, (a.shape, a.stride(), b.shape, b.stride(), a.storage_offset(), b.storage_offset())
+        seen[common] += 1
+    assert min(seen.values()) > 500, seen
+
+
 def test_apart_means_no_element_in_common():
     gen = torch.Generator().manual_seed(0)
 

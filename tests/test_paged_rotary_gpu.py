@@ -149,6 +149,26 @@ def test_in_place(gpu_device):
     check(gpu_device, [50, 9], T=9, inplace=True)
 
 
+@pytest.mark.parametrize("shape,order,at", [((9, 5, 8, 64), (1, 0, 2, 3), 2), ((8, 9, 5, 64), (2, 1, 0, 3), 2),
+                                            ((5, 9, 2, 3, 64), None, 3), ((9, 5, 2, 3, 64), (1, 0, 2, 3, 4), 3)])
+def test_in_place_in_any_order_of_a_projection(shape, order, at, gpu_device):
+    """Time first, or every head's query, key and value side by side: the same
+    bits as into a new tensor, keys and values left as they were."""
+    d, gen = gpu_device, torch.Generator().manual_seed(2)
+    buf = torch.randn(shape, generator=gen).to(BF16).to(d)
+    x = buf if order is None else buf.permute(order)
+    q, k, v = x.split([4, 2, 2], at) if x.ndim == 4 else x.unbind(at)
+    lens = [9, 30, 3, 16, 0]
+    table, P = table_of(lens, 16, gen)
+    table, lens = table.to(d), torch.tensor(lens, dtype=torch.int32, device=d)
+    freq = (10000.0 ** (-torch.arange(32) / 32)).to(d)
+    there, here = ([torch.zeros(P, 16, 2, 64, dtype=BF16, device=d) for _ in range(2)] for _ in range(2))
+    was = [t.clone() for t in (k, v)]
+    want = paged_append_rotary(q, k, v, *there, table, lens, freq)
+    assert paged_append_rotary(q, k, v, *here, table, lens, freq, out=q) is q
+    assert torch.equal(q, want) and all(torch.equal(a, b) for a, b in zip(here + [k, v], there + was))
+
+
 def test_a_missing_page_is_left_out(gpu_device):
     check(gpu_device, [100, 70], T=60, hole=(0, 4))
 
