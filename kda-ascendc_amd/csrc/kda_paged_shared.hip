@@ -717,26 +717,36 @@ __global__ __launch_bounds__(256, 2) void paged_shared_join_kernel(SharedParams 
 
 // ---- launches ----
 
-// Rows of a sequence from which on it is no different from others without a
-// prefix to share: a row tile of the ordinary kernels'.
+// Rows of a sequence from which on a dense call is no different from one without
+// groups: a row tile of the ordinary kernels'.
 constexpr int WHOLE = Shape<MANY>::MT;
 
-// Whether sequences are worked on together at all: not where each fills row
-// tiles by itself, nor where there are more than a plan has room for.
+// Whether a plan has room for the sequences, and the table so many keys that one
+// may pay.
 //
-// Nor where the table is so small that reading the shared keys again for each
-// sequence costs less than the plan and the longer join, 15 us for 9: by the bytes
-// that its rows hold, whose second reading is from the caches. Decode of 8
-// sequences, 32 / 8 heads: 67 MB 15.3 us one by one and 17.9 so, 131 MB 21.3 and
-// 19.4; 2 sequences: 66 MB 18.9 and 22.1, 131 MB 29.0 and 26.5.  Drafts of 5, 24 /
-// 4 heads of 64 (30 rows: their row tiles are full one by one too): 131 MB 24.4
+// Where the table is so small that reading the shared keys again for each
+// sequence costs less than the plan and the longer join, 15 us for 9, it does not:
+// by the bytes that its rows hold, whose second reading is from the caches. Decode
+// of 8 sequences, 32 / 8 heads: 67 MB 15.3 us one by one and 17.9 so, 131 MB 21.3
+// and 19.4; 2 sequences: 66 MB 18.9 and 22.1, 131 MB 29.0 and 26.5.  Drafts of 5, 24
+// / 4 heads of 64 (30 rows: their row tiles are full one by one too): 131 MB 24.4
 // and 27.8, 262 MB 35.9 and 33.5.
-bool together(const SharedParams& p, int D) {
+bool planned(const SharedParams& p, int D) {
     if (p.N < 2 || p.N > MOST || p.NG > MOST || (!p.cu_seqlens && (int64_t)p.T * p.G >= WHOLE)) return false;
     const int64_t row = ((int64_t)p.M << p.page_shift) * p.HKV * D * 4;
     const int64_t least = tokens_of(p) * p.G <= (int64_t)p.N * (ROWS / 2) ? 112 << 20 : 224 << 20;
     return row >= least / p.N;
 }
+// Dense calls of more rows a sequence than fill a row tile, of which the plan lets
+// none share.  In its row tiles of 128, the second one filled in part, they are
+// mostly slower than one by one in one of 256 (32 / 8 heads, 160 rows: 8 sequences
+// behind 12000 tokens 98 us one by one and 150 so, 32 264 and 310, 64 behind 2000
+// 114 and 123; 24 / 4 heads of 64, 162 rows: 64 behind 12000 212 and 253, but 32 216
+// and 130).  Of 128 rows, which share no more, one row tile is full and 256 rows are
+// half empty: 8 behind 12000 88 and 75, 32 229 and 195, 64 behind 2000 102 and 93.
+bool alone(const SharedParams& p) { return !p.cu_seqlens && (int64_t)p.T * p.G > MT; }
+// Whether sequences are worked on together at all.
+bool together(const SharedParams& p, int D) { return planned(p, D) && !alone(p); }
 bool few_only(const SharedParams& p) { return tokens_of(p) * p.G <= ROWS; }
 
 // Row tiles of many rows at most.  Records of many rows have more than ROWS.
@@ -798,7 +808,7 @@ hipError_t launch_shared(SharedParams p, hipStream_t stream) {
     // chunk among single tokens is divided too: 63 of them and a chunk of 300
     // tokens 175 us, with room for as many as run at once 412; the rest end at once.
     const int64_t pairs = (int64_t)p.N * p.HKV;
-    const int64_t rows = std::min((int64_t)p.T * p.G, p.cu_seqlens ? (int64_t)1 << 20 : (int64_t)WHOLE);
+    const int64_t rows = std::min((int64_t)p.T * p.G, (int64_t)1 << 20);
     const bool many = rows > ROWS;
     const int64_t most = (many ? 8 : 1) * Shape<FEW>::SLOTS, all = tokens_of(p) * p.HQ * (D / 4);
     const int fours = (int)std::max((int64_t)64, many ? all / Shape<FEW>::SLOTS : 0);
@@ -810,7 +820,12 @@ hipError_t launch_shared(SharedParams p, hipStream_t stream) {
 }  // namespace
 
 size_t paged_attn_workspace(const SharedParams& p, int D) {
-    if (!together(p, D)) return paged_attn_workspace(static_cast<const PagedParams&>(p), D);
+    if (!together(p, D)) {
+        // (the plan's few KB stay where there is room for one: callers that tell
+        // the calls with one from paged_attention's do so by the size)
+        const size_t one_by_one = paged_attn_workspace(static_cast<const PagedParams&>(p), D);
+        return one_by_one + (planned(p, D) ? plan_bytes(p) : 0);
+    }
     return (size_t)(4 * (D + 2) * room_of(p) * 4 + plan_bytes(p));
 }
 

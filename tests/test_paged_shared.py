@@ -112,6 +112,15 @@ def test_workspace_sizes():
     assert got == (rows + 3) // 4 * 4 * 130 * 4 + (16 + 10 * 16 + 8) * 4
 
 
+def test_workspace_of_dense_rows_past_a_row_tile():
+    """More than 128 rows a sequence: one by one, in what paged_attention takes."""
+    f, plain = _hip.lib().kda_paged_attn_shared_workspace_bytes, _hip.lib().kda_paged_attn_workspace_bytes
+    for heads, T in ((4, 65), (4, 100), (4, 127), (16, 17), (16, 31), (260, 1)):
+        base = dict(T=T, HQ=heads, q_row=T * heads * 128, q_token=heads * 128, M=8000, table_stride=8000)
+        a = shared(base)
+        assert 0 <= f(ctypes.byref(a)) - plain(ctypes.byref(a.paged)) <= 1 << 16, base
+
+
 @fake_pointers
 def test_argument_checks():
     f = _hip.lib().kda_paged_attn_shared_hip

@@ -102,6 +102,17 @@ def test_new_tokens(T, gpu_device):
     check(gpu_device, [(300, 3), (130, 2)], T=T)
 
 
+@pytest.mark.parametrize("T,HQ,HKV,D", [(65, 4, 2, 64), (100, 4, 2, 128), (127, 4, 2, 64), (33, 8, 2, 128), (60, 8, 2, 64), (1, 258, 2, 64)])
+def test_dense_rows_past_a_row_tile_go_one_by_one(T, HQ, HKV, D, gpu_device):
+    """From 129 rows a sequence on none shares: paged_attention's own launches."""
+    d, gen = gpu_device, torch.Generator().manual_seed(17)
+    kc, vc, table, lens, starts, shared = make([(300, 3), (130, 2)], lambda n: T + 9 * n, 16, HKV, D, BF16, gen)
+    q = torch.randn(5, T, HQ, D, generator=gen).to(BF16)
+    o, lse = compare(d, q, kc, vc, table, lens, starts, shared)
+    want, want_lse = paged_attention(q.to(d), kc.to(d), vc.to(d), table.to(d), lens.to(d), return_lse=True)
+    assert torch.equal(o, want) and torch.equal(lse, want_lse)
+
+
 @pytest.mark.parametrize("page", [16, 64, 1024])
 @pytest.mark.parametrize("layout", ["token", "head"])
 def test_pages(page, layout, gpu_device):
