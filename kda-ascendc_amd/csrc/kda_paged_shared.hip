@@ -731,8 +731,18 @@ constexpr int WHOLE = Shape<MANY>::MT;
 // and 19.4; 2 sequences: 66 MB 18.9 and 22.1, 131 MB 29.0 and 26.5.  Drafts of 5, 24
 // / 4 heads of 64 (30 rows: their row tiles are full one by one too): 131 MB 24.4
 // and 27.8, 262 MB 35.9 and 33.5.
+//
+// Nor where rows have room for no more keys than the ordinary kernel takes whole:
+// one launch then instead of three, up to two rounds of its work-groups. Decode of
+// sequences behind 400 to 700 shared tokens, 32 / 8 heads: 64 13.8 to 17.4 us one by
+// one and 26.9 so, 128 24.2 to 32.7 and 33.4 to 33.9, but 256 (four rounds) 45 to 59
+// and 48 to 49; 32 / 16 heads: 64 23.9 to 34.0 and 32.7 to 33.7, 128 44 to 63 and 44
+// to 46; 800 keys, cut and joined: 64 36.5 and 26.1. (Packed single tokens are in
+// the launch with many rows: 64 behind 100 to 700 26 to 38 and 26 to 30.)
 bool planned(const SharedParams& p, int D) {
     if (p.N < 2 || p.N > MOST || p.NG > MOST || (!p.cu_seqlens && (int64_t)p.T * p.G >= WHOLE)) return false;
+    const bool few = !p.cu_seqlens && (int64_t)p.T * p.G <= ROWS;
+    if (few && !may_cut(static_cast<const PagedParams&>(p), FEW) && (int64_t)p.N * p.HKV <= 2 * Shape<FEW>::SLOTS) return false;
     const int64_t row = ((int64_t)p.M << p.page_shift) * p.HKV * D * 4;
     const int64_t least = tokens_of(p) * p.G <= (int64_t)p.N * (ROWS / 2) ? 112 << 20 : 224 << 20;
     return row >= least / p.N;

@@ -362,7 +362,8 @@ def paged_attention_shared(
     new tokens fill a row tile (T * HQ / HKV at least 128), which have nothing to
     gain.  Where the table has room for few keys only (112 MB of keys and values
     in all rows together; 224 MB with more than 16 rows, T * HQ / HKV, a sequence
-    on average) all are worked on one by one, which is faster then.
+    on average), or a decode step's or draft's rows hold up to 768 keys, all are
+    worked on one by one, which is faster then.
     """
     device = k_cache.device
     for name, t in (("cu_groups", cu_groups), ("shared_lens", shared_lens)):

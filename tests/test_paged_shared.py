@@ -121,6 +121,18 @@ def test_workspace_of_dense_rows_past_a_row_tile():
         assert 0 <= f(ctypes.byref(a)) - plain(ctypes.byref(a.paged)) <= 1 << 16, base
 
 
+def test_workspace_of_tables_that_one_launch_takes_whole():
+    """Rows of up to 768 keys, decode and drafts, up to two rounds of row tiles: as
+    without groups, which takes no workspace; else a plan's."""
+    f = _hip.lib().kda_paged_attn_shared_workspace_bytes
+    small = dict(N=512, M=48, table_stride=48)
+    for base in (small, small | dict(T=16), small | dict(N=400)):
+        assert f(ctypes.byref(shared(base))) == 0, base
+    for base in (small | dict(M=49, table_stride=49), small | dict(N=513), small | dict(T=17),
+                 small | dict(cu_seqlens=FAKE, T=512, cu_seqlens_dtype=_hip.DTYPE_I32)):
+        assert f(ctypes.byref(shared(base))) > 0, base
+
+
 @fake_pointers
 def test_argument_checks():
     f = _hip.lib().kda_paged_attn_shared_hip

@@ -113,6 +113,20 @@ def test_dense_rows_past_a_row_tile_go_one_by_one(T, HQ, HKV, D, gpu_device):
     assert torch.equal(o, want) and torch.equal(lse, want_lse)
 
 
+@pytest.mark.parametrize("T,HQ,HKV,D", [(1, 16, 8, 128), (4, 16, 8, 128), (5, 24, 8, 128), (1, 16, 16, 64)])
+def test_rows_that_one_launch_takes_whole_go_one_by_one(T, HQ, HKV, D, gpu_device):
+    """Rows of up to 768 keys: paged_attention's own launch, whatever they hold in
+    all (here 256 MB and more)."""
+    d, gen = gpu_device, torch.Generator().manual_seed(18)
+    N = 1024 // HKV
+    kc, vc, table, lens, starts, shared = make([(600, N - 10), (130, 10)], lambda n: T + n % 9, 16, HKV, D, BF16, gen, wide=False)
+    table = torch.cat([table, torch.full((N, 48 - table.shape[1]), -1, dtype=torch.int32)], 1)
+    q = torch.randn(N, T, HQ, D, generator=gen).to(BF16)
+    o, lse = compare(d, q, kc, vc, table, lens, starts, shared)
+    want, want_lse = paged_attention(q.to(d), kc.to(d), vc.to(d), table.to(d), lens.to(d), return_lse=True)
+    assert torch.equal(o, want) and torch.equal(lse, want_lse)
+
+
 @pytest.mark.parametrize("page", [16, 64, 1024])
 @pytest.mark.parametrize("layout", ["token", "head"])
 def test_pages(page, layout, gpu_device):
