@@ -52,7 +52,7 @@ struct alignas(16) Work {
     int first, count, len, pos;  // as NewTokens, `first` a token of all, or a group's of those that share
     int from, row;               // the first key, a row of the table
     int parts, mt;               // parts of a row tile's keys; row tiles
-    int place;                   // of the partial results, in 4 rows; NONE, or OVER where there is no room
+    int place;                   // of the partial results, in 4 rows; NONE, or OVER where there is no room or unit
     int group;                   // a sequence's record of shared tokens, -1: none
     int few, tiles;              // of few rows; tiles of keys
     int few_end, many_end;       // the units of few and of many rows up to this record's
@@ -133,10 +133,12 @@ constexpr int ROUNDS = 3;
 constexpr int FEW_PARTS = 1024;
 
 // One work-group.  `waves`: those of a work-group of few rows; `fine`: tiles of their
-// parts where they are more than run at once; `rounds`: of parts of many rows, at most; `room`: of the partial results,
-// in 4 rows.
+// parts where they are more than run at once; `rounds`: of parts of many rows, at
+// most; `room`: of the partial results, in 4 rows; `grid`: units.  Both suffice
+// whatever the lengths are; where offsets decrease, and sequences have more tokens
+// than there are, what is past them is left out, and the join makes its rows NaN.
 template <int THREADS>
-__global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams p, int waves, int fine, int rounds, int room) {
+__global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams p, int waves, int fine, int rounds, int room, uint32_t grid) {
     constexpr bool ONE = THREADS < 1024;  // a record a thread
     // (of the groups: their sequences' offsets, the first that shares, how many do,
     // with how many tokens; the shared ones.  Sharing tokens before each sequence.)
@@ -312,6 +314,7 @@ __global__ __launch_bounds__(THREADS) void paged_shared_plan_kernel(SharedParams
         for (int k = 0; k < 3; ++k) at.x[k] += x3.x[k];
         w.few_end = at.x[0];
         w.many_end = at.x[1];
+        if (w.parts > 0 && (w.few ? all3.x[1] + at.x[0] : at.x[1]) > grid) w.place = OVER;
         if (v < p.NG) {
             w.first = w.sharer = before[cu[v]];
         } else {
@@ -660,10 +663,19 @@ __global__ __launch_bounds__(256, 2) void paged_shared_join_kernel(SharedParams 
     // 4 rows behind 2000 tokens took 18.2 us instead of 16.8)
     const int rows = w.count * p.G, items = rows * (D / 4);
     const int each = here ? max(128, fours) : fours, used = min(groups, (items + each - 1) / each);
-    if (group0 >= used || (!here && w.place < 0)) return;
+    if (group0 >= used || (!here && w.place == NONE)) return;
     Work g = {};
     if (w.group >= 0) g = load_work(plan, w.group);
-    if (g.place == OVER) return;
+    if (w.place == OVER || g.place == OVER) {
+        const float nan = __builtin_nanf("");
+        for (int e = group0 * 256 + threadIdx.x; e < items; e += used * 256) {
+            const int r = e / (D / 4), piece = e % (D / 4), tok = r / p.G;
+            const int64_t out = ((int64_t)w.first + tok) * p.HQ + h * p.G + (r - tok * p.G);
+            store_o<E, D>(p, out, piece * 4, nan, nan, nan, nan);
+            if (p.lse && piece == 0) p.lse[out] = nan;
+        }
+        return;
+    }
     const Lds tiles = {lds, lds, lds};
     if (here) {
         Unit u;
@@ -801,11 +813,11 @@ hipError_t launch_shared(SharedParams p, hipStream_t stream) {
     const int V = p.NG + p.N, room = (int)std::min(room_of(p), (int64_t)LIMIT - 1);
     const bool only = few_only(p);
     const int waves = Shape<FEW>::WAVES * (only ? 1 : 2), fine = 4 * waves * (128 / D);
-    if (V <= 256) paged_shared_plan_kernel<256><<<1, 256, 0, stream>>>(p, waves, fine, rounds_of(p), room);
-    else paged_shared_plan_kernel<1024><<<1, 1024, 0, stream>>>(p, waves, fine, rounds_of(p), room);
+    const dim3 grid((unsigned)units_of(p));
+    if (V <= 256) paged_shared_plan_kernel<256><<<1, 256, 0, stream>>>(p, waves, fine, rounds_of(p), room, grid.x);
+    else paged_shared_plan_kernel<1024><<<1, 1024, 0, stream>>>(p, waves, fine, rounds_of(p), room, grid.x);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const dim3 grid((unsigned)units_of(p));
     if (only) paged_shared_kernel<E, D, FEW, false><<<grid, 256, 0, stream>>>(p);
     else if (may_be_wide(p)) paged_shared_kernel<E, D, MIXED, true><<<grid, 512, 0, stream>>>(p);
     else paged_shared_kernel<E, D, MIXED, false><<<grid, 512, 0, stream>>>(p);

@@ -251,6 +251,20 @@ def test_offsets_that_are_none_stay_inside(gpu_device):
     compare(gpu_device, q, kc, vc, table, lens, starts, shared)
 
 
+def test_rows_that_there_is_no_room_for_are_nan(gpu_device):
+    """256 sequences of all 60 tokens each, by offsets that decrease: their group's
+    partial results take 61440 fours of rows, and the room that 60 tokens can need
+    is 23020.  No row is left as it was."""
+    gen, i32 = torch.Generator().manual_seed(19), dict(dtype=torch.int32, device=gpu_device)
+    kc, vc = (torch.randn(64, 16, 16, 64, generator=gen).to(BF16).to(gpu_device) for _ in range(2))
+    table = torch.randint(64, (512, 16), generator=gen, dtype=torch.int32).to(gpu_device)
+    q = torch.randn(1, 60, 16, 64, generator=gen).to(BF16).to(gpu_device)
+    o, lse = paged_attention_shared(q, kc, vc, table, torch.full((512,), 100, **i32), torch.tensor([0, 512], **i32),
+                                    torch.tensor([20], **i32), cu_seqlens=torch.tensor([0, 60] * 256 + [0], **i32),
+                                    return_lse=True)
+    assert bool(o.isnan().all()) and bool(lse.isnan().all())
+
+
 def test_packed_single_tokens_equal_batch_rows(gpu_device):
     gen = torch.Generator().manual_seed(16)
     kc, vc, table, lens, starts, shared = make([(333, 9), (100, 30)], lambda n: 1 + 9 * n, 16, 4, 128, BF16, gen)
