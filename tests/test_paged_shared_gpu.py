@@ -381,3 +381,17 @@ def test_another_stream_and_a_graph(gpu_device):
             want = step()
             torch.cuda.synchronize()
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype,D,HQ,HKV", [(BF16, 128, 128, 32), (FP16, 64, 128, 32), (BF16, 64, 96, 16)])
+@pytest.mark.parametrize("prefix,own", [(200, 20), (9000, 20), (200, 3000)])
+def test_sequences_of_many_rows_share_beside_long_chunks(prefix, own, dtype, D, HQ, HKV, gpu_device):
+    """Row tiles of 256 (chunks of no group bring their number past three rounds'
+    768) beside groups whose records are of many rows too: 12, 20 and 31 new tokens
+    (of 6 heads a kv head 21 at most) share with single tokens; the group's keys, or
+    a member's own, cut into several parts."""
+    G = HQ // HKV
+    new = [12, 20, 31 if G == 4 else 21, 1, 9, 20, 500 if HKV == 32 else 900, 257]
+    assert all(x * G < 128 for x in new[:6]) and sum(-(-x * G // 128) for x in new) * HKV >= 768
+    check(gpu_device, [(prefix, 4), (70, 2)], new=new, HQ=HQ, HKV=HKV, D=D, dtype=dtype, after=2,
+          own=lambda n: new[n] + (own if n in (1, 2) else 20 + n))
