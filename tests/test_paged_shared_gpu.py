@@ -395,3 +395,14 @@ def test_sequences_of_many_rows_share_beside_long_chunks(prefix, own, dtype, D, 
     assert all(x * G < 128 for x in new[:6]) and sum(-(-x * G // 128) for x in new) * HKV >= 768
     check(gpu_device, [(prefix, 4), (70, 2)], new=new, HQ=HQ, HKV=HKV, D=D, dtype=dtype, after=2,
           own=lambda n: new[n] + (own if n in (1, 2) else 20 + n))
+
+
+@pytest.mark.parametrize("D,HQ,HKV,pairs,prefix,own", [
+    # tiles of keys times kv heads: 12000 and 24000 (parts of 32 tiles, 64 of head size 64, are finer than a round's),
+    # 36000 (1024 parts)
+    (128, 32, 32, 4, 3000, 900), (64, 64, 32, 12, 2000, 900), (128, 32, 32, 4, 9000, 60),
+    # with no more than 32 rows altogether: waves of fewer, twice the work-groups
+    (128, 32, 32, 3, 6000, 700), (64, 32, 16, 8, 9000, 60)])
+def test_more_parts_of_few_rows_than_run_at_once(D, HQ, HKV, pairs, prefix, own, gpu_device):
+    check(gpu_device, [(prefix + 171 * i, 2) for i in range(pairs)], HQ=HQ, HKV=HKV, D=D, page=64,
+          own=lambda n: 1 + (n * 397) % own)
