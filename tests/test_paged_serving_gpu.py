@@ -13,6 +13,7 @@ import pytest
 import torch
 
 from kda_bt16 import (
+    paged_append,
     paged_append_rotary,
     paged_attention,
     paged_attention_shared,
@@ -171,3 +172,42 @@ def test_a_stream_gives_its_pages_away(gpu_device):
             k[held], v[held] = want.to(torch.bfloat16), loop.values[n]
             loop.pool[0].copy_(k)
             loop.pool[1].copy_(v)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_pages_given_away_are_another_rows(dtype, gpu_device):
+    """A row under a window with first tokens hands the pages between the two back
+    (filled with NaN), another one's next tokens go into them, and both go on: more
+    tokens altogether than the pool has places for."""
+    d, gen = gpu_device, torch.Generator().manual_seed(4)
+    window, sinks, pages, width = 64, 20, 24, 32
+    i32 = dict(dtype=torch.int32, device=d)
+    pool = torch.full((2, pages, PAGE, HKV, D), float("nan"), dtype=dtype, device=d)
+    table, lens, refs = torch.full((2, width), -1, **i32), torch.zeros(2, **i32), torch.zeros(pages, **i32)
+    # what the rows hold, on the CPU, each in pages of its own one after the other
+    rows = torch.zeros(2, 2 * width, PAGE, HKV, D, dtype=dtype)
+    own = torch.arange(2 * width, dtype=torch.int32).view(2, width)
+    given, total = set(), [0, 0]
+    for new in ([100, 3], [30, 40], [30, 41], [30, 40], [1, 40], [30, 37], [33, 1], [7, 40]):
+        assert bool(paged_reserve(table, lens, refs, torch.tensor(new, **i32), PAGE).all())
+        cu = torch.tensor([0, new[0], sum(new)], **i32)
+        q, k, v = torch.randn(1, sum(new), HQ + 2 * HKV, D, generator=gen).clamp(-6, 6).to(dtype).split([HQ, HKV, HKV], 2)
+        paged_append(k.to(d), v.to(d), pool[0], pool[1], table, lens, cu_seqlens=cu)
+        for n, first in enumerate((0, new[0])):
+            pos = torch.arange(total[n], total[n] + new[n])
+            for c, x in zip(rows, (k, v)):
+                c[own[n, pos // PAGE].long(), pos % PAGE] = x[0, first:first + new[n]]
+            total[n] += new[n]
+        assert lens.tolist() == total
+        got = paged_attention(q.to(d), pool[0], pool[1], table, lens, window=window, sinks=sinks, cu_seqlens=cu, return_lse=True)
+        want = attention(q, rows[0], rows[1], own, total, D ** -0.5, lambda pos, j: (j > pos - window) | (j < sinks), cu.cpu())
+        assert not misses(*got, want, q, total, D ** -0.5, cu.cpu())
+        for n in range(2):
+            gone = table[n, -(-sinks // PAGE):max(0, (total[n] + 1 - window) // PAGE)]
+            at = gone[gone >= 0].long()
+            given |= {(n, p) for p in at.tolist()}
+            pool[:, at] = float("nan")
+            refs[at] -= 1
+            gone[:] = -1
+    held = {(n, p) for n in range(2) for p in table[n].tolist() if p >= 0}
+    assert {(1 - n, p) for n, p in given} & held and sum(total) > pages * PAGE
