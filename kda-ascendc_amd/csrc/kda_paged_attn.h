@@ -210,7 +210,9 @@ __device__ __forceinline__ float sum_halves(float x) {
 // the sums so far have to shrink, by `alpha`.
 // m follows the maximum only when a row's grows by more than a factor of 2^8
 // (any m does as long as nothing overflows: weights stay at most 2^8, and fp32
-// sums and 16-bit weights keep their relative precision), so that the rescaling
+// sums and 16-bit weights keep their relative precision: the weights are rounded
+// for the second product, whose matrix ops take 16 bits, each by half a step at most,
+// while l sums them in fp32 as they were), so that the rescaling
 // of O, 64 multiplications a lane against the softmax's ~130 operations, is
 // rare after the first tiles (a prompt of 8192 tokens: 557 us when m follows
 // every growth, 522 so).

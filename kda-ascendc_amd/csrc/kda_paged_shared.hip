@@ -16,7 +16,7 @@
 // each.  The join, which also works on the own keys of sequences that have few.
 //
 // 64 answers with 10 to 500 tokens of their own behind 16000, 32 / 8 heads: 47 us
-// (400 one by one), where the keys read once at 5.2 TB/s are 19 and the products at
+// (390 to 400 one by one), where the keys read once at 5.2 TB/s are 19 and the products at
 // 1.4 PFLOP/s 12.  The plan takes 4.5: its loads, three sums over the work-group.
 // The parts 29: 1.8 until a work-group has its unit, 3 until its first keys, 16.5
 // for 8 times two tiles (the matrix unit and the softmax in turn, as in
@@ -42,7 +42,7 @@ constexpr int MT = 128;
 // 512 behind 12000 take 251 us so instead of 196, 4 of up to 300 158 instead of 137.
 constexpr int WIDE_MT = Shape<MANY>::MT, WIDE = 3 * Shape<MANY>::SLOTS;
 
-// Sequences and groups that a plan has room for.
+// Sequences, and groups, that a plan has room for (in LDS); more go one by one.
 constexpr int MOST = 2048;
 
 // What is worked on together: the queries of a group over its shared tokens, or
@@ -116,9 +116,13 @@ __device__ __forceinline__ uint32_t limited(int64_t x) { return (uint32_t)min(x,
 
 // Of sequences that share, those with few rows and up to this many tiles of keys
 // of their own have them worked on in the join: not in parts that would only
-// begin when those of the prefixes are over (64 sequences with 10 to 500 tokens of
-// their own behind 16000: 47 us, with up to 8 or 12 tiles 52; drafts with up to 700
-// tokens 31.6, with up to 24 tiles 33.6).
+// begin when those of the prefixes are over.  With 8, 12, 16 and 24 tiles, single
+// tokens of 32 / 8 heads, own tokens spread up to 500: 64 sequences behind 16000 62,
+// 58, 54 and 54 us, 16 behind 8000 37, 38, 34 and 34, 8 behind 4000 20, 21, 22 and 22;
+// up to 1000: 77, 76, 77 and 77, 44, 40, 41 and 43, 22, 22, 24 and 26; up to 2000: 102,
+// 102, 103 and 106, 52, 52, 53 and 55, 22, 25, 25 and 27.  (40 drafts of 5, 24 / 4 heads
+// of 64, behind 4000: up to 500 35, 35, 32 and 32, 1000 41, 41, 41 and 39, 2000 46, 46,
+// 46 and 47; up to 200 own tokens all the same.)
 constexpr int IN_JOIN = 16;
 // Rounds of parts of many rows at most, on 256 CUs each.
 constexpr int ROUNDS = 3;
@@ -738,7 +742,10 @@ constexpr int WHOLE = Shape<MANY>::MT;
 //
 // Where the table is so small that reading the shared keys again for each
 // sequence costs less than the plan and the longer join, 15 us for 9, it does not:
-// by the bytes that its rows hold, whose second reading is from the caches. Decode
+// by the bytes that its rows have room for, whose second reading is from the caches.
+// (The lengths are on the device: a wide table of short rows takes the three
+// launches, 8 sequences behind 2000 tokens in rows of 8000 pages 17.4 us instead of
+// 14.0, 2 16.8 instead of 10.3, 64 behind 100 22.8 instead of 15.8.)  Decode
 // of 8 sequences, 32 / 8 heads: 67 MB 15.3 us one by one and 17.9 so, 131 MB 21.3
 // and 19.4; 2 sequences: 66 MB 18.9 and 22.1, 131 MB 29.0 and 26.5.  Drafts of 5, 24
 // / 4 heads of 64 (30 rows: their row tiles are full one by one too): 131 MB 24.4

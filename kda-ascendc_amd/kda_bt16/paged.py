@@ -360,10 +360,13 @@ def paged_attention_shared(
     sequence whose new tokens do not all come behind the shared ones (a freed
     row) is worked on by itself, and so are rows of no group and sequences whose
     new tokens fill a row tile (T * HQ / HKV at least 128), which have nothing to
-    gain.  Where the table has room for few keys only (112 MB of keys and values
+    gain (packed chunks of thousands of tokens take 2 to 3 % longer than by
+    :func:`paged_attention`).  Beyond 2048 sequences or 2048 groups all are worked
+    on one by one.  Where the table has room for few keys only (112 MB of keys and values
     in all rows together; 224 MB with more than 16 rows, T * HQ / HKV, a sequence
     on average), or a decode step's or draft's rows hold up to 768 keys, all are
-    worked on one by one, which is faster then.
+    worked on one by one, which is faster then; so a table should be no wider than
+    its rows may grow.
     """
     device = k_cache.device
     for name, t in (("cu_groups", cu_groups), ("shared_lens", shared_lens)):
