@@ -118,9 +118,9 @@ int kda_paged_attn_sinks_hip(const KdaPagedSinksArgs* args, void* stream);
  * do not all come behind the shared ones (an ended one's) is worked on by itself,
  * and so are rows of no group, and sequences whose new tokens fill a row tile
  * (T_n * HQ / HKV at least 128), which have nothing to gain.  Beyond 2048 sequences
- * or 2048 groups, with more than 128 rows a sequence without cu_seqlens, and where
- * the table's rows are short (paged_attention_shared() in Python says how short), all
- * are worked on one by one, as by kda_paged_attn_hip. */
+ * or 2048 groups, mostly where every sequence has more than 128 rows (without
+ * cu_seqlens), and where the table's rows are short (paged_attention_shared() in
+ * Python says how short), all are worked on one by one, as by kda_paged_attn_hip. */
 typedef struct KdaPagedSharedArgs {
     KdaPagedArgs paged;
     const int32_t* cu_groups;   /* [num_groups + 1], from 0 to N, non-decreasing */

@@ -768,12 +768,19 @@ bool planned(const SharedParams& p, int D) {
 }
 // Dense calls of more rows a sequence than fill a row tile, of which the plan lets
 // none share.  In its row tiles of 128, the second one filled in part, they are
-// mostly slower than one by one in one of 256 (32 / 8 heads, 160 rows: 8 sequences
-// behind 12000 tokens 98 us one by one and 150 so, 32 264 and 310, 64 behind 2000
-// 114 and 123; 24 / 4 heads of 64, 162 rows: 64 behind 12000 212 and 253, but 32 216
-// and 130).  Of 128 rows, which share no more, one row tile is full and 256 rows are
+// slower than one by one in one of 256 (32 / 8 heads, 160 rows: 8 sequences behind
+// 12000 tokens 98 us one by one and 150 so, 32 264 and 310, 64 behind 2000 114 and
+// 123; 24 / 4 heads of 64, 162 rows: 64 behind 12000 212 and 253), but where row tiles
+// are a quarter to a half of the CUs, which the ordinary kernel cuts in two or three
+// and the plan in three to five (24 / 4 heads of 64: 32 behind 12000 216 and 130, behind
+// 2000 52 and 37; 8 / 8 heads: 16 behind 7400 176 and 128).  Of 90 random calls the
+// former took 0.93 of their time in groups one by one, the latter 1.22 of it.
+// Of 128 rows, which share no more, one row tile is full and 256 rows are
 // half empty: 8 behind 12000 88 and 75, 32 229 and 195, 64 behind 2000 102 and 93.
-bool alone(const SharedParams& p) { return !p.cu_seqlens && (int64_t)p.T * p.G > MT; }
+bool alone(const SharedParams& p) {
+    const int64_t tiles = (int64_t)p.N * p.HKV;
+    return !p.cu_seqlens && (int64_t)p.T * p.G > MT && (tiles <= Shape<MANY>::SLOTS / 4 || tiles > Shape<MANY>::SLOTS / 2);
+}
 // Whether sequences are worked on together at all.
 bool together(const SharedParams& p, int D) { return planned(p, D) && !alone(p); }
 bool few_only(const SharedParams& p) { return tokens_of(p) * p.G <= ROWS; }

@@ -119,6 +119,10 @@ def test_workspace_of_dense_rows_past_a_row_tile():
         base = dict(T=T, HQ=heads, q_row=T * heads * 128, q_token=heads * 128, M=8000, table_stride=8000)
         a = shared(base)
         assert 0 <= f(ctypes.byref(a)) - plain(ctypes.byref(a.paged)) <= 1 << 16, base
+    # (65 to 128 row tiles of 256: in the plan's finer parts)
+    for N, more in ((32, False), (33, True), (64, True), (65, False)):
+        a = shared(base | dict(N=N))
+        assert (f(ctypes.byref(a)) - plain(ctypes.byref(a.paged)) > 1 << 16) == more, N
 
 
 def test_workspace_of_tables_that_one_launch_takes_whole():

@@ -113,6 +113,13 @@ def test_dense_rows_past_a_row_tile_go_one_by_one(T, HQ, HKV, D, gpu_device):
     assert torch.equal(o, want) and torch.equal(lse, want_lse)
 
 
+@pytest.mark.parametrize("T,HQ,HKV,D,dtype", [(65, 4, 2, 64, BF16), (40, 8, 2, 128, FP16), (1, 130, 1, 64, BF16), (127, 2, 1, 64, FP16)])
+def test_dense_rows_past_a_row_tile_in_finer_parts(T, HQ, HKV, D, dtype, gpu_device):
+    """65 to 128 row tiles of 256: by the plan, in row tiles of 128, none shared."""
+    N = 70 // HKV
+    check(gpu_device, [(300, N - 12), (130, 12)], T=T, HQ=HQ, HKV=HKV, D=D, dtype=dtype)
+
+
 @pytest.mark.parametrize("T,HQ,HKV,D", [(1, 16, 8, 128), (4, 16, 8, 128), (5, 24, 8, 128), (1, 16, 16, 64)])
 def test_rows_that_one_launch_takes_whole_go_one_by_one(T, HQ, HKV, D, gpu_device):
     """Rows of up to 768 keys: paged_attention's own launch, whatever they hold in
